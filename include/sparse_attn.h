@@ -454,6 +454,103 @@ int sa_gemm_skinny(int dtype, const void* x, int64_t x_stride, const void* w, in
 int sa_gemm_skinny_swiglu(int dtype, const void* x, int64_t x_stride, const void* w_gate_up, int64_t w_stride,
                           void* out, int64_t out_stride, int M, int I, int K, void* stream);
 
+/*
+ * Operators of a chunk of new tokens over a paged cache: sequences of different lengths in one launch, from one
+ * token each to whole prompts.  No counterpart in the reference, whose cache is contiguous and whose sequences
+ * share one length.
+ *
+ * Packed rows: the new tokens of sequence b are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of tensors of N rows
+ * (device int32, B + 1 entries, not descending); rows outside [cu_seqlens[0], cu_seqlens[B]) belong to no
+ * sequence and their outputs are left as they were.  kv_lens[b] (device int32) counts the tokens of sequence b with the new ones, so new
+ * token i of n sits at position kv_lens[b] - n + i.  Pools [num_pages, Hkv, page, D] (strides in elements: page,
+ * head, token; page a multiple of 16 in 16..128) and block_table [B, max_blocks] (row stride block_table_stride)
+ * as for sa_decode: a position past the table or a page id outside the pool is neither read nor written.  D is
+ * 64 or 128; every head row is 16-byte aligned.
+ */
+
+/*
+ * Per-head RMSNorm and rotary embedding of queries and keys, [B, T, H, D] each with any batch, token and head
+ * strides (a packed [N, H, D] is B = 1):
+ *   n = x * rsqrt(mean(x^2) + eps) * weight      (weight NULL: n = x)
+ *   out[i] = n[i] cos - n[i + D/2] sin,  out[i + D/2] = n[i + D/2] cos + n[i] sin,  angle inv_freq[i] * position
+ * in fp32 with the angle in fp64, rounded once to the element type (sa_qk_rope_kv, which keeps Hugging Face's
+ * roundings, rounds five times on the way).  inv_freq: D/2 fp32; positions[b * pos_sb + t]: device int64.
+ * q_out / k_out may be q / k themselves.  Hq or Hkv may be 0 (that tensor is not touched).
+ */
+int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                    const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                    void* q_out, int64_t qo_sb, int64_t qo_st, int64_t qo_sh,
+                    void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh,
+                    const void* q_weight, const void* k_weight, const float* inv_freq,
+                    const int64_t* positions, int64_t pos_sb,
+                    int B, int T, int Hq, int Hkv, int D, float eps, void* stream);
+
+/*
+ * Writes a chunk's keys and values into the pages: k normed (k_weight, or NULL) and rotated (inv_freq, or NULL:
+ * as they are), v as it is.  With Hq > 0 the queries take the same norm and rotation into q_out in the same
+ * launch.  Arithmetic as in sa_qk_norm_rope; q, k, v may be views of one projection row.
+ * k_bounds (or NULL) [num_pages, Hkv, 2, D] (strides in elements: page, head): the minimum and the maximum of a
+ * page's stored keys in each dim.  A page whose first slot is written gets fresh bounds, another has the new
+ * keys merged into the stored ones.  No two sequences may write one page.
+ */
+int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                    const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                    const void* q_weight, const void* k_weight, const float* inv_freq,
+                    void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st, int num_pages,
+                    void* k_bounds, int64_t bounds_sp, int64_t bounds_sh,
+                    const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                    const int32_t* cu_seqlens, const int32_t* kv_lens,
+                    int N, int B, int Hq, int Hkv, int D, int page, float eps, void* stream);
+
+/*
+ * Causal attention of the new tokens over the pages (their own keys included): the row of a token at position p
+ * sees the keys j <= p of its sequence; o[row] = sum_j softmax_j(q . k_j * sm_scale) v_j with fp32 statistics
+ * and accumulators, 0 for a row that sees no key.  Probabilities are rounded to the element type before the second
+ * product.  Query head h reads KV head h / (Hq / Hkv).
+ * sel (or NULL: all pages): the logical pages that each block of 64 new tokens sees, as sa_paged_block_select
+ * writes them.  Blocks are numbered through the batch, sequence b having ceil(new tokens / 64) of them; the
+ * pages of block i and KV head g, each at most once, are
+ *   sel[i * sel_sr + g * sel_sh + e] for e in [sel_off[i * off_sr + g * off_sh], sel_off[i * off_sr + g * off_sh + 1])
+ * (within sel_width entries).  sel_rows >= N / 64 + min(B, N).
+ * num_splits (1..64): the key range of each row tile is divided over that many workgroups, whose fp32 partials
+ * a second kernel merges; num_splits > 1 needs sa_paged_chunk_workspace_bytes() bytes of workspace, which calls
+ * that may run concurrently must not share.
+ */
+int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64_t q_sh,
+                        const void* k_pages, const void* v_pages,
+                        int64_t pages_sp, int64_t pages_sh, int64_t pages_st, int num_pages,
+                        const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                        const int32_t* cu_seqlens, const int32_t* kv_lens,
+                        const int32_t* sel, int64_t sel_sr, int64_t sel_sh, int sel_rows, int sel_width,
+                        const int32_t* sel_off, int64_t off_sr, int64_t off_sh,
+                        void* o, int64_t o_st, int64_t o_sh,
+                        int N, int B, int Hq, int Hkv, int D, int page, float sm_scale,
+                        int num_splits, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sa_paged_chunk_workspace_bytes(int N, int Hq, int D, int num_splits);
+
+/*
+ * Lists, for each query, the pages worth attending: for one new token per sequence (cu_seqlens NULL, N == B, list
+ * row b; the layout that sa_decode reads) or for each block of 64 new tokens (row i as in sa_paged_chunk_attn), and
+ * each KV head.  The first `sink` pages are kept, the last `recent` (counted back from the page of the row's
+ * first query; all pages up to its last query's), and of the pages between the top_k with the largest
+ *   score(page) = sum over the row's queries and the heads of the group of sum_d max(q_d lo_d, q_d hi_d)
+ * over the page's k_bounds [num_pages, Hkv, 2, D] (lo, hi): an upper bound of the queries' products with its
+ * keys.  fp64 scores; ties go to the lower page; a page whose score is NaN, or which has no valid page id, ranks
+ * last.  sel[i * sel_sr + g * sel_sh + ...] (int32) receives the pages in ascending order, zero-padded to `width`, and
+ * sel_off [rows, Hkv, 2] (contiguous) 0 and their number.  rows == B, or N / 64 + min(B, N) with cu_seqlens (rows
+ * past the last block are empty); width >= sink + top_k + recent - 1 + the pages that a row's queries may lie in
+ * (1, or (62 + page) / page + 1 with cu_seqlens).  The workspace holds scores where the call needs it
+ * (sa_paged_block_select_workspace_bytes, 0: none); calls that may run concurrently must not share it.
+ */
+int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int64_t q_sh,
+                          const void* k_bounds, int64_t bounds_sp, int64_t bounds_sh, int num_pages,
+                          const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                          const int32_t* cu_seqlens, const int32_t* kv_lens,
+                          int N, int B, int Hq, int Hkv, int D, int page, int top_k, int sink, int recent,
+                          int32_t* sel, int64_t sel_sr, int64_t sel_sh, int rows, int width, int32_t* sel_off,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks);
+
 #ifdef __cplusplus
 }
 #endif

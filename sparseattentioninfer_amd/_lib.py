@@ -145,6 +145,52 @@ SIGNATURES = {
     "sa_swiglu": (_i32, [_i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp]),
     "sa_gemm_skinny": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp]),
     "sa_gemm_skinny_swiglu": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp]),
+    "sa_qk_norm_rope": (_i32, [
+        _i32,
+        _vp, _i64, _i64, _i64,
+        _vp, _i64, _i64, _i64,
+        _vp, _i64, _i64, _i64,
+        _vp, _i64, _i64, _i64,
+        _vp, _vp, _vp, _vp, _i64,
+        _i32, _i32, _i32, _i32, _i32, _f32, _vp,
+    ]),
+    "sa_paged_append": (_i32, [
+        _i32,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _vp, _vp, _vp,
+        _vp, _vp, _i64, _i64, _i64, _i32,
+        _vp, _i64, _i64,
+        _vp, _i64, _i32,
+        _vp, _vp,
+        _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp,
+    ]),
+    "sa_paged_chunk_attn": (_i32, [
+        _i32,
+        _vp, _i64, _i64,
+        _vp, _vp, _i64, _i64, _i64, _i32,
+        _vp, _i64, _i32,
+        _vp, _vp,
+        _vp, _i64, _i64, _i32, _i32,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _i32, _i32, _i32, _i32, _i32, _i32, _f32,
+        _i32, _vp, _i64, _vp,
+    ]),
+    "sa_paged_chunk_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "sa_paged_block_select": (_i32, [
+        _i32,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64, _i32,
+        _vp, _i64, _i32,
+        _vp, _vp,
+        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+        _vp, _i64, _i64, _i32, _i32, _vp,
+        _vp, _i64, _vp,
+    ]),
+    "sa_paged_block_select_workspace_bytes": (_i64, [_i32, _i32, _i32]),
 }
 
 

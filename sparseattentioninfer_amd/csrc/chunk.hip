@@ -1,0 +1,535 @@
+// Causal attention of a chunk of new tokens over a paged cache, gfx950 (CDNA4): sequences of different lengths,
+// whole caches or the pages that a selection lists for each 64-query block.
+//
+//   o[row] = sum_j softmax_j(q . k_j * scale) v_j over the keys j <= position of the row (and listed pages),
+//
+// position = kv_len - new tokens + index of the row's token.  fp32 statistics and accumulators; probabilities are
+// rounded to the element type for the second product, which is matrix-core work, and the sum that divides is of
+// the unrounded ones.  A row that sees no key is 0.
+//
+// Rows of an item are (token, query head of one KV head) pairs, flattened with the head fastest, so a tile of 32
+// rows is full whatever the group size, and every K/V tile read serves the whole group.  Keys are read in tiles
+// of 64, each four chunks of 16 keys; a page is a whole number of chunks, so a chunk lies in one page and each of
+// its wave-wide direct loads has one uniform address.  A wave looks its chunks' pages up 64 at a time, one a
+// lane, and takes them lane by lane.
+#include <algorithm>
+
+#include "lds_tile.h"
+#include "ragged.h"
+
+namespace sa {
+
+constexpr int CK_ROWS = 32;        // rows of a wave
+constexpr int CK_KT = 64;          // keys of a tile
+constexpr int CK_BLOCK = 64;       // new tokens that share one selection
+constexpr int CK_NO_KEY = 0x60000000;  // key position of a chunk that is not there: past every row
+// Largest token stride (elements) of the pools: per-lane offsets within a chunk are 32-bit.
+constexpr int64_t CK_MAX_STRIDE = (int64_t)1 << 24;
+
+// 16 readable zero bytes: what lanes of keys that are not there load, so masked keys add 0 * 0.
+__device__ __attribute__((aligned(16))) const uint32_t c_zero16[4] = {0u, 0u, 0u, 0u};
+
+struct ChunkArgs {
+  const elem_t* q;
+  int64_t q_st, q_sh;
+  const elem_t *k, *v;
+  int64_t kv_sp, kv_sh, kv_st;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_blocks, num_pages, page;
+  uint32_t mul_page;
+  Ragged seqs;
+  // selection (NULL: every page): row of query block i, KV head g: sel[i * sel_sr + g * sel_sh + e]
+  const int32_t* sel;
+  int64_t sel_sr, sel_sh;
+  const int32_t* sel_off;
+  int64_t off_sr, off_sh;
+  int sel_rows, sel_width;
+  uint32_t mul_ppc;                // fast_div multiplier of the chunks of a page
+  elem_t* o;
+  int64_t o_st, o_sh;
+  int Hq, Hkv, G;
+  uint32_t mul_G, mul_heads, mul_splits;
+  float scale_log2;
+  int tiles;                       // row tiles of the launch (more than there are: the rest exit)
+  int tiles_per_block;             // with a selection: row tiles of a 64-token block
+  int splits;
+  float* part_acc;                 // splits > 1: [splits, N * Hq, D]
+  float* part_ml;                  // [splits, N * Hq, 2]: row reference (base 2) and row sum
+};
+
+// The rows and keys of one work item.
+struct ChunkItem {
+  int b, kvh, split;
+  int row0, row_end;               // flattened rows of the sequence
+  int tok0;                        // packed row of the sequence's first new token
+  int start;                       // position of its first new token
+  int end;                         // its tokens in all
+  int pos_max;                     // position of the last row
+  int c0, c1;                      // chunks of the item: [c0, c1)
+  const int32_t* list;             // selected pages, or NULL
+  int list_chunks;
+};
+
+__device__ __forceinline__ int tiles_of(const ChunkArgs& a, int rows, int n) {
+  return a.sel ? (n + CK_BLOCK - 1) / CK_BLOCK * a.tiles_per_block
+               : (int)(((int64_t)n * a.G + rows - 1) / rows);
+}
+
+// Work item of workgroup `id` with tiles of `rows` rows, or false.  Heads go fastest (one XCD's workgroups then
+// read one KV head where there are eight of them), then splits; later tiles, which see more keys, come first.
+__device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int rows, int id, ChunkItem& it) {
+  const uint32_t rest = fast_div((uint32_t)id, (uint32_t)a.Hkv, a.mul_heads);
+  it.kvh = id - (int)rest * a.Hkv;
+  const uint32_t t = fast_div(rest, (uint32_t)a.splits, a.mul_splits);
+  it.split = (int)(rest - t * (uint32_t)a.splits);
+  const int x = a.tiles - 1 - (int)t;
+  int local;
+  auto count = [&](int s) {
+    int r0;
+    return tiles_of(a, rows, a.seqs.rows(s, r0));
+  };
+  if (!find_item(a.seqs.B, x, count, it.b, local)) return false;
+  const int n = a.seqs.rows(it.b, it.tok0);
+  it.end = a.seqs.kv_len(it.b);
+  it.start = it.end - n;
+  it.list = nullptr;
+  it.list_chunks = 0;
+  if (a.sel) {
+    const int blk = local / a.tiles_per_block, sub = local % a.tiles_per_block;
+    it.row_end = min(n, (blk + 1) * CK_BLOCK) * a.G;
+    it.row0 = blk * CK_BLOCK * a.G + sub * rows;
+    if (it.row0 >= it.row_end) return false;
+    it.row_end = min(it.row_end, it.row0 + rows);
+    const int sr = x / a.tiles_per_block;
+    if (sr >= a.sel_rows) return false;
+    const int32_t* off = a.sel_off + sr * a.off_sr + it.kvh * a.off_sh;
+    const int e0 = min(max(off[0], 0), a.sel_width), e1 = min(max(off[1], e0), a.sel_width);
+    it.list = a.sel + sr * a.sel_sr + it.kvh * a.sel_sh + e0;
+    it.list_chunks = (e1 - e0) * (a.page / 16);
+  } else {
+    it.row0 = local * rows;
+    it.row_end = (int)min((int64_t)n * a.G, (int64_t)it.row0 + rows);
+  }
+  it.pos_max = it.start + (int)fast_div((uint32_t)(it.row_end - 1), (uint32_t)a.G, a.mul_G);
+  const int chunks = a.sel ? it.list_chunks : it.pos_max < 0 ? 0 : it.pos_max / 16 + 1;
+  const int64_t nt = (chunks + 3) / 4;
+  it.c0 = 4 * (int)(nt * it.split / a.splits);
+  it.c1 = min(chunks, 4 * (int)(nt * (it.split + 1) / a.splits));
+  return true;
+}
+
+// 64 chunks looked up at once: lane i holds where chunk base + i of the item lies in the pools (elements from
+// the KV head's start) and its first key position, CK_NO_KEY if no row of the item sees it.
+struct ChunkWindow {
+  int base;
+  int64_t off;
+  int key;
+
+  __device__ __forceinline__ void fill(const ChunkArgs& a, const ChunkItem& it, int first) {
+    base = first;
+    const int x = first + (int)(threadIdx.x & 63);
+    key = CK_NO_KEY;
+    off = 0;
+    if (x < it.c1) {
+      int lb, slot;
+      if (it.list) {
+        const int e = (int)fast_div((uint32_t)x, (uint32_t)(a.page / 16), a.mul_ppc);
+        lb = it.list[e];
+        slot = (x - e * (a.page / 16)) * 16;
+      } else {
+        lb = (int)fast_div((uint32_t)(16 * x), (uint32_t)a.page, a.mul_page);
+        slot = 16 * x - lb * a.page;
+      }
+      if (lb >= 0 && lb < a.max_blocks && (int64_t)lb * a.page + slot <= it.pos_max) {
+        const int pg = a.table[it.b * a.table_stride + lb];
+        if (pg >= 0 && pg < a.num_pages) {
+          off = (int64_t)pg * a.kv_sp + (int64_t)slot * a.kv_st;
+          key = lb * a.page + slot;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ int key_of(int c) const { return __builtin_amdgcn_readlane(key, c - base); }
+  __device__ __forceinline__ int64_t off_of(int c) const {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uint64_t)off, c - base);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)off >> 32), c - base);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+  }
+};
+
+template <bool BF16, int D>
+struct Chunk : StagedTile {
+  using E = Elem<BF16>;
+  static constexpr int NW = 4;                     // waves; each has the same rows and keys of its own
+  static constexpr int NT = 64 * NW;
+  static constexpr int NCG = D / 32;               // column groups of a staged tile
+  static constexpr int NI = 4 * NCG;               // 1 KiB direct loads of a tile
+  static constexpr int TILE_BYTES = CK_KT * D * 2;
+  static constexpr int LDS_BYTES = NW * 2 * TILE_BYTES;
+  static_assert(LDS_BYTES >= NW * CK_ROWS * D * 4, "the accumulators are merged in the staging buffers");
+  // The row reference is raised when a lane's probabilities of a tile sum past this: no probability then
+  // exceeds 2^16 in bf16 (2^15 in fp16, whose largest is 65,504).
+  static constexpr float REFIT_SUM = BF16 ? 65536.f : 32768.f;
+
+  static __device__ __forceinline__ void wait_reads() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  template <int LEFT>
+  static __device__ __forceinline__ void wait_loads() {  // until at most LEFT of the wave's loads are in flight
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(LEFT) : "memory");
+  }
+
+  // Direct loads of the 64 keys of chunks c .. c + 3 into `tile`.
+  template <bool PERMUTE>
+  static __device__ __forceinline__ void load_tile(const ChunkArgs& a, const ChunkItem& it, const ChunkWindow& w,
+                                                   const elem_t* head, char* tile, int c, int lane, uint32_t lane_off) {
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const int key = w.key_of(c + rb);
+      const elem_t* src = head + w.off_of(c + rb);
+      const uint32_t lds = lds_addr(tile + rb * 1024);
+      if (key + 16 <= it.end) {
+#pragma unroll
+        for (int cg = 0; cg < NCG; ++cg) load_lds16(src + 32 * cg, lane_off, lds + cg * 4096);
+      } else {
+        const int r = PERMUTE ? krow(lane >> 2) : lane >> 2;
+        const bool live = key + r < it.end;
+#pragma unroll
+        for (int cg = 0; cg < NCG; ++cg) {
+          const void* p = live ? (const void*)(src + r * a.kv_st + 32 * cg + dma_col(lane)) : (const void*)c_zero16;
+          load_lds16(p, lds + cg * 4096);
+        }
+      }
+    }
+  }
+
+  static __device__ void run(const ChunkArgs& a) {
+    __shared__ __attribute__((aligned(16))) char s_kv[LDS_BYTES];
+    __shared__ float s_ml[NW * 2 * CK_ROWS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 5, l32 = lane & 31;
+    ChunkItem it;
+    if (!find_chunk_item(a, CK_ROWS, blockIdx.x, it)) return;
+
+    const int row = min(it.row0 + l32, it.row_end - 1);
+    const int token = (int)fast_div((uint32_t)row, (uint32_t)a.G, a.mul_G);
+    const int pos = it.start + token;
+    const int pos_min = it.start + (int)fast_div((uint32_t)it.row0, (uint32_t)a.G, a.mul_G);
+    u32x4 qf[D / 16];
+    {
+      const elem_t* qs = a.q + (int64_t)(it.tok0 + token) * a.q_st + (it.kvh * a.G + row - token * a.G) * a.q_sh + 8 * g;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4*>(qs + 16 * c);
+    }
+    const Frag f(lane);
+    char* sK = s_kv + wave * 2 * TILE_BYTES;
+    char* sV = sK + TILE_BYTES;
+    const elem_t* kh = a.k + it.kvh * a.kv_sh;
+    const elem_t* vh = a.v + it.kvh * a.kv_sh;
+    const uint32_t koff = (uint32_t)((krow(lane >> 2) * a.kv_st + dma_col(lane)) * 2);
+    const uint32_t voff = (uint32_t)(((lane >> 2) * a.kv_st + dma_col(lane)) * 2);
+
+    f32x16 O[NCG];
+#pragma unroll
+    for (int dt = 0; dt < NCG; ++dt) O[dt] = f32x16{};
+    float m_ref = -__builtin_inff(), neg_m = 0.f, l_run = 0.f;
+    bool ref_ok = false;
+    const float c = a.scale_log2;
+
+    // This wave's share of the item's tiles.
+    const int nt = (it.c1 - it.c0 + 3) / 4;
+    const int t0 = nt * wave / NW, t1 = nt * (wave + 1) / NW;
+    ChunkWindow w;
+    w.base = 0;
+    auto look = [&](int ch) {
+      if (ch - w.base >= 64) w.fill(a, it, ch);
+    };
+    auto raise = [&](const f32x16 (&S)[2]) {
+      float mx = S[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[j][r]);
+      const float m_new = fmaxf(m_ref, halves_max(mx) * c);  // -inf stays -inf (c > 0)
+      const float alpha = m_ref == -__builtin_inff() ? 1.f : fast_exp2(m_ref - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NCG; ++dt) O[dt] *= alpha;
+      m_ref = m_new;
+      neg_m = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+      ref_ok = !__any(m_ref == -__builtin_inff());
+    };
+    u32x4 P[2][2];
+    auto probs = [&](const f32x16 (&S)[2]) {
+      float ls = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = fast_exp2(fmaf(S[j][8 * h + 2 * e], c, neg_m));
+            const float p1 = fast_exp2(fmaf(S[j][8 * h + 2 * e + 1], c, neg_m));
+            ls += p0 + p1;
+            P[j][h][e] = E::pack2f(p0, p1);
+          }
+      return ls;
+    };
+
+    if (t0 < t1) {
+      int ch = it.c0 + 4 * t0;
+      w.fill(a, it, ch);
+      load_tile<true>(a, it, w, kh, sK, ch, lane, koff);
+      load_tile<false>(a, it, w, vh, sV, ch, lane, voff);
+      for (int t = t0; t < t1; ++t, ch += 4) {
+        int key[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) key[x] = w.key_of(ch + x);
+        wait_loads<NI>();  // K is in LDS, V may be in flight
+        f32x16 S[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int cc = 0; cc < D / 16; ++cc)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) S[j] = E::mfma32(kfrag(sK, f, j, cc), qf[cc], S[j]);
+        const bool more = t + 1 < t1;
+        if (more) {
+          look(ch + 4);
+          wait_reads();
+          load_tile<true>(a, it, w, kh, sK, ch + 4, lane, koff);
+        }
+        // Keys past a row's position, in the tiles that hold any.
+        if (max(max(key[0], key[1]), max(key[2], key[3])) + 15 > pos_min) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int lim = pos - key[2 * j + h] - 8 * g;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) S[j][8 * h + e] = e > lim ? -__builtin_inff() : S[j][8 * h + e];
+            }
+        }
+        if (!ref_ok) raise(S);
+        float ls = probs(S);
+        if (__any(!(ls <= REFIT_SUM))) {
+          raise(S);
+          ls = probs(S);
+        }
+        l_run += ls;
+        if (more)
+          wait_loads<NI>();  // V is in LDS, the next K may be in flight
+        else
+          wait_loads<0>();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int dt = 0; dt < NCG; ++dt) O[dt] = E::mfma32(vfrag(sV, f, j, h, dt), P[j][h], O[dt]);
+        if (more) {
+          wait_reads();
+          load_tile<false>(a, it, w, vh, sV, ch + 4, lane, voff);
+        }
+      }
+    }
+
+    // Merge of the waves' shares through LDS, in fp32: accumulator row r is D floats at r * 4 D, its 16-byte
+    // chunk x at position x ^ (r % (D / 4)).
+    constexpr int NC4 = D / 4, OC = D / 8 / NW, ACC = CK_ROWS * D * 4;
+    const float lt = halves_sum(l_run);
+    __syncthreads();
+    char* acc = s_kv + wave * ACC;
+#pragma unroll
+    for (int dt = 0; dt < NCG; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {  // d = 32 dt + 8 rq + 4 g + 0..3
+        const int x = 8 * dt + 2 * rq + g;
+        *reinterpret_cast<f32x4*>(acc + l32 * 4 * D + 16 * (x ^ (l32 & (NC4 - 1)))) =
+            f32x4{O[dt][4 * rq], O[dt][4 * rq + 1], O[dt][4 * rq + 2], O[dt][4 * rq + 3]};
+      }
+    if (g == 0) {
+      s_ml[wave * 2 * CK_ROWS + l32] = m_ref;
+      s_ml[wave * 2 * CK_ROWS + CK_ROWS + l32] = lt;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < CK_ROWS * OC / 64; ++k) {
+      const int x = 64 * k + lane;
+      const int r = x / OC, oc = wave * OC + x % OC;
+      float m[NW], l = 0.f, M = -__builtin_inff();
+#pragma unroll
+      for (int s = 0; s < NW; ++s) {
+        m[s] = s_ml[s * 2 * CK_ROWS + r];
+        M = fmaxf(M, m[s]);
+      }
+      const float Mu = M == -__builtin_inff() ? 0.f : M;
+      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+      for (int s = 0; s < NW; ++s) {
+        const float fs = fast_exp2(m[s] - Mu);
+        l += fs * s_ml[s * 2 * CK_ROWS + CK_ROWS + r];
+        const char* p = s_kv + s * ACC + r * 4 * D;
+        lo += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc) ^ (r & (NC4 - 1))));
+        hi += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc + 1) ^ (r & (NC4 - 1))));
+      }
+      if (it.row0 + r < it.row_end) {
+        const int tk = (int)fast_div((uint32_t)(it.row0 + r), (uint32_t)a.G, a.mul_G);
+        const int h = it.kvh * a.G + it.row0 + r - tk * a.G;
+        if (a.splits > 1) {
+          const int64_t at = ((int64_t)it.split * a.seqs.N + it.tok0 + tk) * a.Hq + h;
+          f32x4* d = reinterpret_cast<f32x4*>(a.part_acc + at * D + 8 * oc);
+          d[0] = lo;
+          d[1] = hi;
+          if (oc == 0) {
+            a.part_ml[2 * at] = M;
+            a.part_ml[2 * at + 1] = l;
+          }
+        } else {
+          const float inv = l > 0.f ? 1.f / l : 1.f;
+          *reinterpret_cast<u32x4*>(a.o + (int64_t)(it.tok0 + tk) * a.o_st + h * a.o_sh + 8 * oc) =
+              u32x4{E::pack2f(lo[0] * inv, lo[1] * inv), E::pack2f(lo[2] * inv, lo[3] * inv),
+                    E::pack2f(hi[0] * inv, hi[1] * inv), E::pack2f(hi[2] * inv, hi[3] * inv)};
+        }
+      }
+    }
+  }
+
+  // Merges the splits of one (token, head): D / 8 lanes a row.
+  static __device__ void combine(const ChunkArgs& a) {
+    constexpr int LPR = D / 8;
+    const int64_t row = ((int64_t)blockIdx.x * NT + threadIdx.x) / LPR;
+    const int oc = threadIdx.x % LPR;
+    const int64_t n = row / a.Hq;
+    if (n < a.seqs.cu[0] || n >= a.seqs.N || n >= a.seqs.cu[a.seqs.B]) return;  // not of any sequence
+    const int64_t rows = a.seqs.N * a.Hq;
+    float M = -__builtin_inff(), L = 0.f;
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * rows + row)]);
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    if (M != -__builtin_inff())
+      for (int s = 0; s < a.splits; ++s) {
+        const float m = a.part_ml[2 * (s * rows + row)], l = a.part_ml[2 * (s * rows + row) + 1];
+        if (m == -__builtin_inff()) continue;  // this split saw no key of the row
+        const float fs = fast_exp2(m - M);
+        const f32x4* p = reinterpret_cast<const f32x4*>(a.part_acc + (s * rows + row) * D + 8 * oc);
+        L += fs * l;
+        lo += fs * p[0];
+        hi += fs * p[1];
+      }
+    const float inv = L > 0.f ? 1.f / L : 1.f;
+    *reinterpret_cast<u32x4*>(a.o + n * a.o_st + (row - n * a.Hq) * a.o_sh + 8 * oc) =
+        u32x4{E::pack2f(lo[0] * inv, lo[1] * inv), E::pack2f(lo[2] * inv, lo[3] * inv),
+              E::pack2f(hi[0] * inv, hi[1] * inv), E::pack2f(hi[2] * inv, hi[3] * inv)};
+  }
+};
+
+template <bool BF16, int D>
+__global__ __launch_bounds__(256, 1) void chunk_kernel(const ChunkArgs a) {
+  Chunk<BF16, D>::run(a);
+}
+template <bool BF16, int D>
+__global__ __launch_bounds__(256) void chunk_combine_kernel(const ChunkArgs a) {
+  Chunk<BF16, D>::combine(a);
+}
+
+template <bool BF16, int D>
+static int launch_chunk(const ChunkArgs& a, int64_t groups, hipStream_t s) {
+  hipLaunchKernelGGL((chunk_kernel<BF16, D>), dim3((unsigned)groups), dim3(256), 0, s, a);
+  if (a.splits > 1) {
+    const int64_t rows = a.seqs.N * a.Hq, per = 256 / (D / 8);
+    hipLaunchKernelGGL((chunk_combine_kernel<BF16, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
+  }
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : set_error((int)err, "sa_paged_chunk_attn: launch failed: %s", hipGetErrorString(err));
+}
+
+// Row tiles that any division of N tokens over B sequences may have.
+static int64_t chunk_tiles(int64_t N, int64_t B, int64_t G, bool blocks) {
+  B = std::min(B, N);
+  if (blocks) return (N / CK_BLOCK + B) * ((CK_BLOCK * G + CK_ROWS - 1) / CK_ROWS);
+  return N * G / CK_ROWS + B;
+}
+
+static bool bad_ptr(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" int64_t sa_paged_chunk_workspace_bytes(int N, int Hq, int D, int num_splits) {
+  if (N < 1 || Hq < 1 || D < 1 || num_splits <= 1) return 0;
+  return (int64_t)num_splits * N * Hq * (D + 2) * 4;
+}
+
+extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k_pages,
+                                   const void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
+                                   int num_pages, const int32_t* block_table, int64_t block_table_stride,
+                                   int max_blocks, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                                   const int32_t* sel, int64_t sel_sr, int64_t sel_sh, int sel_rows, int sel_width,
+                                   const int32_t* sel_off, int64_t off_sr, int64_t off_sh, void* o, int64_t o_st,
+                                   int64_t o_sh, int N, int B, int Hq, int Hkv, int D, int page, float sm_scale,
+                                   int num_splits, void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* name = "sa_paged_chunk_attn";
+  if (dtype != SA_DTYPE_BF16 && dtype != SA_DTYPE_F16)
+    return set_error(SA_E_DTYPE, "%s: dtype %d is not bf16 (0) or f16 (1)", name, dtype);
+  if (D != 64 && D != 128) return set_error(SA_E_HEADDIM, "%s: head dim %d not supported (64, 128)", name, D);
+  if (page < 16 || page > 128 || page % 16)
+    return set_error(SA_E_BLOCK, "%s: page %d is not a multiple of 16 in [16, 128]", name, page);
+  if (N < 0 || B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > (1 << 15) || max_blocks < 0 || num_pages < 0 ||
+      block_table_stride < max_blocks || num_splits < 1 || num_splits > 64)
+    return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages, "
+                     "%d splits (1..64)", name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages,
+                     num_splits);
+  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return set_error(SA_E_SHAPE, "%s: scale %g is not positive", name, sm_scale);
+  if ((int64_t)N * Hq > 0x7fffffff) return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d rows are too many", name, N, Hq);
+  if (sel && (!sel_off || sel_width < 0 || sel_rows < (N ? N / CK_BLOCK + std::min(B, N) : 0)))
+    return set_error(SA_E_SHAPE, "%s: a selection needs offsets and %d rows, got %d", name,
+                     N / CK_BLOCK + std::min(B, N), sel_rows);
+  if (N == 0 || B == 0) return 0;
+  if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || !o)
+    return set_error(SA_E_NULL, "%s: NULL pointer", name);
+  if (bad_ptr(q) || bad_ptr(k_pages) || bad_ptr(v_pages) || bad_ptr(o) || bad_ptr(workspace) ||
+      (q_st | q_sh | pages_sp | pages_sh | pages_st | o_st | o_sh) % 8)
+    return set_error(SA_E_ALIGN, "%s: head rows must be 16-byte aligned", name);
+  if (pages_st < 0 || pages_st > CK_MAX_STRIDE)
+    return set_error(SA_E_SHAPE, "%s: token stride %lld of the pools", name, (long long)pages_st);
+  if (num_splits > 1 && (!workspace || workspace_bytes < sa_paged_chunk_workspace_bytes(N, Hq, D, num_splits)))
+    return set_error(SA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", name, (long long)workspace_bytes,
+                     (long long)sa_paged_chunk_workspace_bytes(N, Hq, D, num_splits));
+  ChunkArgs a = {};
+  a.q = static_cast<const elem_t*>(q);
+  a.q_st = q_st, a.q_sh = q_sh;
+  a.k = static_cast<const elem_t*>(k_pages);
+  a.v = static_cast<const elem_t*>(v_pages);
+  a.kv_sp = pages_sp, a.kv_sh = pages_sh, a.kv_st = pages_st;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.max_blocks = max_blocks, a.num_pages = num_pages, a.page = page;
+  a.mul_page = div_mul((uint32_t)page);
+  a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
+  a.sel = sel;
+  a.sel_sr = sel_sr, a.sel_sh = sel_sh, a.sel_rows = sel_rows, a.sel_width = sel_width;
+  a.sel_off = sel_off;
+  a.off_sr = off_sr, a.off_sh = off_sh;
+  a.mul_ppc = div_mul((uint32_t)(page / 16));
+  a.o = static_cast<elem_t*>(o);
+  a.o_st = o_st, a.o_sh = o_sh;
+  a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
+  a.mul_G = div_mul((uint32_t)a.G);
+  a.mul_heads = div_mul((uint32_t)Hkv);
+  a.mul_splits = div_mul((uint32_t)num_splits);
+  a.scale_log2 = sm_scale * 1.44269504088896340736f;
+  a.splits = num_splits;
+  const int64_t tiles = chunk_tiles(N, B, a.G, sel != nullptr);
+  const int64_t groups = tiles * Hkv * num_splits;
+  if (groups > MAX_WORKGROUPS)
+    return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
+  a.tiles = (int)tiles;
+  a.tiles_per_block = (int)((CK_BLOCK * (int64_t)a.G + CK_ROWS - 1) / CK_ROWS);
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = num_splits > 1 ? a.part_acc + (int64_t)num_splits * N * Hq * D : nullptr;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_chunk<true, 128>(a, groups, s) : launch_chunk<true, 64>(a, groups, s);
+  return D == 128 ? launch_chunk<false, 128>(a, groups, s) : launch_chunk<false, 64>(a, groups, s);
+}

@@ -1,0 +1,432 @@
+// Per-head RMS norms and rotary embedding of queries and keys, and the paged write of a chunk's keys and values
+// with the key bounds of the pages (gfx950).
+//
+//   n = x * rsqrt(mean(x^2) + eps) * w                                   (w given; else n = x)
+//   y[i] = n[i] c - n[i + D/2] s,  y[i + D/2] = n[i + D/2] c + n[i] s,   c, s = cos, sin(inv_freq[i] * position)
+//
+// Everything is fp32 and rounded once, to the element type, on the way out.  The angle is the exception: an
+// fp32 product inv_freq * position is off by up to 2^-24 of itself, 0.006 rad at position 100,000, more than the
+// output's rounding.  It is formed in fp64, in turns, reduced to half a turn and only then taken to fp32.
+//
+// Memory bound: each element is read once and written once.  A workgroup takes a window of consecutive tokens and
+// a share of the heads.  It computes the window's cos and sin once, into LDS (one sincos per token and pair
+// whatever the number of heads), then each wave takes whole heads: D/16 lanes hold one token's head, each the two
+// 16-byte chunks that the rotation mixes, so a wave moves 1024 / D tokens of a head per pass and the norm is a
+// reduction over D/16 neighbouring lanes.
+//
+// Pages: windows are aligned to positions, in multiples of the page, so the tokens that a chunk adds to one page
+// belong to one window, and one wave sees all of them for a head.  It keeps their minimum and maximum in
+// registers and updates the page's bounds with plain stores: merged with the stored bounds when the page held
+// tokens before, else written fresh.  Min and max are exact and have no order, so the result has none either.
+#include <algorithm>
+
+#include "ragged.h"
+
+namespace sa {
+
+constexpr int RA_THREADS = 256;
+constexpr int RA_WAVES = RA_THREADS / 64;
+constexpr int RA_MAX_WINDOW = 128;              // tokens of a window
+constexpr int RA_CHUNK = 16;                    // positions that share a page for every page size
+constexpr int RA_UNROLL = 4;                    // passes of a wave whose loads are in flight together
+
+struct RopeArgs {
+  const elem_t *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_st, v_sh;
+  elem_t *qo, *ko;
+  int64_t qo_sb, qo_st, qo_sh, ko_sb, ko_st, ko_sh;
+  const elem_t *qw, *kw;                        // norm weights, or NULL
+  const float* inv_freq;                        // or NULL: no rotation
+  int Hq, Hkv, heads_per_part, window;
+  float eps;
+  // unpaged: token n is row n % T of batch n / T
+  const int64_t* positions;
+  int64_t pos_sb;
+  int64_t N;
+  int T;
+  // paged
+  Ragged seqs;
+  elem_t *k_pages, *v_pages;
+  int64_t pg_sp, pg_sh, pg_st;
+  elem_t* bounds;                               // [pages, Hkv, 2, D], or NULL
+  int64_t bd_sp, bd_sh;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_blocks, num_pages, page;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void unpack8(u32x4 v, float* f) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = Elem<BF16>::to_f32((elem_t)(v[e] & 0xffffu));
+    f[2 * e + 1] = Elem<BF16>::to_f32((elem_t)(v[e] >> 16));
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ u32x4 pack8(const float* f) {
+  u32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = Elem<BF16>::pack2f(f[2 * e], f[2 * e + 1]);
+  return v;
+}
+
+template <bool BF16, int D, bool PAGED>
+struct RopeAppend {
+  static constexpr int LPR = D / 16;            // lanes of one token's head
+  static constexpr int RPI = 64 / LPR;          // tokens of a wave's pass
+  static constexpr int HALF = D / 2;
+  static constexpr int CS_STRIDE = D + 4;       // floats of a token's cos | sin row; the pad spreads tokens over banks
+
+  // A window: `lo` .. `hi` - 1 are the slots (token index within the window) that hold tokens.
+  struct Window {
+    int lo, hi, base;   // base: position of slot 0 (paged), or 0
+    int64_t row0;       // packed row of slot 0 (may lie before the tensor; slots below lo are not touched)
+  };
+
+  static __device__ __forceinline__ bool find_window(const RopeArgs& a, int x, Window& w, int& b) {
+    b = 0;
+    if constexpr (!PAGED) {
+      w.base = 0;
+      w.row0 = (int64_t)x * a.window;
+      w.lo = 0;
+      w.hi = (int)(a.N - w.row0 < a.window ? a.N - w.row0 : a.window);
+      return true;
+    } else {
+      auto windows = [&](int s) {
+        int r0;
+        const int n = a.seqs.rows(s, r0), end = a.seqs.kv_len(s);
+        return n ? floor_div(end - 1, a.window) - floor_div(end - n, a.window) + 1 : 0;
+      };
+      int local;
+      if (!find_item(a.seqs.B, x, windows, b, local)) return false;
+      int r0;
+      const int n = a.seqs.rows(b, r0), end = a.seqs.kv_len(b), start = end - n;
+      w.base = (floor_div(start, a.window) + local) * a.window;
+      w.lo = max(0, start - w.base);
+      w.hi = min(a.window, end - w.base);
+      w.row0 = (int64_t)r0 + w.base - start;
+      return true;
+    }
+  }
+
+  static __device__ void run(const RopeArgs& a) {
+    __shared__ float s_cs[RA_MAX_WINDOW * CS_STRIDE];
+    __shared__ int s_page[RA_MAX_WINDOW / RA_CHUNK], s_slot[RA_MAX_WINDOW / RA_CHUNK];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Window w;
+    int b;
+    if (!find_window(a, blockIdx.x, w, b)) return;
+
+    // cos and sin of the window's tokens
+    if (a.inv_freq) {
+      for (int x = w.lo * HALF + tid; x < w.hi * HALF; x += RA_THREADS) {
+        const int slot = x / HALF, i = x % HALF;
+        int64_t p = w.base + slot;
+        if constexpr (!PAGED) {
+          const int64_t n = w.row0 + slot;
+          p = a.positions[n / a.T * a.pos_sb + n % a.T];
+        }
+        const double turns = (double)p * (double)a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
+        float s, c;
+        sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+        s_cs[slot * CS_STRIDE + i] = c;
+        s_cs[slot * CS_STRIDE + HALF + i] = s;
+      }
+    }
+    if (PAGED && tid < a.window / RA_CHUNK) {
+      const int p = w.base + tid * RA_CHUNK;
+      int pg = -1, slot = 0;
+      if (p >= 0 && p / a.page < a.max_blocks) {
+        pg = a.table[b * a.table_stride + p / a.page];
+        slot = p % a.page;
+        if (pg < 0 || pg >= a.num_pages) pg = -1;
+      }
+      s_page[tid] = pg;
+      s_slot[tid] = slot;
+    }
+    __syncthreads();
+
+    const int heads = a.Hq + a.Hkv + (PAGED ? a.Hkv : 0);
+    const int h_end = min(heads, (int)(blockIdx.y + 1) * a.heads_per_part);
+    for (int h = (int)blockIdx.y * a.heads_per_part + wave; h < h_end; h += RA_WAVES) head(a, w, h, lane, s_cs, s_page, s_slot);
+  }
+
+  // All of the window's tokens of one head.
+  static __device__ __forceinline__ void head(const RopeArgs& a, const Window& w, int h, int lane, const float* s_cs,
+                                              const int* s_page, const int* s_slot) {
+    const int kind = h < a.Hq ? 0 : h < a.Hq + a.Hkv ? 1 : 2;   // query, key, value
+    const int hh = kind == 0 ? h : kind == 1 ? h - a.Hq : h - a.Hq - a.Hkv;
+    const elem_t* src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const int64_t st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
+    const int64_t sb = kind == 0 ? a.q_sb : a.k_sb;
+    src += hh * (kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh);
+    const elem_t* wt = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
+    const bool rotate = a.inv_freq && kind < 2;
+    const bool track = PAGED && kind == 1 && a.bounds;
+    const int c = lane % LPR, g = lane / LPR;
+    float wl[8], wh[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) wl[e] = wh[e] = 1.f;
+    if (wt) {
+      unpack8<BF16>(*reinterpret_cast<const u32x4*>(wt + 8 * c), wl);
+      unpack8<BF16>(*reinterpret_cast<const u32x4*>(wt + HALF + 8 * c), wh);
+    }
+    auto src_of = [&](int slot) {
+      const int64_t n = w.row0 + slot;
+      if constexpr (PAGED) return src + n * st + 8 * c;
+      return src + n / a.T * sb + n % a.T * st + 8 * c;
+    };
+    auto dst_of = [&](int slot) -> elem_t* {
+      const int64_t n = w.row0 + slot;
+      if constexpr (!PAGED) {
+        return (kind == 0 ? a.qo + n / a.T * a.qo_sb + n % a.T * a.qo_st + hh * a.qo_sh
+                          : a.ko + n / a.T * a.ko_sb + n % a.T * a.ko_st + hh * a.ko_sh) + 8 * c;
+      } else {
+        if (kind == 0) return a.qo + n * a.qo_st + hh * a.qo_sh + 8 * c;
+        const int pg = s_page[slot / RA_CHUNK];
+        if (pg < 0) return nullptr;
+        return (kind == 1 ? a.k_pages : a.v_pages) + pg * a.pg_sp + hh * a.pg_sh +
+               (int64_t)(s_slot[slot / RA_CHUNK] + slot % RA_CHUNK) * a.pg_st + 8 * c;
+      }
+    };
+    // With bounds a key head goes page by page, else the window at once.
+    const int seg = track ? min(a.page, a.window) : a.window;
+    for (int s0 = w.lo / seg * seg; s0 < w.hi; s0 += seg) {
+      const int lo = max(w.lo, s0), hi = min(w.hi, s0 + seg);
+      float mn[16], mx[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        mn[e] = __builtin_inff();
+        mx[e] = -__builtin_inff();
+      }
+      for (int t0 = lo / RPI * RPI; t0 < hi; t0 += RPI * RA_UNROLL) {
+        u32x4 xl[RA_UNROLL], xh[RA_UNROLL];
+#pragma unroll
+        for (int u = 0; u < RA_UNROLL; ++u) {
+          const int slot = t0 + u * RPI + g;
+          xl[u] = xh[u] = u32x4{0u, 0u, 0u, 0u};
+          if (slot >= lo && slot < hi) {
+            const elem_t* p = src_of(slot);
+            xl[u] = *reinterpret_cast<const u32x4*>(p);
+            xh[u] = *reinterpret_cast<const u32x4*>(p + HALF);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < RA_UNROLL; ++u) {
+          const int slot = t0 + u * RPI + g;
+          const bool live = slot >= lo && slot < hi;
+          if (kind < 2) {
+            float l[8], r[8];
+            unpack8<BF16>(xl[u], l);
+            unpack8<BF16>(xh[u], r);
+            if (wt) {
+              float ss = 0.f;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) ss += l[e] * l[e] + r[e] * r[e];
+#pragma unroll
+              for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o, 64);
+              const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                l[e] *= inv * wl[e];
+                r[e] *= inv * wh[e];
+              }
+            }
+            if (rotate && live) {
+              const float* cs = s_cs + slot * CS_STRIDE + 8 * c;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float co = cs[e], si = cs[HALF + e];
+                const float y = l[e] * co - r[e] * si;
+                r[e] = r[e] * co + l[e] * si;
+                l[e] = y;
+              }
+            }
+            xl[u] = pack8<BF16>(l);
+            xh[u] = pack8<BF16>(r);
+            if (track && live) {   // bounds of the stored (rounded) keys
+              unpack8<BF16>(xl[u], l);
+              unpack8<BF16>(xh[u], r);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                mn[e] = fminf(mn[e], l[e]);
+                mx[e] = fmaxf(mx[e], l[e]);
+                mn[8 + e] = fminf(mn[8 + e], r[e]);
+                mx[8 + e] = fmaxf(mx[8 + e], r[e]);
+              }
+            }
+          }
+          if (live) {
+            elem_t* d = dst_of(slot);
+            if (d) {
+              *reinterpret_cast<u32x4*>(d) = xl[u];
+              *reinterpret_cast<u32x4*>(d + HALF) = xh[u];
+            }
+          }
+        }
+      }
+      if (track) {
+        const int pg = s_page[lo / RA_CHUNK];
+        if (pg < 0) continue;
+        const bool fresh = s_slot[lo / RA_CHUNK] + lo % RA_CHUNK == 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+          for (int o = LPR; o < 64; o <<= 1) {
+            mn[e] = fminf(mn[e], __shfl_xor(mn[e], o, 64));
+            mx[e] = fmaxf(mx[e], __shfl_xor(mx[e], o, 64));
+          }
+        if (g < 2) {   // lanes of token group 0 write the minima, of group 1 the maxima
+          elem_t* d = a.bounds + pg * a.bd_sp + hh * a.bd_sh + g * D + 8 * c;
+          float y[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[e] = g ? mx[e] : mn[e];
+          if (!fresh) {
+            float old[16];
+            unpack8<BF16>(*reinterpret_cast<const u32x4*>(d), old);
+            unpack8<BF16>(*reinterpret_cast<const u32x4*>(d + HALF), old + 8);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = g ? fmaxf(y[e], old[e]) : fminf(y[e], old[e]);
+          }
+          *reinterpret_cast<u32x4*>(d) = pack8<BF16>(y);
+          *reinterpret_cast<u32x4*>(d + HALF) = pack8<BF16>(y + 8);
+        }
+      }
+    }
+  }
+};
+
+template <bool BF16, int D, bool PAGED>
+__global__ __launch_bounds__(RA_THREADS) void rope_append_kernel(const RopeArgs a) {
+  RopeAppend<BF16, D, PAGED>::run(a);
+}
+
+template <bool PAGED>
+static int launch_rope(const char* name, int dtype, int D, const RopeArgs& a, dim3 grid, hipStream_t s) {
+  const dim3 block(RA_THREADS);
+  if (dtype == SA_DTYPE_BF16 && D == 128)
+    hipLaunchKernelGGL((rope_append_kernel<true, 128, PAGED>), grid, block, 0, s, a);
+  else if (dtype == SA_DTYPE_BF16)
+    hipLaunchKernelGGL((rope_append_kernel<true, 64, PAGED>), grid, block, 0, s, a);
+  else if (D == 128)
+    hipLaunchKernelGGL((rope_append_kernel<false, 128, PAGED>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((rope_append_kernel<false, 64, PAGED>), grid, block, 0, s, a);
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : set_error((int)err, "%s: launch failed: %s", name, hipGetErrorString(err));
+}
+
+// Heads per workgroup: the heads are dealt over workgroups until the launch has about RA_TARGET of them.
+constexpr int64_t RA_TARGET = 1024;
+static int heads_per_part(int64_t windows, int heads) {
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((heads + RA_WAVES - 1) / RA_WAVES, RA_TARGET / std::max<int64_t>(1, windows)));
+  return (int)((heads + parts - 1) / parts);
+}
+
+static bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
+                               int64_t k_sb, int64_t k_st, int64_t k_sh, void* q_out, int64_t qo_sb, int64_t qo_st,
+                               int64_t qo_sh, void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh,
+                               const void* q_weight, const void* k_weight, const float* inv_freq,
+                               const int64_t* positions, int64_t pos_sb, int B, int T, int Hq, int Hkv, int D,
+                               float eps, void* stream) {
+  clear_error();
+  const char* name = "sa_qk_norm_rope";
+  if (dtype != SA_DTYPE_BF16 && dtype != SA_DTYPE_F16)
+    return set_error(SA_E_DTYPE, "%s: dtype %d is not bf16 (0) or f16 (1)", name, dtype);
+  if (D != 64 && D != 128) return set_error(SA_E_HEADDIM, "%s: head dim %d not supported (64, 128)", name, D);
+  if (B < 0 || T < 0 || Hq < 0 || Hkv < 0 || Hq > (1 << 20) || Hkv > (1 << 20))
+    return set_error(SA_E_SHAPE, "%s: bad sizes B=%d T=%d Hq=%d Hkv=%d", name, B, T, Hq, Hkv);
+  if (B == 0 || T == 0 || Hq + Hkv == 0) return 0;
+  if ((Hq && (!q || !q_out)) || (Hkv && (!k || !k_out)) || !inv_freq || !positions)
+    return set_error(SA_E_NULL, "%s: NULL pointer", name);
+  if (misaligned(q) || misaligned(k) || misaligned(q_out) || misaligned(k_out) || misaligned(q_weight) ||
+      misaligned(k_weight) || (q_sb | q_st | q_sh | k_sb | k_st | k_sh | qo_sb | qo_st | qo_sh | ko_sb | ko_st | ko_sh) % 8)
+    return set_error(SA_E_ALIGN, "%s: head rows must be 16-byte aligned", name);
+  RopeArgs a = {};
+  a.q = static_cast<const elem_t*>(q);
+  a.k = static_cast<const elem_t*>(k);
+  a.qo = static_cast<elem_t*>(q_out);
+  a.ko = static_cast<elem_t*>(k_out);
+  a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh, a.k_sb = k_sb, a.k_st = k_st, a.k_sh = k_sh;
+  a.qo_sb = qo_sb, a.qo_st = qo_st, a.qo_sh = qo_sh, a.ko_sb = ko_sb, a.ko_st = ko_st, a.ko_sh = ko_sh;
+  a.qw = static_cast<const elem_t*>(q_weight);
+  a.kw = static_cast<const elem_t*>(k_weight);
+  a.inv_freq = inv_freq;
+  a.positions = positions;
+  a.pos_sb = pos_sb;
+  a.N = (int64_t)B * T;
+  a.T = T;
+  a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
+  a.window = 32;
+  const int64_t windows = (a.N + a.window - 1) / a.window;
+  if (windows > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: %lld tokens are too many", name, (long long)a.N);
+  a.heads_per_part = heads_per_part(windows, Hq + Hkv);
+  const int parts = (Hq + Hkv + a.heads_per_part - 1) / a.heads_per_part;
+  return launch_rope<false>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
+}
+
+extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                               int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st,
+                               int64_t qo_sh, const void* q_weight, const void* k_weight, const float* inv_freq,
+                               void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
+                               int num_pages, void* k_bounds, int64_t bounds_sp, int64_t bounds_sh,
+                               const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                               const int32_t* cu_seqlens, const int32_t* kv_lens, int N, int B, int Hq, int Hkv,
+                               int D, int page, float eps, void* stream) {
+  clear_error();
+  const char* name = "sa_paged_append";
+  if (dtype != SA_DTYPE_BF16 && dtype != SA_DTYPE_F16)
+    return set_error(SA_E_DTYPE, "%s: dtype %d is not bf16 (0) or f16 (1)", name, dtype);
+  if (D != 64 && D != 128) return set_error(SA_E_HEADDIM, "%s: head dim %d not supported (64, 128)", name, D);
+  if (page < 16 || page > 128 || page % 16)
+    return set_error(SA_E_BLOCK, "%s: page %d is not a multiple of 16 in [16, 128]", name, page);
+  if (N < 0 || B < 0 || Hkv < 1 || Hq < 0 || Hq > (1 << 20) || Hkv > (1 << 20) || max_blocks < 0 || num_pages < 0 ||
+      block_table_stride < max_blocks)
+    return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages",
+                     name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages);
+  if (N == 0 || B == 0) return 0;
+  if (!k || !v || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || (Hq && (!q || !q_out)))
+    return set_error(SA_E_NULL, "%s: NULL pointer", name);
+  if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out) || misaligned(q_weight) ||
+      misaligned(k_weight) || misaligned(k_pages) || misaligned(v_pages) || misaligned(k_bounds) ||
+      (q_st | q_sh | k_st | k_sh | v_st | v_sh | qo_st | qo_sh | pages_sp | pages_sh | pages_st | bounds_sp | bounds_sh) % 8)
+    return set_error(SA_E_ALIGN, "%s: head rows must be 16-byte aligned", name);
+  RopeArgs a = {};
+  a.q = static_cast<const elem_t*>(q);
+  a.k = static_cast<const elem_t*>(k);
+  a.v = static_cast<const elem_t*>(v);
+  a.qo = static_cast<elem_t*>(q_out);
+  a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
+  a.qo_st = qo_st, a.qo_sh = qo_sh;
+  a.qw = static_cast<const elem_t*>(q_weight);
+  a.kw = static_cast<const elem_t*>(k_weight);
+  a.inv_freq = inv_freq;
+  a.N = N;
+  a.T = 1;
+  a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
+  a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
+  a.k_pages = static_cast<elem_t*>(k_pages);
+  a.v_pages = static_cast<elem_t*>(v_pages);
+  a.pg_sp = pages_sp, a.pg_sh = pages_sh, a.pg_st = pages_st;
+  a.bounds = static_cast<elem_t*>(k_bounds);
+  a.bd_sp = bounds_sp, a.bd_sh = bounds_sh;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.max_blocks = max_blocks, a.num_pages = num_pages, a.page = page;
+  a.window = 64 % page == 0 ? 64 : page;
+  // n new tokens touch at most (n - 1) / window + 2 windows
+  const int64_t windows = (int64_t)N / a.window + 2 * (int64_t)std::min(B, N);
+  if (windows > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: N=%d B=%d are too many", name, N, B);
+  const int heads = Hq + 2 * Hkv;
+  a.heads_per_part = heads_per_part(windows, heads);
+  const int parts = (heads + a.heads_per_part - 1) / a.heads_per_part;
+  return launch_rope<true>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
+}

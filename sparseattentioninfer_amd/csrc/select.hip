@@ -1,0 +1,425 @@
+// Pages of a paged cache that a cheap score picks for each query, gfx950.
+//
+// Every page keeps the minimum lo and the maximum hi of its keys in each dim (sa_paged_append).  The largest q . k
+// that any key of the page can reach is sum_d max(q_d lo_d, q_d hi_d).  Summed over the queries that share a list (the
+// heads of a KV group, of one token or of a block of 64) it is linear in the queries' positive and negative parts:
+//
+//   score(page) = hi . P + lo . N,   P = sum of max(q, 0),   N = sum of min(q, 0)
+//
+// so a list costs 2 D multiply-adds a page however many queries share it.  Kept are the first `sink` pages, the last
+// `recent` (from the page of the list's first query back, and all up to that of its last), and the top_k best of
+// those between, ties to the lowest page.  Pages between are full and wholly visible to every query of the list.
+//
+// P, N and the scores are fp64: which page is the last one in depends on the order of near-equal scores, and in fp32
+// that order would follow the order of summation.  It costs little: the bounds' bytes are the bound (16,384 tokens
+// of 64, 8 KV heads, 64 sequences: 67 MB, and 4.4 fp64 operations a byte).
+//
+// One workgroup makes a list: scores of all its pages as order-preserving 64-bit keys in LDS, the top_k-th key by
+// radix selection (8 bits a pass), then the kept pages in ascending order by ballots.  Where there are too few lists
+// to fill the chip, or more pages than fit LDS, the scores are computed by workgroups of their own, into the
+// workspace.
+#include <algorithm>
+
+#include "ragged.h"
+
+namespace sa {
+
+constexpr int SEL_THREADS = 256;
+constexpr int SEL_WAVES = SEL_THREADS / 64;
+constexpr int SEL_BLOCK = 64;          // new tokens that share one list
+constexpr int SEL_LDS_PAGES = 4096;    // keys of a list held in LDS
+constexpr int SEL_PAGES_PER_WG = 64;   // pages scored by a workgroup of its own
+
+struct SelectArgs {
+  const elem_t* q;
+  int64_t q_st, q_sh;
+  const elem_t* bounds;                // [pages, Hkv, 2, D]
+  int64_t bd_sp, bd_sh;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_blocks, num_pages, page;
+  Ragged seqs;                         // cu == NULL: one token per sequence, row b
+  int rows, Hkv, G;
+  int top_k, sink, recent;
+  int32_t* sel;
+  int64_t sel_sr, sel_sh;
+  int width;
+  int32_t* off;                        // [rows, Hkv, 2]
+  unsigned long long* keys;            // workspace [rows, Hkv, max_blocks], or NULL: keys stay in LDS
+};
+
+// The queries of one list and the pages it may keep.
+struct SelectItem {
+  int row, g, b;
+  int64_t tok0;      // first query's packed row
+  int n;             // queries (tokens)
+  int pages;         // pages up to the last query's
+  int head;          // pages [0, head) and [lo, pages) are kept; [head, lo) are ranked
+  int lo;
+};
+
+__device__ __forceinline__ bool find_list(const SelectArgs& a, int id, SelectItem& it) {
+  it.g = id % a.Hkv;
+  it.row = id / a.Hkv;
+  int first, last;
+  if (!a.seqs.cu) {
+    it.b = it.row;
+    it.tok0 = it.row;
+    it.n = 1;
+    first = last = a.seqs.kv_len(it.b) - 1;
+  } else {
+    auto blocks = [&](int s) {
+      int r0;
+      return (a.seqs.rows(s, r0) + SEL_BLOCK - 1) / SEL_BLOCK;
+    };
+    int local;
+    if (!find_item(a.seqs.B, it.row, blocks, it.b, local)) return false;
+    int r0;
+    const int n = a.seqs.rows(it.b, r0), start = a.seqs.kv_len(it.b) - n;
+    it.tok0 = r0 + local * SEL_BLOCK;
+    it.n = min(SEL_BLOCK, n - local * SEL_BLOCK);
+    first = start + local * SEL_BLOCK;
+    last = first + it.n - 1;
+  }
+  if (last < 0) return false;
+  it.pages = min(last / a.page + 1, a.max_blocks);
+  it.lo = min(max(0, max(first, 0) / a.page - a.recent + 1), it.pages);
+  it.head = min(a.sink, it.lo);
+  return true;
+}
+
+// Larger scores have larger keys; -0 and 0 share one, and a NaN ranks last.
+__device__ __forceinline__ unsigned long long key_of(double s) {
+  if (!(s == s)) return 0ull;
+  const unsigned long long u = (unsigned long long)__double_as_longlong(s + 0.0);
+  return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+}
+
+template <bool BF16, int D>
+struct Select {
+  static constexpr int LPR = D / 8;                 // lanes of one page's (or query's) row
+  static constexpr int RPP = SEL_THREADS / LPR;     // rows of a pass
+  struct Shared {
+    double pool[SEL_WAVES][2][D];
+    int hist[256];
+    int sums[2][SEL_WAVES];
+    unsigned long long cut;
+    int need, ties;
+  };
+
+  static __device__ __forceinline__ void unpack(u32x4 v, double (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = Elem<BF16>::to_f32((elem_t)(v[e] & 0xffffu));
+      f[2 * e + 1] = Elem<BF16>::to_f32((elem_t)(v[e] >> 16));
+    }
+  }
+
+  // P and N of the list's queries: this lane's 8 dims, in every row of lanes.
+  static __device__ __forceinline__ void pool(const SelectArgs& a, const SelectItem& it, Shared& sh, double (&P)[8],
+                                              double (&N)[8]) {
+    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    double p[8] = {}, n[8] = {};
+    for (int x = r; x < it.n * a.G; x += RPP) {
+      const elem_t* src = a.q + (it.tok0 + x / a.G) * a.q_st + (it.g * a.G + x % a.G) * a.q_sh + 8 * c;
+      double f[8];
+      unpack(*reinterpret_cast<const u32x4*>(src), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] += f[e] > 0. ? f[e] : 0.;
+        n[e] += f[e] < 0. ? f[e] : 0.;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int o = LPR; o < 64; o <<= 1) {
+        p[e] += __shfl_xor(p[e], o, 64);
+        n[e] += __shfl_xor(n[e], o, 64);
+      }
+    if (lane < LPR)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sh.pool[wave][0][8 * c + e] = p[e];
+        sh.pool[wave][1][8 * c + e] = n[e];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      P[e] = N[e] = 0.;
+#pragma unroll
+      for (int w = 0; w < SEL_WAVES; ++w) {
+        P[e] += sh.pool[w][0][8 * c + e];
+        N[e] += sh.pool[w][1][8 * c + e];
+      }
+    }
+  }
+
+  // Keys of pages [p0, p1) into keys[page].
+  static __device__ __forceinline__ void score(const SelectArgs& a, const SelectItem& it, const double (&P)[8],
+                                               const double (&N)[8], int p0, int p1, unsigned long long* keys) {
+    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR;
+    constexpr int U = 4;
+    for (int x0 = p0 + r; x0 < p1; x0 += U * RPP) {
+      int pg[U];
+      u32x4 lo[U], hi[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int x = x0 + u * RPP;
+        pg[u] = x < p1 ? a.table[it.b * a.table_stride + x] : -1;
+        if (pg[u] >= a.num_pages) pg[u] = -1;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        lo[u] = hi[u] = u32x4{0u, 0u, 0u, 0u};
+        if (pg[u] >= 0) {
+          const elem_t* src = a.bounds + pg[u] * a.bd_sp + it.g * a.bd_sh + 8 * c;
+          lo[u] = *reinterpret_cast<const u32x4*>(src);
+          hi[u] = *reinterpret_cast<const u32x4*>(src + D);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        double l[8], h[8], s = 0.;
+        unpack(lo[u], l);
+        unpack(hi[u], h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += h[e] * P[e] + l[e] * N[e];
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o, 64);
+        const int x = x0 + u * RPP;
+        if (c == 0 && x < p1) keys[x] = pg[u] >= 0 ? key_of(s) : 0ull;
+      }
+    }
+  }
+
+  // Radix selection: sh.cut and sh.ties such that the best `need` of the keys [p0, p1) are those above cut and the
+  // first `ties` equal to it.
+  static __device__ __forceinline__ void find_cut(const unsigned long long* keys, int p0, int p1, int need, Shared& sh) {
+    const int tid = threadIdx.x;
+    unsigned long long prefix = 0;
+    for (int byte = 7; byte >= 0; --byte) {
+      sh.hist[tid] = 0;
+      __syncthreads();
+      for (int x = p0 + tid; x < p1; x += SEL_THREADS) {
+        const unsigned long long k = keys[x];
+        if (byte == 7 || (k >> (8 * byte + 8)) == prefix) atomicAdd(&sh.hist[(k >> (8 * byte)) & 255], 1);
+      }
+      __syncthreads();
+      if (tid < 64) {   // lane l: bins 255 - 4 l down to 252 - 4 l
+        int h[4], mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine += h[e] = sh.hist[255 - 4 * tid - e];
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int up = __shfl_up(incl, o, 64);
+          incl += tid >= o ? up : 0;
+        }
+        int above = incl - mine;
+        if (above < need && incl >= need) {
+          int e = 0;
+          while (above + h[e] < need) above += h[e++];
+          sh.cut = (prefix << 8) | (unsigned long long)(255 - 4 * tid - e);
+          sh.need = need - above;
+          sh.ties = h[e];
+        }
+      }
+      __syncthreads();
+      prefix = sh.cut;
+      need = sh.need;
+      if (sh.ties == need) {   // every key with this prefix is in
+        if (byte) prefix = (prefix << (8 * byte)) - 1;   // all above it (prefix > 0: some key has it)
+        else prefix -= 1;
+        need = 0;
+        break;
+      }
+      __syncthreads();
+    }
+    __syncthreads();
+    if (tid == 0) {
+      sh.cut = prefix;
+      sh.ties = need;
+    }
+    __syncthreads();
+  }
+
+  // Exclusive rank of this thread's flag among the workgroup's, and their number.
+  static __device__ __forceinline__ int rank(bool flag, int (&sums)[SEL_WAVES], int& total) {
+    const int wave = threadIdx.x >> 6;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(flag);
+    if ((threadIdx.x & 63) == 0) sums[wave] = __popcll(m);
+    __syncthreads();
+    int before = __popcll(m & ((1ull << (threadIdx.x & 63)) - 1ull));
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < SEL_WAVES; ++w) {
+      if (w < wave) before += sums[w];
+      total += sums[w];
+    }
+    return before;
+  }
+
+  // The kept pages in ascending order; `ranked`: [head, lo) holds more than top_k pages.
+  static __device__ __forceinline__ void write_list(const SelectArgs& a, const SelectItem& it, bool ranked,
+                                                    const unsigned long long* keys, Shared& sh) {
+    int32_t* out = a.sel + it.row * a.sel_sr + it.g * a.sel_sh;
+    int count = 0, tied = 0;
+    for (int p0 = 0; p0 < it.pages; p0 += SEL_THREADS) {
+      const int p = p0 + threadIdx.x;
+      bool keep = p < it.pages && (p < it.head || p >= it.lo);
+      bool tie = false;
+      if (p >= it.head && p < it.lo && a.top_k > 0) {
+        if (!ranked) {
+          keep = true;
+        } else {
+          keep = keys[p] > sh.cut;
+          tie = keys[p] == sh.cut;
+        }
+      }
+      int n;
+      if (ranked) {
+        const int r = rank(tie, sh.sums[0], n) + tied;
+        keep |= tie && r < sh.ties;
+        tied += n;
+      }
+      const int at = count + rank(keep, sh.sums[1], n);
+      if (keep && at < a.width) out[at] = p;
+      count += n;
+      __syncthreads();
+    }
+    count = min(count, a.width);
+    for (int x = count + threadIdx.x; x < a.width; x += SEL_THREADS) out[x] = 0;
+    if (threadIdx.x < 2) a.off[((int64_t)it.row * a.Hkv + it.g) * 2 + threadIdx.x] = threadIdx.x ? count : 0;
+  }
+
+  static __device__ void empty_list(const SelectArgs& a, const SelectItem& it) {
+    int32_t* out = a.sel + it.row * a.sel_sr + it.g * a.sel_sh;
+    for (int x = threadIdx.x; x < a.width; x += SEL_THREADS) out[x] = 0;
+    if (threadIdx.x < 2) a.off[((int64_t)it.row * a.Hkv + it.g) * 2 + threadIdx.x] = 0;
+  }
+};
+
+// Scores of SEL_PAGES_PER_WG pages of a list, into the workspace.
+template <bool BF16, int D>
+__global__ __launch_bounds__(SEL_THREADS) void select_score_kernel(const SelectArgs a) {
+  using S = Select<BF16, D>;
+  __shared__ typename S::Shared sh;
+  SelectItem it;
+  if (!find_list(a, blockIdx.x, it) || it.lo - it.head <= a.top_k || a.top_k == 0) return;
+  const int p0 = it.head + (int)blockIdx.y * SEL_PAGES_PER_WG, p1 = min(it.lo, p0 + SEL_PAGES_PER_WG);
+  if (p0 >= p1) return;
+  double P[8], N[8];
+  S::pool(a, it, sh, P, N);
+  S::score(a, it, P, N, p0, p1, a.keys + (int64_t)blockIdx.x * a.max_blocks);
+}
+
+// A list: with LDS its scores too, else from those of the workspace.
+template <bool BF16, int D, bool LDS>
+__global__ __launch_bounds__(SEL_THREADS) void select_kernel(const SelectArgs a) {
+  using S = Select<BF16, D>;
+  __shared__ typename S::Shared sh;
+  __shared__ unsigned long long s_keys[LDS ? SEL_LDS_PAGES : 1];
+  SelectItem it;
+  if (!find_list(a, blockIdx.x, it)) {
+    S::empty_list(a, it);
+    return;
+  }
+  const bool ranked = it.lo - it.head > a.top_k && a.top_k > 0;
+  unsigned long long* keys = LDS ? s_keys : a.keys + (int64_t)blockIdx.x * a.max_blocks;
+  if (ranked) {
+    if constexpr (LDS) {
+      double P[8], N[8];
+      S::pool(a, it, sh, P, N);
+      S::score(a, it, P, N, it.head, it.lo, keys);
+      __syncthreads();
+    }
+    S::find_cut(keys, it.head, it.lo, a.top_k, sh);
+  }
+  S::write_list(a, it, ranked, keys, sh);
+}
+
+// Whether the scores get workgroups of their own: the pages do not fit LDS, or the lists are too few.
+static bool split_scores(int64_t lists, int max_blocks) {
+  return max_blocks > SEL_LDS_PAGES || (lists < 128 && max_blocks > 2 * SEL_PAGES_PER_WG);
+}
+
+template <bool BF16, int D>
+static int launch_select(const SelectArgs& a, hipStream_t s) {
+  const unsigned lists = (unsigned)((int64_t)a.rows * a.Hkv);
+  if (a.keys) {
+    hipLaunchKernelGGL((select_score_kernel<BF16, D>), dim3(lists, (a.max_blocks + SEL_PAGES_PER_WG - 1) / SEL_PAGES_PER_WG),
+                       dim3(SEL_THREADS), 0, s, a);
+    hipLaunchKernelGGL((select_kernel<BF16, D, false>), dim3(lists), dim3(SEL_THREADS), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((select_kernel<BF16, D, true>), dim3(lists), dim3(SEL_THREADS), 0, s, a);
+  }
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? 0 : set_error((int)err, "sa_paged_block_select: launch failed: %s", hipGetErrorString(err));
+}
+
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks) {
+  if (rows < 1 || Hkv < 1 || max_blocks < 1) return 0;
+  const int64_t lists = (int64_t)rows * Hkv;
+  return split_scores(lists, max_blocks) ? lists * max_blocks * 8 : 0;
+}
+
+extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k_bounds,
+                                     int64_t bounds_sp, int64_t bounds_sh, int num_pages, const int32_t* block_table,
+                                     int64_t block_table_stride, int max_blocks, const int32_t* cu_seqlens,
+                                     const int32_t* kv_lens, int N, int B, int Hq, int Hkv, int D, int page, int top_k,
+                                     int sink, int recent, int32_t* sel, int64_t sel_sr, int64_t sel_sh, int rows,
+                                     int width, int32_t* sel_off, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+  clear_error();
+  const char* name = "sa_paged_block_select";
+  if (dtype != SA_DTYPE_BF16 && dtype != SA_DTYPE_F16)
+    return set_error(SA_E_DTYPE, "%s: dtype %d is not bf16 (0) or f16 (1)", name, dtype);
+  if (D != 64 && D != 128) return set_error(SA_E_HEADDIM, "%s: head dim %d not supported (64, 128)", name, D);
+  if (page < 16 || page > 128 || page % 16)
+    return set_error(SA_E_BLOCK, "%s: page %d is not a multiple of 16 in [16, 128]", name, page);
+  if (N < 0 || B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > (1 << 15) || max_blocks < 0 || num_pages < 0 ||
+      block_table_stride < max_blocks || max_blocks > (1 << 21))
+    return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages", name,
+                     N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages);
+  if (top_k < 0 || sink < 0 || recent < 1 || top_k > (1 << 22) || sink > (1 << 22) || recent > (1 << 22))
+    return set_error(SA_E_SHAPE, "%s: top_k=%d, sink=%d (not negative), recent=%d (at least 1)", name, top_k, sink, recent);
+  const int span = cu_seqlens ? (SEL_BLOCK + page - 2) / page + 1 : 1;   // pages that the queries of a list lie in
+  const int need_rows = cu_seqlens ? N / SEL_BLOCK + std::min(B, N) : B;
+  if (!cu_seqlens && N != B) return set_error(SA_E_SHAPE, "%s: one token per sequence, but N=%d for B=%d", name, N, B);
+  if (rows != need_rows || width < sink + top_k + recent - 1 + span)
+    return set_error(SA_E_SHAPE, "%s: lists [%d, Hkv, %d], needed [%d, Hkv, %d]", name, rows, width, need_rows,
+                     sink + top_k + recent - 1 + span);
+  if (rows == 0) return 0;
+  if (!q || !k_bounds || !block_table || !kv_lens || !sel || !sel_off) return set_error(SA_E_NULL, "%s: NULL pointer", name);
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_bounds) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      (q_st | q_sh | bounds_sp | bounds_sh) % 8)
+    return set_error(SA_E_ALIGN, "%s: rows must be 16-byte aligned", name);
+  const int64_t need = sa_paged_block_select_workspace_bytes(rows, Hkv, max_blocks);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(SA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", name, (long long)workspace_bytes,
+                     (long long)need);
+  if ((int64_t)rows * Hkv > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: %d rows of %d heads are too many", name, rows, Hkv);
+  SelectArgs a = {};
+  a.q = static_cast<const elem_t*>(q);
+  a.q_st = q_st, a.q_sh = q_sh;
+  a.bounds = static_cast<const elem_t*>(k_bounds);
+  a.bd_sp = bounds_sp, a.bd_sh = bounds_sh;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.max_blocks = max_blocks, a.num_pages = num_pages, a.page = page;
+  a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
+  a.rows = rows, a.Hkv = Hkv, a.G = Hq / Hkv;
+  a.top_k = top_k, a.sink = sink, a.recent = recent;
+  a.sel = sel;
+  a.sel_sr = sel_sr, a.sel_sh = sel_sh, a.width = width;
+  a.off = sel_off;
+  a.keys = need ? static_cast<unsigned long long*>(workspace) : nullptr;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_select<true, 128>(a, s) : launch_select<true, 64>(a, s);
+  return D == 128 ? launch_select<false, 128>(a, s) : launch_select<false, 64>(a, s);
+}

@@ -9,7 +9,10 @@ attention, query head ``h`` reads KV head ``h // (Hq / Hkv)``), and the CSR
 may hold one row per KV group.
 
 ``paged_sparse_decode`` is new: one query token per sequence over a paged
-cache.  All work is enqueued on the current HIP stream; nothing synchronises.
+cache.  So are the operators of a chunk of new tokens over a paged cache, for
+sequences of different lengths: ``qk_norm_rope``, ``paged_append``,
+``paged_chunk_attn`` and ``paged_block_select``.  All work is enqueued on the
+current HIP stream; nothing synchronises.
 """
 from __future__ import annotations
 
@@ -785,3 +788,241 @@ def gemm_skinny_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out: torch.Tens
                                                w_gate_up.stride(0), out.data_ptr(), out.stride(0), M, I, K, _stream(x))
     _lib.check("sa_gemm_skinny_swiglu", status)
     return out
+
+
+# ---- a chunk of new tokens over a paged cache: sequences of different lengths --------------------
+
+CHUNK_BLOCK = 64    # new tokens of a sequence that share one selection (include/sparse_attn.h)
+
+
+def _call(name: str, t: torch.Tensor, *args) -> None:
+    """Enqueues C entry ``name`` on the current stream of ``t``'s GPU, whichever GPU is the current one."""
+    fn = getattr(_lib.load(), name)
+    if t.device.index == torch.cuda.current_device():
+        status = fn(*args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            status = fn(*args, _stream(t))
+    _lib.check(name, status)
+
+
+def _check_heads(name: str, like: torch.Tensor, **tensors) -> None:
+    """Every given tensor is on ``like``'s GPU, of its dtype, and has a contiguous last dim."""
+    for label, t in tensors.items():
+        if t is not None:
+            _require(t.device == like.device, f"{name}: {label} is on {t.device}, not {like.device}")
+            _require(t.dtype == like.dtype, f"{name}: {label} is {t.dtype}, not {like.dtype}")
+            _require(t.size(-1) <= 1 or t.stride(-1) == 1, f"{name}: the last dim of {label} must be contiguous")
+
+
+def _check_norms(name: str, D: int, inv_freq, dev, *weights) -> None:
+    for w in weights:
+        _require(w is None or (w.shape == (D,) and w.is_contiguous()), f"{name}: norm weights must be [D={D}]")
+    if inv_freq is not None:
+        _require(inv_freq.dtype == torch.float32 and inv_freq.shape == (D // 2,) and inv_freq.is_contiguous()
+                 and inv_freq.device == dev, f"{name}: inv_freq must be float32 [D/2={D // 2}] on {dev}")
+
+
+def _check_index(name: str, dev, **tensors) -> None:
+    for label, t in tensors.items():
+        _require(t.dtype == torch.int32 and t.device == dev, f"{name}: {label} must be int32 on {dev}")
+        _require(t.size(-1) <= 1 or t.stride(-1) == 1, f"{name}: the last dim of {label} must be contiguous")
+
+
+def _check_ragged(name: str, like: torch.Tensor, block_table, cu_seqlens, kv_lens) -> int:
+    """Validates the tensors that say which rows are whose; returns the number of sequences."""
+    _check_index(name, like.device, block_table=block_table, kv_lens=kv_lens)
+    _require(block_table.dim() == 2, f"{name}: block_table must be [B, max_blocks]")
+    B = block_table.size(0)
+    _require(kv_lens.shape == (B,), f"{name}: kv_lens must be [B={B}], got {tuple(kv_lens.shape)}")
+    if cu_seqlens is not None:
+        _check_index(name, like.device, cu_seqlens=cu_seqlens)
+        _require(cu_seqlens.shape == (B + 1,), f"{name}: cu_seqlens must be [B + 1={B + 1}], got {tuple(cu_seqlens.shape)}")
+    return B
+
+
+def _check_pools(name: str, like: torch.Tensor, k_pages, v_pages) -> None:
+    _require(k_pages.dim() == 4 and k_pages.shape == v_pages.shape, f"{name}: pools must be [P, Hkv, page, D] and alike")
+    _check_heads(name, like, k_pages=k_pages, v_pages=v_pages)
+    _require(k_pages.stride() == v_pages.stride(), f"{name}: k and v pools must share strides")
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMSNorm (where a weight is given) and rotary embedding of queries and keys in one pass.
+
+    ``q [N, Hq, D]`` and ``k [N, Hkv, D]``, or ``[B, T, H, D]``, any strides with the head dim contiguous (views of a
+    projection row, or transposes of ``[B, H, T, D]``); ``positions`` int64 ``[N]`` / ``[B, T]``; ``inv_freq``
+    float32 ``[D/2]``, rotate_half convention.  fp32 inside, angles in fp64, one rounding.  ``q_out`` / ``k_out``
+    may be ``q`` / ``k`` themselves; by default they are new contiguous tensors.
+    """
+    name = "qk_norm_rope"
+    _require(q.is_cuda and q.dtype in _DTYPES, f"{name}: q must be fp16 or bf16 on the GPU")
+    _require(q.dim() in (3, 4) and k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.size(-1) == q.size(-1),
+             f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} must be [N, H, D] or [B, T, H, D] of the same tokens")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+    _require(q_out.shape == q.shape and k_out.shape == k.shape, f"{name}: outputs must have the inputs' shapes")
+    _check_heads(name, q, q=q, k=k, q_out=q_out, k_out=k_out, q_weight=q_weight, k_weight=k_weight)
+    _check_norms(name, q.size(-1), inv_freq, q.device, q_weight, k_weight)
+    _require(positions.dtype == torch.int64 and positions.device == q.device and positions.shape == q.shape[:-2]
+             and (positions.size(-1) <= 1 or positions.stride(-1) == 1),
+             f"{name}: positions must be int64 {tuple(q.shape[:-2])} on {q.device}, contiguous in the last dim")
+    four = [t if t.dim() == 4 else t[None] for t in (q, k, q_out, k_out)]
+    pos = positions if positions.dim() == 2 else positions[None]
+    strides = [(t.data_ptr(), *t.stride()[:3]) for t in four]
+    B, T, Hq, D = four[0].shape
+    _call("sa_qk_norm_rope", q, _DTYPES[q.dtype], *strides[0], *strides[1], *strides[2], *strides[3], _ptr(q_weight),
+          _ptr(k_weight), inv_freq.data_ptr(), pos.data_ptr(), pos.stride(0), B, T, Hq, four[1].size(2), D, float(eps))
+    return q_out, k_out
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *,
+                 inv_freq: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 k_bounds: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                 q_weight: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Writes a chunk's keys (normed and rotated on the way) and values into the pages of a cache.
+
+    ``k, v [N, Hkv, D]`` hold the new tokens of all sequences, those of sequence b in rows ``cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1`` (int32 ``[B + 1]``); ``kv_lens [B]`` int32 counts each sequence's tokens with them.
+    ``inv_freq`` (float32 ``[D/2]``) rotates, ``k_weight [D]`` norms; without them keys are stored as they are.
+    ``k_bounds [P, Hkv, 2, D]`` keeps each page's smallest and largest key per dim (:func:`paged_block_select`
+    reads it).  ``q [N, Hq, D]`` takes the same norm (``q_weight``) and rotation in the same launch; its result is
+    returned (``q_out``, allocated if omitted; rows of no sequence are left as they are).  The pages must
+    be in the table already, and no two sequences may write one page.
+    """
+    name = "paged_append"
+    _require(k.is_cuda and k.dtype in _DTYPES, f"{name}: k must be fp16 or bf16 on the GPU")
+    _require(k.dim() == 3 and v.shape == k.shape, f"{name}: k and v must be [N, Hkv, D] and alike")
+    N, Hkv, D = k.shape
+    _check_pools(name, k, k_pages, v_pages)
+    _require(k_pages.size(1) == Hkv and k_pages.size(3) == D, f"{name}: pools of other heads than k {tuple(k.shape)}")
+    B = _check_ragged(name, k, block_table, cu_seqlens, kv_lens)
+    if q is not None:
+        _require(q.dim() == 3 and q.size(0) == N and q.size(2) == D, f"{name}: q must be [N={N}, Hq, D={D}]")
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        _require(q_out.shape == q.shape, f"{name}: q_out must have q's shape")
+    else:
+        _require(q_out is None and q_weight is None, f"{name}: q_out and q_weight need q")
+    if k_bounds is not None:
+        _require(k_bounds.shape == (k_pages.size(0), Hkv, 2, D) and k_bounds.stride(2) == D,
+                 f"{name}: k_bounds must be [P, Hkv, 2, D] with contiguous [2, D]")
+    _check_heads(name, k, k=k, v=v, q=q, q_out=q_out, k_bounds=k_bounds, q_weight=q_weight, k_weight=k_weight)
+    _check_norms(name, D, inv_freq, k.device, q_weight, k_weight)
+    two = lambda t: (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    _call("sa_paged_append", k, _DTYPES[k.dtype], *two(q), *two(k), *two(v), *two(q_out), _ptr(q_weight), _ptr(k_weight),
+          _ptr(inv_freq), k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.size(0), *two(k_bounds),
+          block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+          N, B, 0 if q is None else q.size(1), Hkv, D, k_pages.size(2), float(eps))
+    return q_out
+
+
+def paged_chunk_splits(N: int, B: int, Hq: int, Hkv: int, max_kv: int) -> int:
+    """Workgroups that share a row tile's keys in :func:`paged_chunk_attn` by default."""
+    tiles = max(1, min(N * (Hq // Hkv) // 32 + min(B, N), N)) * Hkv
+    return max(1, min(256 // tiles, max_kv // 512, 64))
+
+
+def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                     cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *, sel: torch.Tensor | None = None,
+                     sel_off: torch.Tensor | None = None, sm_scale: float | None = None, num_splits: int = 0,
+                     workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of a chunk of new tokens over a paged cache; returns ``[N, Hq, D]``.
+
+    ``q [N, Hq, D]`` packs the new tokens of all sequences as in :func:`paged_append`, whose call has written
+    their keys and values; any number of them per sequence, 0 and 1 included.  The query of a token at position p
+    sees the keys ``j <= p`` of its sequence.  ``sel`` / ``sel_off`` of :func:`paged_block_select` (with
+    ``cu_seqlens``) restrict each block of 64 new tokens to the listed pages.  ``num_splits`` workgroups share
+    the keys of a row tile (0: from the shapes, :func:`paged_chunk_splits`); more than one needs a byte
+    workspace (allocated if omitted), which concurrent calls must not share.  Rows of ``out`` of no sequence are left as
+    they are.
+    """
+    name = "paged_chunk_attn"
+    _require(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, f"{name}: q must be [N, Hq, D], fp16 or bf16 on the GPU")
+    N, Hq, D = q.shape
+    _check_pools(name, q, k_pages, v_pages)
+    P, Hkv, page, _ = k_pages.shape
+    _require(k_pages.size(3) == D and Hkv > 0 and Hq % Hkv == 0, f"{name}: {Hq} query heads of {D} over pools "
+             f"{tuple(k_pages.shape)}")
+    B = _check_ragged(name, q, block_table, cu_seqlens, kv_lens)
+    rows = width = 0
+    sel_strides = off_strides = (0, 0)
+    if sel is not None:
+        _require(sel_off is not None, f"{name}: sel needs sel_off")
+        _check_index(name, q.device, sel=sel, sel_off=sel_off)
+        rows, width = N // CHUNK_BLOCK + min(B, N), sel.size(-1)
+        _require(sel.dim() == 3 and sel.size(1) == Hkv and sel.size(0) >= rows
+                 and sel_off.shape == (sel.size(0), Hkv, 2),
+                 f"{name}: sel must be [{rows} rows, Hkv={Hkv}, width] with sel_off [rows, Hkv, 2]")
+        rows = sel.size(0)
+        sel_strides, off_strides = sel.stride()[:2], sel_off.stride()[:2]
+    else:
+        _require(sel_off is None, f"{name}: sel_off needs sel")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    _require(out.shape == q.shape, f"{name}: out must have q's shape")
+    _check_heads(name, q, q=q, out=out)
+    if num_splits == 0:
+        max_kv = block_table.size(1) * page if sel is None else min(block_table.size(1), width) * page
+        num_splits = paged_chunk_splits(N, B, Hq, Hkv, max_kv)
+    need = int(_lib.load().sa_paged_chunk_workspace_bytes(N, Hq, D, num_splits))
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _require(need == 0 or (have >= need and workspace.device == q.device and workspace.is_contiguous()),
+             f"{name}: needs a contiguous workspace of {need} bytes on {q.device}")
+    _call("sa_paged_chunk_attn", q, _DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(),
+          v_pages.data_ptr(), *k_pages.stride()[:3], P, block_table.data_ptr(), block_table.stride(0),
+          block_table.size(1), cu_seqlens.data_ptr(), kv_lens.data_ptr(), _ptr(sel), *sel_strides, rows, width,
+          _ptr(sel_off), *off_strides, out.data_ptr(), out.stride(0), out.stride(1), N, B, Hq, Hkv, D, page,
+          1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), num_splits, _ptr(workspace), have)
+    return out
+
+
+def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, *,
+                       page: int, top_k: int, sink: int = 1, recent: int = 1, cu_seqlens: torch.Tensor | None = None,
+                       workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The pages worth attending, from the bounds of their keys: ``(sel, sel_off)``.
+
+    For one new token per sequence, ``q [B, Hq, D]`` (the newest, at position ``kv_lens[b] - 1``): ``sel [B, Hkv,
+    width]`` and ``sel_off [B, Hkv, 2]`` as :func:`paged_sparse_decode` reads them.  With ``cu_seqlens``, ``q [N, Hq, D]``
+    packed: a list for each block of 64 new tokens, ``[N // 64 + min(B, N), Hkv, width]``, as
+    :func:`paged_chunk_attn` reads it.  ``k_bounds [P, Hkv, 2, D]`` is :func:`paged_append`'s.
+
+    A list keeps the first ``sink`` pages, the last ``recent`` (counted back from the page of its first query) and
+    the ``top_k`` pages between whose bound of ``q . k``, summed over the list's queries and the heads of the group,
+    is largest; ties go to the lower page.  Lists ascend and are zero-padded.  A byte workspace is used where
+    the call needs one (allocated if omitted); concurrent calls must not share it.
+    """
+    name = "paged_block_select"
+    _require(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, f"{name}: q must be [N, Hq, D], fp16 or bf16 on the GPU")
+    N, Hq, D = q.shape
+    B = _check_ragged(name, q, block_table, cu_seqlens, kv_lens)
+    _require(cu_seqlens is not None or N == B, f"{name}: without cu_seqlens q must hold one token for each of {B} sequences")
+    _require(k_bounds.dim() == 4 and k_bounds.shape[2:] == (2, D) and k_bounds.stride(2) == D and k_bounds.size(1) > 0
+             and Hq % k_bounds.size(1) == 0, f"{name}: k_bounds must be [P, Hkv, 2, D={D}] with contiguous [2, D]")
+    _check_heads(name, q, q=q, k_bounds=k_bounds)
+    _require(page >= 16 and top_k >= 0 and sink >= 0 and recent >= 1, f"{name}: page={page}, top_k={top_k}, sink={sink}, "
+             f"recent={recent}")
+    P, Hkv = k_bounds.shape[:2]
+    span = 1 if cu_seqlens is None else (CHUNK_BLOCK + page - 2) // page + 1
+    rows = B if cu_seqlens is None else N // CHUNK_BLOCK + min(B, N)
+    sel = torch.empty(rows, Hkv, sink + top_k + recent - 1 + span, dtype=torch.int32, device=q.device)
+    sel_off = torch.empty(rows, Hkv, 2, dtype=torch.int32, device=q.device)
+    need = int(_lib.load().sa_paged_block_select_workspace_bytes(rows, Hkv, block_table.size(1)))
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _require(need == 0 or (have >= need and workspace.device == q.device and workspace.is_contiguous()),
+             f"{name}: needs a contiguous workspace of {need} bytes on {q.device}")
+    _call("sa_paged_block_select", q, _DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k_bounds.data_ptr(),
+          k_bounds.stride(0), k_bounds.stride(1), P, block_table.data_ptr(), block_table.stride(0), block_table.size(1),
+          _ptr(cu_seqlens), kv_lens.data_ptr(), N, B, Hq, Hkv, D, page, top_k, sink, recent, sel.data_ptr(), sel.stride(0),
+          sel.stride(1), rows, sel.size(2), sel_off.data_ptr(), _ptr(workspace), have)
+    return sel, sel_off
