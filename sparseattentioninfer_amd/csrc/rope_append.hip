@@ -44,6 +44,7 @@ struct RopeArgs {
   int64_t pos_sb;
   int64_t N;
   int T;
+  uint32_t mul_T;
   // paged
   Ragged seqs;
   elem_t *k_pages, *v_pages;
@@ -84,6 +85,12 @@ struct RopeAppend {
     int64_t row0;       // packed row of slot 0 (may lie before the tensor; slots below lo are not touched)
   };
 
+  // Batch and token of row n of an unpaged tensor.
+  static __device__ __forceinline__ void batch_of(const RopeArgs& a, int64_t n, int& b, int& t) {
+    b = (int)fast_div((uint32_t)n, (uint32_t)a.T, a.mul_T);
+    t = (int)((uint32_t)n - (uint32_t)b * (uint32_t)a.T);
+  }
+
   static __device__ __forceinline__ bool find_window(const RopeArgs& a, int x, Window& w, int& b) {
     b = 0;
     if constexpr (!PAGED) {
@@ -111,7 +118,7 @@ struct RopeAppend {
   }
 
   static __device__ void run(const RopeArgs& a) {
-    __shared__ float s_cs[RA_MAX_WINDOW * CS_STRIDE];
+    extern __shared__ float s_cs[];   // window x CS_STRIDE
     __shared__ int s_page[RA_MAX_WINDOW / RA_CHUNK], s_slot[RA_MAX_WINDOW / RA_CHUNK];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -125,8 +132,9 @@ struct RopeAppend {
         const int slot = x / HALF, i = x % HALF;
         int64_t p = w.base + slot;
         if constexpr (!PAGED) {
-          const int64_t n = w.row0 + slot;
-          p = a.positions[n / a.T * a.pos_sb + n % a.T];
+          int bt, t;
+          batch_of(a, w.row0 + slot, bt, t);
+          p = a.positions[bt * a.pos_sb + t];
         }
         const double turns = (double)p * (double)a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
         float s, c;
@@ -156,13 +164,24 @@ struct RopeAppend {
   // All of the window's tokens of one head.
   static __device__ __forceinline__ void head(const RopeArgs& a, const Window& w, int h, int lane, const float* s_cs,
                                               const int* s_page, const int* s_slot) {
-    const int kind = h < a.Hq ? 0 : h < a.Hq + a.Hkv ? 1 : 2;   // query, key, value
-    const int hh = kind == 0 ? h : kind == 1 ? h - a.Hq : h - a.Hq - a.Hkv;
-    const elem_t* src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const int64_t st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
-    const int64_t sb = kind == 0 ? a.q_sb : a.k_sb;
-    src += hh * (kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh);
-    const elem_t* wt = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
+    // Where this head comes from and goes to: rows of src, then rows of dst or (paged keys and values) pages of it.
+    int kind, hh;                 // query, key, value; head among its kind
+    const elem_t *src, *wt;
+    elem_t* dst;
+    int64_t st, sb, d_st, d_sb;
+    if (h < a.Hq) {
+      kind = 0, hh = h;
+      src = a.q + hh * a.q_sh, st = a.q_st, sb = a.q_sb, wt = a.qw;
+      dst = a.qo + hh * a.qo_sh, d_st = a.qo_st, d_sb = a.qo_sb;
+    } else if (h < a.Hq + a.Hkv) {
+      kind = 1, hh = h - a.Hq;
+      src = a.k + hh * a.k_sh, st = a.k_st, sb = a.k_sb, wt = a.kw;
+      dst = PAGED ? a.k_pages + hh * a.pg_sh : a.ko + hh * a.ko_sh, d_st = PAGED ? a.pg_st : a.ko_st, d_sb = a.ko_sb;
+    } else {
+      kind = 2, hh = h - a.Hq - a.Hkv;
+      src = a.v + hh * a.v_sh, st = a.v_st, sb = 0, wt = nullptr;
+      dst = a.v_pages + hh * a.pg_sh, d_st = a.pg_st, d_sb = 0;
+    }
     const bool rotate = a.inv_freq && kind < 2;
     const bool track = PAGED && kind == 1 && a.bounds;
     const int c = lane % LPR, g = lane / LPR;
@@ -176,20 +195,21 @@ struct RopeAppend {
     auto src_of = [&](int slot) {
       const int64_t n = w.row0 + slot;
       if constexpr (PAGED) return src + n * st + 8 * c;
-      return src + n / a.T * sb + n % a.T * st + 8 * c;
+      int bt, t;
+      batch_of(a, n, bt, t);
+      return src + bt * sb + t * st + 8 * c;
     };
     auto dst_of = [&](int slot) -> elem_t* {
       const int64_t n = w.row0 + slot;
       if constexpr (!PAGED) {
-        return (kind == 0 ? a.qo + n / a.T * a.qo_sb + n % a.T * a.qo_st + hh * a.qo_sh
-                          : a.ko + n / a.T * a.ko_sb + n % a.T * a.ko_st + hh * a.ko_sh) + 8 * c;
-      } else {
-        if (kind == 0) return a.qo + n * a.qo_st + hh * a.qo_sh + 8 * c;
-        const int pg = s_page[slot / RA_CHUNK];
-        if (pg < 0) return nullptr;
-        return (kind == 1 ? a.k_pages : a.v_pages) + pg * a.pg_sp + hh * a.pg_sh +
-               (int64_t)(s_slot[slot / RA_CHUNK] + slot % RA_CHUNK) * a.pg_st + 8 * c;
+        int bt, t;
+        batch_of(a, n, bt, t);
+        return dst + bt * d_sb + t * d_st + 8 * c;
       }
+      if (kind == 0) return dst + n * d_st + 8 * c;
+      const int pg = s_page[slot / RA_CHUNK];
+      if (pg < 0) return nullptr;
+      return dst + pg * a.pg_sp + (int64_t)(s_slot[slot / RA_CHUNK] + slot % RA_CHUNK) * d_st + 8 * c;
     };
     // With bounds a key head goes page by page, else the window at once.
     const int seg = track ? min(a.page, a.window) : a.window;
@@ -306,14 +326,15 @@ __global__ __launch_bounds__(RA_THREADS) void rope_append_kernel(const RopeArgs 
 template <bool PAGED>
 static int launch_rope(const char* name, int dtype, int D, const RopeArgs& a, dim3 grid, hipStream_t s) {
   const dim3 block(RA_THREADS);
+  const size_t lds = a.inv_freq ? (size_t)a.window * (D + 4) * sizeof(float) : 0;
   if (dtype == SA_DTYPE_BF16 && D == 128)
-    hipLaunchKernelGGL((rope_append_kernel<true, 128, PAGED>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<true, 128, PAGED>), grid, block, lds, s, a);
   else if (dtype == SA_DTYPE_BF16)
-    hipLaunchKernelGGL((rope_append_kernel<true, 64, PAGED>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<true, 64, PAGED>), grid, block, lds, s, a);
   else if (D == 128)
-    hipLaunchKernelGGL((rope_append_kernel<false, 128, PAGED>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<false, 128, PAGED>), grid, block, lds, s, a);
   else
-    hipLaunchKernelGGL((rope_append_kernel<false, 64, PAGED>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<false, 64, PAGED>), grid, block, lds, s, a);
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "%s: launch failed: %s", name, hipGetErrorString(err));
 }
@@ -364,6 +385,7 @@ extern "C" int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q
   a.pos_sb = pos_sb;
   a.N = (int64_t)B * T;
   a.T = T;
+  a.mul_T = div_mul((uint32_t)T);
   a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
   a.window = 32;
   const int64_t windows = (a.N + a.window - 1) / a.window;
@@ -410,7 +432,6 @@ extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q
   a.kw = static_cast<const elem_t*>(k_weight);
   a.inv_freq = inv_freq;
   a.N = N;
-  a.T = 1;
   a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
   a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
   a.k_pages = static_cast<elem_t*>(k_pages);

@@ -795,61 +795,62 @@ def gemm_skinny_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, out: torch.Tens
 CHUNK_BLOCK = 64    # new tokens of a sequence that share one selection (include/sparse_attn.h)
 
 
-def _call(name: str, t: torch.Tensor, *args) -> None:
-    """Enqueues C entry ``name`` on the current stream of ``t``'s GPU, whichever GPU is the current one."""
+# Index of the current GPU, without the checks that torch.cuda.current_device makes around it.
+_current_gpu = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _call(name: str, index: int, *args) -> None:
+    """Enqueues C entry ``name`` on the current stream of GPU ``index``, whichever GPU is the current one."""
     fn = getattr(_lib.load(), name)
-    if t.device.index == torch.cuda.current_device():
-        status = fn(*args, _stream(t))
+    if index == _current_gpu():
+        status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(t.device):
-            status = fn(*args, _stream(t))
-    _lib.check(name, status)
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(name, status)
 
 
-def _check_heads(name: str, like: torch.Tensor, **tensors) -> None:
-    """Every given tensor is on ``like``'s GPU, of its dtype, and has a contiguous last dim."""
-    for label, t in tensors.items():
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _refuse(name: str, q: torch.Tensor, *, heads: dict, index: dict, weights=(), inv_freq=None, pools=None, B=None,
+            other: str = "shapes do not fit") -> None:
+    """Says what is wrong with a call whose one test of everything has failed: ``heads`` are the tensors of q's type
+    and GPU with contiguous heads, ``index`` the int32 ones."""
+    D = q.size(-1) if q.dim() else 0
+    _require(q.is_cuda and q.dtype in _DTYPES, f"{name}: tensors must be fp16 or bf16 on the GPU, got {q.dtype} on {q.device}")
+    for label, t in heads.items():
         if t is not None:
-            _require(t.device == like.device, f"{name}: {label} is on {t.device}, not {like.device}")
-            _require(t.dtype == like.dtype, f"{name}: {label} is {t.dtype}, not {like.dtype}")
-            _require(t.size(-1) <= 1 or t.stride(-1) == 1, f"{name}: the last dim of {label} must be contiguous")
-
-
-def _check_norms(name: str, D: int, inv_freq, dev, *weights) -> None:
+            _require(t.device == q.device, f"{name}: {label} is on {t.device}, not {q.device}")
+            _require(t.dtype == q.dtype, f"{name}: {label} is {t.dtype}, not {q.dtype}")
+            _require(t.dim() > 0 and t.stride(-1) == 1, f"{name}: the last dim of {label} must be contiguous")
+    for label, t in index.items():
+        if t is not None:
+            _require(t.dtype == torch.int32 and t.device == q.device, f"{name}: {label} must be int32 on {q.device}")
+            _require(t.dim() > 0 and (t.size(-1) <= 1 or t.stride(-1) == 1), f"{name}: the last dim of {label} must be contiguous")
     for w in weights:
         _require(w is None or (w.shape == (D,) and w.is_contiguous()), f"{name}: norm weights must be [D={D}]")
     if inv_freq is not None:
         _require(inv_freq.dtype == torch.float32 and inv_freq.shape == (D // 2,) and inv_freq.is_contiguous()
-                 and inv_freq.device == dev, f"{name}: inv_freq must be float32 [D/2={D // 2}] on {dev}")
+                 and inv_freq.device == q.device, f"{name}: inv_freq must be float32 [D/2={D // 2}] on {q.device}")
+    if pools is not None:
+        kp, vp = pools
+        _require(kp.dim() == 4 and kp.shape == vp.shape and kp.size(3) == D,
+                 f"{name}: pools must be [P, Hkv, page, D={D}] and alike, got {tuple(kp.shape)} and {tuple(vp.shape)}")
+        _require(kp.stride() == vp.stride(), f"{name}: k and v pools must share strides")
+    if B is not None:
+        _require(index["block_table"].dim() == 2, f"{name}: block_table must be [B, max_blocks]")
+        _require(index["kv_lens"].shape == (B,), f"{name}: kv_lens must be [B={B}], got {tuple(index['kv_lens'].shape)}")
+        cu = index["cu_seqlens"]
+        _require(cu is None or cu.shape == (B + 1,), f"{name}: cu_seqlens must be [B + 1={B + 1}]")
+    _require(False, f"{name}: {other}: " + ", ".join(f"{k} {tuple(t.shape)}" for k, t in {**heads, **index}.items()
+                                                   if t is not None))
 
 
-def _check_index(name: str, dev, **tensors) -> None:
-    for label, t in tensors.items():
-        _require(t.dtype == torch.int32 and t.device == dev, f"{name}: {label} must be int32 on {dev}")
-        _require(t.size(-1) <= 1 or t.stride(-1) == 1, f"{name}: the last dim of {label} must be contiguous")
-
-
-def _check_ragged(name: str, like: torch.Tensor, block_table, cu_seqlens, kv_lens) -> int:
-    """Validates the tensors that say which rows are whose; returns the number of sequences."""
-    _check_index(name, like.device, block_table=block_table, kv_lens=kv_lens)
-    _require(block_table.dim() == 2, f"{name}: block_table must be [B, max_blocks]")
-    B = block_table.size(0)
-    _require(kv_lens.shape == (B,), f"{name}: kv_lens must be [B={B}], got {tuple(kv_lens.shape)}")
-    if cu_seqlens is not None:
-        _check_index(name, like.device, cu_seqlens=cu_seqlens)
-        _require(cu_seqlens.shape == (B + 1,), f"{name}: cu_seqlens must be [B + 1={B + 1}], got {tuple(cu_seqlens.shape)}")
-    return B
-
-
-def _check_pools(name: str, like: torch.Tensor, k_pages, v_pages) -> None:
-    _require(k_pages.dim() == 4 and k_pages.shape == v_pages.shape, f"{name}: pools must be [P, Hkv, page, D] and alike")
-    _check_heads(name, like, k_pages=k_pages, v_pages=v_pages)
-    _require(k_pages.stride() == v_pages.stride(), f"{name}: k and v pools must share strides")
-
-
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
-
+# The calls below test everything in one expression first: a call that passes formats no message.  Their host time
+# is most of a single-token step's (a message per condition made it 24 to 43 us a call).
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
                  q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
@@ -863,23 +864,38 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     may be ``q`` / ``k`` themselves; by default they are new contiguous tensors.
     """
     name = "qk_norm_rope"
-    _require(q.is_cuda and q.dtype in _DTYPES, f"{name}: q must be fp16 or bf16 on the GPU")
-    _require(q.dim() in (3, 4) and k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.size(-1) == q.size(-1),
-             f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} must be [N, H, D] or [B, T, H, D] of the same tokens")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
-    _require(q_out.shape == q.shape and k_out.shape == k.shape, f"{name}: outputs must have the inputs' shapes")
-    _check_heads(name, q, q=q, k=k, q_out=q_out, k_out=k_out, q_weight=q_weight, k_weight=k_weight)
-    _check_norms(name, q.size(-1), inv_freq, q.device, q_weight, k_weight)
-    _require(positions.dtype == torch.int64 and positions.device == q.device and positions.shape == q.shape[:-2]
-             and (positions.size(-1) <= 1 or positions.stride(-1) == 1),
-             f"{name}: positions must be int64 {tuple(q.shape[:-2])} on {q.device}, contiguous in the last dim")
-    four = [t if t.dim() == 4 else t[None] for t in (q, k, q_out, k_out)]
-    pos = positions if positions.dim() == 2 else positions[None]
-    strides = [(t.data_ptr(), *t.stride()[:3]) for t in four]
-    B, T, Hq, D = four[0].shape
-    _call("sa_qk_norm_rope", q, _DTYPES[q.dtype], *strides[0], *strides[1], *strides[2], *strides[3], _ptr(q_weight),
-          _ptr(k_weight), inv_freq.data_ptr(), pos.data_ptr(), pos.stride(0), B, T, Hq, four[1].size(2), D, float(eps))
+    if q_out is None:
+        q_out = _empty_like(q)
+    if k_out is None:
+        k_out = _empty_like(k)
+    qs, ks, dt, dev, n = q.shape, k.shape, q.dtype, q.device, q.dim()
+    D = qs[-1] if n else 0
+    qst, kst, qot, kot = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    if not (q.is_cuda and dt in _DTYPES and (n == 3 or n == 4) and len(ks) == n and qs[:-2] == ks[:-2] and ks[-1] == D
+            and k.dtype == dt and k.device == dev and q_out.shape == qs and q_out.dtype == dt and q_out.device == dev
+            and k_out.shape == ks and k_out.dtype == dt and k_out.device == dev
+            and qst[-1] == 1 and kst[-1] == 1 and qot[-1] == 1 and kot[-1] == 1
+            and (q_weight is None or (q_weight.shape == (D,) and q_weight.dtype == dt and q_weight.device == dev
+                                      and q_weight.is_contiguous()))
+            and (k_weight is None or (k_weight.shape == (D,) and k_weight.dtype == dt and k_weight.device == dev
+                                      and k_weight.is_contiguous()))
+            and inv_freq.dtype == torch.float32 and inv_freq.shape == (D // 2,) and inv_freq.is_contiguous()
+            and inv_freq.device == dev and positions.dtype == torch.int64 and positions.device == dev
+            and positions.shape == qs[:-2] and (positions.size(-1) <= 1 or positions.stride(-1) == 1)):
+        _refuse(name, q, heads=dict(q=q, k=k, q_out=q_out, k_out=k_out, q_weight=q_weight, k_weight=k_weight), index={},
+                weights=(q_weight, k_weight), inv_freq=inv_freq,
+                other="q and k must be [N, H, D] or [B, T, H, D] of the same tokens, outputs like them, positions int64 "
+                      f"of those tokens on {dev}, contiguous in the last dim; got positions {positions.dtype} "
+                      f"{tuple(positions.shape)} on {positions.device}")
+    if n == 3:
+        B, T, pos_sb = 1, qs[0], 0
+        qst, kst, qot, kot = (0, *qst), (0, *kst), (0, *qot), (0, *kot)
+    else:
+        B, T, pos_sb = qs[0], qs[1], positions.stride(0)
+    _call("sa_qk_norm_rope", dev.index, _DTYPES[dt], q.data_ptr(), *qst[:3], k.data_ptr(), *kst[:3], q_out.data_ptr(),
+          *qot[:3], k_out.data_ptr(), *kot[:3], None if q_weight is None else q_weight.data_ptr(),
+          None if k_weight is None else k_weight.data_ptr(), inv_freq.data_ptr(), positions.data_ptr(), pos_sb, B, T,
+          qs[-2], ks[-2], D, eps)
     return q_out, k_out
 
 
@@ -899,28 +915,49 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     be in the table already, and no two sequences may write one page.
     """
     name = "paged_append"
-    _require(k.is_cuda and k.dtype in _DTYPES, f"{name}: k must be fp16 or bf16 on the GPU")
-    _require(k.dim() == 3 and v.shape == k.shape, f"{name}: k and v must be [N, Hkv, D] and alike")
-    N, Hkv, D = k.shape
-    _check_pools(name, k, k_pages, v_pages)
-    _require(k_pages.size(1) == Hkv and k_pages.size(3) == D, f"{name}: pools of other heads than k {tuple(k.shape)}")
-    B = _check_ragged(name, k, block_table, cu_seqlens, kv_lens)
-    if q is not None:
-        _require(q.dim() == 3 and q.size(0) == N and q.size(2) == D, f"{name}: q must be [N={N}, Hq, D={D}]")
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        _require(q_out.shape == q.shape, f"{name}: q_out must have q's shape")
-    else:
-        _require(q_out is None and q_weight is None, f"{name}: q_out and q_weight need q")
-    if k_bounds is not None:
-        _require(k_bounds.shape == (k_pages.size(0), Hkv, 2, D) and k_bounds.stride(2) == D,
-                 f"{name}: k_bounds must be [P, Hkv, 2, D] with contiguous [2, D]")
-    _check_heads(name, k, k=k, v=v, q=q, q_out=q_out, k_bounds=k_bounds, q_weight=q_weight, k_weight=k_weight)
-    _check_norms(name, D, inv_freq, k.device, q_weight, k_weight)
-    two = lambda t: (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
-    _call("sa_paged_append", k, _DTYPES[k.dtype], *two(q), *two(k), *two(v), *two(q_out), _ptr(q_weight), _ptr(k_weight),
-          _ptr(inv_freq), k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], k_pages.size(0), *two(k_bounds),
-          block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(), kv_lens.data_ptr(),
-          N, B, 0 if q is None else q.size(1), Hkv, D, k_pages.size(2), float(eps))
+    dt, dev, ks, ps, B = k.dtype, k.device, k.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    kst, vst, pst = k.stride(), v.stride(), k_pages.stride()
+    ok = (k.is_cuda and dt in _DTYPES and len(ks) == 3 and v.shape == ks and v.dtype == dt and v.device == dev
+          and kst[2] == 1 and vst[2] == 1 and len(ps) == 4 and v_pages.shape == ps and ps[1] == ks[1] and ps[3] == ks[2]
+          and k_pages.dtype == dt and v_pages.dtype == dt and k_pages.device == dev and v_pages.device == dev
+          and pst[3] == 1 and v_pages.stride() == pst
+          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
+          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
+          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+          and (k_weight is None or (k_weight.shape == (ks[2],) and k_weight.dtype == dt and k_weight.device == dev
+                                    and k_weight.is_contiguous()))
+          and (inv_freq is None or (inv_freq.dtype == torch.float32 and inv_freq.shape == (ks[2] // 2,)
+                                    and inv_freq.is_contiguous() and inv_freq.device == dev)))
+    if ok and k_bounds is not None:
+        ok = (k_bounds.shape == (ps[0], ps[1], 2, ps[3]) and k_bounds.dtype == dt and k_bounds.device == dev
+              and k_bounds.stride(3) == 1 and k_bounds.stride(2) == ps[3])
+    qargs, oargs, Hq = (None, 0, 0), (None, 0, 0), 0
+    if q is None:
+        ok = ok and q_out is None and q_weight is None
+    elif ok:
+        if q_out is None:
+            q_out = _empty_like(q)
+        qs, qst, ost = q.shape, q.stride(), q_out.stride()
+        ok = (len(qs) == 3 and qs[0] == ks[0] and qs[2] == ks[2] and q.dtype == dt and q.device == dev and qst[2] == 1
+              and q_out.shape == qs and q_out.dtype == dt and q_out.device == dev and ost[2] == 1
+              and (q_weight is None or (q_weight.shape == (ks[2],) and q_weight.dtype == dt and q_weight.device == dev
+                                        and q_weight.is_contiguous())))
+        if ok:
+            qargs, oargs, Hq = (q.data_ptr(), qst[0], qst[1]), (q_out.data_ptr(), ost[0], ost[1]), qs[1]
+    if not ok:
+        _refuse(name, k, heads=dict(k=k, v=v, k_pages=k_pages, v_pages=v_pages, q=q, q_out=q_out, k_bounds=k_bounds,
+                                    q_weight=q_weight, k_weight=k_weight),
+                index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens), weights=(q_weight, k_weight),
+                inv_freq=inv_freq, pools=(k_pages, v_pages), B=block_table.size(0) if block_table.dim() else 0,
+                other="k and v must be [N, Hkv, D], q [N, Hq, D] (q_out and q_weight need it), pools [P, Hkv, page, D], "
+                      "k_bounds [P, Hkv, 2, D] with contiguous [2, D]")
+    bargs = (None, 0, 0) if k_bounds is None else (k_bounds.data_ptr(), k_bounds.stride(0), k_bounds.stride(1))
+    _call("sa_paged_append", dev.index, _DTYPES[dt], *qargs, k.data_ptr(), kst[0], kst[1], v.data_ptr(), vst[0], vst[1],
+          *oargs, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+          None if inv_freq is None else inv_freq.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pst[0], pst[1], pst[2],
+          ps[0], *bargs, block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
+          kv_lens.data_ptr(), ks[0], B, Hq, ks[1], ks[2], ps[2], eps)
     return q_out
 
 
@@ -945,44 +982,61 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     they are.
     """
     name = "paged_chunk_attn"
-    _require(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, f"{name}: q must be [N, Hq, D], fp16 or bf16 on the GPU")
-    N, Hq, D = q.shape
-    _check_pools(name, q, k_pages, v_pages)
-    P, Hkv, page, _ = k_pages.shape
-    _require(k_pages.size(3) == D and Hkv > 0 and Hq % Hkv == 0, f"{name}: {Hq} query heads of {D} over pools "
-             f"{tuple(k_pages.shape)}")
-    B = _check_ragged(name, q, block_table, cu_seqlens, kv_lens)
-    rows = width = 0
-    sel_strides = off_strides = (0, 0)
-    if sel is not None:
-        _require(sel_off is not None, f"{name}: sel needs sel_off")
-        _check_index(name, q.device, sel=sel, sel_off=sel_off)
-        rows, width = N // CHUNK_BLOCK + min(B, N), sel.size(-1)
-        _require(sel.dim() == 3 and sel.size(1) == Hkv and sel.size(0) >= rows
-                 and sel_off.shape == (sel.size(0), Hkv, 2),
-                 f"{name}: sel must be [{rows} rows, Hkv={Hkv}, width] with sel_off [rows, Hkv, 2]")
-        rows = sel.size(0)
-        sel_strides, off_strides = sel.stride()[:2], sel_off.stride()[:2]
-    else:
-        _require(sel_off is None, f"{name}: sel_off needs sel")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    _require(out.shape == q.shape, f"{name}: out must have q's shape")
-    _check_heads(name, q, q=q, out=out)
+    if out is None:
+        out = _empty_like(q)
+    dt, dev, qs, ps, B = q.dtype, q.device, q.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    qst, ost, pst = q.stride(), out.stride(), k_pages.stride()
+    ok = (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and out.shape == qs and out.dtype == dt
+          and out.device == dev and ost[2] == 1 and len(ps) == 4 and v_pages.shape == ps and ps[3] == qs[2]
+          and ps[1] > 0 and qs[1] % ps[1] == 0
+          and k_pages.dtype == dt and v_pages.dtype == dt and k_pages.device == dev and v_pages.device == dev
+          and pst[3] == 1 and v_pages.stride() == pst
+          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
+          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
+          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+          and (sel is None) == (sel_off is None))
+    sargs = (None, 0, 0, 0, 0, None, 0, 0)
+    max_blocks = block_table.size(-1) if ok else 0
+    keys = max_blocks
+    if ok and sel is not None:
+        ss, sst = sel.shape, sel.stride()
+        ok = (sel.dtype == torch.int32 and sel_off.dtype == torch.int32 and sel.device == dev and sel_off.device == dev
+              and len(ss) == 3 and ss[0] >= qs[0] // CHUNK_BLOCK + min(B, qs[0]) and ss[1] == ps[1]
+              and sel_off.shape == (ss[0], ss[1], 2) and (ss[2] <= 1 or sst[2] == 1) and sel_off.stride(2) == 1)
+        if ok:
+            sargs = (sel.data_ptr(), sst[0], sst[1], ss[0], ss[2], sel_off.data_ptr(), sel_off.stride(0), sel_off.stride(1))
+            keys = min(keys, ss[2])
+    if not ok:
+        _refuse(name, q, heads=dict(q=q, k_pages=k_pages, v_pages=v_pages, out=out),
+                index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens, sel=sel, sel_off=sel_off),
+                pools=(k_pages, v_pages), B=block_table.size(0) if block_table.dim() else 0,
+                other="q and out must be [N, Hq, D], pools [P, Hkv, page, D] with Hq a multiple of Hkv, sel and sel_off "
+                      f"(both or neither) [at least N // {CHUNK_BLOCK} + min(B, N) rows, Hkv, width] and [rows, Hkv, 2]")
+    N, Hq, D = qs
     if num_splits == 0:
-        max_kv = block_table.size(1) * page if sel is None else min(block_table.size(1), width) * page
-        num_splits = paged_chunk_splits(N, B, Hq, Hkv, max_kv)
-    need = int(_lib.load().sa_paged_chunk_workspace_bytes(N, Hq, D, num_splits))
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _require(need == 0 or (have >= need and workspace.device == q.device and workspace.is_contiguous()),
-             f"{name}: needs a contiguous workspace of {need} bytes on {q.device}")
-    _call("sa_paged_chunk_attn", q, _DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(),
-          v_pages.data_ptr(), *k_pages.stride()[:3], P, block_table.data_ptr(), block_table.stride(0),
-          block_table.size(1), cu_seqlens.data_ptr(), kv_lens.data_ptr(), _ptr(sel), *sel_strides, rows, width,
-          _ptr(sel_off), *off_strides, out.data_ptr(), out.stride(0), out.stride(1), N, B, Hq, Hkv, D, page,
-          1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), num_splits, _ptr(workspace), have)
+        num_splits = paged_chunk_splits(N, B, Hq, ps[1], keys * ps[2])
+    ws = _workspace(name, workspace, num_splits * N * Hq * (D + 2) * 4 if num_splits > 1 else 0, dev)
+    _call("sa_paged_chunk_attn", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_pages.data_ptr(),
+          v_pages.data_ptr(), pst[0], pst[1], pst[2], ps[0], block_table.data_ptr(), block_table.stride(0), max_blocks,
+          cu_seqlens.data_ptr(), kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], N, B, Hq, ps[1], D, ps[2],
+          D ** -0.5 if sm_scale is None else sm_scale, num_splits, *_ws_bytes(ws))
     return out
+
+
+def _workspace(name: str, given: torch.Tensor | None, need: int, dev) -> torch.Tensor | None:
+    """The given workspace if a call needs one, after checking it; else a new one, or None."""
+    if not need:
+        return None
+    if given is None:
+        return torch.empty(need, dtype=torch.uint8, device=dev)
+    _require(given.device == dev and given.is_contiguous() and given.numel() * given.element_size() >= need,
+             f"{name}: needs a contiguous workspace of {need} bytes on {dev}")
+    return given
+
+
+def _ws_bytes(ws: torch.Tensor | None):
+    return (None, 0) if ws is None else (ws.data_ptr(), ws.numel() * ws.element_size())
 
 
 def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, *,
@@ -1001,28 +1055,34 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: tor
     the call needs one (allocated if omitted); concurrent calls must not share it.
     """
     name = "paged_block_select"
-    _require(q.is_cuda and q.dtype in _DTYPES and q.dim() == 3, f"{name}: q must be [N, Hq, D], fp16 or bf16 on the GPU")
-    N, Hq, D = q.shape
-    B = _check_ragged(name, q, block_table, cu_seqlens, kv_lens)
-    _require(cu_seqlens is not None or N == B, f"{name}: without cu_seqlens q must hold one token for each of {B} sequences")
-    _require(k_bounds.dim() == 4 and k_bounds.shape[2:] == (2, D) and k_bounds.stride(2) == D and k_bounds.size(1) > 0
-             and Hq % k_bounds.size(1) == 0, f"{name}: k_bounds must be [P, Hkv, 2, D={D}] with contiguous [2, D]")
-    _check_heads(name, q, q=q, k_bounds=k_bounds)
-    _require(page >= 16 and top_k >= 0 and sink >= 0 and recent >= 1, f"{name}: page={page}, top_k={top_k}, sink={sink}, "
-             f"recent={recent}")
-    P, Hkv = k_bounds.shape[:2]
-    span = 1 if cu_seqlens is None else (CHUNK_BLOCK + page - 2) // page + 1
-    rows = B if cu_seqlens is None else N // CHUNK_BLOCK + min(B, N)
-    sel = torch.empty(rows, Hkv, sink + top_k + recent - 1 + span, dtype=torch.int32, device=q.device)
-    sel_off = torch.empty(rows, Hkv, 2, dtype=torch.int32, device=q.device)
-    need = int(_lib.load().sa_paged_block_select_workspace_bytes(rows, Hkv, block_table.size(1)))
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    have = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _require(need == 0 or (have >= need and workspace.device == q.device and workspace.is_contiguous()),
-             f"{name}: needs a contiguous workspace of {need} bytes on {q.device}")
-    _call("sa_paged_block_select", q, _DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k_bounds.data_ptr(),
-          k_bounds.stride(0), k_bounds.stride(1), P, block_table.data_ptr(), block_table.stride(0), block_table.size(1),
-          _ptr(cu_seqlens), kv_lens.data_ptr(), N, B, Hq, Hkv, D, page, top_k, sink, recent, sel.data_ptr(), sel.stride(0),
-          sel.stride(1), rows, sel.size(2), sel_off.data_ptr(), _ptr(workspace), have)
+    dt, dev, qs, bs, B = q.dtype, q.device, q.shape, k_bounds.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    qst, bst = q.stride(), k_bounds.stride()
+    if not (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and len(bs) == 4 and bs[2] == 2 and bs[3] == qs[2]
+            and bs[1] > 0 and qs[1] % bs[1] == 0 and k_bounds.dtype == dt and k_bounds.device == dev and bst[3] == 1
+            and bst[2] == qs[2] and block_table.dtype == torch.int32 and kv_lens.dtype == torch.int32
+            and block_table.device == dev and kv_lens.device == dev and block_table.dim() == 2
+            and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
+            and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+            and (qs[0] == B if cu_seqlens is None else
+                 cu_seqlens.dtype == torch.int32 and cu_seqlens.device == dev and cu_seqlens.shape == (B + 1,)
+                 and cu_seqlens.is_contiguous())
+            and page >= 16 and top_k >= 0 and sink >= 0 and recent >= 1):
+        _refuse(name, q, heads=dict(q=q, k_bounds=k_bounds),
+                index=dict(block_table=block_table, kv_lens=kv_lens, cu_seqlens=cu_seqlens),
+                B=block_table.size(0) if block_table.dim() else 0,
+                other=f"q must be [N, Hq, D] (N == B without cu_seqlens), k_bounds [P, Hkv, 2, D] with contiguous [2, D] "
+                      f"and Hq a multiple of Hkv; page={page} (16 or more), top_k={top_k}, sink={sink} (not negative), "
+                      f"recent={recent} (1 or more)")
+    (N, Hq, D), Hkv, max_blocks = qs, bs[1], block_table.size(1)
+    if cu_seqlens is None:
+        rows, span, cu = B, 1, None
+    else:
+        rows, span, cu = N // CHUNK_BLOCK + min(B, N), (CHUNK_BLOCK + page - 2) // page + 1, cu_seqlens.data_ptr()
+    width = sink + top_k + recent - 1 + span
+    sel = torch.empty((rows, Hkv, width), dtype=torch.int32, device=dev)
+    sel_off = torch.empty((rows, Hkv, 2), dtype=torch.int32, device=dev)
+    ws = _workspace(name, workspace, _lib.load().sa_paged_block_select_workspace_bytes(rows, Hkv, max_blocks), dev)
+    _call("sa_paged_block_select", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_bounds.data_ptr(), bst[0], bst[1],
+          bs[0], block_table.data_ptr(), block_table.stride(0), max_blocks, cu, kv_lens.data_ptr(), N, B, Hq, Hkv, D, page,
+          top_k, sink, recent, sel.data_ptr(), Hkv * width, width, rows, width, sel_off.data_ptr(), *_ws_bytes(ws))
     return sel, sel_off
