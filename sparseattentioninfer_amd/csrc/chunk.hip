@@ -13,6 +13,7 @@
 // its wave-wide direct loads has one uniform address.  A wave looks its chunks' pages up 64 at a time, one a
 // lane, and takes them lane by lane.
 #include <algorithm>
+#include <type_traits>
 
 #include "lds_tile.h"
 #include "ragged.h"
@@ -423,9 +424,360 @@ struct Chunk : StagedTile {
   }
 };
 
+// 256 rows to a workgroup: eight waves of 32 rows share every K/V tile, which direct loads bring into LDS while the
+// tile before is worked on.  One step per tile and one barrier per step.  Block A of a step runs S^T = K Q^T of the
+// next tile on the matrix cores under the exponentials of this one, block B O^T += V^T P^T.  Waves 0..3 run A(i),
+// B(i) in step i and waves 4..7, one on each SIMD beside them, B(i - 1), A(i), so that the two waves of a SIMD run the
+// vector-heavy A and the matrix-only B at the same time.  K is double- and V triple-buffered for that.
+// A row's reference is the maximum of its first tile and is raised only when its probabilities would pass the
+// element type's range (Chunk::REFIT_SUM), so the common step never touches O with vector instructions.
+template <bool BF16, int D>
+struct ChunkWide : StagedTile {
+  using E = Elem<BF16>;
+  static constexpr int NW = 8;
+  static constexpr int NT = 64 * NW;
+  static constexpr int ROWS = NW * CK_ROWS;
+  static constexpr int NCG = D / 32;
+  static constexpr int NIW = 4 * NCG / NW;         // direct loads of a tile per wave: one row block each
+  static constexpr int TILE_BYTES = CK_KT * D * 2;
+  static constexpr int NBK = 2, NBV = 3;
+  static constexpr int STAGE = CK_ROWS * D * 2;    // a wave's share of O
+  static_assert(NW * STAGE <= (NBK + NBV) * TILE_BYTES, "O is staged in the K/V buffers");
+  static constexpr float REFIT_SUM = BF16 ? 65536.f : 32768.f;
+
+  // 64 tiles looked up at once: lane i holds, for tile base + i, the place and first key of the chunk that this
+  // wave loads, and the tile's largest key; the first keys of its four chunks go to LDS, for the tiles that need
+  // a mask.  Tiles are loaded up to two ahead of the one whose mask is due, so a window starts one tile back.
+  struct Window {
+    int base;
+    int64_t off;
+    int key, last;
+
+    static __device__ __forceinline__ int32_t now(const int32_t* p) {
+      int32_t x;
+      asm volatile(
+          "global_load_dword %0, %1, off\n\t"
+          "s_waitcnt vmcnt(0)"
+          : "=v"(x)
+          : "v"(p)
+          : "memory");
+      return x;
+    }
+    __device__ __forceinline__ void fill(const ChunkArgs& a, const ChunkItem& it, int first, int rb, int* s_keys) {
+      base = first;
+      key = CK_NO_KEY;
+      off = 0;
+      last = -1;
+      const int lane = threadIdx.x & 63;
+      int keys[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int c = it.c0 + 4 * (first + lane) + x;
+        keys[x] = CK_NO_KEY;
+        if (c < it.c1) {
+          int lb, slot;
+          if (it.list) {
+            const int e = (int)fast_div((uint32_t)c, (uint32_t)(a.page / 16), a.mul_ppc);
+            lb = now(it.list + e);
+            slot = (c - e * (a.page / 16)) * 16;
+          } else {
+            lb = (int)fast_div((uint32_t)(16 * c), (uint32_t)a.page, a.mul_page);
+            slot = 16 * c - lb * a.page;
+          }
+          if (lb >= 0 && lb < a.max_blocks && (int64_t)lb * a.page + slot <= it.pos_max) {
+            const int pg = now(a.table + it.b * a.table_stride + lb);
+            if (pg >= 0 && pg < a.num_pages) {
+              keys[x] = lb * a.page + slot;
+              if (x == rb) {
+                off = (int64_t)pg * a.kv_sp + (int64_t)slot * a.kv_st;
+                key = keys[x];
+              }
+            }
+          }
+        }
+        last = max(last, keys[x] + 15);
+      }
+      *reinterpret_cast<int4*>(s_keys + 4 * lane) = int4{keys[0], keys[1], keys[2], keys[3]};
+    }
+    __device__ __forceinline__ int key_of(int t) const { return __builtin_amdgcn_readlane(key, t - base); }
+    __device__ __forceinline__ int last_of(int t) const { return __builtin_amdgcn_readlane(last, t - base); }
+    __device__ __forceinline__ int64_t off_of(int t) const {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uint64_t)off, t - base);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)off >> 32), t - base);
+      return (int64_t)(((uint64_t)hi << 32) | lo);
+    }
+  };
+
+  static __device__ void run(const ChunkArgs& a) {
+    __shared__ __attribute__((aligned(16))) char s_kv[(NBK + NBV) * TILE_BYTES];
+    __shared__ __attribute__((aligned(16))) int s_keys[NW][4 * 64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 5, l32 = lane & 31;
+    ChunkItem it;
+    if (!find_chunk_item(a, ROWS, blockIdx.x, it)) return;
+    char* sK = s_kv;
+    char* sV = s_kv + NBK * TILE_BYTES;
+
+    const int row0 = min(it.row0 + CK_ROWS * wave, it.row_end - 1);   // a wave past the rows repeats the last one
+    const int row = min(row0 + l32, it.row_end - 1);
+    const int token = (int)fast_div((uint32_t)row, (uint32_t)a.G, a.mul_G);
+    const int pos_min = it.start + (int)fast_div((uint32_t)row0, (uint32_t)a.G, a.mul_G);
+    const int pos8 = it.start + token - 8 * g;   // a key at offset e of a chunk's lane half is seen if e <= pos8 - key
+    u32x4 Qr[D / 16];
+    {
+      const elem_t* qs = a.q + (int64_t)(it.tok0 + token) * a.q_st + (it.kvh * a.G + row - token * a.G) * a.q_sh + 8 * g;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) Qr[c] = *reinterpret_cast<const u32x4*>(qs + 16 * c);
+    }
+    const Frag f(lane);
+    const float c = a.scale_log2;
+
+    // This wave's direct loads of a tile: NIW column groups of row block rb.
+    const int rb = wave * NIW / NCG, cg0 = wave * NIW % NCG;
+    const char* kh = reinterpret_cast<const char*>(a.k + it.kvh * a.kv_sh + 32 * cg0);
+    const char* vh = reinterpret_cast<const char*>(a.v + it.kvh * a.kv_sh + 32 * cg0);
+    const uint32_t koff = (uint32_t)((krow(lane >> 2) * a.kv_st + dma_col(lane)) * 2);
+    const uint32_t voff = (uint32_t)(((lane >> 2) * a.kv_st + dma_col(lane)) * 2);
+    const uint32_t lds_k = lds_addr(sK + cg0 * 4096 + rb * 1024);
+    const uint32_t lds_v = lds_addr(sV + cg0 * 4096 + rb * 1024);
+    const int nt = (it.c1 - it.c0 + 3) / 4;
+    Window w;
+    auto load = [&](const char* head, uint32_t lane_off, int r, uint32_t lds, int t) {
+      const char* src = head + 2 * w.off_of(t);
+      const int key = w.key_of(t);
+      if (key + 16 <= it.end) {
+        load_lds16_at<0>(src, lane_off, lds);
+        if constexpr (NIW > 1) load_lds16_at<64>(src, lane_off, lds + 4096);
+      } else {   // keys that are not there are zeros
+        const bool live = key + r < it.end;
+#pragma unroll
+        for (int u = 0; u < NIW; ++u)
+          load_lds16(live ? (const void*)(src + lane_off + 64 * u) : (const void*)c_zero16, lds + u * 4096);
+      }
+    };
+    auto load_k = [&](int t, int kb) {
+      if (t - w.base >= 64) w.fill(a, it, t - 1, rb, s_keys[wave]);
+      load(kh, koff, krow(lane >> 2), lds_k + kb * TILE_BYTES, t);
+    };
+    auto load_v = [&](int t, int vb) { load(vh, voff, lane >> 2, lds_v + vb * TILE_BYTES, t); };
+    // Scores of tile t past a row's position become -inf.
+    auto mask = [&](f32x16 (&S)[2], int t) {
+      if (w.last_of(t) <= pos_min) return;
+      const int4 keys = *reinterpret_cast<const int4*>(&s_keys[wave][4 * (t - w.base)]);
+      const int lim[4] = {pos8 - keys.x, pos8 - keys.y, pos8 - keys.z, pos8 - keys.w};
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            S[j][8 * h + e] = e > lim[2 * j + h] ? -__builtin_inff() : S[j][8 * h + e];
+    };
+
+    f32x16 O[NCG];
+#pragma unroll
+    for (int dt = 0; dt < NCG; ++dt) O[dt] = f32x16{};
+    float m_ref = -__builtin_inff(), l_run = 0.f;
+    f32x16 S[2] = {f32x16{}, f32x16{}};
+    if (nt > 0) {
+      w.fill(a, it, 0, rb, s_keys[wave]);
+      load_k(0, 0);
+      load_v(0, 0);
+      if (nt > 1) load_k(1, 1);
+      wait_dma();
+      __syncthreads();
+#pragma unroll
+      for (int cc = 0; cc < D / 16; ++cc)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) S[j] = E::mfma32(kfrag(sK, f, j, cc), Qr[cc], S[j]);
+      mask(S, 0);
+      float mx = S[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[j][r]);
+      m_ref = halves_max(mx) * c;   // -inf stays -inf (c > 0)
+      __syncthreads();              // K of tile 0 has been read
+    }
+    float neg_m = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+    bool ref_ok = !__any(m_ref == -__builtin_inff());
+
+    const bool lag = wave >= NW / 2;
+    int vb_cur = 0;
+    bool pending = false;
+    u32x4 P[2][2];
+    constexpr int NQ = D / 8;    // QK MFMAs of a tile: i -> (key half i % 2, cc = i / 2)
+    constexpr int PE = 32 / NQ;  // probabilities per QK MFMA
+    constexpr int NP = D / 8;    // PV MFMAs: i -> (dt = i % NCG, h, j)
+
+    auto block_b = [&](const char* cV) {
+      auto vfr = [&](int i) { return vfrag(cV, f, i / (2 * NCG), (i / NCG) & 1, i % NCG); };
+      u32x4 vf[2] = {vfr(0), vfr(1)};
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        O[i % NCG] = E::mfma32(vf[i & 1], P[i / (2 * NCG)][(i / NCG) & 1], O[i % NCG]);
+        if (i + 2 < NP) vf[i & 1] = vfr(i + 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto probs = [&](const f32x16 (&Sc)[2], float& ls) {
+      ls = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = fast_exp2(fmaf(Sc[j][8 * h + 2 * e], c, neg_m));
+            const float p1 = fast_exp2(fmaf(Sc[j][8 * h + 2 * e + 1], c, neg_m));
+            ls += p0 + p1;
+            P[j][h][e] = E::pack2f(p0, p1);
+          }
+    };
+    // Rare: a row without a reference yet, or probabilities past REFIT_SUM.
+    auto raise = [&](const f32x16 (&Sc)[2], float& ls) {
+      float mx = Sc[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, Sc[j][r]);
+      const float m_new = fmaxf(m_ref, halves_max(mx) * c);
+      const float alpha = m_ref == -__builtin_inff() ? 1.f : fast_exp2(m_ref - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NCG; ++dt) O[dt] *= alpha;
+      m_ref = m_new;
+      neg_m = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+      ref_ok = !__any(m_ref == -__builtin_inff());
+      probs(Sc, ls);
+    };
+
+    // One step on tile t, whose scores are in Sc and whose K is in buffer KB; fills Sx with the next tile's.
+    auto step = [&](auto kb_tag, int t, f32x16 (&Sc)[2], f32x16 (&Sx)[2]) {
+      constexpr int kb_cur = decltype(kb_tag)::value;
+      const int vb_prev = vb_cur == 0 ? NBV - 1 : vb_cur - 1;
+      const int vb_nxt = vb_cur == NBV - 1 ? 0 : vb_cur + 1;
+      if (t + 2 < nt) load_k(t + 2, kb_cur);
+      load_v(t + 1, vb_nxt);
+      if (lag && pending) block_b(sV + vb_prev * TILE_BYTES);
+      const char* cK = sK + (kb_cur ^ 1) * TILE_BYTES;
+      auto kfr = [&](int i) { return kfrag(cK, f, i & 1, i >> 1); };
+      u32x4 kf[3] = {kfr(0), kfr(1), kfr(2)};
+      Sx[0] = f32x16{};
+      Sx[1] = f32x16{};
+      float ls = 0.f;
+      uint32_t pw[2][2][4];
+      __builtin_amdgcn_s_setprio(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        Sx[i & 1] = E::mfma32(kf[i % 3], Qr[i >> 1], Sx[i & 1]);
+        if (i + 3 < NQ) kf[i % 3] = kfr(i + 3);
+#pragma unroll
+        for (int u = 0; u < PE; u += 2) {
+          const int x = PE * i + u, j = x >> 4, rr = x & 15;
+          const float p0 = fast_exp2(fmaf(Sc[j][rr], c, neg_m));
+          const float p1 = fast_exp2(fmaf(Sc[j][rr + 1], c, neg_m));
+          ls += p0 + p1;
+          uint32_t pk = E::pack2f(p0, p1);
+          asm volatile("" : "+v"(pk), "+v"(ls));   // computed here, not sunk to its use in block B
+          pw[j][rr >> 3][(rr & 7) >> 1] = pk;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) P[j][h] = u32x4{pw[j][h][0], pw[j][h][1], pw[j][h][2], pw[j][h][3]};
+      if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(Sc, ls);
+      l_run += ls;
+      mask(Sx, t + 1);
+      if (!lag) block_b(sV + vb_cur * TILE_BYTES);
+      pending = true;
+      wait_dma();
+      __syncthreads();
+      vb_cur = vb_nxt;
+    };
+    if (nt > 0) {
+      f32x16 Sn[2];
+      int t = 0;
+      while (t + 2 < nt) {
+        step(std::integral_constant<int, 0>{}, t, S, Sn);
+        step(std::integral_constant<int, 1>{}, t + 1, Sn, S);
+        t += 2;
+      }
+      if (t + 1 < nt) {
+        step(std::integral_constant<int, 0>{}, t, S, Sn);
+        S[0] = Sn[0];
+        S[1] = Sn[1];
+      }
+      // The last tile: no next one, nothing to load.
+      if (lag && pending) block_b(sV + (vb_cur == 0 ? NBV - 1 : vb_cur - 1) * TILE_BYTES);
+      float ls;
+      probs(S, ls);
+      if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(S, ls);
+      l_run += ls;
+      block_b(sV + vb_cur * TILE_BYTES);
+    }
+    __syncthreads();   // the K/V buffers are free
+    const float lt = halves_sum(l_run);
+    if (a.splits > 1) {
+      if (it.row0 + CK_ROWS * wave + l32 < it.row_end) {
+        const int64_t at = ((int64_t)it.split * a.seqs.N + it.tok0 + token) * a.Hq + it.kvh * a.G + row - token * a.G;
+#pragma unroll
+        for (int dt = 0; dt < NCG; ++dt)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq)
+            *reinterpret_cast<f32x4*>(a.part_acc + at * D + 32 * dt + 8 * rq + 4 * g) =
+                f32x4{O[dt][4 * rq], O[dt][4 * rq + 1], O[dt][4 * rq + 2], O[dt][4 * rq + 3]};
+        if (g == 0) {
+          a.part_ml[2 * at] = m_ref;
+          a.part_ml[2 * at + 1] = lt;
+        }
+      }
+      return;
+    }
+    // O / l through this wave's 32 x D staging area: 16-byte chunk x of row r at position x ^ (r % (D / 8)); each
+    // store instruction then writes whole rows.
+    constexpr int NCH = D / 8, RPI = 64 / NCH;
+    const float inv = lt > 0.f ? 1.f / lt : 1.f;
+    char* stage = s_kv + wave * STAGE;
+#pragma unroll
+    for (int dt = 0; dt < NCG; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int x = 4 * dt + rq;
+        *reinterpret_cast<u32x2*>(stage + l32 * 2 * D + 16 * (x ^ (l32 & (NCH - 1))) + 8 * g) =
+            u32x2{E::pack2f(O[dt][4 * rq] * inv, O[dt][4 * rq + 1] * inv),
+                  E::pack2f(O[dt][4 * rq + 2] * inv, O[dt][4 * rq + 3] * inv)};
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave reads back what its own lanes wrote
+    const int p = lane % NCH;
+#pragma unroll
+    for (int k = 0; k < CK_ROWS / RPI; ++k) {
+      const int r = RPI * k + lane / NCH;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * 2 * D + 16 * p);
+      const int fr = it.row0 + CK_ROWS * wave + r;
+      if (fr < it.row_end) {
+        const int tk = (int)fast_div((uint32_t)fr, (uint32_t)a.G, a.mul_G);
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(a.o + (int64_t)(it.tok0 + tk) * a.o_st +
+                                                                 (it.kvh * a.G + fr - tk * a.G) * a.o_sh +
+                                                                 8 * (p ^ (r & (NCH - 1)))));
+      }
+    }
+  }
+};
+
 template <bool BF16, int D>
 __global__ __launch_bounds__(256, 1) void chunk_kernel(const ChunkArgs a) {
   Chunk<BF16, D>::run(a);
+}
+template <bool BF16, int D>
+__global__ __launch_bounds__(512, 2) void chunk_wide_kernel(const ChunkArgs a) {
+  ChunkWide<BF16, D>::run(a);
 }
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(const ChunkArgs a) {
@@ -433,8 +785,11 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(const ChunkArgs a) {
 }
 
 template <bool BF16, int D>
-static int launch_chunk(const ChunkArgs& a, int64_t groups, hipStream_t s) {
-  hipLaunchKernelGGL((chunk_kernel<BF16, D>), dim3((unsigned)groups), dim3(256), 0, s, a);
+static int launch_chunk(const ChunkArgs& a, int rows, int64_t groups, hipStream_t s) {
+  if (rows > CK_ROWS)
+    hipLaunchKernelGGL((chunk_wide_kernel<BF16, D>), dim3((unsigned)groups), dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((chunk_kernel<BF16, D>), dim3((unsigned)groups), dim3(256), 0, s, a);
   if (a.splits > 1) {
     const int64_t rows = a.seqs.N * a.Hq, per = 256 / (D / 8);
     hipLaunchKernelGGL((chunk_combine_kernel<BF16, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
@@ -444,10 +799,10 @@ static int launch_chunk(const ChunkArgs& a, int64_t groups, hipStream_t s) {
 }
 
 // Row tiles that any division of N tokens over B sequences may have.
-static int64_t chunk_tiles(int64_t N, int64_t B, int64_t G, bool blocks) {
+static int64_t chunk_tiles(int64_t N, int64_t B, int64_t G, int rows, bool blocks) {
   B = std::min(B, N);
-  if (blocks) return (N / CK_BLOCK + B) * ((CK_BLOCK * G + CK_ROWS - 1) / CK_ROWS);
-  return N * G / CK_ROWS + B;
+  if (blocks) return (N / CK_BLOCK + B) * ((CK_BLOCK * G + rows - 1) / rows);
+  return N * G / rows + B;
 }
 
 static bool bad_ptr(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
@@ -521,15 +876,16 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
   a.mul_splits = div_mul((uint32_t)num_splits);
   a.scale_log2 = sm_scale * 1.44269504088896340736f;
   a.splits = num_splits;
-  const int64_t tiles = chunk_tiles(N, B, a.G, sel != nullptr);
+  const int rows = (int64_t)N * a.G >= 64 * (int64_t)std::min(N, B) ? 8 * CK_ROWS : CK_ROWS;
+  const int64_t tiles = chunk_tiles(N, B, a.G, rows, sel != nullptr);
   const int64_t groups = tiles * Hkv * num_splits;
   if (groups > MAX_WORKGROUPS)
     return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
   a.tiles = (int)tiles;
-  a.tiles_per_block = (int)((CK_BLOCK * (int64_t)a.G + CK_ROWS - 1) / CK_ROWS);
+  a.tiles_per_block = (int)((CK_BLOCK * (int64_t)a.G + rows - 1) / rows);
   a.part_acc = static_cast<float*>(workspace);
   a.part_ml = num_splits > 1 ? a.part_acc + (int64_t)num_splits * N * Hq * D : nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_chunk<true, 128>(a, groups, s) : launch_chunk<true, 64>(a, groups, s);
-  return D == 128 ? launch_chunk<false, 128>(a, groups, s) : launch_chunk<false, 64>(a, groups, s);
+  if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_chunk<true, 128>(a, rows, groups, s) : launch_chunk<true, 64>(a, rows, groups, s);
+  return D == 128 ? launch_chunk<false, 128>(a, rows, groups, s) : launch_chunk<false, 64>(a, rows, groups, s);
 }
