@@ -512,9 +512,13 @@ int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const 
  * pages of block i and KV head g, each at most once, are
  *   sel[i * sel_sr + g * sel_sh + e] for e in [sel_off[i * off_sr + g * off_sh], sel_off[i * off_sr + g * off_sh + 1])
  * (within sel_width entries).  sel_rows >= N / 64 + min(B, N).
- * num_splits (1..64): the key range of each row tile is divided over that many workgroups, whose fp32 partials
- * a second kernel merges; num_splits > 1 needs sa_paged_chunk_workspace_bytes() bytes of workspace, which calls
- * that may run concurrently must not share.
+ * num_splits: how many workgroups share the keys of a row tile, leaving fp32 partials in the workspace that a
+ * second kernel merges.  0: worked out on the device from the lengths, so that the workgroups' key tiles come out
+ * about even, within the workspace given (any size; sa_paged_chunk_workspace_bytes() is enough, none means no
+ * division); 1: one; 2..64: that many for every sequence (at most one per 64 keys), which needs all of those bytes.
+ * max_keys there is the most keys that a row may see: max_blocks * page, or with sel the smaller of that and
+ * sel_width * page.  The workspace is 16-byte aligned, its contents arbitrary; calls that may run concurrently must
+ * not share it.
  */
 int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64_t q_sh,
                         const void* k_pages, const void* v_pages,
@@ -526,7 +530,7 @@ int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64_t q_sh,
                         void* o, int64_t o_st, int64_t o_sh,
                         int N, int B, int Hq, int Hkv, int D, int page, float sm_scale,
                         int num_splits, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t sa_paged_chunk_workspace_bytes(int N, int Hq, int D, int num_splits);
+int64_t sa_paged_chunk_workspace_bytes(int N, int B, int Hq, int Hkv, int D, int max_keys, int num_splits);
 
 /*
  * Lists, for each query, the pages worth attending: for one new token per sequence (cu_seqlens NULL, N == B, list

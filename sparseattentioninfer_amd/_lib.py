@@ -179,7 +179,7 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32, _i32, _f32,
         _i32, _vp, _i64, _vp,
     ]),
-    "sa_paged_chunk_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "sa_paged_chunk_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "sa_paged_block_select": (_i32, [
         _i32,
         _vp, _i64, _i64,

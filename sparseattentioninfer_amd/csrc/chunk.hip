@@ -23,12 +23,19 @@ namespace sa {
 constexpr int CK_ROWS = 32;        // rows of a wave
 constexpr int CK_KT = 64;          // keys of a tile
 constexpr int CK_BLOCK = 64;       // new tokens that share one selection
+constexpr int64_t CK_PART_ROWS = 1 << 17;  // rows of partials (68 MB at head dim 128) that a planned division uses at most
 constexpr int CK_NO_KEY = 0x60000000;  // key position of a chunk that is not there: past every row
 // Largest token stride (elements) of the pools: per-lane offsets within a chunk are 32-bit.
 constexpr int64_t CK_MAX_STRIDE = (int64_t)1 << 24;
 
 // 16 readable zero bytes: what lanes of keys that are not there load, so masked keys add 0 * 0.
 __device__ __attribute__((aligned(16))) const uint32_t c_zero16[4] = {0u, 0u, 0u, 0u};
+
+// Where a sequence's partial results are (splits > 1).
+struct SeqPart {
+  int first, splits, n;
+  int any;           // whether any sequence is split
+};
 
 struct ChunkArgs {
   const elem_t* q;
@@ -50,73 +57,260 @@ struct ChunkArgs {
   elem_t* o;
   int64_t o_st, o_sh;
   int Hq, Hkv, G;
-  uint32_t mul_G, mul_heads, mul_splits;
+  uint32_t mul_G, mul_heads, mul_Hq;
   float scale_log2;
-  int tiles;                       // row tiles of the launch (more than there are: the rest exit)
-  int tiles_per_block;             // with a selection: row tiles of a 64-token block
-  int splits;
-  float* part_acc;                 // splits > 1: [splits, N * Hq, D]
-  float* part_ml;                  // [splits, N * Hq, 2]: row reference (base 2) and row sum
+  int items;                       // (row tile, split) pairs of the launch at most; workgroups past the last exit
+  int tiles_per_block;             // with a selection: wide row tiles of a 64-token block
+  int key_tiles;                   // key tiles that a row may see at most: the table's, or the longest list's
+  int cus;
+  int splits;                      // of every sequence; 0: planned, 1: none
+  // Partial results of sequences whose keys are split: row (split, token, head) of sequence b at part[b].first +
+  // (split * tokens + token) * Hq + head.
+  SeqPart* part;                   // [B], written by the launch's first workgroup
+  float* part_acc;                 // [part_rows, D]
+  float* part_ml;                  // [part_rows, 2]: row reference (base 2) and row sum
+  int64_t part_rows;
 };
+
+// ---- which workgroup does what ----------------------------------------------------------------
+//
+// A sequence of few rows (CK_NARROW or less: one token, a few drafts) is read by narrow items, 32 rows whose keys
+// four waves divide; others by wide items, 256 rows that share every key tile.  Where there are fewer items than
+// CUs, or one sequence is much longer than the rest, each item's keys are divided over `splits` workgroups.  The
+// lengths are device memory, so the launch is as large as any lengths need and every workgroup works out the
+// division for itself, the same in all of them: `limit` key tiles to a workgroup, from the total.
+//
+// A key tile takes a narrow item about as long as a wide one when the chip is full (32 KB at a CU's share of HBM,
+// 1.5 us; 256 rows on its matrix cores, 1.3 us), so tiles are what is balanced, and a workgroup costs CK_START of them
+// besides its own (its first loads, the row tile's partials: 7 to 10 us).
+constexpr float CK_START = 6.f;
+constexpr int CK_NARROW = 64;
+constexpr int CK_WIDE_ROWS = 256;
+
+// Sum over the lanes that differ in bits 3..5 only, in every lane.
+__device__ __forceinline__ float over_eights(float x) {
+  x += dpp<0x128>(x);   // row_ror:8
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return halves_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
+}
+
+struct SeqShape {
+  int n, end;       // new tokens; tokens in all
+  int row;          // packed row of the first new token
+  int tiles;        // row tiles
+  int nt, nt0;      // key tiles of the last row tile; of the first
+};
+
+__device__ __forceinline__ bool is_narrow(const ChunkArgs& a, int n) { return (int64_t)n * a.G <= CK_NARROW; }
+
+__device__ __forceinline__ SeqShape seq_shape(const ChunkArgs& a, int b) {
+  SeqShape s;
+  s.n = a.seqs.rows(b, s.row);
+  s.end = a.seqs.kv_len(b);
+  const int64_t rows = (int64_t)s.n * a.G;
+  if (is_narrow(a, s.n))
+    s.tiles = ((int)rows + CK_ROWS - 1) / CK_ROWS;
+  else
+    s.tiles = a.sel ? (s.n + CK_BLOCK - 1) / CK_BLOCK * a.tiles_per_block : (int)((rows + CK_WIDE_ROWS - 1) / CK_WIDE_ROWS);
+  s.nt = min((s.end + CK_KT - 1) / CK_KT, a.key_tiles);
+  s.nt0 = min((max(s.end - s.n, 0) + CK_KT) / CK_KT, s.nt);
+  return s;
+}
+
+// Workgroups that share a row tile's keys when one takes at most `limit` key tiles.  A wide one leaves 133 KB of
+// partials (as long as 5 tiles take), so it has at least 8 tiles; a narrow one at least one for each wave.
+constexpr int CK_NO_LIMIT = 0x40000000;   // at or past this: no division
+struct SplitRule {
+  int limit;
+  float rcp_wide, rcp_narrow;   // of the key tiles that a wide and that a narrow workgroup may take
+  static __device__ __forceinline__ int most(int limit, int narrow) { return max(limit, narrow ? 4 : 8); }
+  __device__ __forceinline__ explicit SplitRule(int l) {
+    limit = l;
+    rcp_wide = __builtin_amdgcn_rcpf((float)most(l, 0));
+    rcp_narrow = __builtin_amdgcn_rcpf((float)most(l, 1));
+  }
+  __device__ __forceinline__ int splits(int fixed, int narrow, int nt) const {
+    if (limit >= CK_NO_LIMIT) return 1;
+    if (fixed) return max(1, min(fixed, nt));
+    // ceil(nt / m): nt < 2^24, so the rounded product is off by one at most.
+    const int m = most(limit, narrow), x = nt + m - 1;
+    int q = (int)((float)x * (narrow ? rcp_narrow : rcp_wide));
+    q += (q + 1) * m <= x ? 1 : 0;
+    q -= q * m > x ? 1 : 0;
+    return max(1, q);
+  }
+};
+
+// Key tiles that one workgroup takes (a.splits: any number below CK_NO_LIMIT stands for that division).  Every
+// workgroup comes through here before its first load, so the choices are weighed side by side: lane 8 y + x adds up
+// choice x over the sequences y, y + 8, ...  The sums are fp32: exact where they decide between neighbouring choices
+// (below 2^24), and the room for partials is kept with a margin above their rounding; a fixed division, which fills
+// its room exactly, is summed in 64 bits.
+__device__ __forceinline__ int plan_limit(const ChunkArgs& a, const SeqShape& first64) {
+  const int lane = threadIdx.x & 63;
+  if (a.splits) {
+    int64_t x = 0;
+    for (int b = lane; b < a.seqs.B; b += 64) {
+      const SeqShape s = b < 64 ? first64 : seq_shape(a, b);
+      const int k = SplitRule(1).splits(a.splits, is_narrow(a, s.n), s.nt);
+      x += k > 1 ? (int64_t)s.n * k * a.Hq : 0;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x > a.part_rows ? CK_NO_LIMIT : 1;
+  }
+  const float heads = (float)a.Hkv, cus = (float)a.cus;
+  float work = 0.f, longest = 0.f, tiles = 0.f;
+  for (int b0 = 0; b0 < a.seqs.B; b0 += 64)
+    if (b0 + lane < a.seqs.B) {
+      const SeqShape s = b0 ? seq_shape(a, b0 + lane) : first64;
+      work += (float)s.tiles * (float)(s.nt + s.nt0);
+      tiles += (float)s.tiles;
+      longest = fmaxf(longest, (float)s.nt);
+    }
+  work = wave_sum(work) * (0.5f * heads);
+  tiles = wave_sum(tiles);
+  longest = wave_max(longest);
+  const float even = fminf(ceilf(work / cus), (float)(CK_NO_LIMIT / 16));
+  if (longest <= 0.5f * even) return CK_NO_LIMIT;   // there are row tiles enough
+  // Choices: 1/2, 3/4, 1, 5/4, 3/2, 2 and 3 even shares, and no division.
+  const int quarters = (0x0C865432u >> (4 * (lane & 7))) & 15;
+  const SplitRule r(quarters ? max(1, (int)ceilf(even * (float)quarters * 0.25f)) : CK_NO_LIMIT);
+  float groups = 0.f, rows = 0.f;
+  for (int b0 = 0; b0 < a.seqs.B; b0 += 64) {
+    SeqShape s = {};
+    if (b0 + lane < a.seqs.B) s = b0 ? seq_shape(a, b0 + lane) : first64;
+    const int narrow = is_narrow(a, s.n);
+    for (int y = 0; y < min(64, a.seqs.B - b0); y += 8) {
+      const int from = y + (lane >> 3);   // sequences past the last have no tiles
+      const int st = __shfl(s.tiles, from, 64), nt = __shfl(2 * s.nt + narrow, from, 64), n = __shfl(s.n, from, 64);
+      const int k = r.splits(0, nt & 1, nt >> 1);
+      groups += (float)st * (float)k;
+      rows += k > 1 ? (float)n * (float)k : 0.f;
+    }
+  }
+  groups = over_eights(groups) * heads;
+  rows = over_eights(rows) * (float)a.Hq;
+  // The division that ends first among those whose partials fit and which add no more workgroups than there are CUs
+  // (chunk_items: the launch has that many to spare, and idle ones cost time too).  Workgroups in one round end with the longest; in
+  // several, half a workgroup after an even share of all tiles and starts.
+  const float one = fminf((float)max(r.limit, 8), longest) + CK_START;
+  float time = groups <= cus ? one : fmaxf(one, (work + groups * CK_START) / cus + 0.5f * one);
+  if (rows * 1.001f > (float)a.part_rows || groups > tiles * heads + cus) time = __builtin_inff();
+  int limit = CK_NO_LIMIT;
+  float best = __builtin_inff();
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const float t = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(time), x));
+    const int l = __builtin_amdgcn_readlane(r.limit, x);
+    if (t < best) {
+      best = t;
+      limit = l;
+    }
+  }
+  return limit;
+}
 
 // The rows and keys of one work item.
 struct ChunkItem {
-  int b, kvh, split;
+  int b, kvh, split, splits;
+  bool narrow;
   int row0, row_end;               // flattened rows of the sequence
-  int tok0;                        // packed row of the sequence's first new token
+  int n, tok0;                     // its new tokens, and the packed row of the first
   int start;                       // position of its first new token
   int end;                         // its tokens in all
   int pos_max;                     // position of the last row
   int c0, c1;                      // chunks of the item: [c0, c1)
   const int32_t* list;             // selected pages, or NULL
   int list_chunks;
+  int64_t part;                    // first row of the sequence's partials
+
+  // Row of the partials of flattened row r.
+  __device__ __forceinline__ int64_t part_row(const ChunkArgs& a, int token, int head) const {
+    return part + ((int64_t)split * n + token) * a.Hq + head;
+  }
 };
 
-__device__ __forceinline__ int tiles_of(const ChunkArgs& a, int rows, int n) {
-  return a.sel ? (n + CK_BLOCK - 1) / CK_BLOCK * a.tiles_per_block
-               : (int)(((int64_t)n * a.G + rows - 1) / rows);
-}
-
-// Work item of workgroup `id` with tiles of `rows` rows, or false.  Heads go fastest (one XCD's workgroups then
-// read one KV head where there are eight of them), then splits; later tiles, which see more keys, come first.
-__device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int rows, int id, ChunkItem& it) {
-  const uint32_t rest = fast_div((uint32_t)id, (uint32_t)a.Hkv, a.mul_heads);
-  it.kvh = id - (int)rest * a.Hkv;
-  const uint32_t t = fast_div(rest, (uint32_t)a.splits, a.mul_splits);
-  it.split = (int)(rest - t * (uint32_t)a.splits);
-  const int x = a.tiles - 1 - (int)t;
-  int local;
-  auto count = [&](int s) {
-    int r0;
-    return tiles_of(a, rows, a.seqs.rows(s, r0));
-  };
-  if (!find_item(a.seqs.B, x, count, it.b, local)) return false;
-  const int n = a.seqs.rows(it.b, it.tok0);
-  it.end = a.seqs.kv_len(it.b);
-  it.start = it.end - n;
+// Work item of workgroup `id`, or false.  Heads go fastest (one XCD's workgroups then read one KV head where there
+// are eight of them); later row tiles, which see more keys, come first.
+__device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, ChunkItem& it) {
+  const int lane = threadIdx.x & 63;
+  const int t = (int)fast_div((uint32_t)id, (uint32_t)a.Hkv, a.mul_heads);
+  it.kvh = id - t * a.Hkv;
+  SeqShape s64 = {};
+  if (lane < a.seqs.B) s64 = seq_shape(a, lane);
+  const bool split = a.part != nullptr;
+  const SplitRule rule(split ? plan_limit(a, s64) : CK_NO_LIMIT);
+  const bool first = id == 0 && split && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
+  int total = 0;
+  for (int b0 = 0; b0 < a.seqs.B; b0 += 64) {
+    SeqShape s = {};
+    if (b0 + lane < a.seqs.B) s = b0 ? seq_shape(a, b0 + lane) : s64;
+    total += __builtin_amdgcn_readlane(scan_lanes(s.tiles * rule.splits(a.splits, is_narrow(a, s.n), s.nt)), 63);
+  }
+  const int x = total - 1 - t;
+  if (x < 0 && !first) return false;
+  int base = 0, block0 = 0;
+  int part0 = 0;
+  bool found = false;
+  for (int b0 = 0; b0 < a.seqs.B && (first || !found); b0 += 64) {
+    SeqShape s = {};
+    if (b0 + lane < a.seqs.B) s = b0 ? seq_shape(a, b0 + lane) : s64;
+    const int k = rule.splits(a.splits, is_narrow(a, s.n), s.nt);
+    const int c = s.tiles * k, blocks = a.sel ? (s.n + CK_BLOCK - 1) / CK_BLOCK : 0;
+    const int rows = k > 1 ? s.n * k * a.Hq : 0;   // all of them fit 31 bits: part_rows does
+    const int ic = scan_lanes(c), ib = a.sel ? scan_lanes(blocks) : 0, ir = split ? scan_lanes(rows) : 0;
+    if (first && b0 + lane < a.seqs.B) a.part[b0 + lane] = SeqPart{part0 + ir - rows, k, s.n, rule.limit < CK_NO_LIMIT};
+    const uint64_t past = __builtin_amdgcn_ballot_w64(base + ic > x);
+    if (past && !found && x >= 0) {
+      found = true;
+      const int l = __builtin_ctzll(past);
+      auto lane_of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      it.b = b0 + l;
+      it.n = lane_of(s.n);
+      it.tok0 = lane_of(s.row);
+      it.end = lane_of(s.end);
+      it.splits = lane_of(k);
+      const int local = x - base - lane_of(ic - c);
+      const int tile = local / it.splits;
+      it.split = local - tile * it.splits;
+      it.narrow = is_narrow(a, it.n);
+      it.start = it.end - it.n;
+      it.part = part0 + lane_of(ir - rows);
+      it.row0 = tile;   // resolved below
+      block0 += lane_of(ib - blocks);
+    }
+    if (!found) block0 += __builtin_amdgcn_readlane(ib, 63);
+    base += __builtin_amdgcn_readlane(ic, 63);
+    part0 += __builtin_amdgcn_readlane(ir, 63);
+  }
+  if (!found) return false;
+  const int tile = it.row0, rows = it.narrow ? CK_ROWS : CK_WIDE_ROWS;
   it.list = nullptr;
   it.list_chunks = 0;
   if (a.sel) {
-    const int blk = local / a.tiles_per_block, sub = local % a.tiles_per_block;
-    it.row_end = min(n, (blk + 1) * CK_BLOCK) * a.G;
+    const int blk = it.narrow ? 0 : tile / a.tiles_per_block, sub = it.narrow ? tile : tile % a.tiles_per_block;
+    it.row_end = min(it.n, (blk + 1) * CK_BLOCK) * a.G;
     it.row0 = blk * CK_BLOCK * a.G + sub * rows;
     if (it.row0 >= it.row_end) return false;
     it.row_end = min(it.row_end, it.row0 + rows);
-    const int sr = x / a.tiles_per_block;
+    const int sr = block0 + blk;
     if (sr >= a.sel_rows) return false;
     const int32_t* off = a.sel_off + sr * a.off_sr + it.kvh * a.off_sh;
     const int e0 = min(max(off[0], 0), a.sel_width), e1 = min(max(off[1], e0), a.sel_width);
     it.list = a.sel + sr * a.sel_sr + it.kvh * a.sel_sh + e0;
-    it.list_chunks = (e1 - e0) * (a.page / 16);
+    it.list_chunks = a.max_blocks > 0 ? (e1 - e0) * (a.page / 16) : 0;
   } else {
-    it.row0 = local * rows;
-    it.row_end = (int)min((int64_t)n * a.G, (int64_t)it.row0 + rows);
+    it.row0 = tile * rows;
+    it.row_end = (int)min((int64_t)it.n * a.G, (int64_t)it.row0 + rows);
   }
   it.pos_max = it.start + (int)fast_div((uint32_t)(it.row_end - 1), (uint32_t)a.G, a.mul_G);
-  const int chunks = a.sel ? it.list_chunks : it.pos_max < 0 ? 0 : it.pos_max / 16 + 1;
+  // Lengths past the table end with it.
+  const int last = (int)min((int64_t)it.pos_max, (int64_t)a.max_blocks * a.page - 1);
+  const int chunks = a.sel ? it.list_chunks : last < 0 ? 0 : last / 16 + 1;
   const int64_t nt = (chunks + 3) / 4;
-  it.c0 = 4 * (int)(nt * it.split / a.splits);
-  it.c1 = min(chunks, 4 * (int)(nt * (it.split + 1) / a.splits));
+  it.c0 = 4 * (int)(nt * it.split / it.splits);
+  it.c1 = min(chunks, 4 * (int)(nt * (it.split + 1) / it.splits));
   return true;
 }
 
@@ -159,11 +353,12 @@ struct ChunkWindow {
   }
 };
 
+// 32 rows to a workgroup: its first four waves hold the same rows and divide the keys, each with tiles of its own in
+// LDS and no barrier before they merge.  Bound by the keys' bytes: a wave keeps 32 KB of loads in flight.
 template <bool BF16, int D>
-struct Chunk : StagedTile {
+struct ChunkNarrow : StagedTile {
   using E = Elem<BF16>;
-  static constexpr int NW = 4;                     // waves; each has the same rows and keys of its own
-  static constexpr int NT = 64 * NW;
+  static constexpr int NW = 4;
   static constexpr int NCG = D / 32;               // column groups of a staged tile
   static constexpr int NI = 4 * NCG;               // 1 KiB direct loads of a tile
   static constexpr int TILE_BYTES = CK_KT * D * 2;
@@ -205,15 +400,16 @@ struct Chunk : StagedTile {
     }
   }
 
-  static __device__ void run(const ChunkArgs& a) {
-    __shared__ __attribute__((aligned(16))) char s_kv[LDS_BYTES];
-    __shared__ float s_ml[NW * 2 * CK_ROWS];
+  // s_ml: 2 * CK_ROWS floats a wave.
+  static __device__ void run(const ChunkArgs& a, const ChunkItem& it, char* s_kv, float* s_ml) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 5, l32 = lane & 31;
-    ChunkItem it;
-    if (!find_chunk_item(a, CK_ROWS, blockIdx.x, it)) return;
-
+    if (wave >= NW) {   // the barriers of the merge below
+      __syncthreads();
+      __syncthreads();
+      return;
+    }
     const int row = min(it.row0 + l32, it.row_end - 1);
     const int token = (int)fast_div((uint32_t)row, (uint32_t)a.G, a.mul_G);
     const int pos = it.start + token;
@@ -377,8 +573,8 @@ struct Chunk : StagedTile {
       if (it.row0 + r < it.row_end) {
         const int tk = (int)fast_div((uint32_t)(it.row0 + r), (uint32_t)a.G, a.mul_G);
         const int h = it.kvh * a.G + it.row0 + r - tk * a.G;
-        if (a.splits > 1) {
-          const int64_t at = ((int64_t)it.split * a.seqs.N + it.tok0 + tk) * a.Hq + h;
+        if (it.splits > 1) {
+          const int64_t at = it.part_row(a, tk, h);
           f32x4* d = reinterpret_cast<f32x4*>(a.part_acc + at * D + 8 * oc);
           d[0] = lo;
           d[1] = hi;
@@ -395,105 +591,90 @@ struct Chunk : StagedTile {
       }
     }
   }
-
-  // Merges the splits of one (token, head): D / 8 lanes a row.
-  static __device__ void combine(const ChunkArgs& a) {
-    constexpr int LPR = D / 8;
-    const int64_t row = ((int64_t)blockIdx.x * NT + threadIdx.x) / LPR;
-    const int oc = threadIdx.x % LPR;
-    const int64_t n = row / a.Hq;
-    if (n < a.seqs.cu[0] || n >= a.seqs.N || n >= a.seqs.cu[a.seqs.B]) return;  // not of any sequence
-    const int64_t rows = a.seqs.N * a.Hq;
-    float M = -__builtin_inff(), L = 0.f;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * rows + row)]);
-    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-    if (M != -__builtin_inff())
-      for (int s = 0; s < a.splits; ++s) {
-        const float m = a.part_ml[2 * (s * rows + row)], l = a.part_ml[2 * (s * rows + row) + 1];
-        if (m == -__builtin_inff()) continue;  // this split saw no key of the row
-        const float fs = fast_exp2(m - M);
-        const f32x4* p = reinterpret_cast<const f32x4*>(a.part_acc + (s * rows + row) * D + 8 * oc);
-        L += fs * l;
-        lo += fs * p[0];
-        hi += fs * p[1];
-      }
-    const float inv = L > 0.f ? 1.f / L : 1.f;
-    *reinterpret_cast<u32x4*>(a.o + n * a.o_st + (row - n * a.Hq) * a.o_sh + 8 * oc) =
-        u32x4{E::pack2f(lo[0] * inv, lo[1] * inv), E::pack2f(lo[2] * inv, lo[3] * inv),
-              E::pack2f(hi[0] * inv, hi[1] * inv), E::pack2f(hi[2] * inv, hi[3] * inv)};
-  }
 };
 
 // 256 rows to a workgroup: eight waves of 32 rows share every K/V tile, which direct loads bring into LDS while the
 // tile before is worked on.  One step per tile and one barrier per step.  Block A of a step runs S^T = K Q^T of the
 // next tile on the matrix cores under the exponentials of this one, block B O^T += V^T P^T.  Waves 0..3 run A(i),
 // B(i) in step i and waves 4..7, one on each SIMD beside them, B(i - 1), A(i), so that the two waves of a SIMD run the
-// vector-heavy A and the matrix-only B at the same time.  K is double- and V triple-buffered for that.
+// vector-heavy A and the matrix-only B at the same time.  Step i issues the loads of K(i + 3) and V(i + 2) and ends
+// with a wait for those of the step before, so a tile has two steps to arrive; the waves read K(i + 1), V(i) and
+// V(i - 1) meanwhile, hence three K and four V buffers.
 // A row's reference is the maximum of its first tile and is raised only when its probabilities would pass the
 // element type's range (Chunk::REFIT_SUM), so the common step never touches O with vector instructions.
 template <bool BF16, int D>
 struct ChunkWide : StagedTile {
   using E = Elem<BF16>;
   static constexpr int NW = 8;
-  static constexpr int NT = 64 * NW;
-  static constexpr int ROWS = NW * CK_ROWS;
+  static_assert(NW * CK_ROWS == CK_WIDE_ROWS, "rows of a wide item");
   static constexpr int NCG = D / 32;
   static constexpr int NIW = 4 * NCG / NW;         // direct loads of a tile per wave: one row block each
   static constexpr int TILE_BYTES = CK_KT * D * 2;
-  static constexpr int NBK = 2, NBV = 3;
+  static constexpr int NBK = 3, NBV = 4;
   static constexpr int STAGE = CK_ROWS * D * 2;    // a wave's share of O
-  static_assert(NW * STAGE <= (NBK + NBV) * TILE_BYTES, "O is staged in the K/V buffers");
+  static constexpr int LDS_BYTES = (NBK + NBV) * TILE_BYTES;
+  static constexpr int KEYS = NW * 4 * 64;         // ints of LDS for the tiles' first keys
+  static_assert(NW * STAGE <= LDS_BYTES, "O is staged in the K/V buffers");
   static constexpr float REFIT_SUM = BF16 ? 65536.f : 32768.f;
 
   // 64 tiles looked up at once: lane i holds, for tile base + i, the place and first key of the chunk that this
   // wave loads, and the tile's largest key; the first keys of its four chunks go to LDS, for the tiles that need
-  // a mask.  Tiles are loaded up to two ahead of the one whose mask is due, so a window starts one tile back.
+  // a mask.  Tiles are loaded two ahead of the one whose mask is due, so a window starts two tiles back.
   struct Window {
     int base;
     int64_t off;
     int key, last;
 
-    static __device__ __forceinline__ int32_t now(const int32_t* p) {
-      int32_t x;
+    // Four 32-bit reads that have completed when it returns: one opaque block, so that the compiler has no pending
+    // load whose wait would cover the direct loads in the tile loop.
+    static __device__ __forceinline__ void read4(const int32_t* const (&p)[4], int (&x)[4]) {
       asm volatile(
-          "global_load_dword %0, %1, off\n\t"
+          "global_load_dword %0, %4, off\n\t"
+          "global_load_dword %1, %5, off\n\t"
+          "global_load_dword %2, %6, off\n\t"
+          "global_load_dword %3, %7, off\n\t"
           "s_waitcnt vmcnt(0)"
-          : "=v"(x)
-          : "v"(p)
+          : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+          : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3])
           : "memory");
-      return x;
     }
     __device__ __forceinline__ void fill(const ChunkArgs& a, const ChunkItem& it, int first, int rb, int* s_keys) {
       base = first;
-      key = CK_NO_KEY;
-      off = 0;
-      last = -1;
       const int lane = threadIdx.x & 63;
-      int keys[4];
+      int lb[4], slot[4], page[4], keys[4];
+      const int32_t* p[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int c = it.c0 + 4 * (first + lane) + x;
-        keys[x] = CK_NO_KEY;
-        if (c < it.c1) {
-          int lb, slot;
-          if (it.list) {
-            const int e = (int)fast_div((uint32_t)c, (uint32_t)(a.page / 16), a.mul_ppc);
-            lb = now(it.list + e);
-            slot = (c - e * (a.page / 16)) * 16;
-          } else {
-            lb = (int)fast_div((uint32_t)(16 * c), (uint32_t)a.page, a.mul_page);
-            slot = 16 * c - lb * a.page;
-          }
-          if (lb >= 0 && lb < a.max_blocks && (int64_t)lb * a.page + slot <= it.pos_max) {
-            const int pg = now(a.table + it.b * a.table_stride + lb);
-            if (pg >= 0 && pg < a.num_pages) {
-              keys[x] = lb * a.page + slot;
-              if (x == rb) {
-                off = (int64_t)pg * a.kv_sp + (int64_t)slot * a.kv_st;
-                key = keys[x];
-              }
-            }
-          }
+        keys[x] = c < it.c1 ? 0 : CK_NO_KEY;
+        if (it.list) {
+          const int e = (int)fast_div((uint32_t)c, (uint32_t)(a.page / 16), a.mul_ppc);
+          p[x] = it.list + (c < it.c1 ? e : 0);   // there is an entry: the item has a chunk
+          slot[x] = (c - e * (a.page / 16)) * 16;
+        } else {
+          lb[x] = (int)fast_div((uint32_t)(16 * c), (uint32_t)a.page, a.mul_page);
+          slot[x] = 16 * c - lb[x] * a.page;
+        }
+      }
+      if (it.list) read4(p, lb);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        // (a page whose first key no row sees is not looked up; neither are ids that are no column)
+        if (lb[x] < 0 || lb[x] >= a.max_blocks || (int64_t)lb[x] * a.page + slot[x] > it.pos_max) keys[x] = CK_NO_KEY;
+        p[x] = a.table + it.b * a.table_stride + (keys[x] ? 0 : lb[x]);
+      }
+      read4(p, page);
+      key = CK_NO_KEY;
+      off = 0;
+      last = -1;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (page[x] < 0 || page[x] >= a.num_pages) keys[x] = CK_NO_KEY;
+        if (!keys[x]) keys[x] = lb[x] * a.page + slot[x];
+        else keys[x] = CK_NO_KEY;
+        if (x == rb && keys[x] != CK_NO_KEY) {
+          off = (int64_t)page[x] * a.kv_sp + (int64_t)slot[x] * a.kv_st;
+          key = keys[x];
         }
         last = max(last, keys[x] + 15);
       }
@@ -508,14 +689,11 @@ struct ChunkWide : StagedTile {
     }
   };
 
-  static __device__ void run(const ChunkArgs& a) {
-    __shared__ __attribute__((aligned(16))) char s_kv[(NBK + NBV) * TILE_BYTES];
-    __shared__ __attribute__((aligned(16))) int s_keys[NW][4 * 64];
+  static __device__ void run(const ChunkArgs& a, const ChunkItem& it, char* s_kv, int* s_all_keys) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 5, l32 = lane & 31;
-    ChunkItem it;
-    if (!find_chunk_item(a, ROWS, blockIdx.x, it)) return;
+    int* s_keys = s_all_keys + 4 * 64 * wave;
     char* sK = s_kv;
     char* sV = s_kv + NBK * TILE_BYTES;
 
@@ -557,14 +735,14 @@ struct ChunkWide : StagedTile {
       }
     };
     auto load_k = [&](int t, int kb) {
-      if (t - w.base >= 64) w.fill(a, it, t - 1, rb, s_keys[wave]);
+      if (t - w.base >= 64) w.fill(a, it, t - 2, rb, s_keys);
       load(kh, koff, krow(lane >> 2), lds_k + kb * TILE_BYTES, t);
     };
     auto load_v = [&](int t, int vb) { load(vh, voff, lane >> 2, lds_v + vb * TILE_BYTES, t); };
     // Scores of tile t past a row's position become -inf.
     auto mask = [&](f32x16 (&S)[2], int t) {
       if (w.last_of(t) <= pos_min) return;
-      const int4 keys = *reinterpret_cast<const int4*>(&s_keys[wave][4 * (t - w.base)]);
+      const int4 keys = *reinterpret_cast<const int4*>(&s_keys[4 * (t - w.base)]);
       const int lim[4] = {pos8 - keys.x, pos8 - keys.y, pos8 - keys.z, pos8 - keys.w};
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -581,10 +759,14 @@ struct ChunkWide : StagedTile {
     float m_ref = -__builtin_inff(), l_run = 0.f;
     f32x16 S[2] = {f32x16{}, f32x16{}};
     if (nt > 0) {
-      w.fill(a, it, 0, rb, s_keys[wave]);
+      w.fill(a, it, 0, rb, s_keys);
       load_k(0, 0);
       load_v(0, 0);
-      if (nt > 1) load_k(1, 1);
+      if (nt > 1) {
+        load_k(1, 1);
+        load_v(1, 1);
+      }
+      if (nt > 2) load_k(2, 2);
       wait_dma();
       __syncthreads();
 #pragma unroll
@@ -604,8 +786,9 @@ struct ChunkWide : StagedTile {
     bool ref_ok = !__any(m_ref == -__builtin_inff());
 
     const bool lag = wave >= NW / 2;
-    int vb_cur = 0;
+    int vb_cur = 0, kb_cur = 0;   // buffers of the current tile
     bool pending = false;
+    auto ring = [](int x, int n) { return x >= n ? x - n : x; };
     u32x4 P[2][2];
     constexpr int NQ = D / 8;    // QK MFMAs of a tile: i -> (key half i % 2, cc = i / 2)
     constexpr int PE = 32 / NQ;  // probabilities per QK MFMA
@@ -655,15 +838,13 @@ struct ChunkWide : StagedTile {
       probs(Sc, ls);
     };
 
-    // One step on tile t, whose scores are in Sc and whose K is in buffer KB; fills Sx with the next tile's.
-    auto step = [&](auto kb_tag, int t, f32x16 (&Sc)[2], f32x16 (&Sx)[2]) {
-      constexpr int kb_cur = decltype(kb_tag)::value;
-      const int vb_prev = vb_cur == 0 ? NBV - 1 : vb_cur - 1;
-      const int vb_nxt = vb_cur == NBV - 1 ? 0 : vb_cur + 1;
-      if (t + 2 < nt) load_k(t + 2, kb_cur);
-      load_v(t + 1, vb_nxt);
-      if (lag && pending) block_b(sV + vb_prev * TILE_BYTES);
-      const char* cK = sK + (kb_cur ^ 1) * TILE_BYTES;
+    // One step on tile t, whose scores are in Sc; fills Sx with the next tile's.
+    auto step = [&](int t, f32x16 (&Sc)[2], f32x16 (&Sx)[2]) {
+      const bool ahead = t + 3 < nt;
+      if (ahead) load_k(t + 3, kb_cur);
+      if (t + 2 < nt) load_v(t + 2, ring(vb_cur + 2, NBV));
+      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES);
+      const char* cK = sK + ring(kb_cur + 1, NBK) * TILE_BYTES;
       auto kfr = [&](int i) { return kfrag(cK, f, i & 1, i >> 1); };
       u32x4 kf[3] = {kfr(0), kfr(1), kfr(2)};
       Sx[0] = f32x16{};
@@ -697,25 +878,29 @@ struct ChunkWide : StagedTile {
       mask(Sx, t + 1);
       if (!lag) block_b(sV + vb_cur * TILE_BYTES);
       pending = true;
-      wait_dma();
+      if (ahead)
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * NIW));   // vmcnt: this step's loads may be in flight
+      else
+        wait_dma();
       __syncthreads();
-      vb_cur = vb_nxt;
+      vb_cur = ring(vb_cur + 1, NBV);
+      kb_cur = ring(kb_cur + 1, NBK);
     };
     if (nt > 0) {
       f32x16 Sn[2];
       int t = 0;
       while (t + 2 < nt) {
-        step(std::integral_constant<int, 0>{}, t, S, Sn);
-        step(std::integral_constant<int, 1>{}, t + 1, Sn, S);
+        step(t, S, Sn);
+        step(t + 1, Sn, S);
         t += 2;
       }
       if (t + 1 < nt) {
-        step(std::integral_constant<int, 0>{}, t, S, Sn);
+        step(t, S, Sn);
         S[0] = Sn[0];
         S[1] = Sn[1];
       }
       // The last tile: no next one, nothing to load.
-      if (lag && pending) block_b(sV + (vb_cur == 0 ? NBV - 1 : vb_cur - 1) * TILE_BYTES);
+      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES);
       float ls;
       probs(S, ls);
       if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(S, ls);
@@ -724,9 +909,9 @@ struct ChunkWide : StagedTile {
     }
     __syncthreads();   // the K/V buffers are free
     const float lt = halves_sum(l_run);
-    if (a.splits > 1) {
+    if (it.splits > 1) {
       if (it.row0 + CK_ROWS * wave + l32 < it.row_end) {
-        const int64_t at = ((int64_t)it.split * a.seqs.N + it.tok0 + token) * a.Hq + it.kvh * a.G + row - token * a.G;
+        const int64_t at = it.part_row(a, token, it.kvh * a.G + row - token * a.G);
 #pragma unroll
         for (int dt = 0; dt < NCG; ++dt)
 #pragma unroll
@@ -772,38 +957,135 @@ struct ChunkWide : StagedTile {
 };
 
 template <bool BF16, int D>
-__global__ __launch_bounds__(256, 1) void chunk_kernel(const ChunkArgs a) {
-  Chunk<BF16, D>::run(a);
+__global__ __launch_bounds__(512, 2) void chunk_kernel(const ChunkArgs a) {
+  using W = ChunkWide<BF16, D>;
+  using S = ChunkNarrow<BF16, D>;
+  __shared__ __attribute__((aligned(16))) char s_kv[W::LDS_BYTES > S::LDS_BYTES ? W::LDS_BYTES : S::LDS_BYTES];
+  __shared__ __attribute__((aligned(16))) int s_aux[W::KEYS];
+  ChunkItem it;
+  if (!find_chunk_item(a, blockIdx.x, it)) return;
+  if (it.narrow)
+    S::run(a, it, s_kv, reinterpret_cast<float*>(s_aux));
+  else
+    W::run(a, it, s_kv, s_aux);
 }
-template <bool BF16, int D>
-__global__ __launch_bounds__(512, 2) void chunk_wide_kernel(const ChunkArgs a) {
-  ChunkWide<BF16, D>::run(a);
-}
+
+// Merges the partials of the rows (token, head), D / 8 lanes a row, after the workgroups of the launch before have left
+// them; rows of sequences that were not split are done.  Each lane of a wave holds one sequence's range of
+// rows and place, so a row finds its own without a chain of reads.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(const ChunkArgs a) {
-  Chunk<BF16, D>::combine(a);
+  using E = Elem<BF16>;
+  constexpr int LPR = D / 8, U = 4;
+  const int lane = threadIdx.x & 63, oc = threadIdx.x % LPR;
+  const int64_t rows = a.seqs.N * a.Hq;
+  for (int b0 = 0; b0 < a.seqs.B; b0 += 64) {
+    SeqPart sp = {0, 1, 0, 0};
+    int r0 = 0, n_of = 0;
+    if (b0 + lane < a.seqs.B) {
+      sp = a.part[b0 + lane];
+      n_of = a.seqs.rows(b0 + lane, r0);
+    }
+    if (!__any(sp.any != 0)) return;
+    if (sp.n != n_of) sp.splits = 1;   // lengths that changed under the launch
+    const uint64_t split = __builtin_amdgcn_ballot_w64(sp.splits > 1 && n_of > 0);
+    for (int64_t w0 = ((int64_t)blockIdx.x * 256 + threadIdx.x - lane) / LPR; w0 < rows && split;
+         w0 += (int64_t)gridDim.x * (256 / LPR)) {
+      const int64_t row = w0 + lane / LPR;
+      const int n = row < rows ? (int)fast_div((uint32_t)row, (uint32_t)a.Hq, a.mul_Hq) : -1;
+      int first = 0, k = 0, tokens = 0, at0 = 0;
+      for (uint64_t m = split; m; m &= m - 1) {
+        const int l = __builtin_ctzll(m);
+        const int s0 = __builtin_amdgcn_readlane(r0, l), sn = __builtin_amdgcn_readlane(n_of, l);
+        if (n >= s0 && n < s0 + sn) {
+          first = __builtin_amdgcn_readlane(sp.first, l);
+          k = __builtin_amdgcn_readlane(sp.splits, l);
+          tokens = sn;
+          at0 = s0;
+        }
+      }
+      if (k <= 1) continue;
+      const int h = (int)(row - (int64_t)n * a.Hq);
+      const int64_t step = (int64_t)tokens * a.Hq, at = first + (int64_t)(n - at0) * a.Hq + h;
+      float M = -__builtin_inff(), L = 0.f;
+      f32x4 acc[2] = {f32x4{}, f32x4{}};
+      for (int s0 = 0; s0 < k; s0 += U) {
+        float m[U], l[U];
+        f32x4 v[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t p = at + min(s0 + u, k - 1) * step;   // past the last: a repeat, not used
+          m[u] = a.part_ml[2 * p];
+          l[u] = a.part_ml[2 * p + 1];
+          v[u][0] = reinterpret_cast<const f32x4*>(a.part_acc + p * D + 8 * oc)[0];
+          v[u][1] = reinterpret_cast<const f32x4*>(a.part_acc + p * D + 8 * oc)[1];
+        }
+        float Mc = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (s0 + u < k) Mc = fmaxf(Mc, m[u]);
+        if (Mc == -__builtin_inff()) continue;   // no key of the row yet
+        const float f0 = fast_exp2(M - Mc);
+        L *= f0;
+        acc[0] *= f0;
+        acc[1] *= f0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (s0 + u < k && m[u] != -__builtin_inff()) {
+            const float fs = fast_exp2(m[u] - Mc);
+            L += fs * l[u];
+            acc[0] += fs * v[u][0];
+            acc[1] += fs * v[u][1];
+          }
+        M = Mc;
+      }
+      const float inv = L > 0.f ? 1.f / L : 1.f;
+      *reinterpret_cast<u32x4*>(a.o + (int64_t)n * a.o_st + h * a.o_sh + 8 * oc) =
+          u32x4{E::pack2f(acc[0][0] * inv, acc[0][1] * inv), E::pack2f(acc[0][2] * inv, acc[0][3] * inv),
+                E::pack2f(acc[1][0] * inv, acc[1][1] * inv), E::pack2f(acc[1][2] * inv, acc[1][3] * inv)};
+    }
+  }
 }
 
 template <bool BF16, int D>
-static int launch_chunk(const ChunkArgs& a, int rows, int64_t groups, hipStream_t s) {
-  if (rows > CK_ROWS)
-    hipLaunchKernelGGL((chunk_wide_kernel<BF16, D>), dim3((unsigned)groups), dim3(512), 0, s, a);
-  else
-    hipLaunchKernelGGL((chunk_kernel<BF16, D>), dim3((unsigned)groups), dim3(256), 0, s, a);
-  if (a.splits > 1) {
+static int launch_chunk(const ChunkArgs& a, int64_t groups, hipStream_t s) {
+  hipLaunchKernelGGL((chunk_kernel<BF16, D>), dim3((unsigned)groups), dim3(512), 0, s, a);
+  if (a.part) {
     const int64_t rows = a.seqs.N * a.Hq, per = 256 / (D / 8);
-    hipLaunchKernelGGL((chunk_combine_kernel<BF16, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((chunk_combine_kernel<BF16, D>), dim3((unsigned)std::min<int64_t>((rows + per - 1) / per, 2048)), dim3(256), 0, s, a);
   }
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "sa_paged_chunk_attn: launch failed: %s", hipGetErrorString(err));
 }
 
-// Row tiles that any division of N tokens over B sequences may have.
-static int64_t chunk_tiles(int64_t N, int64_t B, int64_t G, int rows, bool blocks) {
-  B = std::min(B, N);
-  if (blocks) return (N / CK_BLOCK + B) * ((CK_BLOCK * G + rows - 1) / rows);
-  return N * G / rows + B;
+static int chunk_cus() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (!cached[dev]) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+    cached[dev] = n;
+  }
+  return cached[dev];
 }
+
+// Row tiles that any division of N tokens over B sequences may have: a narrow sequence has at most two, a wide one
+// its rows over 256 rounded up (or, with a selection, those of its blocks).
+static int64_t chunk_tiles(int64_t N, int64_t B, int64_t G, bool blocks) {
+  B = std::min(B, N);
+  const int64_t per_block = (CK_BLOCK * G + CK_WIDE_ROWS - 1) / CK_WIDE_ROWS;
+  if (blocks) return (N / CK_BLOCK + B) * std::max<int64_t>(per_block, CK_NARROW / CK_ROWS);
+  return N * G / CK_WIDE_ROWS + std::min(B * (CK_NARROW / CK_ROWS), N * G / CK_ROWS + B);
+}
+
+// Row tiles and splits: a planned division has at most a workgroup per CU more than the row tiles need.
+static int64_t chunk_items(int64_t N, int64_t B, int64_t G, int64_t Hkv, bool blocks, int splits) {
+  const int64_t tiles = chunk_tiles(N, B, G, blocks);
+  return splits ? tiles * splits : tiles + chunk_cus() / Hkv;
+}
+
+static int64_t chunk_part_header(int64_t B) { return (B * (int64_t)sizeof(SeqPart) + 255) / 256 * 256; }
 
 static bool bad_ptr(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 
@@ -811,9 +1093,14 @@ static bool bad_ptr(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15;
 
 using namespace sa;
 
-extern "C" int64_t sa_paged_chunk_workspace_bytes(int N, int Hq, int D, int num_splits) {
-  if (N < 1 || Hq < 1 || D < 1 || num_splits <= 1) return 0;
-  return (int64_t)num_splits * N * Hq * (D + 2) * 4;
+extern "C" int64_t sa_paged_chunk_workspace_bytes(int N, int B, int Hq, int Hkv, int D, int max_keys, int num_splits) {
+  if (N < 1 || B < 1 || Hkv < 1 || Hq < Hkv || D < 1 || max_keys < 1 || num_splits == 1 || num_splits < 0) return 0;
+  const int64_t key_tiles = (max_keys + CK_KT - 1) / CK_KT;
+  const int64_t all = (int64_t)N * Hq;
+  if (num_splits > 1) return chunk_part_header(B) + all * std::min<int64_t>(num_splits, key_tiles) * (D + 2) * 4;
+  // Nothing is gained where the row tiles fill the chip several times over.
+  if (key_tiles <= 4 || (int64_t)N * (Hq / Hkv) / CK_WIDE_ROWS * Hkv >= 8 * (int64_t)chunk_cus()) return 0;
+  return chunk_part_header(B) + std::min(all * std::min<int64_t>(key_tiles / 4 + 1, 64), CK_PART_ROWS) * (D + 2) * 4;
 }
 
 extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k_pages,
@@ -832,9 +1119,9 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
   if (page < 16 || page > 128 || page % 16)
     return set_error(SA_E_BLOCK, "%s: page %d is not a multiple of 16 in [16, 128]", name, page);
   if (N < 0 || B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > (1 << 15) || max_blocks < 0 || num_pages < 0 ||
-      block_table_stride < max_blocks || num_splits < 1 || num_splits > 64)
+      block_table_stride < max_blocks || num_splits < 0 || num_splits > 64)
     return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages, "
-                     "%d splits (1..64)", name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages,
+                     "%d splits (0..64)", name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages,
                      num_splits);
   if (!(sm_scale > 0.f) || sm_scale > 1e30f) return set_error(SA_E_SHAPE, "%s: scale %g is not positive", name, sm_scale);
   if ((int64_t)N * Hq > 0x7fffffff) return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d rows are too many", name, N, Hq);
@@ -849,9 +1136,13 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
     return set_error(SA_E_ALIGN, "%s: head rows must be 16-byte aligned", name);
   if (pages_st < 0 || pages_st > CK_MAX_STRIDE)
     return set_error(SA_E_SHAPE, "%s: token stride %lld of the pools", name, (long long)pages_st);
-  if (num_splits > 1 && (!workspace || workspace_bytes < sa_paged_chunk_workspace_bytes(N, Hq, D, num_splits)))
+  if (num_splits > 1 && (int64_t)N * Hq * num_splits > 0x7fffffff)
+    return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d x %d splits are too many partial rows", name, N, Hq, num_splits);
+  const int64_t max_keys = std::min<int64_t>((int64_t)(sel ? std::min(max_blocks, sel_width) : max_blocks) * page, 1 << 30);
+  const int64_t need = sa_paged_chunk_workspace_bytes(N, B, Hq, Hkv, D, (int)max_keys, num_splits);
+  if (num_splits > 1 && need && (!workspace || workspace_bytes < need))
     return set_error(SA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", name, (long long)workspace_bytes,
-                     (long long)sa_paged_chunk_workspace_bytes(N, Hq, D, num_splits));
+                     (long long)need);
   ChunkArgs a = {};
   a.q = static_cast<const elem_t*>(q);
   a.q_st = q_st, a.q_sh = q_sh;
@@ -873,19 +1164,25 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
   a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
   a.mul_G = div_mul((uint32_t)a.G);
   a.mul_heads = div_mul((uint32_t)Hkv);
-  a.mul_splits = div_mul((uint32_t)num_splits);
+  a.mul_Hq = div_mul((uint32_t)Hq);
   a.scale_log2 = sm_scale * 1.44269504088896340736f;
-  a.splits = num_splits;
-  const int rows = (int64_t)N * a.G >= 64 * (int64_t)std::min(N, B) ? 8 * CK_ROWS : CK_ROWS;
-  const int64_t tiles = chunk_tiles(N, B, a.G, rows, sel != nullptr);
-  const int64_t groups = tiles * Hkv * num_splits;
-  if (groups > MAX_WORKGROUPS)
+  a.tiles_per_block = (int)((CK_BLOCK * (int64_t)a.G + CK_WIDE_ROWS - 1) / CK_WIDE_ROWS);
+  a.key_tiles = (int)((max_keys + CK_KT - 1) / CK_KT);
+  a.cus = chunk_cus();
+  // Without room for partials nothing is split.
+  const int64_t room = std::min<int64_t>((workspace_bytes - chunk_part_header(B)) / ((int64_t)(D + 2) * 4), 0x7fffffff);
+  a.splits = need && workspace && room > 0 ? num_splits : 1;
+  if (a.splits != 1) {
+    a.part = static_cast<SeqPart*>(workspace);
+    a.part_rows = room;
+    a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + chunk_part_header(B));
+    a.part_ml = a.part_acc + room * D;
+  }
+  const int64_t items = chunk_items(N, B, a.G, Hkv, sel != nullptr, a.splits), groups = items * Hkv;
+  if (groups > MAX_WORKGROUPS / 2)
     return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
-  a.tiles = (int)tiles;
-  a.tiles_per_block = (int)((CK_BLOCK * (int64_t)a.G + rows - 1) / rows);
-  a.part_acc = static_cast<float*>(workspace);
-  a.part_ml = num_splits > 1 ? a.part_acc + (int64_t)num_splits * N * Hq * D : nullptr;
+  a.items = (int)items;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_chunk<true, 128>(a, rows, groups, s) : launch_chunk<true, 64>(a, rows, groups, s);
-  return D == 128 ? launch_chunk<false, 128>(a, rows, groups, s) : launch_chunk<false, 64>(a, rows, groups, s);
+  if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_chunk<true, 128>(a, groups, s) : launch_chunk<true, 64>(a, groups, s);
+  return D == 128 ? launch_chunk<false, 128>(a, groups, s) : launch_chunk<false, 64>(a, groups, s);
 }

@@ -31,6 +31,18 @@ struct Ragged {
 
 __device__ __forceinline__ int floor_div(int a, int d) { return a >= 0 ? a / d : -((d - 1 - a) / d); }
 
+// Sum of x over this lane and those before it, without LDS: four shifts within rows of 16 lanes, then the last
+// lane of a row to the next and of the lower half to the upper.
+__device__ __forceinline__ int scan_lanes(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
 // Sequence b and index `local` within it of item x, where sequence b has count(b) items.  Called by whole
 // waves; 64 sequences are counted at a time.  False if x is past the last item.
 template <class Count>
@@ -39,12 +51,7 @@ __device__ __forceinline__ bool find_item(int B, int x, Count count, int& b, int
   int base = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     const int c = b0 + lane < B ? count(b0 + lane) : 0;
-    int incl = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(incl, o, 64);
-      incl += lane >= o ? up : 0;
-    }
+    const int incl = scan_lanes(c);
     const uint64_t past = __builtin_amdgcn_ballot_w64(base + incl > x);
     if (past) {
       const int l = __builtin_ctzll(past);

@@ -961,12 +961,6 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     return q_out
 
 
-def paged_chunk_splits(N: int, B: int, Hq: int, Hkv: int, max_kv: int) -> int:
-    """Workgroups that share a row tile's keys in :func:`paged_chunk_attn` by default."""
-    tiles = max(1, min(N * (Hq // Hkv) // 32 + min(B, N), N)) * Hkv
-    return max(1, min(256 // tiles, max_kv // 512, 64))
-
-
 def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                      cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *, sel: torch.Tensor | None = None,
                      sel_off: torch.Tensor | None = None, sm_scale: float | None = None, num_splits: int = 0,
@@ -977,9 +971,9 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     their keys and values; any number of them per sequence, 0 and 1 included.  The query of a token at position p
     sees the keys ``j <= p`` of its sequence.  ``sel`` / ``sel_off`` of :func:`paged_block_select` (with
     ``cu_seqlens``) restrict each block of 64 new tokens to the listed pages.  ``num_splits`` workgroups share
-    the keys of a row tile (0: from the shapes, :func:`paged_chunk_splits`); more than one needs a byte
-    workspace (allocated if omitted), which concurrent calls must not share.  Rows of ``out`` of no sequence are left as
-    they are.
+    the keys of a row tile: by default as many as make the workgroups' shares about even, worked out on the device
+    from the lengths; 1 for none.  Their partial results take a byte workspace (allocated if omitted), which
+    concurrent calls must not share.  Rows of ``out`` of no sequence are left as they are.
     """
     name = "paged_chunk_attn"
     if out is None:
@@ -1014,9 +1008,8 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                 other="q and out must be [N, Hq, D], pools [P, Hkv, page, D] with Hq a multiple of Hkv, sel and sel_off "
                       f"(both or neither) [at least N // {CHUNK_BLOCK} + min(B, N) rows, Hkv, width] and [rows, Hkv, 2]")
     N, Hq, D = qs
-    if num_splits == 0:
-        num_splits = paged_chunk_splits(N, B, Hq, ps[1], keys * ps[2])
-    ws = _workspace(name, workspace, num_splits * N * Hq * (D + 2) * 4 if num_splits > 1 else 0, dev)
+    ws = _workspace(name, workspace, _lib.load().sa_paged_chunk_workspace_bytes(
+        N, B, Hq, ps[1], D, min(keys * ps[2], 1 << 30), num_splits), dev)
     _call("sa_paged_chunk_attn", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_pages.data_ptr(),
           v_pages.data_ptr(), pst[0], pst[1], pst[2], ps[0], block_table.data_ptr(), block_table.stride(0), max_blocks,
           cu_seqlens.data_ptr(), kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], N, B, Hq, ps[1], D, ps[2],
