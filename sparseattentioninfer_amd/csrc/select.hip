@@ -15,20 +15,20 @@
 // of 64, 8 KV heads, 64 sequences: 67 MB, and 4.4 fp64 operations a byte).
 //
 // One workgroup makes a list: scores of all its pages as order-preserving 64-bit keys in LDS, the top_k-th key by
-// radix selection (8 bits a pass), then the kept pages in ascending order by ballots.  Where there are too few lists
-// to fill the chip, or more pages than fit LDS, the scores are computed by workgroups of their own, into the
-// workspace.
+// radix selection (8 bits a pass, from the highest bit in which the keys differ), then the kept pages in ascending
+// order by ballots.  Few lists get workgroups of 1,024 threads, many of 512.  All of it runs
+// once or a few times, so its time is latency and instruction fetch: loops are kept rolled.  Where a list has more pages than fit
+// LDS, the scores are computed by workgroups of their own, into the workspace.
 #include <algorithm>
 
 #include "ragged.h"
 
 namespace sa {
 
-constexpr int SEL_THREADS = 256;
-constexpr int SEL_WAVES = SEL_THREADS / 64;
 constexpr int SEL_BLOCK = 64;          // new tokens that share one list
 constexpr int SEL_LDS_PAGES = 4096;    // keys of a list held in LDS
-constexpr int SEL_PAGES_PER_WG = 64;   // pages scored by a workgroup of its own
+constexpr int SEL_FEW_LISTS = 256;     // up to one workgroup per CU: of 1,024 threads
+constexpr int SEL_PAGES_PER_WG = 128;  // pages scored by a workgroup of its own
 
 struct SelectArgs {
   const elem_t* q;
@@ -40,6 +40,7 @@ struct SelectArgs {
   int max_blocks, num_pages, page;
   Ragged seqs;                         // cu == NULL: one token per sequence, row b
   int rows, Hkv, G;
+  uint32_t mul_G;
   int top_k, sink, recent;
   int32_t* sel;
   int64_t sel_sr, sel_sh;
@@ -95,19 +96,24 @@ __device__ __forceinline__ unsigned long long key_of(double s) {
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, int T>
 struct Select {
-  static constexpr int LPR = D / 8;                 // lanes of one page's (or query's) row
-  static constexpr int RPP = SEL_THREADS / LPR;     // rows of a pass
+  static constexpr int WAVES = T / 64;
+  static constexpr int LPR = D / 8;     // lanes of one page's (or query's) row
+  static constexpr int RPP = T / LPR;   // rows of a pass
+  static constexpr int U = 4;           // rows of queries whose loads are in flight together
+  static constexpr int POOL_ROWS = 256 / LPR;   // rows of lanes that sum the queries: a single token's heads are few
   struct Shared {
-    double pool[SEL_WAVES][2][D];
+    double share[POOL_ROWS][2 * D];
+    double pool[2 * D];   // P, N
     int hist[256];
-    int sums[2][SEL_WAVES];
+    int sums[2][WAVES];
+    unsigned long long hi[WAVES], lo[WAVES];
     unsigned long long cut;
     int need, ties;
   };
 
-  static __device__ __forceinline__ void unpack(u32x4 v, double (&f)[8]) {
+  static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       f[2 * e] = Elem<BF16>::to_f32((elem_t)(v[e] & 0xffffu));
@@ -115,112 +121,144 @@ struct Select {
     }
   }
 
-  // P and N of the list's queries: this lane's 8 dims, in every row of lanes.
-  static __device__ __forceinline__ void pool(const SelectArgs& a, const SelectItem& it, Shared& sh, double (&P)[8],
-                                              double (&N)[8]) {
-    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    double p[8] = {}, n[8] = {};
-    for (int x = r; x < it.n * a.G; x += RPP) {
-      const elem_t* src = a.q + (it.tok0 + x / a.G) * a.q_st + (it.g * a.G + x % a.G) * a.q_sh + 8 * c;
-      double f[8];
-      unpack(*reinterpret_cast<const u32x4*>(src), f);
+  // P and N of the list's queries, into sh.pool.  Each row of lanes sums its share of the (query, head) rows; one
+  // thread per dim then adds the shares.
+  static __device__ __forceinline__ void pool(const SelectArgs& a, const SelectItem& it, Shared& sh) {
+    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR, rows = it.n * a.G;
+    if (r < POOL_ROWS) {
+      double p[8] = {}, n[8] = {};
+      for (int x0 = r; x0 < rows; x0 += U * POOL_ROWS) {
+        u32x4 v[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] += f[e] > 0. ? f[e] : 0.;
-        n[e] += f[e] < 0. ? f[e] : 0.;
-      }
-    }
+        for (int u = 0; u < U; ++u) {
+          const int x = x0 + u * POOL_ROWS;
+          v[u] = u32x4{0u, 0u, 0u, 0u};
+          if (x < rows) {
+            const int t = (int)fast_div((uint32_t)x, (uint32_t)a.G, a.mul_G);
+            v[u] = *reinterpret_cast<const u32x4*>(a.q + (it.tok0 + t) * a.q_st + (it.g * a.G + x - t * a.G) * a.q_sh + 8 * c);
+          }
+        }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+        for (int u = 0; u < U; ++u) {
+          float f[8];
+          unpack(v[u], f);
 #pragma unroll
-      for (int o = LPR; o < 64; o <<= 1) {
-        p[e] += __shfl_xor(p[e], o, 64);
-        n[e] += __shfl_xor(n[e], o, 64);
-      }
-    if (lane < LPR)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        sh.pool[wave][0][8 * c + e] = p[e];
-        sh.pool[wave][1][8 * c + e] = n[e];
-      }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      P[e] = N[e] = 0.;
-#pragma unroll
-      for (int w = 0; w < SEL_WAVES; ++w) {
-        P[e] += sh.pool[w][0][8 * c + e];
-        N[e] += sh.pool[w][1][8 * c + e];
-      }
-    }
-  }
-
-  // Keys of pages [p0, p1) into keys[page].
-  static __device__ __forceinline__ void score(const SelectArgs& a, const SelectItem& it, const double (&P)[8],
-                                               const double (&N)[8], int p0, int p1, unsigned long long* keys) {
-    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR;
-    constexpr int U = 4;
-    for (int x0 = p0 + r; x0 < p1; x0 += U * RPP) {
-      int pg[U];
-      u32x4 lo[U], hi[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int x = x0 + u * RPP;
-        pg[u] = x < p1 ? a.table[it.b * a.table_stride + x] : -1;
-        if (pg[u] >= a.num_pages) pg[u] = -1;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        lo[u] = hi[u] = u32x4{0u, 0u, 0u, 0u};
-        if (pg[u] >= 0) {
-          const elem_t* src = a.bounds + pg[u] * a.bd_sp + it.g * a.bd_sh + 8 * c;
-          lo[u] = *reinterpret_cast<const u32x4*>(src);
-          hi[u] = *reinterpret_cast<const u32x4*>(src + D);
+          for (int e = 0; e < 8; ++e) {
+            p[e] += (double)fmaxf(f[e], 0.f);
+            n[e] += (double)fminf(f[e], 0.f);
+          }
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        double l[8], h[8], s = 0.;
-        unpack(lo[u], l);
-        unpack(hi[u], h);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += h[e] * P[e] + l[e] * N[e];
-#pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o, 64);
-        const int x = x0 + u * RPP;
-        if (c == 0 && x < p1) keys[x] = pg[u] >= 0 ? key_of(s) : 0ull;
+      for (int e = 0; e < 8; ++e) {
+        sh.share[r][8 * c + e] = p[e];
+        sh.share[r][D + 8 * c + e] = n[e];
       }
+    }
+    __syncthreads();
+    if (threadIdx.x < 2 * D) {
+      double s = 0.;
+#pragma unroll 4
+      for (int x = 0; x < POOL_ROWS; ++x) s += sh.share[x][threadIdx.x];
+      sh.pool[threadIdx.x] = s;
+    }
+    __syncthreads();
+  }
+
+  // Keys of pages [p0, p1) into keys[page].  The bounds of the pages after these are on their way meanwhile.
+  static __device__ __forceinline__ void score(const SelectArgs& a, const SelectItem& it, const Shared& sh, int p0, int p1,
+                                               unsigned long long* keys) {
+    const int c = threadIdx.x % LPR, r = threadIdx.x / LPR;
+    const int32_t* table = a.table + it.b * a.table_stride;
+    const elem_t* bounds = a.bounds + it.g * a.bd_sh + 8 * c;
+    double P[8], N[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      P[e] = sh.pool[8 * c + e];
+      N[e] = sh.pool[D + 8 * c + e];
+    }
+    auto page_of = [&](int x) {
+      const int pg = x < p1 ? table[x] : -1;
+      return pg < a.num_pages ? pg : -1;
+    };
+    u32x4 lo = {0u, 0u, 0u, 0u}, hi = lo;
+    auto load = [&](int pg) {
+      if (pg >= 0) {
+        lo = *reinterpret_cast<const u32x4*>(bounds + pg * a.bd_sp);
+        hi = *reinterpret_cast<const u32x4*>(bounds + pg * a.bd_sp + D);
+      }
+    };
+    int pg = page_of(p0 + r), pg1 = page_of(p0 + r + RPP);
+    load(pg);
+    for (int x = p0 + r; x < p1; x += RPP) {
+      const u32x4 l4 = lo, h4 = hi;
+      const bool live = pg >= 0;
+      const int pg2 = page_of(x + 2 * RPP);
+      load(pg1);
+      float l[8], h[8];
+      double s = 0.;
+      unpack(l4, l);
+      unpack(h4, h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (double)h[e] * P[e] + (double)l[e] * N[e];
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o, 64);
+      if (c == 0) keys[x] = live ? key_of(s) : 0ull;
+      pg = pg1;
+      pg1 = pg2;
     }
   }
 
   // Radix selection: sh.cut and sh.ties such that the best `need` of the keys [p0, p1) are those above cut and the
   // first `ties` equal to it.
   static __device__ __forceinline__ void find_cut(const unsigned long long* keys, int p0, int p1, int need, Shared& sh) {
-    const int tid = threadIdx.x;
-    unsigned long long prefix = 0;
-    for (int byte = 7; byte >= 0; --byte) {
-      sh.hist[tid] = 0;
-      __syncthreads();
-      for (int x = p0 + tid; x < p1; x += SEL_THREADS) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    unsigned long long hi = 0, lo = ~0ull;
+    for (int x = p0 + tid; x < p1; x += T) {
+      const unsigned long long k = keys[x];
+      hi = k > hi ? k : hi;
+      lo = k < lo ? k : lo;
+    }
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned long long h = __shfl_xor(hi, o, 64), l = __shfl_xor(lo, o, 64);
+      hi = h > hi ? h : hi;
+      lo = l < lo ? l : lo;
+    }
+    if (lane == 0) {
+      sh.hi[wave] = hi;
+      sh.lo[wave] = lo;
+    }
+    if (tid < 256) sh.hist[tid] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < WAVES; ++w) {
+      hi = sh.hi[w] > hi ? sh.hi[w] : hi;
+      lo = sh.lo[w] < lo ? sh.lo[w] : lo;
+    }
+    // `left` bits are undecided; the keys that may hold the cut are those whose bits above are `prefix`.
+    int left = hi == lo ? 0 : 64 - __builtin_clzll(hi ^ lo);
+    unsigned long long prefix = left == 64 ? 0ull : hi >> left;
+    int count = p1 - p0;
+    while (left > 0 && count != need) {
+      const int bits = min(8, left), shift = left - bits;
+      for (int x = p0 + tid; x < p1; x += T) {
         const unsigned long long k = keys[x];
-        if (byte == 7 || (k >> (8 * byte + 8)) == prefix) atomicAdd(&sh.hist[(k >> (8 * byte)) & 255], 1);
+        if (left == 64 || (k >> left) == prefix) atomicAdd(&sh.hist[(int)(k >> shift) & ((1 << bits) - 1)], 1);
       }
       __syncthreads();
-      if (tid < 64) {   // lane l: bins 255 - 4 l down to 252 - 4 l
+      if (tid < 64) {   // lane l: digits 255 - 4 l down to 252 - 4 l
         int h[4], mine = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine += h[e] = sh.hist[255 - 4 * tid - e];
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int up = __shfl_up(incl, o, 64);
-          incl += tid >= o ? up : 0;
+        for (int e = 0; e < 4; ++e) {
+          mine += h[e] = sh.hist[255 - 4 * tid - e];
+          sh.hist[255 - 4 * tid - e] = 0;
         }
-        int above = incl - mine;
-        if (above < need && incl >= need) {
+        int above = scan_lanes(mine) - mine;
+        if (above < need && above + mine >= need) {
           int e = 0;
           while (above + h[e] < need) above += h[e++];
-          sh.cut = (prefix << 8) | (unsigned long long)(255 - 4 * tid - e);
+          sh.cut = (prefix << bits) | (unsigned long long)(255 - 4 * tid - e);
           sh.need = need - above;
           sh.ties = h[e];
         }
@@ -228,24 +266,21 @@ struct Select {
       __syncthreads();
       prefix = sh.cut;
       need = sh.need;
-      if (sh.ties == need) {   // every key with this prefix is in
-        if (byte) prefix = (prefix << (8 * byte)) - 1;   // all above it (prefix > 0: some key has it)
-        else prefix -= 1;
-        need = 0;
-        break;
-      }
-      __syncthreads();
+      count = sh.ties;
+      left = shift;
     }
     __syncthreads();
     if (tid == 0) {
-      sh.cut = prefix;
-      sh.ties = need;
+      // All `count` keys with the prefix are in (those above prefix << left, less one), or, all bits decided,
+      // `need` of the equal ones.  A prefix of zeros with all of its keys in would mean that every key is.
+      sh.cut = count == need ? (prefix << left) - 1ull : prefix;
+      sh.ties = count == need ? 0 : need;
     }
     __syncthreads();
   }
 
   // Exclusive rank of this thread's flag among the workgroup's, and their number.
-  static __device__ __forceinline__ int rank(bool flag, int (&sums)[SEL_WAVES], int& total) {
+  static __device__ __forceinline__ int rank(bool flag, int (&sums)[WAVES], int& total) {
     const int wave = threadIdx.x >> 6;
     const uint64_t m = __builtin_amdgcn_ballot_w64(flag);
     if ((threadIdx.x & 63) == 0) sums[wave] = __popcll(m);
@@ -253,7 +288,7 @@ struct Select {
     int before = __popcll(m & ((1ull << (threadIdx.x & 63)) - 1ull));
     total = 0;
 #pragma unroll
-    for (int w = 0; w < SEL_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       if (w < wave) before += sums[w];
       total += sums[w];
     }
@@ -265,7 +300,7 @@ struct Select {
                                                     const unsigned long long* keys, Shared& sh) {
     int32_t* out = a.sel + it.row * a.sel_sr + it.g * a.sel_sh;
     int count = 0, tied = 0;
-    for (int p0 = 0; p0 < it.pages; p0 += SEL_THREADS) {
+    for (int p0 = 0; p0 < it.pages; p0 += T) {
       const int p = p0 + threadIdx.x;
       bool keep = p < it.pages && (p < it.head || p >= it.lo);
       bool tie = false;
@@ -289,37 +324,36 @@ struct Select {
       __syncthreads();
     }
     count = min(count, a.width);
-    for (int x = count + threadIdx.x; x < a.width; x += SEL_THREADS) out[x] = 0;
+    for (int x = count + threadIdx.x; x < a.width; x += T) out[x] = 0;
     if (threadIdx.x < 2) a.off[((int64_t)it.row * a.Hkv + it.g) * 2 + threadIdx.x] = threadIdx.x ? count : 0;
   }
 
   static __device__ void empty_list(const SelectArgs& a, const SelectItem& it) {
     int32_t* out = a.sel + it.row * a.sel_sr + it.g * a.sel_sh;
-    for (int x = threadIdx.x; x < a.width; x += SEL_THREADS) out[x] = 0;
+    for (int x = threadIdx.x; x < a.width; x += T) out[x] = 0;
     if (threadIdx.x < 2) a.off[((int64_t)it.row * a.Hkv + it.g) * 2 + threadIdx.x] = 0;
   }
 };
 
 // Scores of SEL_PAGES_PER_WG pages of a list, into the workspace.
 template <bool BF16, int D>
-__global__ __launch_bounds__(SEL_THREADS) void select_score_kernel(const SelectArgs a) {
-  using S = Select<BF16, D>;
+__global__ __launch_bounds__(256) void select_score_kernel(const SelectArgs a) {
+  using S = Select<BF16, D, 256>;
   __shared__ typename S::Shared sh;
   SelectItem it;
   if (!find_list(a, blockIdx.x, it) || it.lo - it.head <= a.top_k || a.top_k == 0) return;
   const int p0 = it.head + (int)blockIdx.y * SEL_PAGES_PER_WG, p1 = min(it.lo, p0 + SEL_PAGES_PER_WG);
   if (p0 >= p1) return;
-  double P[8], N[8];
-  S::pool(a, it, sh, P, N);
-  S::score(a, it, P, N, p0, p1, a.keys + (int64_t)blockIdx.x * a.max_blocks);
+  S::pool(a, it, sh);
+  S::score(a, it, sh, p0, p1, a.keys + (int64_t)blockIdx.x * a.max_blocks);
 }
 
 // A list: with LDS its scores too, else from those of the workspace.
-template <bool BF16, int D, bool LDS>
-__global__ __launch_bounds__(SEL_THREADS) void select_kernel(const SelectArgs a) {
-  using S = Select<BF16, D>;
+template <bool BF16, int D, int T, bool LDS>
+__global__ __launch_bounds__(T) void select_kernel(const SelectArgs a) {
+  using S = Select<BF16, D, T>;
   __shared__ typename S::Shared sh;
-  __shared__ unsigned long long s_keys[LDS ? SEL_LDS_PAGES : 1];
+  extern __shared__ unsigned long long s_keys[];   // max_blocks
   SelectItem it;
   if (!find_list(a, blockIdx.x, it)) {
     S::empty_list(a, it);
@@ -329,9 +363,8 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(const SelectArgs a)
   unsigned long long* keys = LDS ? s_keys : a.keys + (int64_t)blockIdx.x * a.max_blocks;
   if (ranked) {
     if constexpr (LDS) {
-      double P[8], N[8];
-      S::pool(a, it, sh, P, N);
-      S::score(a, it, P, N, it.head, it.lo, keys);
+      S::pool(a, it, sh);
+      S::score(a, it, sh, it.head, it.lo, keys);
       __syncthreads();
     }
     S::find_cut(keys, it.head, it.lo, a.top_k, sh);
@@ -339,20 +372,19 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(const SelectArgs a)
   S::write_list(a, it, ranked, keys, sh);
 }
 
-// Whether the scores get workgroups of their own: the pages do not fit LDS, or the lists are too few.
-static bool split_scores(int64_t lists, int max_blocks) {
-  return max_blocks > SEL_LDS_PAGES || (lists < 128 && max_blocks > 2 * SEL_PAGES_PER_WG);
-}
-
 template <bool BF16, int D>
 static int launch_select(const SelectArgs& a, hipStream_t s) {
-  const unsigned lists = (unsigned)((int64_t)a.rows * a.Hkv);
+  const int64_t lists = (int64_t)a.rows * a.Hkv;
+  const dim3 grid((unsigned)lists);
+  const size_t lds = a.keys ? 0 : (size_t)a.max_blocks * 8;
   if (a.keys) {
-    hipLaunchKernelGGL((select_score_kernel<BF16, D>), dim3(lists, (a.max_blocks + SEL_PAGES_PER_WG - 1) / SEL_PAGES_PER_WG),
-                       dim3(SEL_THREADS), 0, s, a);
-    hipLaunchKernelGGL((select_kernel<BF16, D, false>), dim3(lists), dim3(SEL_THREADS), 0, s, a);
+    hipLaunchKernelGGL((select_score_kernel<BF16, D>),
+                       dim3((unsigned)lists, (a.max_blocks + SEL_PAGES_PER_WG - 1) / SEL_PAGES_PER_WG), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((select_kernel<BF16, D, 1024, false>), grid, dim3(1024), lds, s, a);
+  } else if (lists <= SEL_FEW_LISTS) {
+    hipLaunchKernelGGL((select_kernel<BF16, D, 1024, true>), grid, dim3(1024), lds, s, a);
   } else {
-    hipLaunchKernelGGL((select_kernel<BF16, D, true>), dim3(lists), dim3(SEL_THREADS), 0, s, a);
+    hipLaunchKernelGGL((select_kernel<BF16, D, 512, true>), grid, dim3(512), lds, s, a);
   }
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "sa_paged_block_select: launch failed: %s", hipGetErrorString(err));
@@ -365,7 +397,7 @@ using namespace sa;
 extern "C" int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks) {
   if (rows < 1 || Hkv < 1 || max_blocks < 1) return 0;
   const int64_t lists = (int64_t)rows * Hkv;
-  return split_scores(lists, max_blocks) ? lists * max_blocks * 8 : 0;
+  return max_blocks > SEL_LDS_PAGES ? lists * max_blocks * 8 : 0;
 }
 
 extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k_bounds,
@@ -414,6 +446,7 @@ extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int
   a.max_blocks = max_blocks, a.num_pages = num_pages, a.page = page;
   a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
   a.rows = rows, a.Hkv = Hkv, a.G = Hq / Hkv;
+  a.mul_G = div_mul((uint32_t)a.G);
   a.top_k = top_k, a.sink = sink, a.recent = recent;
   a.sel = sel;
   a.sel_sr = sel_sr, a.sel_sh = sel_sh, a.width = width;
