@@ -1098,8 +1098,8 @@ extern "C" int64_t sa_paged_chunk_workspace_bytes(int N, int B, int Hq, int Hkv,
   const int64_t key_tiles = (max_keys + CK_KT - 1) / CK_KT;
   const int64_t all = (int64_t)N * Hq;
   if (num_splits > 1) return chunk_part_header(B) + all * std::min<int64_t>(num_splits, key_tiles) * (D + 2) * 4;
-  // Nothing is gained where the row tiles fill the chip several times over.
-  if (key_tiles <= 4 || (int64_t)N * (Hq / Hkv) / CK_WIDE_ROWS * Hkv >= 8 * (int64_t)chunk_cus()) return 0;
+  // Nothing is gained where the row tiles fill the chip several times over, twice for those of one sequence.
+  if (key_tiles <= 4 || (int64_t)N * (Hq / Hkv) / CK_WIDE_ROWS * Hkv >= (B == 1 ? 2 : 8) * (int64_t)chunk_cus()) return 0;
   return chunk_part_header(B) + std::min(all * std::min<int64_t>(key_tiles / 4 + 1, 64), CK_PART_ROWS) * (D + 2) * 4;
 }
 

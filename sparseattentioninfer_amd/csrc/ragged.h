@@ -29,8 +29,6 @@ struct Ragged {
   __device__ __forceinline__ int kv_len(int b) const { return min(max(kv_lens[b], 0), MAX_KV_LEN); }
 };
 
-__device__ __forceinline__ int floor_div(int a, int d) { return a >= 0 ? a / d : -((d - 1 - a) / d); }
-
 // Sum of x over this lane and those before it, without LDS: four shifts within rows of 16 lanes, then the last
 // lane of a row to the next and of the lower half to the upper.
 __device__ __forceinline__ int scan_lanes(int x) {

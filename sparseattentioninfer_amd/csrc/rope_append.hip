@@ -12,7 +12,8 @@
 // a share of the heads.  It computes the window's cos and sin once, into LDS (one sincos per token and pair
 // whatever the number of heads), then each wave takes whole heads: D/16 lanes hold one token's head, each the two
 // 16-byte chunks that the rotation mixes, so a wave moves 1024 / D tokens of a head per pass and the norm is a
-// reduction over D/16 neighbouring lanes.
+// reduction over D/16 neighbouring lanes.  One pass's loads run under the pass before (loops are kept rolled: short
+// calls are bound by latency and instruction fetch).
 //
 // Pages: windows are aligned to positions, in multiples of the page, so the tokens that a chunk adds to one page
 // belong to one window, and one wave sees all of them for a head.  It keeps their minimum and maximum in
@@ -20,6 +21,7 @@
 // tokens before, else written fresh.  Min and max are exact and have no order, so the result has none either.
 #include <algorithm>
 
+#include "lds_tile.h"
 #include "ragged.h"
 
 namespace sa {
@@ -28,7 +30,6 @@ constexpr int RA_THREADS = 256;
 constexpr int RA_WAVES = RA_THREADS / 64;
 constexpr int RA_MAX_WINDOW = 128;              // tokens of a window
 constexpr int RA_CHUNK = 16;                    // positions that share a page for every page size
-constexpr int RA_UNROLL = 4;                    // passes of a wave whose loads are in flight together
 
 struct RopeArgs {
   const elem_t *q, *k, *v;
@@ -45,6 +46,7 @@ struct RopeArgs {
   int64_t N;
   int T;
   uint32_t mul_T;
+  uint32_t mul_window, mul_page;
   // paged
   Ragged seqs;
   elem_t *k_pages, *v_pages;
@@ -91,6 +93,52 @@ struct RopeAppend {
     t = (int)((uint32_t)n - (uint32_t)b * (uint32_t)a.T);
   }
 
+  // Norm weights of a lane's 16 dims.
+  struct Weights {
+    u32x4 l, h;
+  };
+
+  // Where a head comes from and goes to: rows of src, then rows of dst or (paged keys and values) pages of it.
+  struct Head {
+    int kind, hh;                 // query, key, value; head among its kind
+    const elem_t* src;
+    elem_t* dst;
+    int64_t s_sb, s_st, d_sb, d_st;
+  };
+  static __device__ __forceinline__ Head head_of(const RopeArgs& a, int h) {
+    Head x;
+    if (h < a.Hq) {
+      x.kind = 0, x.hh = h;
+      x.src = a.q + x.hh * a.q_sh, x.s_st = a.q_st, x.s_sb = a.q_sb;
+      x.dst = a.qo + x.hh * a.qo_sh, x.d_st = a.qo_st, x.d_sb = a.qo_sb;
+    } else if (h < a.Hq + a.Hkv) {
+      x.kind = 1, x.hh = h - a.Hq;
+      x.src = a.k + x.hh * a.k_sh, x.s_st = a.k_st, x.s_sb = a.k_sb;
+      x.dst = PAGED ? a.k_pages + x.hh * a.pg_sh : a.ko + x.hh * a.ko_sh;
+      x.d_st = PAGED ? a.pg_st : a.ko_st, x.d_sb = a.ko_sb;
+    } else {
+      x.kind = 2, x.hh = h - a.Hq - a.Hkv;
+      x.src = a.v + x.hh * a.v_sh, x.s_st = a.v_st, x.s_sb = 0;
+      x.dst = a.v_pages + x.hh * a.pg_sh, x.d_st = a.pg_st, x.d_sb = 0;
+    }
+    return x;
+  }
+
+  // Offset of packed row n (paged), or of token n % T of batch n / T.
+  static __device__ __forceinline__ int64_t row_at(const RopeArgs& a, int64_t n, int64_t sb, int64_t st) {
+    if constexpr (PAGED) return n * st;
+    int bt, t;
+    batch_of(a, n, bt, t);
+    return bt * sb + t * st;
+  }
+
+  // Window of position p, rounded down; a position may be negative where a sequence has fewer tokens than new ones.
+  static __device__ __forceinline__ int window_of(const RopeArgs& a, int p) {
+    const uint32_t m = (uint32_t)(p < 0 ? a.window - 1 - p : p);
+    const int q = (int)fast_div(m, (uint32_t)a.window, a.mul_window);
+    return p < 0 ? -q : q;
+  }
+
   static __device__ __forceinline__ bool find_window(const RopeArgs& a, int x, Window& w, int& b) {
     b = 0;
     if constexpr (!PAGED) {
@@ -103,13 +151,13 @@ struct RopeAppend {
       auto windows = [&](int s) {
         int r0;
         const int n = a.seqs.rows(s, r0), end = a.seqs.kv_len(s);
-        return n ? floor_div(end - 1, a.window) - floor_div(end - n, a.window) + 1 : 0;
+        return n ? window_of(a, end - 1) - window_of(a, end - n) + 1 : 0;
       };
       int local;
       if (!find_item(a.seqs.B, x, windows, b, local)) return false;
       int r0;
       const int n = a.seqs.rows(b, r0), end = a.seqs.kv_len(b), start = end - n;
-      w.base = (floor_div(start, a.window) + local) * a.window;
+      w.base = (window_of(a, start) + local) * a.window;
       w.lo = max(0, start - w.base);
       w.hi = min(a.window, end - w.base);
       w.row0 = (int64_t)r0 + w.base - start;
@@ -126,29 +174,37 @@ struct RopeAppend {
     int b;
     if (!find_window(a, blockIdx.x, w, b)) return;
 
-    // cos and sin of the window's tokens
+    // The norm weights of this lane's dims, and cos and sin of the window's tokens: one pair to a thread.
+    const int c = lane % LPR;
+    Weights qw = {}, kw = {};
+    if (a.qw) qw = {*reinterpret_cast<const u32x4*>(a.qw + 8 * c), *reinterpret_cast<const u32x4*>(a.qw + HALF + 8 * c)};
+    if (a.kw) kw = {*reinterpret_cast<const u32x4*>(a.kw + 8 * c), *reinterpret_cast<const u32x4*>(a.kw + HALF + 8 * c)};
     if (a.inv_freq) {
-      for (int x = w.lo * HALF + tid; x < w.hi * HALF; x += RA_THREADS) {
-        const int slot = x / HALF, i = x % HALF;
-        int64_t p = w.base + slot;
-        if constexpr (!PAGED) {
+      const int i = tid % HALF;
+      const double freq = (double)a.inv_freq[i] * 0.15915494309189533577;   // / 2 pi: turns
+      for (int slot = w.lo + tid / HALF; slot < w.hi; slot += RA_THREADS / HALF) {
+        double p;
+        if constexpr (PAGED) {
+          p = (double)(w.base + slot);
+        } else {
           int bt, t;
           batch_of(a, w.row0 + slot, bt, t);
-          p = a.positions[bt * a.pos_sb + t];
+          p = (double)a.positions[bt * a.pos_sb + t];
         }
-        const double turns = (double)p * (double)a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
-        float s, c;
-        sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-        s_cs[slot * CS_STRIDE + i] = c;
-        s_cs[slot * CS_STRIDE + HALF + i] = s;
+        const double turns = p * freq;
+        float si, co;
+        sincospif(2.f * (float)(turns - rint(turns)), &si, &co);
+        s_cs[slot * CS_STRIDE + i] = co;
+        s_cs[slot * CS_STRIDE + HALF + i] = si;
       }
     }
     if (PAGED && tid < a.window / RA_CHUNK) {
       const int p = w.base + tid * RA_CHUNK;
       int pg = -1, slot = 0;
-      if (p >= 0 && p / a.page < a.max_blocks) {
-        pg = a.table[b * a.table_stride + p / a.page];
-        slot = p % a.page;
+      const int lb = p < 0 ? -1 : (int)fast_div((uint32_t)p, (uint32_t)a.page, a.mul_page);
+      if (lb >= 0 && lb < a.max_blocks) {
+        pg = a.table[b * a.table_stride + lb];
+        slot = p - lb * a.page;
         if (pg < 0 || pg >= a.num_pages) pg = -1;
       }
       s_page[tid] = pg;
@@ -156,164 +212,145 @@ struct RopeAppend {
     }
     __syncthreads();
 
+    // Passes of RPI tokens of a head, head by head; the loads of the next pass are in flight meanwhile.
     const int heads = a.Hq + a.Hkv + (PAGED ? a.Hkv : 0);
     const int h_end = min(heads, (int)(blockIdx.y + 1) * a.heads_per_part);
-    for (int h = (int)blockIdx.y * a.heads_per_part + wave; h < h_end; h += RA_WAVES) head(a, w, h, lane, s_cs, s_page, s_slot);
+    const int g = lane / LPR, t_first = w.lo / RPI * RPI;
+    u32x4 nl = {0u, 0u, 0u, 0u}, nh = nl;
+    auto load = [&](const Head& hd, int slot) {
+      if (slot >= w.lo && slot < w.hi) {
+        const elem_t* p = hd.src + row_at(a, w.row0 + slot, hd.s_sb, hd.s_st) + 8 * c;
+        nl = *reinterpret_cast<const u32x4*>(p);
+        nh = *reinterpret_cast<const u32x4*>(p + HALF);
+      }
+    };
+    int h = (int)blockIdx.y * a.heads_per_part + wave, t0 = t_first;
+    if (h >= h_end) return;
+    Head hd = head_of(a, h);
+    load(hd, t0 + g);
+    float mn[16], mx[16];
+    int from = w.lo;              // first slot of the page at hand (bounds)
+#pragma unroll 1
+    while (true) {
+      const Head cur = hd;
+      const int slot = t0 + g;
+      const bool live = slot >= w.lo && slot < w.hi;
+      u32x4 vl = nl, vh = nh;
+      t0 += RPI;
+      const bool head_done = t0 >= w.hi;
+      if (head_done) {
+        h += RA_WAVES;
+        t0 = t_first;
+        if (h < h_end) hd = head_of(a, h);
+      }
+      if (h < h_end) load(hd, t0 + g);
+      if (cur.kind < 2) {
+        float l[8], r[8];
+        unpack8<BF16>(vl, l);
+        unpack8<BF16>(vh, r);
+        if (cur.kind ? a.kw != nullptr : a.qw != nullptr) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss += l[e] * l[e] + r[e] * r[e];
+          ss = row_total(ss);
+          const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+          float wl[8], wh[8];
+          unpack8<BF16>(cur.kind ? kw.l : qw.l, wl);
+          unpack8<BF16>(cur.kind ? kw.h : qw.h, wh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            l[e] *= inv * wl[e];
+            r[e] *= inv * wh[e];
+          }
+        }
+        if (a.inv_freq && live) {
+          const float* cs = s_cs + slot * CS_STRIDE + 8 * c;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float co = cs[e], si = cs[HALF + e];
+            const float y = l[e] * co - r[e] * si;
+            r[e] = r[e] * co + l[e] * si;
+            l[e] = y;
+          }
+        }
+        vl = pack8<BF16>(l);
+        vh = pack8<BF16>(r);
+      }
+      if (live) {
+        elem_t* d = nullptr;
+        if (!PAGED || cur.kind == 0) {
+          d = cur.dst + row_at(a, w.row0 + slot, cur.d_sb, cur.d_st) + 8 * c;
+        } else {
+          const int pg = s_page[slot / RA_CHUNK];
+          if (pg >= 0)
+            d = cur.dst + pg * a.pg_sp + (int64_t)(s_slot[slot / RA_CHUNK] + slot % RA_CHUNK) * cur.d_st + 8 * c;
+        }
+        if (d) {
+          *reinterpret_cast<u32x4*>(d) = vl;
+          *reinterpret_cast<u32x4*>(d + HALF) = vh;
+        }
+      }
+      if (PAGED && cur.kind == 1 && a.bounds) {   // bounds of the stored (rounded) keys
+        float y[16];
+        unpack8<BF16>(vl, y);
+        unpack8<BF16>(vh, y + 8);
+        const int first_slot = slot - g;          // of the pass
+        const bool first = first_slot <= from;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          mn[e] = fminf(first ? __builtin_inff() : mn[e], live ? y[e] : __builtin_inff());
+          mx[e] = fmaxf(first ? -__builtin_inff() : mx[e], live ? y[e] : -__builtin_inff());
+        }
+        const int page_end = min(w.hi, from + a.page - (s_slot[from / RA_CHUNK] + from % RA_CHUNK));
+        if (first_slot + RPI >= page_end) {
+          bound_page(a, mn, mx, s_page[from / RA_CHUNK], s_slot[from / RA_CHUNK] + from % RA_CHUNK == 0, cur.hh, c, g);
+          from = head_done ? w.lo : page_end;
+        }
+      }
+      if (h >= h_end) break;
+    }
   }
 
-  // All of the window's tokens of one head.
-  static __device__ __forceinline__ void head(const RopeArgs& a, const Window& w, int h, int lane, const float* s_cs,
-                                              const int* s_page, const int* s_slot) {
-    // Where this head comes from and goes to: rows of src, then rows of dst or (paged keys and values) pages of it.
-    int kind, hh;                 // query, key, value; head among its kind
-    const elem_t *src, *wt;
-    elem_t* dst;
-    int64_t st, sb, d_st, d_sb;
-    if (h < a.Hq) {
-      kind = 0, hh = h;
-      src = a.q + hh * a.q_sh, st = a.q_st, sb = a.q_sb, wt = a.qw;
-      dst = a.qo + hh * a.qo_sh, d_st = a.qo_st, d_sb = a.qo_sb;
-    } else if (h < a.Hq + a.Hkv) {
-      kind = 1, hh = h - a.Hq;
-      src = a.k + hh * a.k_sh, st = a.k_st, sb = a.k_sb, wt = a.kw;
-      dst = PAGED ? a.k_pages + hh * a.pg_sh : a.ko + hh * a.ko_sh, d_st = PAGED ? a.pg_st : a.ko_st, d_sb = a.ko_sb;
-    } else {
-      kind = 2, hh = h - a.Hq - a.Hkv;
-      src = a.v + hh * a.v_sh, st = a.v_st, sb = 0, wt = nullptr;
-      dst = a.v_pages + hh * a.pg_sh, d_st = a.pg_st, d_sb = 0;
+  // Sum over the LPR (4 or 8) lanes of a token's head, in every one.
+  static __device__ __forceinline__ float row_total(float x) {
+    x += dpp<0xB1>(x);    // lane pairs
+    x += dpp<0x4E>(x);    // quads
+    if constexpr (LPR == 8) x += dpp<0x141>(x);   // the two quads of 8 lanes
+    return x;
+  }
+
+  // Brings a page's bounds up to date with the minimum and maximum of new keys of head hh that the lanes hold.
+  static __device__ __forceinline__ void bound_page(const RopeArgs& a, float (&mn)[16], float (&mx)[16], int pg, bool fresh,
+                                                    int hh, int c, int g) {
+    if (pg < 0) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      // Over the lanes that differ in the bits of the token.
+      if constexpr (LPR == 4) {
+        mn[e] = fminf(mn[e], __shfl_xor(mn[e], 4, 64));
+        mx[e] = fmaxf(mx[e], __shfl_xor(mx[e], 4, 64));
+      }
+      mn[e] = fminf(mn[e], dpp<0x128>(mn[e]));   // row_ror:8
+      mx[e] = fmaxf(mx[e], dpp<0x128>(mx[e]));
+      auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(mn[e]), __float_as_uint(mn[e]), false, false);
+      mn[e] = -halves_max(-fminf(__uint_as_float(s[0]), __uint_as_float(s[1])));
+      s = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx[e]), __float_as_uint(mx[e]), false, false);
+      mx[e] = halves_max(fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])));
     }
-    const bool rotate = a.inv_freq && kind < 2;
-    const bool track = PAGED && kind == 1 && a.bounds;
-    const int c = lane % LPR, g = lane / LPR;
-    float wl[8], wh[8];
+    if (g < 2) {   // lanes of token group 0 write the minima, of group 1 the maxima
+      elem_t* d = a.bounds + pg * a.bd_sp + hh * a.bd_sh + g * D + 8 * c;
+      float y[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wl[e] = wh[e] = 1.f;
-    if (wt) {
-      unpack8<BF16>(*reinterpret_cast<const u32x4*>(wt + 8 * c), wl);
-      unpack8<BF16>(*reinterpret_cast<const u32x4*>(wt + HALF + 8 * c), wh);
-    }
-    auto src_of = [&](int slot) {
-      const int64_t n = w.row0 + slot;
-      if constexpr (PAGED) return src + n * st + 8 * c;
-      int bt, t;
-      batch_of(a, n, bt, t);
-      return src + bt * sb + t * st + 8 * c;
-    };
-    auto dst_of = [&](int slot) -> elem_t* {
-      const int64_t n = w.row0 + slot;
-      if constexpr (!PAGED) {
-        int bt, t;
-        batch_of(a, n, bt, t);
-        return dst + bt * d_sb + t * d_st + 8 * c;
+      for (int e = 0; e < 16; ++e) y[e] = g ? mx[e] : mn[e];
+      if (!fresh) {
+        float old[16];
+        unpack8<BF16>(*reinterpret_cast<const u32x4*>(d), old);
+        unpack8<BF16>(*reinterpret_cast<const u32x4*>(d + HALF), old + 8);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = g ? fmaxf(y[e], old[e]) : fminf(y[e], old[e]);
       }
-      if (kind == 0) return dst + n * d_st + 8 * c;
-      const int pg = s_page[slot / RA_CHUNK];
-      if (pg < 0) return nullptr;
-      return dst + pg * a.pg_sp + (int64_t)(s_slot[slot / RA_CHUNK] + slot % RA_CHUNK) * d_st + 8 * c;
-    };
-    // With bounds a key head goes page by page, else the window at once.
-    const int seg = track ? min(a.page, a.window) : a.window;
-    for (int s0 = w.lo / seg * seg; s0 < w.hi; s0 += seg) {
-      const int lo = max(w.lo, s0), hi = min(w.hi, s0 + seg);
-      float mn[16], mx[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        mn[e] = __builtin_inff();
-        mx[e] = -__builtin_inff();
-      }
-      for (int t0 = lo / RPI * RPI; t0 < hi; t0 += RPI * RA_UNROLL) {
-        u32x4 xl[RA_UNROLL], xh[RA_UNROLL];
-#pragma unroll
-        for (int u = 0; u < RA_UNROLL; ++u) {
-          const int slot = t0 + u * RPI + g;
-          xl[u] = xh[u] = u32x4{0u, 0u, 0u, 0u};
-          if (slot >= lo && slot < hi) {
-            const elem_t* p = src_of(slot);
-            xl[u] = *reinterpret_cast<const u32x4*>(p);
-            xh[u] = *reinterpret_cast<const u32x4*>(p + HALF);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < RA_UNROLL; ++u) {
-          const int slot = t0 + u * RPI + g;
-          const bool live = slot >= lo && slot < hi;
-          if (kind < 2) {
-            float l[8], r[8];
-            unpack8<BF16>(xl[u], l);
-            unpack8<BF16>(xh[u], r);
-            if (wt) {
-              float ss = 0.f;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) ss += l[e] * l[e] + r[e] * r[e];
-#pragma unroll
-              for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o, 64);
-              const float inv = rsqrtf(ss * (1.f / D) + a.eps);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                l[e] *= inv * wl[e];
-                r[e] *= inv * wh[e];
-              }
-            }
-            if (rotate && live) {
-              const float* cs = s_cs + slot * CS_STRIDE + 8 * c;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float co = cs[e], si = cs[HALF + e];
-                const float y = l[e] * co - r[e] * si;
-                r[e] = r[e] * co + l[e] * si;
-                l[e] = y;
-              }
-            }
-            xl[u] = pack8<BF16>(l);
-            xh[u] = pack8<BF16>(r);
-            if (track && live) {   // bounds of the stored (rounded) keys
-              unpack8<BF16>(xl[u], l);
-              unpack8<BF16>(xh[u], r);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                mn[e] = fminf(mn[e], l[e]);
-                mx[e] = fmaxf(mx[e], l[e]);
-                mn[8 + e] = fminf(mn[8 + e], r[e]);
-                mx[8 + e] = fmaxf(mx[8 + e], r[e]);
-              }
-            }
-          }
-          if (live) {
-            elem_t* d = dst_of(slot);
-            if (d) {
-              *reinterpret_cast<u32x4*>(d) = xl[u];
-              *reinterpret_cast<u32x4*>(d + HALF) = xh[u];
-            }
-          }
-        }
-      }
-      if (track) {
-        const int pg = s_page[lo / RA_CHUNK];
-        if (pg < 0) continue;
-        const bool fresh = s_slot[lo / RA_CHUNK] + lo % RA_CHUNK == 0;
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-#pragma unroll
-          for (int o = LPR; o < 64; o <<= 1) {
-            mn[e] = fminf(mn[e], __shfl_xor(mn[e], o, 64));
-            mx[e] = fmaxf(mx[e], __shfl_xor(mx[e], o, 64));
-          }
-        if (g < 2) {   // lanes of token group 0 write the minima, of group 1 the maxima
-          elem_t* d = a.bounds + pg * a.bd_sp + hh * a.bd_sh + g * D + 8 * c;
-          float y[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = g ? mx[e] : mn[e];
-          if (!fresh) {
-            float old[16];
-            unpack8<BF16>(*reinterpret_cast<const u32x4*>(d), old);
-            unpack8<BF16>(*reinterpret_cast<const u32x4*>(d + HALF), old + 8);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = g ? fmaxf(y[e], old[e]) : fminf(y[e], old[e]);
-          }
-          *reinterpret_cast<u32x4*>(d) = pack8<BF16>(y);
-          *reinterpret_cast<u32x4*>(d + HALF) = pack8<BF16>(y + 8);
-        }
-      }
+      *reinterpret_cast<u32x4*>(d) = pack8<BF16>(y);
+      *reinterpret_cast<u32x4*>(d + HALF) = pack8<BF16>(y + 8);
     }
   }
 };
@@ -339,10 +376,15 @@ static int launch_rope(const char* name, int dtype, int D, const RopeArgs& a, di
   return err == hipSuccess ? 0 : set_error((int)err, "%s: launch failed: %s", name, hipGetErrorString(err));
 }
 
-// Heads per workgroup: the heads are dealt over workgroups until the launch has about RA_TARGET of them.
-constexpr int64_t RA_TARGET = 1024;
-static int heads_per_part(int64_t windows, int heads) {
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((heads + RA_WAVES - 1) / RA_WAVES, RA_TARGET / std::max<int64_t>(1, windows)));
+// Heads per workgroup: the heads of a window are dealt over up to target / windows workgroups, each of which computes
+// the window's cos and sin again.  Paged, four workgroups fit a CU and one round of them is best (8K tokens in 8
+// sequences, 521 windows: 46.6 us with one workgroup each, 53.8 with 4, 50.0 with 7; 64 single tokens 9.1 us with 12,
+// 10.3 with 7).  Unpaged, seven fit, and a round and a bit is worse than several (32K tokens, 2,048 windows: 146 us with
+// one workgroup each, 139 with two).
+constexpr int64_t RA_TARGET_PAGED = 1024, RA_TARGET = 4096;
+static int heads_per_part(int64_t windows, int heads, int64_t target) {
+  const int64_t most = (heads + RA_WAVES - 1) / RA_WAVES;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(most, target / std::max<int64_t>(1, windows)));
   return (int)((heads + parts - 1) / parts);
 }
 
@@ -387,10 +429,10 @@ extern "C" int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q
   a.T = T;
   a.mul_T = div_mul((uint32_t)T);
   a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
-  a.window = 32;
+  a.window = 16;
   const int64_t windows = (a.N + a.window - 1) / a.window;
   if (windows > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: %lld tokens are too many", name, (long long)a.N);
-  a.heads_per_part = heads_per_part(windows, Hq + Hkv);
+  a.heads_per_part = heads_per_part(windows, Hq + Hkv, RA_TARGET);
   const int parts = (Hq + Hkv + a.heads_per_part - 1) / a.heads_per_part;
   return launch_rope<false>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
 }
@@ -442,12 +484,15 @@ extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q
   a.table = block_table;
   a.table_stride = block_table_stride;
   a.max_blocks = max_blocks, a.num_pages = num_pages, a.page = page;
-  a.window = 64 % page == 0 ? 64 : page;
-  // n new tokens touch at most (n - 1) / window + 2 windows
-  const int64_t windows = (int64_t)N / a.window + 2 * (int64_t)std::min(B, N);
+  // Bounds want whole pages; else the shortest window, whose cos and sin are soonest done.
+  a.window = k_bounds ? page : RA_CHUNK;
+  a.mul_window = div_mul((uint32_t)a.window);
+  a.mul_page = div_mul((uint32_t)page);
+  // n new tokens touch at most (n - 1) / window + 2 windows, and at most n
+  const int64_t windows = std::min<int64_t>(N, (int64_t)N / a.window + 2 * (int64_t)std::min(B, N));
   if (windows > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: N=%d B=%d are too many", name, N, B);
   const int heads = Hq + 2 * Hkv;
-  a.heads_per_part = heads_per_part(windows, heads);
+  a.heads_per_part = heads_per_part(windows, heads, RA_TARGET_PAGED);
   const int parts = (heads + a.heads_per_part - 1) / a.heads_per_part;
   return launch_rope<true>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
 }
