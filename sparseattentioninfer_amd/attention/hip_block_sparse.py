@@ -212,3 +212,35 @@ class HipBlockSparseBackend(AttentionBackend):
         self.last_kernel = "decode"
         self._last_actual_backend = "hip_block_sparse"
         return out
+
+    def forward_packed(self, q: torch.Tensor, store, chunk, pattern: PatternMetadata) -> torch.Tensor:
+        """Causal attention of a chunk of new tokens over a paged store; returns ``[N, H, D]``.
+
+        ``q [N, H, D]`` packs the new tokens of all sequences, any number of them each, as the ``chunk`` that
+        :meth:`~sparseattentioninfer_amd.models.kv_cache.PagedKVStore.append` returned lists them; the store
+        already holds their keys and values.  ``kind == "dense"`` attends the whole cache; ``"block_topk"`` the
+        pages that the store's key bounds rank highest for each query (single tokens) or block of 64 queries.
+        """
+        if not q.is_cuda:
+            raise RuntimeError("hip_block_sparse runs on ROCm GPU tensors only")
+        paged = (store.k_pages, store.v_pages, store.block_table)
+        if pattern.kind == "dense":
+            out = ops.paged_chunk_attn(q, *paged, chunk.cu_seqlens, store.kv_lens)
+        elif pattern.kind == "block_topk":
+            if store.k_bounds is None:
+                raise ValueError("block_topk needs a paged store with key bounds (bounds=True)")
+            if pattern.block_size != store.page:
+                raise ValueError(f"pattern block {pattern.block_size} differs from the cache page {store.page}")
+            pick = dict(page=store.page, top_k=pattern.topk, sink=pattern.sink, recent=pattern.recent)
+            if chunk.single_tokens:
+                sel, off = ops.paged_block_select(q, store.k_bounds, store.block_table, store.kv_lens, **pick)
+                out = ops.paged_sparse_decode(q, *paged, store.kv_lens, sel, off, num_splits=0)
+            else:
+                sel, off = ops.paged_block_select(q, store.k_bounds, store.block_table, store.kv_lens,
+                                                  cu_seqlens=chunk.cu_seqlens, **pick)
+                out = ops.paged_chunk_attn(q, *paged, chunk.cu_seqlens, store.kv_lens, sel=sel, sel_off=off)
+        else:
+            raise NotImplementedError(f"forward_packed runs dense and block_topk patterns, not {pattern.kind!r}")
+        self.last_kernel = "decode" if chunk.single_tokens else "chunk"
+        self._last_actual_backend = "hip_block_sparse"
+        return out

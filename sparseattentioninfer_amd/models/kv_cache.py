@@ -12,11 +12,16 @@ copy) only when exceeded.
 ``PagedKVStore`` holds one layer's pages ``[P, H, page, D]``, a block table
 ``[B, max_blocks]`` (logical block -> page) and the sequence lengths; pages
 are taken from a free list as sequences grow.  It is the layout
-``sa_decode`` reads in paged mode.
+``sa_decode`` reads in paged mode.  ``append`` takes a chunk of new tokens whose
+number differs from sequence to sequence.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
+
+from .. import ops
 
 
 def _round_up(x: int, m: int) -> int:
@@ -108,18 +113,35 @@ class KVCache:
         return self._view(layer_idx)
 
 
+@dataclass
+class PagedChunk:
+    """New tokens that :meth:`PagedKVStore.append` has written: those of sequence b are rows
+    ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` of the packed tensors."""
+    cu_seqlens: torch.Tensor            # [B + 1] int32, on the store's device
+    counts: tuple[int, ...]             # new tokens of each sequence
+    q: torch.Tensor | None              # the normed and rotated queries, if any were given
+
+    @property
+    def single_tokens(self) -> bool:
+        """Whether every sequence has exactly one."""
+        return all(n == 1 for n in self.counts)
+
+
 class PagedKVStore:
     """One layer's paged K/V: ``k_pages, v_pages [P, H, page, D]``, ``block_table [B, max_blocks]``.
 
     Pages are handed out from a free list (in a seeded shuffled order when
     ``shuffle_seed`` is given, to exercise non-contiguous tables) as
     sequences grow; ``lens`` counts the valid tokens per sequence on the host
-    and ``kv_lens`` mirrors it on the device.
+    and ``kv_lens`` mirrors it on the device.  With ``bounds`` (on the GPU) ``k_bounds [P, H, 2, D]`` keeps
+    the smallest and largest key of each page in each dim, which ``ops.paged_block_select`` ranks pages by.
     """
 
     def __init__(self, batch: int, heads: int, head_dim: int, max_len: int, *, page: int = 64,
                  dtype=torch.bfloat16, device="cuda", num_pages: int | None = None,
-                 shuffle_seed: int | None = None):
+                 shuffle_seed: int | None = None, bounds: bool = False):
+        if bounds and torch.device(device).type != "cuda":
+            raise ValueError("a PagedKVStore with key bounds lives on the GPU (its append kernel keeps them)")
         if page % 16 or not 16 <= page <= 128:
             raise ValueError(f"page {page} must be a multiple of 16 in [16, 128]")
         self.batch, self.heads, self.head_dim, self.page = batch, heads, head_dim, page
@@ -127,6 +149,7 @@ class PagedKVStore:
         self.num_pages = num_pages if num_pages is not None else batch * self.max_blocks
         self.k_pages = torch.empty(self.num_pages, heads, page, head_dim, dtype=dtype, device=device)
         self.v_pages = torch.empty_like(self.k_pages)
+        self.k_bounds = torch.zeros(self.num_pages, heads, 2, head_dim, dtype=dtype, device=device) if bounds else None
         self.block_table = torch.zeros(batch, self.max_blocks, dtype=torch.int32, device=device)
         self.kv_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.lens = [0] * batch
@@ -155,6 +178,52 @@ class PagedKVStore:
         self.block_table[:, have:need] = torch.tensor(added, dtype=torch.int32).to(self.block_table.device)
         self._page_cols.clear()
 
+    def _grow_each(self, new_lens: list[int]) -> None:
+        """Gives each sequence the pages that its ``new_lens`` tokens need (one table update), or none of them."""
+        need = [-(-n // self.page) for n in new_lens]
+        if max(need) > self.max_blocks:
+            raise ValueError(f"sequences need {max(need)} blocks > max_blocks {self.max_blocks}")
+        more = [max(0, n - len(row)) for n, row in zip(need, self._table_host)]
+        if not any(more):
+            return
+        if len(self._free) < sum(more):
+            raise RuntimeError("paged KV cache: out of pages")
+        table = torch.zeros(self.batch, self.max_blocks, dtype=torch.int32)
+        for b, (row, n) in enumerate(zip(self._table_host, more)):
+            row.extend(self._free.pop() for _ in range(n))
+            table[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
+        self.block_table.copy_(table)
+        self._page_cols.clear()
+
+    def _uniform_len(self, what: str) -> int:
+        if any(n != self.lens[0] for n in self.lens):
+            raise ValueError(f"{what} needs sequences of one length, got {self.lens}")
+        return self.lens[0]
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, counts, *, inv_freq: torch.Tensor | None = None,
+               k_weight: torch.Tensor | None = None, eps: float = 1e-6, q: torch.Tensor | None = None,
+               q_weight: torch.Tensor | None = None) -> PagedChunk:
+        """Appends ``counts[b]`` new tokens to each sequence b, packed in ``k_new, v_new [N, H, D]`` (on the GPU).
+
+        Keys are normed (``k_weight``) and rotated (``inv_freq``) on the way where those are given, and queries
+        ``q [N, Hq, D]`` with them (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).
+        """
+        counts = tuple(int(n) for n in counts)
+        if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k_new.size(0):
+            raise ValueError(f"counts {counts} do not split {k_new.size(0)} tokens over {self.batch} sequences")
+        new_lens = [n + t for n, t in zip(self.lens, counts)]
+        self._grow_each(new_lens)
+        cu = [0]
+        for t in counts:
+            cu.append(cu[-1] + t)
+        cu = torch.tensor(cu, dtype=torch.int32).to(self.kv_lens.device)
+        self.kv_lens.copy_(torch.tensor(new_lens, dtype=torch.int32))
+        q_out = ops.paged_append(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
+                                 inv_freq=inv_freq, k_weight=k_weight, eps=eps, k_bounds=self.k_bounds, q=q,
+                                 q_weight=q_weight)
+        self.lens = new_lens
+        return PagedChunk(cu, counts, q_out)
+
     def _page_col(self, lb: int) -> torch.Tensor:
         """Pages of logical block ``lb`` for every sequence, as a device index tensor (cached)."""
         col = self._page_cols.get(lb)
@@ -169,7 +238,11 @@ class PagedKVStore:
         if (B, H, D) != (self.batch, self.heads, self.head_dim) or v_new.shape != k_new.shape:
             raise ValueError(f"write of {tuple(k_new.shape)} into a [{self.batch}, {self.heads}, *, "
                              f"{self.head_dim}] store")
-        start = self.lens[0]
+        start = self._uniform_len("write")
+        if self.k_bounds is not None:      # the append kernel keeps the bounds
+            k, v = (x.to(self.k_pages.dtype).transpose(1, 2).reshape(B * t, H, D) for x in (k_new, v_new))
+            self.append(k, v, [t] * B)
+            return
         self._grow_all(start + t)
         if t == 1:   # decode: one slot of one page per sequence
             idx = self._page_col(start // self.page)
@@ -188,7 +261,7 @@ class PagedKVStore:
 
     def gather(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Contiguous ``[B, H, T, D]`` copies of the cached K/V (slow path for generic callers)."""
-        T = self.lens[0]
+        T = self._uniform_len("gather")
         nb = -(-T // self.page)
         pages = self.block_table[:, :nb].long()                         # [B, nb]
         k = self.k_pages[pages].permute(0, 2, 1, 3, 4).reshape(self.batch, self.heads, nb * self.page, -1)
@@ -196,7 +269,7 @@ class PagedKVStore:
         return k[:, :, :T].contiguous(), v[:, :, :T].contiguous()
 
     def seq_len(self) -> int:
-        return self.lens[0]
+        return self._uniform_len("seq_len")
 
     def reset(self) -> None:
         """Returns every page to the free list (contents are left as they are)."""

@@ -29,7 +29,7 @@ class PatternMetadata:
     ``H / H_kv`` query heads of the group; the backends tell the two apart by
     the row count.
     """
-    kind: str                                   # "dense" | "mask" | "topk" | "local"
+    kind: str                                   # "dense" | "mask" | "topk" | "local" | "block_topk"
     mask: torch.Tensor | None = None            # [H, T_q, T_k] bool, True = keep
     topk: int | None = None
     keep_ratio: float = 1.0
@@ -38,6 +38,8 @@ class PatternMetadata:
     kv_block_list: torch.Tensor | None = None   # [H, NQB, MAX_KV] int32, -1 = padding
     block_pairs: torch.Tensor | None = None     # [R, max_pairs] int32
     block_pair_offsets: torch.Tensor | None = None  # [R, NQB + 1] int32
+    sink: int = 0                               # "block_topk": first and last blocks kept beside the best `topk`
+    recent: int = 1
 
 
 class SparsePattern(ABC):

@@ -155,6 +155,8 @@ class GraphDecoder:
         if not self.chunk:
             raise ValueError(f"vocab {V} has no power-of-two chunk for the two-stage argmax")
         for layer in self.layers:
+            if layer.self_attn.pattern_name == "block_topk":
+                raise ValueError("GraphDecoder builds its selections before the run; block_topk selects at every step")
             if not hasattr(layer.self_attn.sparse_backend, "forward_paged"):
                 raise ValueError("GraphDecoder needs a backend with paged decode (hip_block_sparse)")
         # one selection table per distinct pattern (dense causal layers all share one)

@@ -24,6 +24,10 @@ update, pattern build, backend call, output projection.  Differences:
   shared per KV group) and ``"dense"`` (full causal, on the same kernels);
   ``config.sparse_attention_layers`` lists the sparse layers, the others run
   ``"dense"``.
+* ``"block_topk"``: the pages of a ``PagedKVCache(bounds=True)`` that rank highest for
+  each query, for prompts, chunks of them and single tokens alike.  Norms, rotation,
+  the paged write and the pages' bounds are one launch (one rounding where Hugging
+  Face's modules round five times), and no step gathers the cache.
 """
 from __future__ import annotations
 
@@ -38,8 +42,8 @@ from transformers.models.qwen3.modeling_qwen3 import (Qwen3Attention, Qwen3ForCa
 
 from ..attention import get_backend
 from ..models.attention_layer import repeat_kv
-from ..patterns import (BigBirdKeepRatioPattern, BigBirdPattern, DenseCausalPattern, LocalWindowPattern,
-                        SeededBigBirdPattern)
+from ..patterns import (BigBirdKeepRatioPattern, BigBirdPattern, BlockTopKPattern, DenseCausalPattern,
+                        LocalWindowPattern, SeededBigBirdPattern)
 from .paged_cache import PagedKVCache
 from .sparse_config import (KERNEL_BACKEND, GroupSparsitySpec, backend_candidates, config_value,
                             ensure_attn_implementation, is_plain_causal_mask, pattern_stats,
@@ -107,6 +111,15 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
                 global_blocks=config_value(config, "sparse_attention_bigbird_global", 2),
                 random_blocks=config_value(config, "sparse_attention_bigbird_random", 3),
                 seed=config_value(config, "sparse_attention_seed", 0) + layer_idx)
+        if self.pattern_name == "block_topk":
+            rope = config_value(config, "rope_parameters", None) or {}
+            if rope.get("rope_type", "default") != "default":
+                raise NotImplementedError(f"block_topk rotates with the default rope, not {rope['rope_type']!r}")
+            self._rope_theta = float(rope.get("rope_theta", 10000.0))
+            self._inv_freq: Optional[torch.Tensor] = None
+            return BlockTopKPattern(config_value(config, "sparse_attention_topk_pages", 16), block_size=self.block_size,
+                                    sink=config_value(config, "sparse_attention_sink_pages", 1),
+                                    recent=config_value(config, "sparse_attention_recent_pages", 2))
         if self.pattern_name == "dense":
             return DenseCausalPattern()
         if self.pattern_name == "local":
@@ -148,6 +161,8 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
         cache = past_key_values if past_key_values is not None else kwargs.get("past_key_value")
         input_shape = hidden_states.shape[:-1]
         bsz, q_len = input_shape
+        if self.pattern_name == "block_topk":
+            return self._forward_block_topk(hidden_states, attention_mask, cache), None
         hidden_shape = (*input_shape, -1, self.head_dim)
         q = self.q_norm(self.q_proj(hidden_states).view(hidden_shape)).transpose(1, 2)
         k = self.k_norm(self.k_proj(hidden_states).view(hidden_shape)).transpose(1, 2)
@@ -195,6 +210,33 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
             raise ValueError(f"`attn_output` should be of size {expected}, but is {tuple(out.size())}.")
         out = out.transpose(1, 2).reshape(*input_shape, -1).contiguous()
         return self.o_proj(out), None
+
+
+    def _forward_block_topk(self, hidden_states: torch.Tensor, attention_mask, cache) -> torch.Tensor:
+        """Projections, one append launch, page selection and attention over the chosen pages."""
+        if not isinstance(cache, PagedKVCache) or not cache.layers[self.layer_idx].bounds:
+            raise ValueError("the block_topk pattern needs past_key_values=PagedKVCache(..., bounds=True)")
+        bsz, q_len = hidden_states.shape[:-1]
+        layer = cache.layers[self.layer_idx]
+        if self.validate_causal_mask and not is_plain_causal_mask(attention_mask, q_len=q_len,
+                                                                  k_len=layer.get_seq_length() + q_len):
+            raise NotImplementedError("Sparse kernel path supports plain causal masks only; padding-aware or "
+                                      "custom attention masks are not wired up.")
+        backend = self.sparse_backend = self.sparse_backends[self.backend_name]
+        if not hasattr(backend, "forward_packed"):
+            raise NotImplementedError(f"backend {self.backend_name!r} has no attention over packed chunks (block_topk)")
+        if self._inv_freq is None or self._inv_freq.device != hidden_states.device:
+            half = torch.arange(0, self.head_dim, 2, dtype=torch.float64) / self.head_dim
+            self._inv_freq = (1.0 / self._rope_theta ** half).float().to(hidden_states.device)
+        q, k, v = (proj(hidden_states).view(bsz * q_len, -1, self.head_dim)
+                   for proj in (self.q_proj, self.k_proj, self.v_proj))
+        chunk = layer.append(q, k, v, [q_len] * bsz, inv_freq=self._inv_freq, k_weight=self.k_norm.weight,
+                             q_weight=self.q_norm.weight, eps=self.q_norm.variance_epsilon)
+        store = layer.store
+        pattern = self.sparse_pattern.build(q, q.new_empty((bsz, self.num_key_value_heads, store.seq_len(), 0)), causal=True)
+        self.last_pattern_stats = pattern_stats(pattern) if self.collect_pattern_stats else None
+        out = backend.forward_packed(chunk.q, store, chunk, pattern)
+        return self.o_proj(out.reshape(bsz, q_len, -1))
 
 
 def build_sparse_attention_from_dense(attention: nn.Module, *, backend_name: str = "hip_block_sparse",

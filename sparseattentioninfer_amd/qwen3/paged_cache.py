@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
-from ..models.kv_cache import PagedKVStore
+from ..models.kv_cache import PagedChunk, PagedKVStore
 
 
 class PagedKVLayer(CacheLayerMixin):
@@ -22,17 +22,26 @@ class PagedKVLayer(CacheLayerMixin):
     is_sliding = False
     is_compileable = False
 
-    def __init__(self, max_len: int, *, page: int = 64, shuffle_seed: int | None = None):
+    def __init__(self, max_len: int, *, page: int = 64, shuffle_seed: int | None = None, bounds: bool = False):
         super().__init__()
-        self.max_len, self.page, self.shuffle_seed = max_len, page, shuffle_seed
+        self.max_len, self.page, self.shuffle_seed, self.bounds = max_len, page, shuffle_seed, bounds
         self.store: PagedKVStore | None = None
 
     def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
         B, H, _, D = key_states.shape
-        self.dtype, self.device = key_states.dtype, key_states.device
-        self.store = PagedKVStore(B, H, D, self.max_len, page=self.page, dtype=key_states.dtype,
-                                  device=key_states.device, shuffle_seed=self.shuffle_seed)
+        self._make_store(B, H, D, key_states)
+
+    def _make_store(self, B: int, H: int, D: int, like: torch.Tensor) -> None:
+        self.dtype, self.device = like.dtype, like.device
+        self.store = PagedKVStore(B, H, D, self.max_len, page=self.page, dtype=like.dtype, device=like.device,
+                                  shuffle_seed=self.shuffle_seed, bounds=self.bounds)
         self.is_initialized = True
+
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts, **rope) -> PagedChunk:
+        """:meth:`PagedKVStore.append` of packed ``[N, H, D]`` projections (queries too), allocating on first use."""
+        if not self.is_initialized:
+            self._make_store(len(counts), k.size(1), k.size(2), k)
+        return self.store.append(k, v, counts, q=q, **rope)
 
     def write(self, key_states: torch.Tensor, value_states: torch.Tensor) -> PagedKVStore:
         """Appends ``[B, H_kv, t, D]`` K/V to the pages; returns the store."""
@@ -73,10 +82,12 @@ class PagedKVLayer(CacheLayerMixin):
 
 
 class PagedKVCache(Cache):
-    """``num_layers`` paged layers of up to ``max_len`` tokens per sequence."""
+    """``num_layers`` paged layers of up to ``max_len`` tokens per sequence; with ``bounds`` their pages keep the
+    key bounds that the ``"block_topk"`` pattern selects by."""
 
-    def __init__(self, num_layers: int, max_len: int, *, page: int = 64, shuffle_seed: int | None = None):
-        super().__init__(layers=[PagedKVLayer(max_len, page=page, shuffle_seed=shuffle_seed)
+    def __init__(self, num_layers: int, max_len: int, *, page: int = 64, shuffle_seed: int | None = None,
+                 bounds: bool = False):
+        super().__init__(layers=[PagedKVLayer(max_len, page=page, shuffle_seed=shuffle_seed, bounds=bounds)
                                  for _ in range(num_layers)])
         self.page = page
 

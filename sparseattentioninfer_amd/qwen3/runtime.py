@@ -88,7 +88,8 @@ def greedy_generate(model, input_ids: torch.Tensor, steps: int, *, cache: str = 
     cfg = model.config
     if cache == "paged":
         pkv = PagedKVCache(cfg.num_hidden_layers, max_len or (T + steps + 1),
-                           page=getattr(cfg, "sparse_attention_block_size", 64), shuffle_seed=shuffle_seed)
+                           page=getattr(cfg, "sparse_attention_block_size", 64), shuffle_seed=shuffle_seed,
+                           bounds=getattr(cfg, "sparse_attention_pattern", None) == "block_topk")
     elif cache == "dynamic":
         from transformers.cache_utils import DynamicCache
         pkv = DynamicCache(config=cfg)
