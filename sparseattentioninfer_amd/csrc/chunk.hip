@@ -57,7 +57,7 @@ struct ChunkArgs {
   elem_t* o;
   int64_t o_st, o_sh;
   int Hq, Hkv, G;
-  uint32_t mul_G, mul_heads, mul_Hq;
+  uint32_t mul_G, mul_heads, mul_Hq, mul_tpb;
   float scale_log2;
   int items;                       // (row tile, split) pairs of the launch at most; workgroups past the last exit
   int tiles_per_block;             // with a selection: wide row tiles of a 64-token block
@@ -80,18 +80,23 @@ struct ChunkArgs {
 // lengths are device memory, so the launch is as large as any lengths need and every workgroup works out the
 // division for itself, the same in all of them: `limit` key tiles to a workgroup, from the total.
 //
-// A key tile takes a narrow item about as long as a wide one when the chip is full (32 KB at a CU's share of HBM,
-// 1.5 us; 256 rows on its matrix cores, 1.3 us), so tiles are what is balanced, and a workgroup costs CK_START of them
-// besides its own (its first loads, the row tile's partials: 7 to 10 us).
-constexpr float CK_START = 6.f;
+// Key tiles are what is balanced.  With the chip full a wide item takes 1.75 us for one (256 rows on its matrix
+// cores), a narrow one 1.45 us where narrow items are most of the work (32 KB at a CU's share of HBM) and about half of
+// a wide one's beside wide ones.  A workgroup costs CK_START of them besides its own: 9.6 us, of which finding its item
+// takes 2.5, the pages of its first tiles 2.6, the tiles 1.5 and the end 3.
+constexpr float CK_START = 5.5f;
 constexpr int CK_NARROW = 64;
 constexpr int CK_WIDE_ROWS = 256;
 
-// Sum over the lanes that differ in bits 3..5 only, in every lane.
+// Sum or maximum over the lanes that differ in bits 3..5 only, in every lane.
+enum : int { SUM = 0, MAX = 1 };
+template <int OP>
 __device__ __forceinline__ float over_eights(float x) {
-  x += dpp<0x128>(x);   // row_ror:8
+  auto op = [](float a, float b) { return OP == MAX ? fmaxf(a, b) : a + b; };
+  x = op(x, dpp<0x128>(x));   // row_ror:8
   const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return halves_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
+  x = op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  return OP == MAX ? halves_max(x) : halves_sum(x);
 }
 
 struct SeqShape {
@@ -119,83 +124,118 @@ __device__ __forceinline__ SeqShape seq_shape(const ChunkArgs& a, int b) {
 
 // Workgroups that share a row tile's keys when one takes at most `limit` key tiles.  A wide one leaves 133 KB of
 // partials (as long as 5 tiles take), so it has at least 8 tiles; a narrow one at least one for each wave.
+constexpr int CK_MAX_SPLITS = 64;
 constexpr int CK_NO_LIMIT = 0x40000000;   // at or past this: no division
 struct SplitRule {
   int limit;
-  float rcp_wide, rcp_narrow;   // of the key tiles that a wide and that a narrow workgroup may take
-  static __device__ __forceinline__ int most(int limit, int narrow) { return max(limit, narrow ? 4 : 8); }
-  __device__ __forceinline__ explicit SplitRule(int l) {
+  int most_wide, most_narrow;    // key tiles of a workgroup
+  float rcp_wide, rcp_narrow;
+  // half: a narrow item's key tile counts half of a wide one's.
+  __device__ __forceinline__ SplitRule(int l, int half) {
     limit = l;
-    rcp_wide = __builtin_amdgcn_rcpf((float)most(l, 0));
-    rcp_narrow = __builtin_amdgcn_rcpf((float)most(l, 1));
+    most_wide = max(l, 8);
+    most_narrow = max(l >= CK_NO_LIMIT ? l : l << half, 4);
+    rcp_wide = __builtin_amdgcn_rcpf((float)most_wide);
+    rcp_narrow = __builtin_amdgcn_rcpf((float)most_narrow);
   }
   __device__ __forceinline__ int splits(int fixed, int narrow, int nt) const {
     if (limit >= CK_NO_LIMIT) return 1;
     if (fixed) return max(1, min(fixed, nt));
     // ceil(nt / m): nt < 2^24, so the rounded product is off by one at most.
-    const int m = most(limit, narrow), x = nt + m - 1;
+    const int m = narrow ? most_narrow : most_wide, x = nt + m - 1;
     int q = (int)((float)x * (narrow ? rcp_narrow : rcp_wide));
     q += (q + 1) * m <= x ? 1 : 0;
     q -= q * m > x ? 1 : 0;
-    return max(1, q);
+    return min(max(1, q), CK_MAX_SPLITS);
   }
 };
 
-// Key tiles that one workgroup takes (a.splits: any number below CK_NO_LIMIT stands for that division).  Every
-// workgroup comes through here before its first load, so the choices are weighed side by side: lane 8 y + x adds up
-// choice x over the sequences y, y + 8, ...  The sums are fp32: exact where they decide between neighbouring choices
-// (below 2^24), and the room for partials is kept with a margin above their rounding; a fixed division, which fills
-// its room exactly, is summed in 64 bits.
-__device__ __forceinline__ int plan_limit(const ChunkArgs& a, const SeqShape& first64) {
+// The division of the keys (a.splits: any limit below CK_NO_LIMIT stands for that division).  Every workgroup comes
+// through here before its first load, so eight choices are weighed side by side: lane 8 y + x adds up choice x over
+// the sequences y, y + 8, ...  The sums are fp32: exact where they decide between neighbouring choices (below 2^24),
+// and the room for partials is kept with a margin above their rounding; a fixed division, which fills its room
+// exactly, is summed in 64 bits.
+__device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqShape& first64) {
   const int lane = threadIdx.x & 63;
   if (a.splits) {
     int64_t x = 0;
     for (int b = lane; b < a.seqs.B; b += 64) {
       const SeqShape s = b < 64 ? first64 : seq_shape(a, b);
-      const int k = SplitRule(1).splits(a.splits, is_narrow(a, s.n), s.nt);
+      const int k = SplitRule(1, 0).splits(a.splits, is_narrow(a, s.n), s.nt);
       x += k > 1 ? (int64_t)s.n * k * a.Hq : 0;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x > a.part_rows ? CK_NO_LIMIT : 1;
+    return SplitRule(x > a.part_rows ? CK_NO_LIMIT : 1, 0);
   }
   const float heads = (float)a.Hkv, cus = (float)a.cus;
-  float work = 0.f, longest = 0.f, tiles = 0.f;
+  float wide = 0.f, narrow = 0.f, longest = 0.f, tiles = 0.f;
   for (int b0 = 0; b0 < a.seqs.B; b0 += 64)
     if (b0 + lane < a.seqs.B) {
       const SeqShape s = b0 ? seq_shape(a, b0 + lane) : first64;
-      work += (float)s.tiles * (float)(s.nt + s.nt0);
+      const float w = (float)s.tiles * (float)(s.nt + s.nt0);
+      (is_narrow(a, s.n) ? narrow : wide) += w;
       tiles += (float)s.tiles;
       longest = fmaxf(longest, (float)s.nt);
     }
-  work = wave_sum(work) * (0.5f * heads);
+  wide = wave_sum(wide) * (0.5f * heads);
+  narrow = wave_sum(narrow) * (0.5f * heads);
   tiles = wave_sum(tiles);
   longest = wave_max(longest);
+  const int half = narrow > wide ? 0 : 1;
+  const float nw = half ? 0.5f : 1.f, work = wide + nw * narrow;
   const float even = fminf(ceilf(work / cus), (float)(CK_NO_LIMIT / 16));
-  if (longest <= 0.5f * even) return CK_NO_LIMIT;   // there are row tiles enough
+  if (longest <= 0.5f * even) return SplitRule(CK_NO_LIMIT, half);   // there are row tiles enough
   // Choices: 1/2, 3/4, 1, 5/4, 3/2, 2 and 3 even shares, and no division.
   const int quarters = (0x0C865432u >> (4 * (lane & 7))) & 15;
-  const SplitRule r(quarters ? max(1, (int)ceilf(even * (float)quarters * 0.25f)) : CK_NO_LIMIT);
-  float groups = 0.f, rows = 0.f;
-  for (int b0 = 0; b0 < a.seqs.B; b0 += 64) {
-    SeqShape s = {};
-    if (b0 + lane < a.seqs.B) s = b0 ? seq_shape(a, b0 + lane) : first64;
-    const int narrow = is_narrow(a, s.n);
-    for (int y = 0; y < min(64, a.seqs.B - b0); y += 8) {
-      const int from = y + (lane >> 3);   // sequences past the last have no tiles
-      const int st = __shfl(s.tiles, from, 64), nt = __shfl(2 * s.nt + narrow, from, 64), n = __shfl(s.n, from, 64);
-      const int k = r.splits(0, nt & 1, nt >> 1);
-      groups += (float)st * (float)k;
-      rows += k > 1 ? (float)n * (float)k : 0.f;
+  const SplitRule r(quarters ? max(1, (int)ceilf(even * (float)quarters * 0.25f)) : CK_NO_LIMIT, half);
+  auto each = [&](auto f) {   // f(sequence's row tiles, splits, longest, shortest key tiles, new tokens, weight)
+    for (int b0 = 0; b0 < a.seqs.B; b0 += 64) {
+      SeqShape s = first64;
+      if (b0) {
+        s = SeqShape{};
+        if (b0 + lane < a.seqs.B) s = seq_shape(a, b0 + lane);
+      }
+      const int nar = is_narrow(a, s.n);
+      for (int y = 0; y < min(64, a.seqs.B - b0); y += 8) {
+        const int from = y + (lane >> 3);   // sequences past the last have no tiles
+        const int st = __shfl(s.tiles, from, 64), nt = __shfl(2 * s.nt + nar, from, 64);
+        const int nt0 = __shfl(s.nt0, from, 64), n = __shfl(s.n, from, 64);
+        const int k = r.splits(0, nt & 1, nt >> 1);
+        f((float)st, (float)k, (float)(nt >> 1), (float)nt0, (float)n, nt & 1 ? nw : 1.f);
+      }
     }
-  }
-  groups = over_eights(groups) * heads;
-  rows = over_eights(rows) * (float)a.Hq;
-  // The division that ends first among those whose partials fit and which add no more workgroups than there are CUs
-  // (chunk_items: the launch has that many to spare, and idle ones cost time too).  Workgroups in one round end with the longest; in
-  // several, half a workgroup after an even share of all tiles and starts.
-  const float one = fminf((float)max(r.limit, 8), longest) + CK_START;
-  float time = groups <= cus ? one : fmaxf(one, (work + groups * CK_START) / cus + 0.5f * one);
+  };
+  float groups = 0.f, rows = 0.f;
+  each([&](float st, float k, float, float, float n, float) {
+    groups += st * k;
+    rows += k > 1.f ? n * k : 0.f;
+  });
+  groups = over_eights<SUM>(groups) * heads;
+  rows = over_eights<SUM>(rows) * (float)a.Hq;
+  // When it ends.  In one round: with the longest workgroup.  Else, handed out longest first: the mean load, or
+  // two of those longer than half of it where they outnumber the CUs (their lengths taken as spread evenly).
+  const float mean = (work + groups * CK_START) / cus;
+  float one = 0.f, many = 0.f, lo = __builtin_inff(), hi = 0.f;
+  each([&](float st, float k, float nt, float nt0, float, float w) {
+    if (st == 0.f) return;
+    const float x = w * __builtin_amdgcn_rcpf(k), h = nt * x + CK_START, l = nt0 * x + CK_START;
+    one = fmaxf(one, h);
+    if (h <= 0.5f * mean) return;
+    const float from = fmaxf(l, 0.5f * mean);
+    many += st * k * (l >= 0.5f * mean ? 1.f : (h - from) * __builtin_amdgcn_rcpf(h - l));
+    lo = fminf(lo, from);
+    hi = fmaxf(hi, h);
+  });
+  one = over_eights<MAX>(one);
+  many = over_eights<SUM>(many) * heads;
+  lo = -over_eights<MAX>(-lo);
+  hi = over_eights<MAX>(hi);
+  float time = one;
+  if (groups > cus) time = fmaxf(one, 1.08f * mean);
+  if (groups > cus && many > cus) time = fmaxf(time, 2.f * (lo + (hi - lo) * (many - cus) / many));
+  // The partials must fit, and no more workgroups are added than there are CUs (chunk_items: the launch has that
+  // many to spare, and idle ones cost time too).  No division always does.
   if (rows * 1.001f > (float)a.part_rows || groups > tiles * heads + cus) time = __builtin_inff();
   int limit = CK_NO_LIMIT;
   float best = __builtin_inff();
@@ -208,7 +248,7 @@ __device__ __forceinline__ int plan_limit(const ChunkArgs& a, const SeqShape& fi
       limit = l;
     }
   }
-  return limit;
+  return SplitRule(limit, half);
 }
 
 // The rows and keys of one work item.
@@ -232,7 +272,9 @@ struct ChunkItem {
 };
 
 // Work item of workgroup `id`, or false.  Heads go fastest (one XCD's workgroups then read one KV head where there
-// are eight of them); later row tiles, which see more keys, come first.
+// are eight of them).  Longest first, so that the launch ends evenly: up to 64 sequences in the order of their
+// workgroups' key tiles (a narrow one's take half as long while the matrix cores bound the rest), more as they come;
+// within a sequence later row tiles, which see more keys, first.
 __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, ChunkItem& it) {
   const int lane = threadIdx.x & 63;
   const int t = (int)fast_div((uint32_t)id, (uint32_t)a.Hkv, a.mul_heads);
@@ -240,56 +282,66 @@ __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, Chun
   SeqShape s64 = {};
   if (lane < a.seqs.B) s64 = seq_shape(a, lane);
   const bool split = a.part != nullptr;
-  const SplitRule rule(split ? plan_limit(a, s64) : CK_NO_LIMIT);
+  const SplitRule rule = split ? plan_splits(a, s64) : SplitRule(CK_NO_LIMIT, 0);
   const bool first = id == 0 && split && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
-  int total = 0;
-  for (int b0 = 0; b0 < a.seqs.B; b0 += 64) {
-    SeqShape s = {};
-    if (b0 + lane < a.seqs.B) s = b0 ? seq_shape(a, b0 + lane) : s64;
-    total += __builtin_amdgcn_readlane(scan_lanes(s.tiles * rule.splits(a.splits, is_narrow(a, s.n), s.nt)), 63);
-  }
-  const int x = total - 1 - t;
-  if (x < 0 && !first) return false;
-  int base = 0, block0 = 0;
-  int part0 = 0;
+  const bool ranked = a.seqs.B > 1 && a.seqs.B <= 64;
+  int base = 0, block0 = 0, part0 = 0, local = 0;
   bool found = false;
   for (int b0 = 0; b0 < a.seqs.B && (first || !found); b0 += 64) {
-    SeqShape s = {};
-    if (b0 + lane < a.seqs.B) s = b0 ? seq_shape(a, b0 + lane) : s64;
-    const int k = rule.splits(a.splits, is_narrow(a, s.n), s.nt);
+    SeqShape s = s64;
+    if (b0) {
+      s = SeqShape{};
+      if (b0 + lane < a.seqs.B) s = seq_shape(a, b0 + lane);
+    }
+    const int narrow = is_narrow(a, s.n), k = rule.splits(a.splits, narrow, s.nt);
     const int c = s.tiles * k, blocks = a.sel ? (s.n + CK_BLOCK - 1) / CK_BLOCK : 0;
     const int rows = k > 1 ? s.n * k * a.Hq : 0;   // all of them fit 31 bits: part_rows does
-    const int ic = scan_lanes(c), ib = a.sel ? scan_lanes(blocks) : 0, ir = split ? scan_lanes(rows) : 0;
+    const int ib = a.sel ? scan_lanes(blocks) : 0, ir = split ? scan_lanes(rows) : 0;
     if (first && b0 + lane < a.seqs.B) a.part[b0 + lane] = SeqPart{part0 + ir - rows, k, s.n, rule.limit < CK_NO_LIMIT};
-    const uint64_t past = __builtin_amdgcn_ballot_w64(base + ic > x);
-    if (past && !found && x >= 0) {
+    // The sequences in their order: lane i then holds the item count and the lane of the i-th.
+    int co = c, from = lane;
+    if (ranked) {
+      const float len = (float)((s.nt + s.nt0) << (1 - narrow)) * __builtin_amdgcn_rcpf((float)k);
+      int rank = 0;
+      for (int j = 0; j < a.seqs.B; ++j) {
+        const float lj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(len), j));
+        rank += lj > len || (lj == len && j < lane) ? 1 : 0;
+      }
+      rank = lane < a.seqs.B ? rank : lane;
+      co = __builtin_amdgcn_ds_permute(4 * rank, c);
+      from = __builtin_amdgcn_ds_permute(4 * rank, lane);
+    }
+    const int io = scan_lanes(co);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(base + io > t);
+    if (past && !found) {
       found = true;
-      const int l = __builtin_ctzll(past);
+      const int lo = __builtin_ctzll(past), l = __builtin_amdgcn_readlane(from, lo);
       auto lane_of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      local = base + __builtin_amdgcn_readlane(io, lo) - 1 - t;   // from the sequence's last item back
       it.b = b0 + l;
       it.n = lane_of(s.n);
       it.tok0 = lane_of(s.row);
       it.end = lane_of(s.end);
       it.splits = lane_of(k);
-      const int local = x - base - lane_of(ic - c);
-      const int tile = local / it.splits;
-      it.split = local - tile * it.splits;
       it.narrow = is_narrow(a, it.n);
       it.start = it.end - it.n;
       it.part = part0 + lane_of(ir - rows);
-      it.row0 = tile;   // resolved below
       block0 += lane_of(ib - blocks);
     }
     if (!found) block0 += __builtin_amdgcn_readlane(ib, 63);
-    base += __builtin_amdgcn_readlane(ic, 63);
+    base += __builtin_amdgcn_readlane(io, 63);
     part0 += __builtin_amdgcn_readlane(ir, 63);
   }
   if (!found) return false;
-  const int tile = it.row0, rows = it.narrow ? CK_ROWS : CK_WIDE_ROWS;
+  const uint32_t mul_k = it.splits > 1 ? 0xFFFFFFFFu / (uint32_t)it.splits : 0xFFFFFFFFu;
+  const int tile = (int)fast_div((uint32_t)local, (uint32_t)it.splits, mul_k);
+  it.split = local - tile * it.splits;
+  const int rows = it.narrow ? CK_ROWS : CK_WIDE_ROWS;
   it.list = nullptr;
   it.list_chunks = 0;
   if (a.sel) {
-    const int blk = it.narrow ? 0 : tile / a.tiles_per_block, sub = it.narrow ? tile : tile % a.tiles_per_block;
+    const int blk = it.narrow ? 0 : (int)fast_div((uint32_t)tile, (uint32_t)a.tiles_per_block, a.mul_tpb);
+    const int sub = it.narrow ? tile : tile - blk * a.tiles_per_block;
     it.row_end = min(it.n, (blk + 1) * CK_BLOCK) * a.G;
     it.row0 = blk * CK_BLOCK * a.G + sub * rows;
     if (it.row0 >= it.row_end) return false;
@@ -308,9 +360,9 @@ __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, Chun
   // Lengths past the table end with it.
   const int last = (int)min((int64_t)it.pos_max, (int64_t)a.max_blocks * a.page - 1);
   const int chunks = a.sel ? it.list_chunks : last < 0 ? 0 : last / 16 + 1;
-  const int64_t nt = (chunks + 3) / 4;
-  it.c0 = 4 * (int)(nt * it.split / it.splits);
-  it.c1 = min(chunks, 4 * (int)(nt * (it.split + 1) / it.splits));
+  const int nt = (chunks + 3) / 4;   // at most 2^24, and 64 splits
+  it.c0 = 4 * (int)fast_div((uint32_t)(nt * it.split), (uint32_t)it.splits, mul_k);
+  it.c1 = min(chunks, 4 * (int)fast_div((uint32_t)(nt * (it.split + 1)), (uint32_t)it.splits, mul_k));
   return true;
 }
 
@@ -1119,7 +1171,7 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
   if (page < 16 || page > 128 || page % 16)
     return set_error(SA_E_BLOCK, "%s: page %d is not a multiple of 16 in [16, 128]", name, page);
   if (N < 0 || B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > (1 << 15) || max_blocks < 0 || num_pages < 0 ||
-      block_table_stride < max_blocks || num_splits < 0 || num_splits > 64)
+      block_table_stride < max_blocks || num_splits < 0 || num_splits > CK_MAX_SPLITS)
     return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages, "
                      "%d splits (0..64)", name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages,
                      num_splits);
@@ -1167,6 +1219,7 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
   a.mul_Hq = div_mul((uint32_t)Hq);
   a.scale_log2 = sm_scale * 1.44269504088896340736f;
   a.tiles_per_block = (int)((CK_BLOCK * (int64_t)a.G + CK_WIDE_ROWS - 1) / CK_WIDE_ROWS);
+  a.mul_tpb = div_mul((uint32_t)a.tiles_per_block);
   a.key_tiles = (int)((max_keys + CK_KT - 1) / CK_KT);
   a.cus = chunk_cus();
   // Without room for partials nothing is split.
