@@ -511,7 +511,7 @@ int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const 
  * writes them.  Blocks are numbered through the batch, sequence b having ceil(new tokens / 64) of them; the
  * pages of block i and KV head g, each at most once, are
  *   sel[i * sel_sr + g * sel_sh + e] for e in [sel_off[i * off_sr + g * off_sh], sel_off[i * off_sr + g * off_sh + 1])
- * (within sel_width entries).  sel_rows >= N / 64 + min(B, N).
+ * (within sel_width entries).  sel_rows >= N / 64 + B.
  * num_splits: how many workgroups share the keys of a row tile, leaving fp32 partials in the workspace that a
  * second kernel merges.  0: worked out on the device from the lengths, so that the workgroups' key tiles come out
  * about even, within the workspace given (any size; sa_paged_chunk_workspace_bytes() is enough, none means no
@@ -541,7 +541,7 @@ int64_t sa_paged_chunk_workspace_bytes(int N, int B, int Hq, int Hkv, int D, int
  * over the page's k_bounds [num_pages, Hkv, 2, D] (lo, hi): an upper bound of the queries' products with its
  * keys.  fp64 scores; ties go to the lower page; a page whose score is NaN, or which has no valid page id, ranks
  * last.  sel[i * sel_sr + g * sel_sh + ...] (int32) receives the pages in ascending order, zero-padded to `width`, and
- * sel_off [rows, Hkv, 2] (contiguous) 0 and their number.  rows == B, or N / 64 + min(B, N) with cu_seqlens (rows
+ * sel_off [rows, Hkv, 2] (contiguous) 0 and their number.  rows == B, or N / 64 + B with cu_seqlens (rows
  * past the last block are empty); width >= sink + top_k + recent - 1 + the pages that a row's queries may lie in
  * (1, or (62 + page) / page + 1 with cu_seqlens).  The workspace holds scores where the call needs it
  * (sa_paged_block_select_workspace_bytes, 0: none); calls that may run concurrently must not share it.

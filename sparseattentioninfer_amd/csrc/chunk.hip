@@ -1177,9 +1177,9 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
                      num_splits);
   if (!(sm_scale > 0.f) || sm_scale > 1e30f) return set_error(SA_E_SHAPE, "%s: scale %g is not positive", name, sm_scale);
   if ((int64_t)N * Hq > 0x7fffffff) return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d rows are too many", name, N, Hq);
-  if (sel && (!sel_off || sel_width < 0 || sel_rows < (N ? N / CK_BLOCK + std::min(B, N) : 0)))
-    return set_error(SA_E_SHAPE, "%s: a selection needs offsets and %d rows, got %d", name,
-                     N / CK_BLOCK + std::min(B, N), sel_rows);
+  if (sel && (!sel_off || sel_width < 0 || sel_rows < (int64_t)N / CK_BLOCK + B))
+    return set_error(SA_E_SHAPE, "%s: a selection needs offsets and %lld rows, got %d", name,
+                     (long long)N / CK_BLOCK + B, sel_rows);
   if (N == 0 || B == 0) return 0;
   if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || !o)
     return set_error(SA_E_NULL, "%s: NULL pointer", name);

@@ -421,13 +421,13 @@ extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int
   if (top_k < 0 || sink < 0 || recent < 1 || top_k > (1 << 22) || sink > (1 << 22) || recent > (1 << 22))
     return set_error(SA_E_SHAPE, "%s: top_k=%d, sink=%d (not negative), recent=%d (at least 1)", name, top_k, sink, recent);
   const int span = cu_seqlens ? (SEL_BLOCK + page - 2) / page + 1 : 1;   // pages that the queries of a list lie in
-  const int need_rows = cu_seqlens ? N / SEL_BLOCK + std::min(B, N) : B;
+  const int64_t need_rows = cu_seqlens ? (int64_t)N / SEL_BLOCK + B : B;
   if (!cu_seqlens && N != B) return set_error(SA_E_SHAPE, "%s: one token per sequence, but N=%d for B=%d", name, N, B);
   if (rows != need_rows || width < sink + top_k + recent - 1 + span)
-    return set_error(SA_E_SHAPE, "%s: lists [%d, Hkv, %d], needed [%d, Hkv, %d]", name, rows, width, need_rows,
+    return set_error(SA_E_SHAPE, "%s: lists [%d, Hkv, %d], needed [%lld, Hkv, %d]", name, rows, width, (long long)need_rows,
                      sink + top_k + recent - 1 + span);
   if (rows == 0) return 0;
-  if (!q || !k_bounds || !block_table || !kv_lens || !sel || !sel_off) return set_error(SA_E_NULL, "%s: NULL pointer", name);
+  if ((N && !q) || !k_bounds || !block_table || !kv_lens || !sel || !sel_off) return set_error(SA_E_NULL, "%s: NULL pointer", name);
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_bounds) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (q_st | q_sh | bounds_sp | bounds_sh) % 8)
     return set_error(SA_E_ALIGN, "%s: rows must be 16-byte aligned", name);

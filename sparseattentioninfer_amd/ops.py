@@ -996,7 +996,7 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if ok and sel is not None:
         ss, sst = sel.shape, sel.stride()
         ok = (sel.dtype == torch.int32 and sel_off.dtype == torch.int32 and sel.device == dev and sel_off.device == dev
-              and len(ss) == 3 and ss[0] >= qs[0] // CHUNK_BLOCK + min(B, qs[0]) and ss[1] == ps[1]
+              and len(ss) == 3 and ss[0] >= qs[0] // CHUNK_BLOCK + B and ss[1] == ps[1]
               and sel_off.shape == (ss[0], ss[1], 2) and (ss[2] <= 1 or sst[2] == 1) and sel_off.stride(2) == 1)
         if ok:
             sargs = (sel.data_ptr(), sst[0], sst[1], ss[0], ss[2], sel_off.data_ptr(), sel_off.stride(0), sel_off.stride(1))
@@ -1006,7 +1006,7 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                 index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens, sel=sel, sel_off=sel_off),
                 pools=(k_pages, v_pages), B=block_table.size(0) if block_table.dim() else 0,
                 other="q and out must be [N, Hq, D], pools [P, Hkv, page, D] with Hq a multiple of Hkv, sel and sel_off "
-                      f"(both or neither) [at least N // {CHUNK_BLOCK} + min(B, N) rows, Hkv, width] and [rows, Hkv, 2]")
+                      f"(both or neither) [at least N // {CHUNK_BLOCK} + B rows, Hkv, width] and [rows, Hkv, 2]")
     N, Hq, D = qs
     ws = _workspace(name, workspace, _lib.load().sa_paged_chunk_workspace_bytes(
         N, B, Hq, ps[1], D, min(keys * ps[2], 1 << 30), num_splits), dev)
@@ -1039,7 +1039,7 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: tor
 
     For one new token per sequence, ``q [B, Hq, D]`` (the newest, at position ``kv_lens[b] - 1``): ``sel [B, Hkv,
     width]`` and ``sel_off [B, Hkv, 2]`` as :func:`paged_sparse_decode` reads them.  With ``cu_seqlens``, ``q [N, Hq, D]``
-    packed: a list for each block of 64 new tokens, ``[N // 64 + min(B, N), Hkv, width]``, as
+    packed: a list for each block of 64 new tokens, ``[N // 64 + B, Hkv, width]`` (rows past the last block are empty), as
     :func:`paged_chunk_attn` reads it.  ``k_bounds [P, Hkv, 2, D]`` is :func:`paged_append`'s.
 
     A list keeps the first ``sink`` pages, the last ``recent`` (counted back from the page of its first query) and
@@ -1070,7 +1070,7 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: tor
     if cu_seqlens is None:
         rows, span, cu = B, 1, None
     else:
-        rows, span, cu = N // CHUNK_BLOCK + min(B, N), (CHUNK_BLOCK + page - 2) // page + 1, cu_seqlens.data_ptr()
+        rows, span, cu = N // CHUNK_BLOCK + B, (CHUNK_BLOCK + page - 2) // page + 1, cu_seqlens.data_ptr()
     width = sink + top_k + recent - 1 + span
     sel = torch.empty((rows, Hkv, width), dtype=torch.int32, device=dev)
     sel_off = torch.empty((rows, Hkv, 2), dtype=torch.int32, device=dev)

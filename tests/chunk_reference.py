@@ -150,7 +150,7 @@ def select(r: Ragged, q, bounds, *, top_k, sink, recent, tokens):
                 per_head.append(sorted(list(range(min(sink, lo))) + [free[i] for i in best] + list(range(lo, pages))))
             lists.append(per_head)
     N, B = q.size(0), len(r.lens)
-    rows = B if tokens else N // BLOCK + min(B, N)
+    rows = B if tokens else N // BLOCK + B
     span = 1 if tokens else (BLOCK + r.page - 2) // r.page + 1
     sel = torch.zeros(rows, r.Hkv, sink + top_k + recent - 1 + span, dtype=torch.int32)
     off = torch.zeros(rows, r.Hkv, 2, dtype=torch.int32)

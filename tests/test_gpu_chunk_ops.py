@@ -221,7 +221,7 @@ def test_chunk_attention_over_a_selection(case, splits):
     _say("chunk sel", *SHAPES[case], "splits", splits)
     r = Ragged(q_lens, kv_lens, page=page, Hkv=Hkv, D=D, dtype=dtype, seed=90 + case, pad_rows=70)
     q = randn(r.N, Hq, D, seed=120 + case, dtype=dtype)
-    rows = r.N // 64 + min(len(q_lens), r.N)
+    rows = r.N // 64 + len(q_lens)
     g = torch.Generator().manual_seed(case)
     cols = r.table.size(1)
     sel = torch.stack([torch.stack([torch.randperm(cols, generator=g) for _ in range(Hkv)]) for _ in range(rows)]).to(torch.int32)
@@ -347,6 +347,25 @@ def test_select_chunks_and_attend(page, D, dtype, top_k, sink, recent):
     got = _attend(r, q, sel=sel, sel_off=off)
     want, tol, live = attention(r, q, sel.cpu(), off.cpu())
     _check(got, want, tol, live, "selected chunk")
+
+
+def test_more_sequences_than_new_tokens():
+    """Two new tokens among nine sequences, and none at all: rows of lists past the last block are empty."""
+    r, q, (sel, off) = _select_case([0, 0, 1, 0, 0, 0, 1, 0, 0], [70, 0, 900, 1, 5, 64, 333, 8, 2], 64, 4, 2, 128, BF, 2, 1, 1,
+                                    False)
+    assert sel.size(0) == 9 and not off[2:].any()
+    want, tol, live = attention(r, q, sel.cpu(), off.cpu())
+    _check(_attend(r, q, sel=sel, sel_off=off), want, tol, live, "two of nine")
+    for n in (0, 3):
+        q = torch.zeros(0, 4, 64, dtype=BF, device="cuda")
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        bd, table = torch.zeros(2, 2, 2, 64, dtype=BF, device="cuda"), torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+        cu, lens = i32(*[0] * (n + 1)), i32(*[9] * n)
+        sel, off = ops.paged_block_select(q, bd, table, lens, page=64, top_k=1, cu_seqlens=cu)
+        assert sel.shape[:2] == (n, 2) and not sel.any() and not off.any()
+        pool = torch.zeros(2, 2, 64, 64, dtype=BF, device="cuda")
+        assert ops.paged_chunk_attn(q, pool, pool, table, cu, lens, sel=sel, sel_off=off).shape == q.shape
+        ops.paged_append(q[:, :2], q[:, :2], pool, pool.clone(), table, cu, lens, k_bounds=bd)
 
 
 @pytest.mark.parametrize("tokens", [True, False])
