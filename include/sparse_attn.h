@@ -490,8 +490,10 @@ int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_
  * as they are), v as it is.  With Hq > 0 the queries take the same norm and rotation into q_out in the same
  * launch.  Arithmetic as in sa_qk_norm_rope; q, k, v may be views of one projection row.
  * k_bounds (or NULL) [num_pages, Hkv, 2, D] (strides in elements: page, head): the minimum and the maximum of a
- * page's stored keys in each dim.  A page whose first slot is written gets fresh bounds, another has the new
- * keys merged into the stored ones.  No two sequences may write one page.
+ * page's stored keys in each dim (NaN ones are left out).  A page whose first slot is written gets fresh bounds,
+ * another has the new keys merged into the stored ones; so where tokens are dropped and others written in their
+ * place, the bounds of a page that is kept in part stay those of all it held, which is still an upper bound of its
+ * products.  No two sequences may write one page.
  */
 int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                     const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
@@ -506,7 +508,9 @@ int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const 
  * Causal attention of the new tokens over the pages (their own keys included): the row of a token at position p
  * sees the keys j <= p of its sequence; o[row] = sum_j softmax_j(q . k_j * sm_scale) v_j with fp32 statistics
  * and accumulators, 0 for a row that sees no key.  Probabilities are rounded to the element type before the second
- * product.  Query head h reads KV head h / (Hq / Hkv).
+ * product.  Query head h reads KV head h / (Hq / Hkv).  Slots past kv_lens[b] and pages that are not listed are
+ * not used, whatever they hold; the values of the tokens that are there are taken to be finite, as a row that does
+ * not see one of its tile may still multiply it by 0.
  * sel (or NULL: all pages): the logical pages that each block of 64 new tokens sees, as sa_paged_block_select
  * writes them.  Blocks are numbered through the batch, sequence b having ceil(new tokens / 64) of them; the
  * pages of block i and KV head g, each at most once, are

@@ -59,7 +59,6 @@ struct ChunkArgs {
   int Hq, Hkv, G;
   uint32_t mul_G, mul_heads, mul_Hq, mul_tpb;
   float scale_log2;
-  int items;                       // (row tile, split) pairs of the launch at most; workgroups past the last exit
   int tiles_per_block;             // with a selection: wide row tiles of a 64-token block
   int key_tiles;                   // key tiles that a row may see at most: the table's, or the longest list's
   int cus;
@@ -1104,7 +1103,8 @@ static int launch_chunk(const ChunkArgs& a, int64_t groups, hipStream_t s) {
   hipLaunchKernelGGL((chunk_kernel<BF16, D>), dim3((unsigned)groups), dim3(512), 0, s, a);
   if (a.part) {
     const int64_t rows = a.seqs.N * a.Hq, per = 256 / (D / 8);
-    hipLaunchKernelGGL((chunk_combine_kernel<BF16, D>), dim3((unsigned)std::min<int64_t>((rows + per - 1) / per, 2048)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((chunk_combine_kernel<BF16, D>), 
+                       dim3((unsigned)std::min<int64_t>((rows + per - 1) / per, 2048)), dim3(256), 0, s, a);
   }
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "sa_paged_chunk_attn: launch failed: %s", hipGetErrorString(err));
@@ -1175,7 +1175,8 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
     return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages, "
                      "%d splits (0..64)", name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages,
                      num_splits);
-  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return set_error(SA_E_SHAPE, "%s: scale %g is not positive", name, sm_scale);
+  if (!(sm_scale >= 1e-30f && sm_scale <= 1e30f))
+    return set_error(SA_E_SHAPE, "%s: scale %g is not in [1e-30, 1e30]", name, sm_scale);
   if ((int64_t)N * Hq > 0x7fffffff) return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d rows are too many", name, N, Hq);
   if (sel && (!sel_off || sel_width < 0 || sel_rows < (int64_t)N / CK_BLOCK + B))
     return set_error(SA_E_SHAPE, "%s: a selection needs offsets and %lld rows, got %d", name,
@@ -1231,10 +1232,10 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
     a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + chunk_part_header(B));
     a.part_ml = a.part_acc + room * D;
   }
-  const int64_t items = chunk_items(N, B, a.G, Hkv, sel != nullptr, a.splits), groups = items * Hkv;
+  // As many workgroups as any lengths need; those past the last item exit.
+  const int64_t groups = chunk_items(N, B, a.G, Hkv, sel != nullptr, a.splits) * Hkv;
   if (groups > MAX_WORKGROUPS / 2)
     return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
-  a.items = (int)items;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_chunk<true, 128>(a, groups, s) : launch_chunk<true, 64>(a, groups, s);
   return D == 128 ? launch_chunk<false, 128>(a, groups, s) : launch_chunk<false, 64>(a, groups, s);

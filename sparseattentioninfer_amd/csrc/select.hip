@@ -435,7 +435,8 @@ extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int
   if (need && (!workspace || workspace_bytes < need))
     return set_error(SA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", name, (long long)workspace_bytes,
                      (long long)need);
-  if ((int64_t)rows * Hkv > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: %d rows of %d heads are too many", name, rows, Hkv);
+  if ((int64_t)rows * Hkv > MAX_WORKGROUPS / 4)   // of up to 1,024 threads
+    return set_error(SA_E_SHAPE, "%s: %d rows of %d heads are too many", name, rows, Hkv);
   SelectArgs a = {};
   a.q = static_cast<const elem_t*>(q);
   a.q_st = q_st, a.q_sh = q_sh;

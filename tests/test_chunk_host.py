@@ -83,7 +83,7 @@ def _chunk(lib, **o):
 @pytest.mark.parametrize("change,code,text", [
     (dict(dtype=2), -1, b"dtype"), (dict(D=256), -3, b"head dim 256"), (dict(page=40), -4, b"page 40"),
     (dict(Hq=7), -2, b"Hq=7"), (dict(splits=65), -2, b"65 splits"), (dict(splits=-1), -2, b"-1 splits"),
-    (dict(scale=0.0), -2, b"scale"), (dict(scale=float("nan")), -2, b"scale"), (dict(N=1 << 30), -2, b"too many"),
+    (dict(scale=0.0), -2, b"scale"), (dict(scale=1e-40), -2, b"scale"), (dict(scale=-1.0), -2, b"scale"), (dict(scale=float("nan")), -2, b"scale"), (dict(N=1 << 30), -2, b"too many"),
     (dict(sel=FAKE), -2, b"selection"), (dict(sel=FAKE, off=FAKE, rows=1, width=4), -2, b"selection"),
     (dict(q=None), -6, b"NULL"), (dict(lens=None), -6, b"NULL"), (dict(o=FAKE + 2), -8, b"aligned"),
     (dict(st=1026), -8, b"aligned"), (dict(pst=1 << 25), -2, b"token stride"), (dict(pst=-128), -2, b"token stride"),
@@ -118,7 +118,7 @@ def _select(lib, **o):
     (dict(topk=-1), -2, b"top_k=-1"), (dict(recent=0), -2, b"recent=0"), (dict(sink=-2), -2, b"sink=-2"),
     (dict(N=3), -2, b"one token per sequence"), (dict(rows=3), -2, b"lists [3"), (dict(width=3), -2, b"needed [2"),
     (dict(cu=FAKE, N=70, rows=2, width=9), -2, b"needed [3"), (dict(ts=2), -2, b"columns"),
-    (dict(mb=(1 << 21) + 1, ts=1 << 22), -2, b"columns"), (dict(bd=None), -6, b"NULL"), (dict(off=None), -6, b"NULL"),
+    (dict(mb=(1 << 21) + 1, ts=1 << 22), -2, b"columns"), (dict(N=1 << 22, B=1 << 22, rows=1 << 22), -2, b"too many"), (dict(bd=None), -6, b"NULL"), (dict(off=None), -6, b"NULL"),
     (dict(q=FAKE + 4), -8, b"aligned"), (dict(mb=5000, ts=5000), -7, b"workspace")])
 def test_select_refusals(lib, change, code, text):
     assert _select(lib, **change) == code and text in lib.sa_last_error()
