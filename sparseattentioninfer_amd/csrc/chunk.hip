@@ -84,6 +84,9 @@ struct ChunkArgs {
 // a wide one's beside wide ones.  A workgroup costs CK_START of them besides its own: 9.6 us, of which finding its item
 // takes 2.5, the pages of its first tiles 2.6, the tiles 1.5 and the end 3.
 constexpr float CK_START = 5.5f;
+// A division costs the merge, 4 us after narrow and 6.5 after wide items, and for each row of partials its write and
+// read: 1,040 bytes at D = 128, 0.2 ns at the rate of a copy.
+constexpr float CK_MERGE_WIDE = 4.f, CK_MERGE_NARROW = 2.5f, CK_MERGE_ROW = 1.3e-4f;
 constexpr int CK_NARROW = 64;
 constexpr int CK_WIDE_ROWS = 256;
 
@@ -121,8 +124,9 @@ __device__ __forceinline__ SeqShape seq_shape(const ChunkArgs& a, int b) {
   return s;
 }
 
-// Workgroups that share a row tile's keys when one takes at most `limit` key tiles.  A wide one leaves 133 KB of
-// partials (as long as 5 tiles take), so it has at least 8 tiles; a narrow one at least one for each wave.
+// Workgroups that share a row tile's keys when one takes at most `limit` key tiles.  At least
+// 4: one for each wave of a narrow one; of a wide one, whose 256 rows leave 133 KB of partials, fewer do not pay (64 new
+// tokens over 1,024 keys, 32/8 heads, bf16, D = 128: 28.7 us in one, 24.7 in 2, 20.7 in 4, 20.6 in 8, 25.1 in 16).
 constexpr int CK_MAX_SPLITS = 64;
 constexpr int CK_NO_LIMIT = 0x40000000;   // at or past this: no division
 struct SplitRule {
@@ -132,7 +136,7 @@ struct SplitRule {
   // half: a narrow item's key tile counts half of a wide one's.
   __device__ __forceinline__ SplitRule(int l, int half) {
     limit = l;
-    most_wide = max(l, 8);
+    most_wide = max(l, 4);
     most_narrow = max(l >= CK_NO_LIMIT ? l : l << half, 4);
     rcp_wide = __builtin_amdgcn_rcpf((float)most_wide);
     rcp_narrow = __builtin_amdgcn_rcpf((float)most_narrow);
@@ -215,10 +219,12 @@ __device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqSh
   // When it ends.  In one round: with the longest workgroup.  Else, handed out longest first: the mean load, or
   // two of those longer than half of it where they outnumber the CUs (their lengths taken as spread evenly).
   const float mean = (work + groups * CK_START) / cus;
+  // Narrow items that do not fill the chip are not bound by HBM: 0.5 us for a tile instead of 1.45.
+  const float alone = half ? 1.f : fminf(fmaxf(0.35f, groups / cus), 1.f);
   float one = 0.f, many = 0.f, lo = __builtin_inff(), hi = 0.f;
   each([&](float st, float k, float nt, float nt0, float, float w) {
     if (st == 0.f) return;
-    const float x = w * __builtin_amdgcn_rcpf(k), h = nt * x + CK_START, l = nt0 * x + CK_START;
+    const float x = w * alone * __builtin_amdgcn_rcpf(k), h = nt * x + CK_START, l = nt0 * x + CK_START;
     one = fmaxf(one, h);
     if (h <= 0.5f * mean) return;
     const float from = fmaxf(l, 0.5f * mean);
@@ -233,6 +239,7 @@ __device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqSh
   float time = one;
   if (groups > cus) time = fmaxf(one, 1.08f * mean);
   if (groups > cus && many > cus) time = fmaxf(time, 2.f * (lo + (hi - lo) * (many - cus) / many));
+  if (rows > 0.f) time += (half ? CK_MERGE_WIDE : CK_MERGE_NARROW) + CK_MERGE_ROW * rows;
   // The partials must fit, and no more workgroups are added than there are CUs (chunk_items: the launch has that
   // many to spare, and idle ones cost time too).  No division always does.
   if (rows * 1.001f > (float)a.part_rows || groups > tiles * heads + cus) time = __builtin_inff();
@@ -1150,8 +1157,15 @@ extern "C" int64_t sa_paged_chunk_workspace_bytes(int N, int B, int Hq, int Hkv,
   const int64_t key_tiles = (max_keys + CK_KT - 1) / CK_KT;
   const int64_t all = (int64_t)N * Hq;
   if (num_splits > 1) return chunk_part_header(B) + all * std::min<int64_t>(num_splits, key_tiles) * (D + 2) * 4;
-  // Nothing is gained where the row tiles fill the chip several times over, twice for those of one sequence.
-  if (key_tiles <= 4 || (int64_t)N * (Hq / Hkv) / CK_WIDE_ROWS * Hkv >= (B == 1 ? 2 : 8) * (int64_t)chunk_cus()) return 0;
+  // Nothing is gained where the row tiles fill the chip several times over, twice for those of one sequence, nor by
+  // dividing few keys.  bf16, D = 128, 32/8 heads, divided against not: 8 sequences of 4 new tokens 13.6 us against 9.8 at
+  // 512 keys, 18.6 against 15.2 at 1,024; 4 of 128 (wide) 22.1 against 19.0 at 512, but one of 64 21.9 against 28.8 at
+  // 1,024.  One sequence of one token takes 11.7 against 12.9 at 1,024: less than the 3.5 us of host time that the
+  // workspace and the second launch cost, so narrow items are not divided there either.
+  const bool narrow = (int64_t)N * (Hq / Hkv) <= CK_NARROW * (int64_t)B;
+  if (key_tiles <= (narrow ? 16 : 8) ||
+      (int64_t)N * (Hq / Hkv) / CK_WIDE_ROWS * Hkv >= (B == 1 ? 2 : 8) * (int64_t)chunk_cus())
+    return 0;
   return chunk_part_header(B) + std::min(all * std::min<int64_t>(key_tiles / 4 + 1, 64), CK_PART_ROWS) * (D + 2) * 4;
 }
 

@@ -100,6 +100,7 @@ def test_chunk_workspace_sizes(lib):
     assert size(4, 2, 8, 2, 128, 100, 3) == 256 + 2 * 4 * 8 * 130 * 4    # at most one for 64 keys
     assert size(4, 2, 8, 2, 128, 1 << 16, 0) > 0
     assert size(4, 2, 8, 2, 128, 256, 0) == 0                    # too few keys to divide
+    assert size(4, 2, 8, 2, 128, 1024, 0) == 0 and size(40, 2, 8, 2, 128, 512, 0) == 0
     assert size(0, 2, 8, 2, 128, 1 << 16, 0) == 0 and size(4, 2, 8, 2, 128, 0, 4) == 0
 
 
