@@ -864,29 +864,36 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     may be ``q`` / ``k`` themselves; by default they are new contiguous tensors.
     """
     name = "qk_norm_rope"
-    if q_out is None:
-        q_out = _empty_like(q)
-    if k_out is None:
-        k_out = _empty_like(k)
     qs, ks, dt, dev, n = q.shape, k.shape, q.dtype, q.device, q.dim()
     D = qs[-1] if n else 0
-    qst, kst, qot, kot = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-    if not (q.is_cuda and dt in _DTYPES and (n == 3 or n == 4) and len(ks) == n and qs[:-2] == ks[:-2] and ks[-1] == D
-            and k.dtype == dt and k.device == dev and q_out.shape == qs and q_out.dtype == dt and q_out.device == dev
-            and k_out.shape == ks and k_out.dtype == dt and k_out.device == dev
-            and qst[-1] == 1 and kst[-1] == 1 and qot[-1] == 1 and kot[-1] == 1
-            and (q_weight is None or (q_weight.shape == (D,) and q_weight.dtype == dt and q_weight.device == dev
-                                      and q_weight.is_contiguous()))
-            and (k_weight is None or (k_weight.shape == (D,) and k_weight.dtype == dt and k_weight.device == dev
-                                      and k_weight.is_contiguous()))
-            and inv_freq.dtype == torch.float32 and inv_freq.shape == (D // 2,) and inv_freq.is_contiguous()
-            and inv_freq.device == dev and positions.dtype == torch.int64 and positions.device == dev
-            and positions.shape == qs[:-2] and (positions.size(-1) <= 1 or positions.stride(-1) == 1)):
+    qst, kst = q.stride(), k.stride()
+    ok = (q.is_cuda and dt in _DTYPES and (n == 3 or n == 4) and k.dtype == dt and k.device == dev and len(ks) == n
+          and ks[-1] == D and qst[-1] == 1 and kst[-1] == 1
+          and (q_weight is None or (q_weight.shape == (D,) and q_weight.dtype == dt and q_weight.device == dev
+                                    and q_weight.is_contiguous()))
+          and (k_weight is None or (k_weight.shape == (D,) and k_weight.dtype == dt and k_weight.device == dev
+                                    and k_weight.is_contiguous()))
+          and inv_freq.dtype == torch.float32 and inv_freq.shape == (D // 2,) and inv_freq.is_contiguous()
+          and inv_freq.device == dev and positions.dtype == torch.int64 and positions.device == dev)
+    if n == 3:
+        ok = ok and ks[0] == qs[0] and positions.shape == (qs[0],) and (qs[0] < 2 or positions.stride(0) == 1)
+    else:
+        ok = ok and ks[:2] == qs[:2] and positions.shape == qs[:2] and (qs[1] < 2 or positions.stride(1) == 1)
+    if q_out is None:
+        q_out = _empty_like(q)
+    elif ok:
+        ok = q_out.shape == qs and q_out.dtype == dt and q_out.device == dev and q_out.stride(-1) == 1
+    if k_out is None:
+        k_out = _empty_like(k)
+    elif ok:
+        ok = k_out.shape == ks and k_out.dtype == dt and k_out.device == dev and k_out.stride(-1) == 1
+    if not ok:
         _refuse(name, q, heads=dict(q=q, k=k, q_out=q_out, k_out=k_out, q_weight=q_weight, k_weight=k_weight), index={},
                 weights=(q_weight, k_weight), inv_freq=inv_freq,
                 other="q and k must be [N, H, D] or [B, T, H, D] of the same tokens, outputs like them, positions int64 "
                       f"of those tokens on {dev}, contiguous in the last dim; got positions {positions.dtype} "
                       f"{tuple(positions.shape)} on {positions.device}")
+    qot, kot = q_out.stride(), k_out.stride()
     if n == 3:
         B, T, pos_sb = 1, qs[0], 0
         qst, kst, qot, kot = (0, *qst), (0, *kst), (0, *qot), (0, *kot)
@@ -976,12 +983,9 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     concurrent calls must not share.  Rows of ``out`` of no sequence are left as they are.
     """
     name = "paged_chunk_attn"
-    if out is None:
-        out = _empty_like(q)
     dt, dev, qs, ps, B = q.dtype, q.device, q.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
-    qst, ost, pst = q.stride(), out.stride(), k_pages.stride()
-    ok = (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and out.shape == qs and out.dtype == dt
-          and out.device == dev and ost[2] == 1 and len(ps) == 4 and v_pages.shape == ps and ps[3] == qs[2]
+    qst, pst = q.stride(), k_pages.stride()
+    ok = (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and len(ps) == 4 and v_pages.shape == ps and ps[3] == qs[2]
           and ps[1] > 0 and qs[1] % ps[1] == 0
           and k_pages.dtype == dt and v_pages.dtype == dt and k_pages.device == dev and v_pages.device == dev
           and pst[3] == 1 and v_pages.stride() == pst
@@ -990,6 +994,10 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
           and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
           and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
           and (sel is None) == (sel_off is None))
+    if out is None:
+        out = _empty_like(q)
+    elif ok:
+        ok = out.shape == qs and out.dtype == dt and out.device == dev and out.stride(2) == 1
     sargs = (None, 0, 0, 0, 0, None, 0, 0)
     max_blocks = block_table.size(-1) if ok else 0
     keys = max_blocks
@@ -1008,6 +1016,7 @@ def paged_chunk_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                 other="q and out must be [N, Hq, D], pools [P, Hkv, page, D] with Hq a multiple of Hkv, sel and sel_off "
                       f"(both or neither) [at least N // {CHUNK_BLOCK} + B rows, Hkv, width] and [rows, Hkv, 2]")
     N, Hq, D = qs
+    ost = out.stride()
     ws = _workspace(name, workspace, _lib.load().sa_paged_chunk_workspace_bytes(
         N, B, Hq, ps[1], D, min(keys * ps[2], 1 << 30), num_splits), dev)
     _call("sa_paged_chunk_attn", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_pages.data_ptr(),
