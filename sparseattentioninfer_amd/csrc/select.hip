@@ -11,14 +11,13 @@
 // those between, ties to the lowest page.  Pages between are full and wholly visible to every query of the list.
 //
 // P, N and the scores are fp64: which page is the last one in depends on the order of near-equal scores, and in fp32
-// that order would follow the order of summation.  It costs little: the bounds' bytes are the bound (16,384 tokens
-// of 64, 8 KV heads, 64 sequences: 67 MB, and 4.4 fp64 operations a byte).
+// that order would follow the order of summation.  It costs little: a page's 4 D bytes take 2 D fp64 multiply-adds.
 //
 // One workgroup makes a list: scores of all its pages as order-preserving 64-bit keys in LDS, the top_k-th key by
 // radix selection (8 bits a pass, from the highest bit in which the keys differ), then the kept pages in ascending
-// order by ballots.  Few lists get workgroups of 1,024 threads, many of 512.  All of it runs
-// once or a few times, so its time is latency and instruction fetch: loops are kept rolled.  Where a list has more pages than fit
-// LDS, the scores are computed by workgroups of their own, into the workspace.
+// order by ballots.  All of it runs once or a few times, so its time is latency and instruction fetch: loops are kept
+// rolled.  Few lists of many pages, and those of more pages than fit LDS, are scored by workgroups of their own first,
+// into the workspace.
 #include <algorithm>
 
 #include "ragged.h"
@@ -27,8 +26,18 @@ namespace sa {
 
 constexpr int SEL_BLOCK = 64;          // new tokens that share one list
 constexpr int SEL_LDS_PAGES = 4096;    // keys of a list held in LDS
-constexpr int SEL_FEW_LISTS = 256;     // up to one workgroup per CU: of 1,024 threads
-constexpr int SEL_PAGES_PER_WG = 128;  // pages scored by a workgroup of its own
+// Few lists of many pages leave most CUs idle, so their pages are scored by workgroups of their own first.  One token a
+// sequence, D = 128, bf16, us in one workgroup a list against apart: 8 lists of 512 pages 17.2 / 10.7, of 4,096 70.6 / 22;
+// 64 of 512 17.5 / 14.7, of 4,096 77.4 / 49.5; but 128 of 512 20.2 / 20.7, 256 of 1,024 31 / 42.  Of 256 pages, 12.7 / 10.1 for
+// 8 lists, it is less than the host time of the second launch and the workspace (3.5).
+constexpr int SEL_APART_LISTS = 64, SEL_APART_PAGES = 256;
+// Pages of such a workgroup: as many as make SEL_SCORE_GROUPS of them within these limits.  Each sums the queries again,
+// so more cost time (32 lists of 2,048 pages: 32 a workgroup 30 us, 64 23.7, 128 23.0; 512 lists of 4,096: 128 284, 4,096
+// 355), and fewer leave CUs idle (8 lists of 512 pages: 64 a workgroup 11.7, 32 10.6).
+constexpr int SEL_SCORE_GROUPS = 512, SEL_SCORE_MIN = 32, SEL_SCORE_MAX = 128;
+// Threads of a workgroup that scores its own list: 1,024 up to one workgroup per CU, if its pages are many, else 512 (256
+// lists of 1,024 pages: 31 us with 1,024, 34 with 512; of 128: 14.0, 10.9; 264 lists of 1,024: 55, 43).
+constexpr int SEL_FEW_LISTS = 256, SEL_FEW_PAGES = 512;
 
 struct SelectArgs {
   const elem_t* q;
@@ -46,7 +55,8 @@ struct SelectArgs {
   int64_t sel_sr, sel_sh;
   int width;
   int32_t* off;                        // [rows, Hkv, 2]
-  unsigned long long* keys;            // workspace [rows, Hkv, max_blocks], or NULL: keys stay in LDS
+  int score_pages;                     // pages scored by a workgroup of its own
+  unsigned long long* keys;            // workspace [rows, Hkv, max_blocks], or NULL: a list's workgroup scores its pages
 };
 
 // The queries of one list and the pages it may keep.
@@ -335,20 +345,20 @@ struct Select {
   }
 };
 
-// Scores of SEL_PAGES_PER_WG pages of a list, into the workspace.
+// Scores of a.score_pages pages of a list, into the workspace.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void select_score_kernel(const SelectArgs a) {
   using S = Select<BF16, D, 256>;
   __shared__ typename S::Shared sh;
   SelectItem it;
   if (!find_list(a, blockIdx.x, it) || it.lo - it.head <= a.top_k || a.top_k == 0) return;
-  const int p0 = it.head + (int)blockIdx.y * SEL_PAGES_PER_WG, p1 = min(it.lo, p0 + SEL_PAGES_PER_WG);
+  const int p0 = it.head + (int)blockIdx.y * a.score_pages, p1 = min(it.lo, p0 + a.score_pages);
   if (p0 >= p1) return;
   S::pool(a, it, sh);
   S::score(a, it, sh, p0, p1, a.keys + (int64_t)blockIdx.x * a.max_blocks);
 }
 
-// A list: with LDS its scores too, else from those of the workspace.
+// A list, of the workspace's scores or its own.  LDS: it has the keys there.
 template <bool BF16, int D, int T, bool LDS>
 __global__ __launch_bounds__(T) void select_kernel(const SelectArgs a) {
   using S = Select<BF16, D, T>;
@@ -363,8 +373,13 @@ __global__ __launch_bounds__(T) void select_kernel(const SelectArgs a) {
   unsigned long long* keys = LDS ? s_keys : a.keys + (int64_t)blockIdx.x * a.max_blocks;
   if (ranked) {
     if constexpr (LDS) {
-      S::pool(a, it, sh);
-      S::score(a, it, sh, it.head, it.lo, keys);
+      if (a.keys) {
+        const unsigned long long* from = a.keys + (int64_t)blockIdx.x * a.max_blocks;
+        for (int x = it.head + threadIdx.x; x < it.lo; x += T) keys[x] = from[x];
+      } else {
+        S::pool(a, it, sh);
+        S::score(a, it, sh, it.head, it.lo, keys);
+      }
       __syncthreads();
     }
     S::find_cut(keys, it.head, it.lo, a.top_k, sh);
@@ -376,16 +391,17 @@ template <bool BF16, int D>
 static int launch_select(const SelectArgs& a, hipStream_t s) {
   const int64_t lists = (int64_t)a.rows * a.Hkv;
   const dim3 grid((unsigned)lists);
-  const size_t lds = a.keys ? 0 : (size_t)a.max_blocks * 8;
-  if (a.keys) {
+  const bool in_lds = a.max_blocks <= SEL_LDS_PAGES;
+  const size_t lds = in_lds ? (size_t)a.max_blocks * 8 : 0;
+  if (a.keys)
     hipLaunchKernelGGL((select_score_kernel<BF16, D>),
-                       dim3((unsigned)lists, (a.max_blocks + SEL_PAGES_PER_WG - 1) / SEL_PAGES_PER_WG), dim3(256), 0, s, a);
+                       dim3((unsigned)lists, (a.max_blocks + a.score_pages - 1) / a.score_pages), dim3(256), 0, s, a);
+  if (!in_lds)
     hipLaunchKernelGGL((select_kernel<BF16, D, 1024, false>), grid, dim3(1024), lds, s, a);
-  } else if (lists <= SEL_FEW_LISTS) {
+  else if (!a.keys && lists <= SEL_FEW_LISTS && a.max_blocks > SEL_FEW_PAGES)
     hipLaunchKernelGGL((select_kernel<BF16, D, 1024, true>), grid, dim3(1024), lds, s, a);
-  } else {
+  else
     hipLaunchKernelGGL((select_kernel<BF16, D, 512, true>), grid, dim3(512), lds, s, a);
-  }
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "sa_paged_block_select: launch failed: %s", hipGetErrorString(err));
 }
@@ -397,7 +413,8 @@ using namespace sa;
 extern "C" int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks) {
   if (rows < 1 || Hkv < 1 || max_blocks < 1) return 0;
   const int64_t lists = (int64_t)rows * Hkv;
-  return max_blocks > SEL_LDS_PAGES ? lists * max_blocks * 8 : 0;
+  const bool apart = max_blocks > SEL_LDS_PAGES || (lists <= SEL_APART_LISTS && max_blocks > SEL_APART_PAGES);
+  return apart ? lists * max_blocks * 8 : 0;
 }
 
 extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k_bounds,
@@ -453,6 +470,8 @@ extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int
   a.sel_sr = sel_sr, a.sel_sh = sel_sh, a.width = width;
   a.off = sel_off;
   a.keys = need ? static_cast<unsigned long long*>(workspace) : nullptr;
+  const int64_t pages = (int64_t)rows * Hkv * max_blocks;
+  a.score_pages = (int)std::min<int64_t>(std::max<int64_t>(pages / SEL_SCORE_GROUPS, SEL_SCORE_MIN), SEL_SCORE_MAX);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == SA_DTYPE_BF16) return D == 128 ? launch_select<true, 128>(a, s) : launch_select<true, 64>(a, s);
   return D == 128 ? launch_select<false, 128>(a, s) : launch_select<false, 64>(a, s);

@@ -104,6 +104,14 @@ def test_chunk_workspace_sizes(lib):
     assert size(0, 2, 8, 2, 128, 1 << 16, 0) == 0 and size(4, 2, 8, 2, 128, 0, 4) == 0
 
 
+def test_select_workspace_sizes(lib):
+    size = lib.sa_paged_block_select_workspace_bytes
+    assert size(8, 8, 257) == 64 * 257 * 8 and size(1, 1, 4096) == 4096 * 8     # few lists of many pages
+    assert size(8, 8, 256) == 0 and size(9, 8, 257) == 0 and size(9, 8, 4096) == 0
+    assert size(9, 8, 4097) == 72 * 4097 * 8
+    assert size(0, 8, 5000) == 0 and size(8, 8, 0) == 0
+
+
 def _select(lib, **o):
     a = dict(dtype=0, q=FAKE, st=1024, sh=128, bd=FAKE, pages=8, table=FAKE, ts=4, mb=4, cu=None, lens=FAKE, N=2, B=2, Hq=8,
              Hkv=2, D=128, page=64, topk=2, sink=1, recent=1, sel=FAKE, rows=2, width=4, off=FAKE, ws=None, wsb=0)

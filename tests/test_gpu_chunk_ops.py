@@ -332,6 +332,39 @@ def test_select_many_pages(lists):
     _select_case([1] * lists, [16 * 300 + 3 + 16 * (b % 40) for b in range(lists)], 16, 2, 1, 64, BF, 33, 1, 2, True)
 
 
+@pytest.mark.parametrize("lists,pages", [(1, 257), (64, 257), (65, 257), (3, 600), (65, 513), (1, 4096)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_select_borders_of_the_forms(lists, pages, ties):
+    """On both sides of where pages are scored apart, and of where a list takes a larger workgroup; short lists among them."""
+    _say("select borders", lists, pages, ties)
+    _select_case([1] * lists, [16 * pages - 7 * b for b in range(lists - 1)] + [16 * pages if lists == 1 else 20], 16, 2, 1,
+                 64, BF, 33, 1, 2, True, ties=ties, seed=230)
+
+
+def test_select_chunks_scored_apart():
+    _say("select chunks apart")
+    _select_case([130, 0, 1, 64, 65], [16 * 300, 50, 16 * 280 + 3, 64, 16 * 520], 16, 4, 2, 128, HF, 20, 1, 1, False, seed=240)
+
+
+def test_select_apart_on_a_replayed_graph():
+    """Each replay scores the queries of that moment, in the same workspace."""
+    _say("select graph")
+    r, q, (sel, off) = _select_case([1] * 2, [16 * 400, 16 * 300 + 3], 16, 4, 2, 64, BF, 9, 1, 1, True, seed=250)
+    bounds, (table, lens) = bounds_of(r).cuda(), r.gpu("table", "kv_lens")
+    x = q.cuda()
+    pick = dict(page=16, top_k=9, sink=1, recent=1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.paged_block_select(x, bounds, table, lens, **pick)
+    for i in range(4):
+        x.copy_(randn(*q.shape, seed=260 + i))
+        g.replay()
+        want = ops.paged_block_select(x, bounds, table, lens, **pick)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+        assert torch.equal(got[0].cpu(), select(r, x.cpu(), bounds.cpu(), tokens=True, top_k=9, sink=1, recent=1)[0]), i
+
+
 @pytest.mark.parametrize("ties", [False, True])
 def test_select_more_pages_than_lds_holds(ties):
     _say("select 5000 pages")
