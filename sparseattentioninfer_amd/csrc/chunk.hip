@@ -412,7 +412,8 @@ struct ChunkWindow {
 };
 
 // 32 rows to a workgroup: its first four waves hold the same rows and divide the keys, each with tiles of its own in
-// LDS and no barrier before they merge.  Bound by the keys' bytes: a wave keeps 32 KB of loads in flight.
+// LDS and no barrier before they merge.  Bound by the keys' bytes: a wave keeps 32 KB of loads in flight.  8 sequences of
+// 4 new tokens over 4,096 keys, 32/8 heads, bf16, D = 128: 31 us with the merge, 134 MB.
 template <bool BF16, int D>
 struct ChunkNarrow : StagedTile {
   using E = Elem<BF16>;
@@ -659,7 +660,9 @@ struct ChunkNarrow : StagedTile {
 // with a wait for those of the step before, so a tile has two steps to arrive; the waves read K(i + 1), V(i) and
 // V(i - 1) meanwhile, hence three K and four V buffers.
 // A row's reference is the maximum of its first tile and is raised only when its probabilities would pass the
-// element type's range (Chunk::REFIT_SUM), so the common step never touches O with vector instructions.
+// element type's range (REFIT_SUM), so the common step never touches O with vector instructions.
+// Bound by the step: 1.75 us of it per tile at D = 128 with the chip full, 1.35 at D = 64 (exponentials).  8K new tokens
+// over 32K keys, 32/8 heads, bf16, take 3.2 ms, 1.20 PFLOP/s where a large matrix product reaches 1.44.
 template <bool BF16, int D>
 struct ChunkWide : StagedTile {
   using E = Elem<BF16>;

@@ -15,10 +15,14 @@
 // reduction over D/16 neighbouring lanes.  One pass's loads run under the pass before (loops are kept rolled: short
 // calls are bound by latency and instruction fetch).
 //
-// Pages: windows are aligned to positions, in multiples of the page, so the tokens that a chunk adds to one page
-// belong to one window, and one wave sees all of them for a head.  It keeps their minimum and maximum in
+// Pages: with bounds a window is the positions of one page, else 16, so the tokens that a chunk adds to one page
+// belong to one window where bounds need it, and one wave sees all of them for a head.  It keeps their minimum and maximum in
 // registers and updates the page's bounds with plain stores: merged with the stored bounds when the page held
 // tokens before, else written fresh.  Min and max are exact and have no order, so the result has none either.
+//
+// Measured, bf16, D = 128, 32 + 8 heads: 32K tokens unpaged 136 us, 4.9 TB/s (a copy reaches 5.4); 8K tokens in 8
+// sequences into pages of 16 with bounds 50 us, 4.0 TB/s, of which the kernel takes 45 to 47; 64 single tokens 7.3 us,
+// the latency of four dependent reads (lengths, table, rows, bounds).
 #include <algorithm>
 
 #include "lds_tile.h"

@@ -1083,8 +1083,10 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: tor
     width = sink + top_k + recent - 1 + span
     sel = torch.empty((rows, Hkv, width), dtype=torch.int32, device=dev)
     sel_off = torch.empty((rows, Hkv, 2), dtype=torch.int32, device=dev)
-    ws = _workspace(name, workspace, _lib.load().sa_paged_block_select_workspace_bytes(rows, Hkv, max_blocks), dev)
+    need = _lib.load().sa_paged_block_select_workspace_bytes(rows, Hkv, max_blocks)
+    ws = _workspace(name, workspace, need, dev)
     _call("sa_paged_block_select", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_bounds.data_ptr(), bst[0], bst[1],
           bs[0], block_table.data_ptr(), block_table.stride(0), max_blocks, cu, kv_lens.data_ptr(), N, B, Hq, Hkv, D, page,
-          top_k, sink, recent, sel.data_ptr(), Hkv * width, width, rows, width, sel_off.data_ptr(), *_ws_bytes(ws))
+          top_k, sink, recent, sel.data_ptr(), Hkv * width, width, rows, width, sel_off.data_ptr(),
+          None if ws is None else ws.data_ptr(), need)
     return sel, sel_off
