@@ -365,6 +365,21 @@ def test_select_apart_on_a_replayed_graph():
         assert torch.equal(got[0].cpu(), select(r, x.cpu(), bounds.cpu(), tokens=True, top_k=9, sink=1, recent=1)[0]), i
 
 
+def test_select_in_a_given_workspace():
+    """What the workspace holds does not matter, and what is behind the bytes needed stays; one too small is refused."""
+    _say("select workspace")
+    r, q, (sel, off) = _select_case([1] * 2, [16 * 400, 16 * 300 + 3], 16, 4, 2, 64, BF, 9, 1, 1, True, seed=270)
+    bounds, (table, lens) = bounds_of(r).cuda(), r.gpu("table", "kv_lens")
+    need = 2 * 2 * table.size(1) * 8
+    ws = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")
+    pick = dict(page=16, top_k=9, sink=1, recent=1)
+    got = ops.paged_block_select(q.cuda(), bounds, table, lens, workspace=ws, **pick)
+    assert torch.equal(got[0], sel) and torch.equal(got[1], off)
+    assert (ws[need:] == 255).all()
+    with pytest.raises(AssertionError, match="workspace"):
+        ops.paged_block_select(q.cuda(), bounds, table, lens, workspace=ws[:need - 16], **pick)
+
+
 @pytest.mark.parametrize("ties", [False, True])
 def test_select_more_pages_than_lds_holds(ties):
     _say("select 5000 pages")
