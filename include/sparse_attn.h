@@ -511,8 +511,8 @@ int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const 
  * product.  Query head h reads KV head h / (Hq / Hkv).  Slots past kv_lens[b] and pages that are not listed are
  * not used, whatever they hold; the values of the tokens that are there are taken to be finite, as a row that does
  * not see one of its tile may still multiply it by 0.
- * sel (or NULL: all pages): the logical pages that each block of 64 new tokens sees, as sa_paged_block_select
- * writes them.  Blocks are numbered through the batch, sequence b having ceil(new tokens / 64) of them; the
+ * sel with sel_off (both NULL: all pages): the logical pages that each block of 64 new tokens sees, as
+ * sa_paged_block_select writes them (with a sel_width of 0, where sel may be NULL, no row sees a key).  Blocks are numbered through the batch, sequence b having ceil(new tokens / 64) of them; the
  * pages of block i and KV head g, each at most once, are
  *   sel[i * sel_sr + g * sel_sh + e] for e in [sel_off[i * off_sr + g * off_sh], sel_off[i * off_sr + g * off_sh + 1])
  * (within sel_width entries).  sel_rows >= N / 64 + B.

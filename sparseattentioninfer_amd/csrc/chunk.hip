@@ -47,7 +47,8 @@ struct ChunkArgs {
   int max_blocks, num_pages, page;
   uint32_t mul_page;
   Ragged seqs;
-  // selection (NULL: every page): row of query block i, KV head g: sel[i * sel_sr + g * sel_sh + e]
+  // selection (sel_off NULL: every page): row of query block i, KV head g: sel[i * sel_sr + g * sel_sh + e]; sel is NULL
+  // where its rows have no entry
   const int32_t* sel;
   int64_t sel_sr, sel_sh;
   const int32_t* sel_off;
@@ -118,7 +119,7 @@ __device__ __forceinline__ SeqShape seq_shape(const ChunkArgs& a, int b) {
   if (is_narrow(a, s.n))
     s.tiles = ((int)rows + CK_ROWS - 1) / CK_ROWS;
   else
-    s.tiles = a.sel ? (s.n + CK_BLOCK - 1) / CK_BLOCK * a.tiles_per_block : (int)((rows + CK_WIDE_ROWS - 1) / CK_WIDE_ROWS);
+    s.tiles = a.sel_off ? (s.n + CK_BLOCK - 1) / CK_BLOCK * a.tiles_per_block : (int)((rows + CK_WIDE_ROWS - 1) / CK_WIDE_ROWS);
   s.nt = min((s.end + CK_KT - 1) / CK_KT, a.key_tiles);
   s.nt0 = min((max(s.end - s.n, 0) + CK_KT) / CK_KT, s.nt);
   return s;
@@ -300,9 +301,9 @@ __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, Chun
       if (b0 + lane < a.seqs.B) s = seq_shape(a, b0 + lane);
     }
     const int narrow = is_narrow(a, s.n), k = rule.splits(a.splits, narrow, s.nt);
-    const int c = s.tiles * k, blocks = a.sel ? (s.n + CK_BLOCK - 1) / CK_BLOCK : 0;
+    const int c = s.tiles * k, blocks = a.sel_off ? (s.n + CK_BLOCK - 1) / CK_BLOCK : 0;
     const int rows = k > 1 ? s.n * k * a.Hq : 0;   // all of them fit 31 bits: part_rows does
-    const int ib = a.sel ? scan_lanes(blocks) : 0, ir = split ? scan_lanes(rows) : 0;
+    const int ib = a.sel_off ? scan_lanes(blocks) : 0, ir = split ? scan_lanes(rows) : 0;
     if (first && b0 + lane < a.seqs.B) a.part[b0 + lane] = SeqPart{part0 + ir - rows, k, s.n, rule.limit < CK_NO_LIMIT};
     // The sequences in their order: lane i then holds the item count and the lane of the i-th.
     int co = c, from = lane;
@@ -345,7 +346,7 @@ __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, Chun
   const int rows = it.narrow ? CK_ROWS : CK_WIDE_ROWS;
   it.list = nullptr;
   it.list_chunks = 0;
-  if (a.sel) {
+  if (a.sel_off) {
     const int blk = it.narrow ? 0 : (int)fast_div((uint32_t)tile, (uint32_t)a.tiles_per_block, a.mul_tpb);
     const int sub = it.narrow ? tile : tile - blk * a.tiles_per_block;
     it.row_end = min(it.n, (blk + 1) * CK_BLOCK) * a.G;
@@ -365,7 +366,7 @@ __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, Chun
   it.pos_max = it.start + (int)fast_div((uint32_t)(it.row_end - 1), (uint32_t)a.G, a.mul_G);
   // Lengths past the table end with it.
   const int last = (int)min((int64_t)it.pos_max, (int64_t)a.max_blocks * a.page - 1);
-  const int chunks = a.sel ? it.list_chunks : last < 0 ? 0 : last / 16 + 1;
+  const int chunks = a.sel_off ? it.list_chunks : last < 0 ? 0 : last / 16 + 1;
   const int nt = (chunks + 3) / 4;   // at most 2^24, and 64 splits
   it.c0 = 4 * (int)fast_div((uint32_t)(nt * it.split), (uint32_t)it.splits, mul_k);
   it.c1 = min(chunks, 4 * (int)fast_div((uint32_t)(nt * (it.split + 1)), (uint32_t)it.splits, mul_k));
@@ -1195,11 +1196,12 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
   if (!(sm_scale >= 1e-30f && sm_scale <= 1e30f))
     return set_error(SA_E_SHAPE, "%s: scale %g is not in [1e-30, 1e30]", name, sm_scale);
   if ((int64_t)N * Hq > 0x7fffffff) return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d rows are too many", name, N, Hq);
-  if (sel && (!sel_off || sel_width < 0 || sel_rows < (int64_t)N / CK_BLOCK + B))
+  const bool selected = sel || sel_off;
+  if (selected && (!sel_off || sel_width < 0 || sel_rows < (int64_t)N / CK_BLOCK + B))
     return set_error(SA_E_SHAPE, "%s: a selection needs offsets and %lld rows, got %d", name,
                      (long long)N / CK_BLOCK + B, sel_rows);
   if (N == 0 || B == 0) return 0;
-  if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || !o)
+  if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || !o || (selected && sel_width && !sel))
     return set_error(SA_E_NULL, "%s: NULL pointer", name);
   if (bad_ptr(q) || bad_ptr(k_pages) || bad_ptr(v_pages) || bad_ptr(o) || bad_ptr(workspace) ||
       (q_st | q_sh | pages_sp | pages_sh | pages_st | o_st | o_sh) % 8)
@@ -1208,7 +1210,7 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
     return set_error(SA_E_SHAPE, "%s: token stride %lld of the pools", name, (long long)pages_st);
   if (num_splits > 1 && (int64_t)N * Hq * num_splits > 0x7fffffff)
     return set_error(SA_E_SHAPE, "%s: N=%d x Hq=%d x %d splits are too many partial rows", name, N, Hq, num_splits);
-  const int64_t max_keys = std::min<int64_t>((int64_t)(sel ? std::min(max_blocks, sel_width) : max_blocks) * page, 1 << 30);
+  const int64_t max_keys = std::min<int64_t>((int64_t)(selected ? std::min(max_blocks, sel_width) : max_blocks) * page, 1 << 30);
   const int64_t need = sa_paged_chunk_workspace_bytes(N, B, Hq, Hkv, D, (int)max_keys, num_splits);
   if (num_splits > 1 && need && (!workspace || workspace_bytes < need))
     return set_error(SA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", name, (long long)workspace_bytes,
@@ -1250,7 +1252,7 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
     a.part_ml = a.part_acc + room * D;
   }
   // As many workgroups as any lengths need; those past the last item exit.
-  const int64_t groups = chunk_items(N, B, a.G, Hkv, sel != nullptr, a.splits) * Hkv;
+  const int64_t groups = chunk_items(N, B, a.G, Hkv, selected, a.splits) * Hkv;
   if (groups > MAX_WORKGROUPS / 2)
     return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
