@@ -1086,15 +1086,17 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(const ChunkArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (s0 + u < k) Mc = fmaxf(Mc, m[u]);
-        if (Mc == -__builtin_inff()) continue;   // no key of the row yet
-        const float f0 = fast_exp2(M - Mc);
+        // A share without a key of the row has a reference of -inf and sums of 0.  One whose scores are all NaN has a
+        // reference of -inf or NaN, which the maximum passes over, and sums of NaN, which reach the row from here.
+        const float Mu = Mc == -__builtin_inff() ? 0.f : Mc;
+        const float f0 = fast_exp2(M - Mu);
         L *= f0;
         acc[0] *= f0;
         acc[1] *= f0;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (s0 + u < k && m[u] != -__builtin_inff()) {
-            const float fs = fast_exp2(m[u] - Mc);
+          if (s0 + u < k) {
+            const float fs = fast_exp2(m[u] - Mu);
             L += fs * l[u];
             acc[0] += fs * v[u][0];
             acc[1] += fs * v[u][1];
