@@ -542,9 +542,9 @@ int64_t sa_paged_chunk_workspace_bytes(int N, int B, int Hq, int Hkv, int D, int
  * each KV head.  The first `sink` pages are kept, the last `recent` (counted back from the page of the row's
  * first query; all pages up to its last query's), and of the pages between the top_k with the largest
  *   score(page) = sum over the row's queries and the heads of the group of sum_d max(q_d lo_d, q_d hi_d)
- * over the page's k_bounds [num_pages, Hkv, 2, D] (lo, hi): an upper bound of the queries' products with its
- * keys.  fp64 scores; ties go to the lower page; a page whose score is NaN, or which has no valid page id, ranks
- * last.  sel[i * sel_sr + g * sel_sh + ...] (int32) receives the pages in ascending order, zero-padded to `width`, and
+ * over the page's k_bounds [num_pages, Hkv, 2, D] (lo <= hi): an upper bound of the queries' products with its
+ * keys.  fp64 scores; ties go to the lower page; a page whose score is NaN (NaN bounds or queries, infinities of both
+ * signs), or which has no valid page id, ranks last.  0 times an infinite bound counts as 0.  sel[i * sel_sr + g * sel_sh + ...] (int32) receives the pages in ascending order, zero-padded to `width`, and
  * sel_off [rows, Hkv, 2] (contiguous) 0 and their number.  rows == B, or N / 64 + B with cu_seqlens (rows
  * past the last block are empty); width >= sink + top_k + recent - 1 + the pages that a row's queries may lie in
  * (1, or (62 + page) / page + 1 with cu_seqlens).  The workspace holds scores where the call needs it

@@ -6,9 +6,10 @@
 //
 //   score(page) = hi . P + lo . N,   P = sum of max(q, 0),   N = sum of min(q, 0)
 //
-// so a list costs 2 D multiply-adds a page however many queries share it.  Kept are the first `sink` pages, the last
-// `recent` (from the page of the list's first query back, and all up to that of its last), and the top_k best of
-// those between, ties to the lowest page.  Pages between are full and wholly visible to every query of the list.
+// with 0 times an infinite bound counted as 0, so a list costs 2 D multiply-adds a page however many queries share
+// it.  Kept are the first `sink` pages, the last `recent` (from the page of the list's first query back, and all up to
+// that of its last), and the top_k best of those between, ties to the lowest page.  Pages between are full and wholly
+// visible to every query of the list.
 //
 // P, N and the scores are fp64: which page is the last one in depends on the order of near-equal scores, and in fp32
 // that order would follow the order of summation.  It costs little: a page's 4 D bytes take 2 D fp64 multiply-adds.
@@ -154,8 +155,8 @@ struct Select {
           unpack(v[u], f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            p[e] += (double)fmaxf(f[e], 0.f);
-            n[e] += (double)fminf(f[e], 0.f);
+            p[e] += f[e] < 0.f ? 0. : (double)f[e];   // a NaN too: its list's scores are NaN
+            n[e] += f[e] < 0.f ? (double)f[e] : 0.;
           }
         }
       }
@@ -211,6 +212,11 @@ struct Select {
       unpack(h4, h);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += (double)h[e] * P[e] + (double)l[e] * N[e];
+      if (!(s == s)) {   // rare: a bound may be infinite, and a sign that no query has takes nothing of it
+        s = 0.;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (P[e] != 0. ? (double)h[e] * P[e] : 0.) + (N[e] != 0. ? (double)l[e] * N[e] : 0.);
+      }
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o, 64);
       if (c == 0) keys[x] = live ? key_of(s) : 0ull;

@@ -62,3 +62,65 @@ def test_nan_rows_stay_nan_however_the_keys_are_divided(q_lens, kv_lens, D, dtyp
     # a whole share of the keys
     r.k_pages[r.table[0, 0].long(), 0] = math.nan
     assert _attend(r, q, num_splits=splits)[:t, :4].isnan().all()
+
+
+@pytest.mark.parametrize("tokens", [True, False])
+def test_select_ranks_infinite_bounds_by_the_definition(tokens):
+    """Largest products of +inf rank first (ties to the lower page); an infinite bound on the side that a query's sign
+    does not take changes nothing."""
+    _say("infinite bounds", tokens)
+    r = Ragged([1, 1], [64 * 20, 64 * 14 + 3], page=64, Hkv=2, D=64, seed=420, poison=False)
+    bounds = bounds_of(r)
+    q = randn(2, 2, 64, seed=421)           # one head a group: one sign for each dim
+    for b in range(2):
+        for g in range(2):
+            up, down = (q[b, g] > 0).nonzero().flatten(), (q[b, g] < 0).nonzero().flatten()
+            pg = r.table[b].long()
+            bounds[pg[9], g, 1, up[3]] = math.inf
+            bounds[pg[5], g, 0, down[2]] = -math.inf
+            bounds[pg[7], g, 1, down[1]] = math.inf         # not the side that counts
+            bounds[pg[8], g, 0, up[1]] = -math.inf
+    for top_k in (1, 2, 4):
+        args = dict(top_k=top_k, sink=1, recent=1)
+        want = select(r, q, bounds, tokens=tokens, **args)
+        got = ops.paged_block_select(q.cuda(), bounds.cuda(), *r.gpu("table", "kv_lens"), page=64,
+                                     cu_seqlens=None if tokens else r.cu.cuda(), **args)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+        kept = got[0][..., :top_k + 2].cpu()
+        assert (kept == 5).any(-1).all() and (top_k == 1 or (kept == 9).any(-1).all())
+
+
+def test_select_infinite_bounds_and_a_zero_query():
+    """0 times an infinite bound counts as 0: the page is ranked by its other dims."""
+    _say("infinite bounds, zero query")
+    r = Ragged([1], [64 * 10], page=64, Hkv=1, D=64, seed=425, poison=False)
+    q = randn(1, 2, 64, seed=426)
+    q[:, :, 7] = 0
+    bounds = bounds_of(r)
+    bounds[..., 7] = 0
+    args = dict(top_k=4, sink=0, recent=1)
+    want = select(r, q, bounds, tokens=True, **args)
+    bounds[r.table[0, 2].long(), 0, 1, 7] = math.inf
+    bounds[r.table[0, 4].long(), 0, 0, 7] = -math.inf
+    got = ops.paged_block_select(q.cuda(), bounds.cuda(), *r.gpu("table", "kv_lens"), page=64, **args)
+    assert torch.equal(got[0].cpu(), want[0])
+
+
+def test_select_nan_queries_leave_the_lowest_pages():
+    """Every score of a list with a NaN query is NaN: all rank last, so the lowest pages are kept.  Other lists, the same
+    block's of another KV head among them, are as without it."""
+    _say("nan queries")
+    r = Ragged([1, 130], [64 * 20, 64 * 12], page=64, Hkv=2, D=128, seed=430, poison=False)
+    bounds = bounds_of(r)
+    args = dict(top_k=3, sink=1, recent=1)
+    q = randn(131, 4, 128, seed=431)
+    clean = select(r, q, bounds, tokens=False, **args)[0]
+    q[0, 3, 5] = math.nan           # list 0, KV head 1
+    q[1 + 64 + 9, 0, 77] = math.nan     # second block of the second sequence, KV head 0
+    got = ops.paged_block_select(q.cuda(), bounds.cuda(), *r.gpu("table", "kv_lens"), page=64, cu_seqlens=r.cu.cuda(),
+                                 **args)[0].cpu()
+    assert got[0, 1].tolist()[:5] == [0, 1, 2, 3, 19]
+    assert got[2, 0].tolist()[:4] == [0, 1, 2, 3]
+    same = torch.ones(got.shape[:2], dtype=torch.bool)
+    same[0, 1] = same[2, 0] = False
+    assert torch.equal(got[same], clean[same])
