@@ -505,6 +505,20 @@ int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const 
                     int N, int B, int Hq, int Hkv, int D, int page, float eps, void* stream);
 
 /*
+ * sa_paged_append with angles of positions that are given: positions[n * pos_st] (device int64, pos_st >= 0) for packed
+ * row n.  Places in the cache follow kv_lens all the same.  inv_freq is needed.
+ */
+int sa_paged_append_at(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                       const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                       const void* q_weight, const void* k_weight, const float* inv_freq,
+                       const int64_t* positions, int64_t pos_st,
+                       void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
+                       int num_pages, void* k_bounds, int64_t bounds_sp, int64_t bounds_sh,
+                       const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                       const int32_t* cu_seqlens, const int32_t* kv_lens,
+                       int N, int B, int Hq, int Hkv, int D, int page, float eps, void* stream);
+
+/*
  * Causal attention of the new tokens over the pages (their own keys included): the row of a token at position p
  * sees the keys j <= p of its sequence; o[row] = sum_j softmax_j(q . k_j * sm_scale) v_j with fp32 statistics
  * and accumulators, 0 for a row that sees no key.  Probabilities are rounded to the element type before the second

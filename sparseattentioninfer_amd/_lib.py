@@ -167,6 +167,19 @@ SIGNATURES = {
         _vp, _vp,
         _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp,
     ]),
+    "sa_paged_append_at": (_i32, [
+        _i32,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _vp, _i64, _i64,
+        _vp, _vp, _vp, _vp, _i64,
+        _vp, _vp, _i64, _i64, _i64, _i32,
+        _vp, _i64, _i64,
+        _vp, _i64, _i32,
+        _vp, _vp,
+        _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp,
+    ]),
     "sa_paged_chunk_attn": (_i32, [
         _i32,
         _vp, _i64, _i64,

@@ -44,9 +44,10 @@ struct RopeArgs {
   const float* inv_freq;                        // or NULL: no rotation
   int Hq, Hkv, heads_per_part, window;
   float eps;
-  // unpaged: token n is row n % T of batch n / T
+  // What the angles follow.  Unpaged: token n is row n % T of batch n / T.  Paged: of packed row n, or NULL, where they
+  // follow the tokens' places in their sequences.
   const int64_t* positions;
-  int64_t pos_sb;
+  int64_t pos_sb, pos_st;
   int64_t N;
   int T;
   uint32_t mul_T;
@@ -189,7 +190,7 @@ struct RopeAppend {
       for (int slot = w.lo + tid / HALF; slot < w.hi; slot += RA_THREADS / HALF) {
         double p;
         if constexpr (PAGED) {
-          p = (double)(w.base + slot);
+          p = a.positions ? (double)a.positions[(w.row0 + slot) * a.pos_st] : (double)(w.base + slot);
         } else {
           int bt, t;
           batch_of(a, w.row0 + slot, bt, t);
@@ -441,16 +442,13 @@ extern "C" int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q
   return launch_rope<false>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
 }
 
-extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
-                               int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st,
-                               int64_t qo_sh, const void* q_weight, const void* k_weight, const float* inv_freq,
-                               void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
-                               int num_pages, void* k_bounds, int64_t bounds_sp, int64_t bounds_sh,
-                               const int32_t* block_table, int64_t block_table_stride, int max_blocks,
-                               const int32_t* cu_seqlens, const int32_t* kv_lens, int N, int B, int Hq, int Hkv,
-                               int D, int page, float eps, void* stream) {
-  clear_error();
-  const char* name = "sa_paged_append";
+static int append(const char* name, int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                  const void* q_weight, const void* k_weight, const float* inv_freq, const int64_t* positions,
+                  int64_t pos_st, void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
+                  int num_pages, void* k_bounds, int64_t bounds_sp, int64_t bounds_sh, const int32_t* block_table,
+                  int64_t block_table_stride, int max_blocks, const int32_t* cu_seqlens, const int32_t* kv_lens, int N,
+                  int B, int Hq, int Hkv, int D, int page, float eps, void* stream) {
   if (dtype != SA_DTYPE_BF16 && dtype != SA_DTYPE_F16)
     return set_error(SA_E_DTYPE, "%s: dtype %d is not bf16 (0) or f16 (1)", name, dtype);
   if (D != 64 && D != 128) return set_error(SA_E_HEADDIM, "%s: head dim %d not supported (64, 128)", name, D);
@@ -477,6 +475,8 @@ extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q
   a.qw = static_cast<const elem_t*>(q_weight);
   a.kw = static_cast<const elem_t*>(k_weight);
   a.inv_freq = inv_freq;
+  a.positions = positions;
+  a.pos_st = pos_st;
   a.N = N;
   a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
   a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
@@ -499,4 +499,38 @@ extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q
   a.heads_per_part = heads_per_part(windows, heads, RA_TARGET_PAGED);
   const int parts = (heads + a.heads_per_part - 1) / a.heads_per_part;
   return launch_rope<true>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
+}
+
+extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                               int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st,
+                               int64_t qo_sh, const void* q_weight, const void* k_weight, const float* inv_freq,
+                               void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
+                               int num_pages, void* k_bounds, int64_t bounds_sp, int64_t bounds_sh,
+                               const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                               const int32_t* cu_seqlens, const int32_t* kv_lens, int N, int B, int Hq, int Hkv,
+                               int D, int page, float eps, void* stream) {
+  clear_error();
+  return append("sa_paged_append", dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight,
+                k_weight, inv_freq, nullptr, 0, k_pages, v_pages, pages_sp, pages_sh, pages_st, num_pages, k_bounds,
+                bounds_sp, bounds_sh, block_table, block_table_stride, max_blocks, cu_seqlens, kv_lens, N, B, Hq, Hkv, D,
+                page, eps, stream);
+}
+
+extern "C" int sa_paged_append_at(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st,
+                                  int64_t qo_sh, const void* q_weight, const void* k_weight, const float* inv_freq,
+                                  const int64_t* positions, int64_t pos_st, void* k_pages, void* v_pages,
+                                  int64_t pages_sp, int64_t pages_sh, int64_t pages_st, int num_pages, void* k_bounds,
+                                  int64_t bounds_sp, int64_t bounds_sh, const int32_t* block_table,
+                                  int64_t block_table_stride, int max_blocks, const int32_t* cu_seqlens,
+                                  const int32_t* kv_lens, int N, int B, int Hq, int Hkv, int D, int page, float eps,
+                                  void* stream) {
+  clear_error();
+  const char* name = "sa_paged_append_at";
+  if (N > 0 && B > 0 && (!inv_freq || !positions)) return set_error(SA_E_NULL, "%s: NULL inv_freq or positions", name);
+  if (pos_st < 0) return set_error(SA_E_SHAPE, "%s: positions of stride %lld", name, (long long)pos_st);
+  return append(name, dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight, k_weight,
+                inv_freq, positions, pos_st, k_pages, v_pages, pages_sp, pages_sh, pages_st, num_pages, k_bounds,
+                bounds_sp, bounds_sh, block_table, block_table_stride, max_blocks, cu_seqlens, kv_lens, N, B, Hq, Hkv, D,
+                page, eps, stream);
 }

@@ -201,12 +201,12 @@ class PagedKVStore:
         return self.lens[0]
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, counts, *, inv_freq: torch.Tensor | None = None,
-               k_weight: torch.Tensor | None = None, eps: float = 1e-6, q: torch.Tensor | None = None,
-               q_weight: torch.Tensor | None = None) -> PagedChunk:
+               positions: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+               q: torch.Tensor | None = None, q_weight: torch.Tensor | None = None) -> PagedChunk:
         """Appends ``counts[b]`` new tokens to each sequence b, packed in ``k_new, v_new [N, H, D]`` (on the GPU).
 
-        Keys are normed (``k_weight``) and rotated (``inv_freq``) on the way where those are given, and queries
-        ``q [N, Hq, D]`` with them (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).
+        Keys are normed (``k_weight``) and rotated (``inv_freq``, by their places in the cache or by ``positions``
+        int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).
         """
         counts = tuple(int(n) for n in counts)
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k_new.size(0):
@@ -219,8 +219,8 @@ class PagedKVStore:
         cu = torch.tensor(cu, dtype=torch.int32).to(self.kv_lens.device)
         self.kv_lens.copy_(torch.tensor(new_lens, dtype=torch.int32))
         q_out = ops.paged_append(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
-                                 inv_freq=inv_freq, k_weight=k_weight, eps=eps, k_bounds=self.k_bounds, q=q,
-                                 q_weight=q_weight)
+                                 inv_freq=inv_freq, positions=positions, k_weight=k_weight, eps=eps,
+                                 k_bounds=self.k_bounds, q=q, q_weight=q_weight)
         self.lens = new_lens
         return PagedChunk(cu, counts, q_out)
 

@@ -908,14 +908,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *,
-                 inv_freq: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
-                 k_bounds: torch.Tensor | None = None, q: torch.Tensor | None = None,
-                 q_weight: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+                 inv_freq: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, eps: float = 1e-6, k_bounds: torch.Tensor | None = None,
+                 q: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
     """Writes a chunk's keys (normed and rotated on the way) and values into the pages of a cache.
 
     ``k, v [N, Hkv, D]`` hold the new tokens of all sequences, those of sequence b in rows ``cu_seqlens[b] ..
     cu_seqlens[b + 1] - 1`` (int32 ``[B + 1]``); ``kv_lens [B]`` int32 counts each sequence's tokens with them.
-    ``inv_freq`` (float32 ``[D/2]``) rotates, ``k_weight [D]`` norms; without them keys are stored as they are.
+    ``inv_freq`` (float32 ``[D/2]``) rotates, ``k_weight [D]`` norms; without them keys are stored as they are.  The
+    angles follow each token's place in its sequence, or ``positions`` (int64 ``[N]``) where those are given.
     ``k_bounds [P, Hkv, 2, D]`` keeps each page's smallest and largest key per dim (:func:`paged_block_select`
     reads it).  ``q [N, Hq, D]`` takes the same norm (``q_weight``) and rotation in the same launch; its result is
     returned (``q_out``, allocated if omitted; rows of no sequence are left as they are).  The pages must
@@ -935,7 +937,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
           and (k_weight is None or (k_weight.shape == (ks[2],) and k_weight.dtype == dt and k_weight.device == dev
                                     and k_weight.is_contiguous()))
           and (inv_freq is None or (inv_freq.dtype == torch.float32 and inv_freq.shape == (ks[2] // 2,)
-                                    and inv_freq.is_contiguous() and inv_freq.device == dev)))
+                                    and inv_freq.is_contiguous() and inv_freq.device == dev))
+          and (positions is None or (inv_freq is not None and positions.dtype == torch.int64 and positions.device == dev
+                                     and positions.shape == (ks[0],))))
     if ok and k_bounds is not None:
         ok = (k_bounds.shape == (ps[0], ps[1], 2, ps[3]) and k_bounds.dtype == dt and k_bounds.device == dev
               and k_bounds.stride(3) == 1 and k_bounds.stride(2) == ps[3])
@@ -958,12 +962,17 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                 index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens), weights=(q_weight, k_weight),
                 inv_freq=inv_freq, pools=(k_pages, v_pages), B=block_table.size(0) if block_table.dim() else 0,
                 other="k and v must be [N, Hkv, D], q [N, Hq, D] (q_out and q_weight need it), pools [P, Hkv, page, D], "
-                      "k_bounds [P, Hkv, 2, D] with contiguous [2, D]")
+                      "k_bounds [P, Hkv, 2, D] with contiguous [2, D], positions (with inv_freq) int64 [N]"
+                      + ("" if positions is None else f"; got positions {positions.dtype} {tuple(positions.shape)} on "
+                         f"{positions.device}"))
     bargs = (None, 0, 0) if k_bounds is None else (k_bounds.data_ptr(), k_bounds.stride(0), k_bounds.stride(1))
-    _call("sa_paged_append", dev.index, _DTYPES[dt], *qargs, k.data_ptr(), kst[0], kst[1], v.data_ptr(), vst[0], vst[1],
+    entry, at = "sa_paged_append", ()
+    if positions is not None:
+        entry, at = "sa_paged_append_at", (positions.data_ptr(), positions.stride(0))
+    _call(entry, dev.index, _DTYPES[dt], *qargs, k.data_ptr(), kst[0], kst[1], v.data_ptr(), vst[0], vst[1],
           *oargs, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-          None if inv_freq is None else inv_freq.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pst[0], pst[1], pst[2],
-          ps[0], *bargs, block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
+          None if inv_freq is None else inv_freq.data_ptr(), *at, k_pages.data_ptr(), v_pages.data_ptr(), pst[0], pst[1],
+          pst[2], ps[0], *bargs, block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
           kv_lens.data_ptr(), ks[0], B, Hq, ks[1], ks[2], ps[2], eps)
     return q_out
 

@@ -162,7 +162,8 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
         input_shape = hidden_states.shape[:-1]
         bsz, q_len = input_shape
         if self.pattern_name == "block_topk":
-            return self._forward_block_topk(hidden_states, attention_mask, cache), None
+            return self._forward_block_topk(hidden_states, position_embeddings, attention_mask, cache,
+                                            kwargs.get("position_ids")), None
         hidden_shape = (*input_shape, -1, self.head_dim)
         q = self.q_norm(self.q_proj(hidden_states).view(hidden_shape)).transpose(1, 2)
         k = self.k_norm(self.k_proj(hidden_states).view(hidden_shape)).transpose(1, 2)
@@ -212,8 +213,13 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
         return self.o_proj(out), None
 
 
-    def _forward_block_topk(self, hidden_states: torch.Tensor, attention_mask, cache) -> torch.Tensor:
-        """Projections, one append launch, page selection and attention over the chosen pages."""
+    def _forward_block_topk(self, hidden_states: torch.Tensor, position_embeddings, attention_mask, cache,
+                            position_ids) -> torch.Tensor:
+        """Projections, one append launch, page selection and attention over the chosen pages.
+
+        The append rotates at ``position_ids [1 or B, T]`` (the model passes them); without them the heads are normed and
+        rotated before it with the cos and sin of ``position_embeddings``, as the other patterns do.
+        """
         if not isinstance(cache, PagedKVCache) or not cache.layers[self.layer_idx].bounds:
             raise ValueError("the block_topk pattern needs past_key_values=PagedKVCache(..., bounds=True)")
         bsz, q_len = hidden_states.shape[:-1]
@@ -225,13 +231,19 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
         backend = self.sparse_backend = self.sparse_backends[self.backend_name]
         if not hasattr(backend, "forward_packed"):
             raise NotImplementedError(f"backend {self.backend_name!r} has no attention over packed chunks (block_topk)")
-        if self._inv_freq is None or self._inv_freq.device != hidden_states.device:
-            half = torch.arange(0, self.head_dim, 2, dtype=torch.float64) / self.head_dim
-            self._inv_freq = (1.0 / self._rope_theta ** half).float().to(hidden_states.device)
-        q, k, v = (proj(hidden_states).view(bsz * q_len, -1, self.head_dim)
+        q, k, v = (proj(hidden_states).view(bsz, q_len, -1, self.head_dim)
                    for proj in (self.q_proj, self.k_proj, self.v_proj))
-        chunk = layer.append(q, k, v, [q_len] * bsz, inv_freq=self._inv_freq, k_weight=self.k_norm.weight,
-                             q_weight=self.q_norm.weight, eps=self.q_norm.variance_epsilon)
+        if position_ids is not None:
+            if self._inv_freq is None or self._inv_freq.device != hidden_states.device:
+                half = torch.arange(0, self.head_dim, 2, dtype=torch.float64) / self.head_dim
+                self._inv_freq = (1.0 / self._rope_theta ** half).float().to(hidden_states.device)
+            rope = dict(inv_freq=self._inv_freq, positions=position_ids.expand(bsz, q_len).reshape(-1).long(),
+                        k_weight=self.k_norm.weight, q_weight=self.q_norm.weight, eps=self.q_norm.variance_epsilon)
+        else:
+            rope = {}
+            q, k = apply_rotary_pos_emb(self.q_norm(q), self.k_norm(k), *position_embeddings, unsqueeze_dim=2)
+        q, k, v = (x.flatten(0, 1) for x in (q, k, v))
+        chunk = layer.append(q, k, v, [q_len] * bsz, **rope)
         store = layer.store
         pattern = self.sparse_pattern.build(q, q.new_empty((bsz, self.num_key_value_heads, store.seq_len(), 0)), causal=True)
         self.last_pattern_stats = pattern_stats(pattern) if self.collect_pattern_stats else None

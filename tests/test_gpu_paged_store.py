@@ -1,0 +1,131 @@
+"""Callers of the paged append on the GPU: positions that are given, refusals that leave the cache as it was, no upload
+that waits for the stream, key bounds after a captured decode."""
+import pytest
+import torch
+from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
+
+from sparseattentioninfer_amd import ops
+from sparseattentioninfer_amd.attention import HipBlockSparseBackend
+from sparseattentioninfer_amd.models import PagedChunk, PagedKVStore
+from sparseattentioninfer_amd.qwen3 import PagedKVCache
+from sparseattentioninfer_amd.qwen3.graph_decode import GraphDecoder
+from sparseattentioninfer_amd.qwen3.runtime import build_model, qwen3_config
+from tests.chunk_reference import Ragged, assert_rotated, bounds_of, randn, rotate
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+EPS = 1e-6
+
+
+def _say(*msg):
+    print("[paged-store]", *msg, flush=True)
+
+
+def _view(store):
+    r = Ragged.__new__(Ragged)
+    r.lens, r.page, r.Hkv, r.D, r.dtype = list(store.lens), store.page, store.heads, store.head_dim, store.k_pages.dtype
+    r.table, r.k_pages, r.v_pages = store.block_table.cpu(), store.k_pages.cpu(), store.v_pages.cpu()
+    return r
+
+
+def _state(st):
+    return (list(st.lens), st.kv_lens.tolist(), [list(r) for r in st._table_host], list(st._free), st.block_table.tolist())
+
+
+def _inv(D):
+    return (1.0 / 1e6 ** (torch.arange(0, D, 2, dtype=torch.float64) / D)).float()
+
+
+@pytest.mark.parametrize("stride", [1, 0, 3])
+@pytest.mark.parametrize("D,dtype,norm,bounds", [(128, BF, True, True), (64, HF, False, False)])
+def test_append_at_given_positions(D, dtype, norm, bounds, stride):
+    """Angles follow ``positions``; places in the cache, and so what attention sees, follow the lengths."""
+    _say("positions", D, dtype, norm, bounds, stride)
+    q_lens, kv_lens = [40, 0, 1, 100], [40, 5, 300, 131]
+    r = Ragged(q_lens, kv_lens, page=32, Hkv=2, D=D, dtype=dtype, seed=600, pad_rows=2, poison=False)
+    q, k, v = (randn(r.N, h, D, seed=601 + h, dtype=dtype) for h in (6, 2, 2))
+    w = randn(D, seed=610, dtype=dtype, scale=0.3) + 1 if norm else None
+    wide = torch.randint(0, 131072, (r.N, max(stride, 1)), generator=torch.Generator().manual_seed(611))
+    positions = wide[:1, 0].expand(r.N) if stride == 0 else wide[:, 0]
+    dev = wide.cuda()
+    dev_positions = dev[:1, 0].expand(r.N) if stride == 0 else dev[:, 0]
+    kp, vp, table, cu, lens = r.gpu("k_pages", "v_pages", "table", "cu", "kv_lens")
+    bd = torch.zeros(kp.size(0), 2, 2, D, dtype=dtype, device="cuda") if bounds else None
+    q_out = torch.full((r.N, 6, D), 7.0, dtype=dtype, device="cuda")
+    gw = None if w is None else w.cuda()
+    ops.paged_append(k.cuda(), v.cuda(), kp, vp, table, cu, lens, inv_freq=_inv(D).cuda(), positions=dev_positions,
+                     k_weight=gw, q=q.cuda(), q_weight=gw, q_out=q_out, eps=EPS, k_bounds=bd)
+    kp, vp = kp.cpu(), vp.cpu()
+    for b, at, t, n in r.rows():
+        rows, p = slice(at, at + t), torch.arange(n - t, n)
+        phys, slot = r.table[b, p // 32].long(), p % 32
+        assert_rotated(q_out[rows], *rotate(q[rows], w, positions[rows], _inv(D), EPS), f"q of {b}")
+        assert_rotated(kp[phys, :, slot], *rotate(k[rows], w, positions[rows], _inv(D), EPS), f"k of {b}")
+        assert torch.equal(vp[phys, :, slot], v[rows])
+    assert (q_out[r.N - 2:] == 7.0).all()
+
+
+def test_append_refuses_positions_that_do_not_fit():
+    r = Ragged([4], [70], page=64, Hkv=2, D=64, seed=615)
+    kp, vp, table, cu, lens = r.gpu("k_pages", "v_pages", "table", "cu", "kv_lens")
+    k, inv = randn(4, 2, 64, seed=616).cuda(), _inv(64).cuda()
+    pos = torch.arange(4, device="cuda")
+    for bad in (dict(positions=pos, inv_freq=None), dict(positions=pos[:3]), dict(positions=pos.int()),
+                dict(positions=pos.cpu()), dict(positions=pos[None])):
+        with pytest.raises(AssertionError, match="positions"):
+            ops.paged_append(k, k, kp, vp, table, cu, lens, **{"inv_freq": inv, **bad})
+
+
+def _model(pattern="block_topk", block_size=32):
+    cfg = qwen3_config(pattern=pattern, block_size=block_size, vocab_size=512, hidden_size=256, intermediate_size=256,
+                       num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=128)
+    return build_model(cfg, seed=8)
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("per_row", [False, True])
+def test_qwen3_block_topk_rotates_at_the_positions_it_is_given(per_row):
+    """A prompt, a chunk and a token whose position_ids are not the cache's own: one row for the batch, or a row each."""
+    _say("qwen3 positions", per_row)
+    model = _model()
+    cache = PagedKVCache(2, 400, page=32, shuffle_seed=4, bounds=True)
+    seen = []
+    for layer in model.model.layers:
+        layer.self_attn.register_forward_pre_hook(lambda m, a, kw: seen.append((m, kw["hidden_states"])), with_kwargs=True)
+    at = 0
+    for t in (150, 40, 1):
+        ids = torch.randint(0, 512, (2, t), generator=torch.Generator().manual_seed(t)).cuda()
+        pos = (torch.arange(at, at + t) + 1000)[None]
+        if per_row:
+            pos = torch.cat([pos, pos + 777])
+        model(input_ids=ids, position_ids=pos.cuda(), past_key_values=cache, use_cache=True, logits_to_keep=1)
+        at += t
+        for attn, x in seen:
+            r = _view(cache.layers[attn.layer_idx].store)
+            keys = torch.cat([r.cached(r.k_pages, b, at)[:, at - t:].transpose(0, 1) for b in range(2)]).to(BF)
+            proj = attn.k_proj(x).view(2 * t, -1, 128).cpu()
+            assert_rotated(keys, *rotate(proj, attn.k_norm.weight.cpu(), pos.expand(2, t).reshape(-1), attn._inv_freq.cpu(),
+                                         model.config.rms_norm_eps), "k")
+        seen.clear()
+
+
+@torch.no_grad()
+def test_qwen3_block_topk_called_with_cos_and_sin_alone():
+    """The attention module called by itself, without position_ids: it rotates with the cos and sin it is given."""
+    _say("qwen3 cos sin")
+    model = _model()
+    attn = model.model.layers[1].self_attn
+    cache = PagedKVCache(2, 200, page=32, bounds=True)
+    x = randn(2, 70, 256, seed=640).cuda()
+    cos, sin = model.model.rotary_emb(x, (torch.arange(70, device="cuda") * 3 + 11)[None])
+    out, _ = attn(x, (cos, sin), None, past_key_values=cache)
+    q = attn.q_norm(attn.q_proj(x).view(2, 70, -1, 128)).transpose(1, 2)
+    k = attn.k_norm(attn.k_proj(x).view(2, 70, -1, 128)).transpose(1, 2)
+    q, k = apply_rotary_pos_emb(q, k, cos, sin)
+    store = cache.layers[1].store
+    assert torch.equal(store.gather()[0], k)
+    assert torch.equal(store.gather()[1], attn.v_proj(x).view(2, 70, -1, 128).transpose(1, 2))
+    chunk = PagedChunk(torch.tensor([0, 70, 140], dtype=torch.int32, device="cuda"), (70, 70), None)
+    want = HipBlockSparseBackend().forward_packed(q.transpose(1, 2).reshape(140, 4, 128), store, chunk,
+                                                  attn.sparse_pattern.build(q, k))
+    assert torch.equal(out, attn.o_proj(want.reshape(2, 70, -1)))
