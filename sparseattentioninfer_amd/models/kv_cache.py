@@ -188,9 +188,22 @@ class PagedKVStore:
             return
         if len(self._free) < sum(more):
             raise RuntimeError("paged KV cache: out of pages")
-        table = torch.zeros(self.batch, self.max_blocks, dtype=torch.int32)
-        for b, (row, n) in enumerate(zip(self._table_host, more)):
+        for row, n in zip(self._table_host, more):
             row.extend(self._free.pop() for _ in range(n))
+        self._upload_table()
+
+    def _shrink_each(self, blocks: list[int]) -> None:
+        """Takes each sequence's pages past its first ``blocks[b]`` back, in the order that undoes :meth:`_grow_each`."""
+        if all(len(row) == n for row, n in zip(self._table_host, blocks)):
+            return
+        for row, n in zip(reversed(self._table_host), reversed(blocks)):
+            while len(row) > n:
+                self._free.append(row.pop())
+        self._upload_table()
+
+    def _upload_table(self) -> None:
+        table = torch.zeros(self.batch, self.max_blocks, dtype=torch.int32)
+        for b, row in enumerate(self._table_host):
             table[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
         self.block_table.copy_(table)
         self._page_cols.clear()
@@ -206,21 +219,28 @@ class PagedKVStore:
         """Appends ``counts[b]`` new tokens to each sequence b, packed in ``k_new, v_new [N, H, D]`` (on the GPU).
 
         Keys are normed (``k_weight``) and rotated (``inv_freq``, by their places in the cache or by ``positions``
-        int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).
+        int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).  A
+        call that is refused leaves the store as it was.
         """
         counts = tuple(int(n) for n in counts)
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k_new.size(0):
             raise ValueError(f"counts {counts} do not split {k_new.size(0)} tokens over {self.batch} sequences")
         new_lens = [n + t for n, t in zip(self.lens, counts)]
+        blocks = [len(row) for row in self._table_host]
         self._grow_each(new_lens)
-        cu = [0]
-        for t in counts:
-            cu.append(cu[-1] + t)
-        cu = torch.tensor(cu, dtype=torch.int32).to(self.kv_lens.device)
-        self.kv_lens.copy_(torch.tensor(new_lens, dtype=torch.int32))
-        q_out = ops.paged_append(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
-                                 inv_freq=inv_freq, positions=positions, k_weight=k_weight, eps=eps,
-                                 k_bounds=self.k_bounds, q=q, q_weight=q_weight)
+        try:
+            cu = [0]
+            for t in counts:
+                cu.append(cu[-1] + t)
+            cu = torch.tensor(cu, dtype=torch.int32).to(self.kv_lens.device)
+            self.kv_lens.copy_(torch.tensor(new_lens, dtype=torch.int32))
+            q_out = ops.paged_append(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
+                                     inv_freq=inv_freq, positions=positions, k_weight=k_weight, eps=eps,
+                                     k_bounds=self.k_bounds, q=q, q_weight=q_weight)
+        except BaseException:
+            self._shrink_each(blocks)
+            self.kv_lens.copy_(torch.tensor(self.lens, dtype=torch.int32))
+            raise
         self.lens = new_lens
         return PagedChunk(cu, counts, q_out)
 

@@ -39,9 +39,14 @@ class PagedKVLayer(CacheLayerMixin):
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts, **rope) -> PagedChunk:
         """:meth:`PagedKVStore.append` of packed ``[N, H, D]`` projections (queries too), allocating on first use."""
-        if not self.is_initialized:
-            self._make_store(len(counts), k.size(1), k.size(2), k)
-        return self.store.append(k, v, counts, q=q, **rope)
+        if self.is_initialized:
+            return self.store.append(k, v, counts, q=q, **rope)
+        self._make_store(len(counts), k.size(1), k.size(2), k)
+        try:
+            return self.store.append(k, v, counts, q=q, **rope)
+        except BaseException:      # a store of the refused tensors' type and device would refuse the right ones
+            self.store, self.is_initialized = None, False
+            raise
 
     def write(self, key_states: torch.Tensor, value_states: torch.Tensor) -> PagedKVStore:
         """Appends ``[B, H_kv, t, D]`` K/V to the pages; returns the store."""

@@ -76,6 +76,24 @@ def test_append_refuses_positions_that_do_not_fit():
             ops.paged_append(k, k, kp, vp, table, cu, lens, **{"inv_freq": inv, **bad})
 
 
+def test_appends_from_many_refusals_go_on_where_they_were():
+    _say("refused appends")
+    st = PagedKVStore(2, 2, 64, 400, page=16, shuffle_seed=2, bounds=True)
+    k = randn(60, 2, 64, seed=620).cuda()
+    st.append(k[:21], k[:21], [20, 1])
+    before = _state(st)
+    for bad in (dict(k_new=k.float(), v_new=k), dict(k_new=k[:, :1], v_new=k), dict(k_new=k, v_new=k[:50]),
+                dict(k_new=k, v_new=k, k_weight=torch.ones(32, dtype=BF, device="cuda")),
+                dict(k_new=k, v_new=k, q_weight=torch.ones(64, dtype=BF, device="cuda"))):
+        with pytest.raises(AssertionError):
+            st.append(counts=[59, 1], **bad)
+        assert _state(st) == before
+    st.append(k[21:], k[21:], [9, 30])
+    r = _view(st)
+    assert torch.equal(r.cached(r.k_pages, 0, 29), torch.cat([k[:20], k[21:30]]).cpu().double().transpose(0, 1))
+    assert torch.equal(r.cached(r.k_pages, 1, 31), torch.cat([k[20:21], k[30:]]).cpu().double().transpose(0, 1))
+
+
 def _model(pattern="block_topk", block_size=32):
     cfg = qwen3_config(pattern=pattern, block_size=block_size, vocab_size=512, hidden_size=256, intermediate_size=256,
                        num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=128)

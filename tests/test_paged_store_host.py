@@ -1,0 +1,43 @@
+"""The paged store's bookkeeping on the CPU: a refused append changes nothing, sequences of unequal page counts grow
+into pages of their own, and what the block_topk pattern's refusals say."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from sparseattentioninfer_amd import _lib
+from sparseattentioninfer_amd.attention import get_backend
+from sparseattentioninfer_amd.models import PagedKVStore
+from sparseattentioninfer_amd.patterns import BlockTopKPattern
+from sparseattentioninfer_amd.qwen3.paged_cache import PagedKVLayer
+
+BF = torch.bfloat16
+
+
+def _state(st):
+    return (list(st.lens), st.kv_lens.tolist(), [list(r) for r in st._table_host], list(st._free), st.block_table.tolist())
+
+
+def test_a_refused_append_leaves_the_store_as_it_was():
+    """The operator runs on the GPU only, so here it refuses each call, with pages to hand out and without."""
+    st = PagedKVStore(2, 1, 64, 100, page=16, device="cpu", shuffle_seed=3)
+    before = _state(st)
+    k = torch.zeros(5, 1, 64, dtype=BF)
+    for counts in ([3, 2], [5, 0], [0, 5]):
+        with pytest.raises(AssertionError, match="GPU"):
+            st.append(k, k, counts)
+        assert _state(st) == before
+    st.write(torch.ones(2, 1, 20, 64, dtype=BF), torch.ones(2, 1, 20, 64, dtype=BF))
+    before = _state(st)
+    with pytest.raises(AssertionError, match="GPU"):
+        st.append(torch.zeros(40, 1, 64, dtype=BF), torch.zeros(40, 1, 64, dtype=BF), [1, 39])
+    assert _state(st) == before and st.seq_len() == 20
+
+
+def test_a_layer_whose_first_append_is_refused_has_no_store():
+    """It would keep the refused tensors' type and device."""
+    layer = PagedKVLayer(64, page=16)
+    x = torch.zeros(4, 1, 64)
+    with pytest.raises(AssertionError):
+        layer.append(x, x, x, [4])
+    assert layer.store is None and not layer.is_initialized and layer.get_seq_length() == 0
