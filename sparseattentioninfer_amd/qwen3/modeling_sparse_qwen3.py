@@ -231,6 +231,8 @@ class Qwen3SparseKernelAttention(Qwen3Attention):
         backend = self.sparse_backend = self.sparse_backends[self.backend_name]
         if not hasattr(backend, "forward_packed"):
             raise NotImplementedError(f"backend {self.backend_name!r} has no attention over packed chunks (block_topk)")
+        if self.sparse_pattern.block_size != layer.page:      # before the append, which a refusal would not undo
+            raise ValueError(f"pattern block {self.sparse_pattern.block_size} differs from the cache page {layer.page}")
         q, k, v = (proj(hidden_states).view(bsz, q_len, -1, self.head_dim)
                    for proj in (self.q_proj, self.k_proj, self.v_proj))
         if position_ids is not None:

@@ -147,3 +147,13 @@ def test_qwen3_block_topk_called_with_cos_and_sin_alone():
     want = HipBlockSparseBackend().forward_packed(q.transpose(1, 2).reshape(140, 4, 128), store, chunk,
                                                   attn.sparse_pattern.build(q, k))
     assert torch.equal(out, attn.o_proj(want.reshape(2, 70, -1)))
+
+
+@torch.no_grad()
+def test_qwen3_block_topk_refuses_a_page_that_is_not_its_block_before_it_appends():
+    _say("qwen3 page")
+    model = _model()
+    cache = PagedKVCache(2, 400, page=64, bounds=True)
+    with pytest.raises(ValueError, match="page"):
+        model(input_ids=torch.zeros(1, 40, dtype=torch.long, device="cuda"), past_key_values=cache, use_cache=True)
+    assert cache.get_seq_length() == 0
