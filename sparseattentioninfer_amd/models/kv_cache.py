@@ -162,21 +162,7 @@ class PagedKVStore:
 
     def _grow_all(self, new_len: int) -> None:
         """Gives every sequence the pages that ``new_len`` tokens need (one table update)."""
-        need = -(-new_len // self.page)
-        if need > self.max_blocks:
-            raise ValueError(f"sequences need {need} blocks > max_blocks {self.max_blocks}")
-        have = len(self._table_host[0])
-        if need <= have:
-            return
-        if len(self._free) < self.batch * (need - have):
-            raise RuntimeError("paged KV cache: out of pages")
-        added = []
-        for row in self._table_host:
-            for _ in range(need - have):
-                row.append(self._free.pop())
-            added.append(row[have:need])
-        self.block_table[:, have:need] = torch.tensor(added, dtype=torch.int32).to(self.block_table.device)
-        self._page_cols.clear()
+        self._grow_each([new_len] * self.batch)
 
     def _grow_each(self, new_lens: list[int]) -> None:
         """Gives each sequence the pages that its ``new_lens`` tokens need (one table update), or none of them."""
@@ -188,24 +174,25 @@ class PagedKVStore:
             return
         if len(self._free) < sum(more):
             raise RuntimeError("paged KV cache: out of pages")
+        first = min(len(row) for row, n in zip(self._table_host, more) if n)
         for row, n in zip(self._table_host, more):
             row.extend(self._free.pop() for _ in range(n))
-        self._upload_table()
+        self._upload_table(first, max(need))
 
     def _shrink_each(self, blocks: list[int]) -> None:
         """Takes each sequence's pages past its first ``blocks[b]`` back, in the order that undoes :meth:`_grow_each`."""
+        last = max(len(row) for row in self._table_host)
         if all(len(row) == n for row, n in zip(self._table_host, blocks)):
             return
         for row, n in zip(reversed(self._table_host), reversed(blocks)):
             while len(row) > n:
                 self._free.append(row.pop())
-        self._upload_table()
+        self._upload_table(min(blocks), last)
 
-    def _upload_table(self) -> None:
-        table = torch.zeros(self.batch, self.max_blocks, dtype=torch.int32)
-        for b, row in enumerate(self._table_host):
-            table[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
-        self.block_table.copy_(table)
+    def _upload_table(self, first: int, last: int) -> None:
+        """Brings columns ``first .. last - 1`` of the device's table up to date; 0 where a sequence has no page."""
+        cols = [row[first:last] + [0] * (last - max(first, len(row))) for row in self._table_host]
+        self.block_table[:, first:last] = torch.tensor(cols, dtype=torch.int32).to(self.block_table.device)
         self._page_cols.clear()
 
     def _uniform_len(self, what: str) -> int:
@@ -219,8 +206,8 @@ class PagedKVStore:
         """Appends ``counts[b]`` new tokens to each sequence b, packed in ``k_new, v_new [N, H, D]`` (on the GPU).
 
         Keys are normed (``k_weight``) and rotated (``inv_freq``, by their places in the cache or by ``positions``
-        int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).  A
-        call that is refused leaves the store as it was.
+        int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them
+        (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).  A call that is refused leaves the store as it was.
         """
         counts = tuple(int(n) for n in counts)
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k_new.size(0):

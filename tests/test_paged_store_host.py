@@ -41,3 +41,17 @@ def test_a_layer_whose_first_append_is_refused_has_no_store():
     with pytest.raises(AssertionError):
         layer.append(x, x, x, [4])
     assert layer.store is None and not layer.is_initialized and layer.get_seq_length() == 0
+
+
+def test_sequences_with_unequal_page_counts_grow_into_their_own_pages():
+    st = PagedKVStore(2, 1, 64, 200, page=16, device="cpu", dtype=torch.float32)
+    st._grow_each([70, 3])
+    k = torch.arange(2 * 60, dtype=torch.float32).view(2, 1, 60, 1).expand(2, 1, 60, 64) + 1
+    st.write(k, -k)
+    assert [len(r) for r in st._table_host] == [5, 4] and len(set(sum(st._table_host, []))) == 9
+    got_k, got_v = st.gather()
+    assert torch.equal(got_k, k) and torch.equal(got_v, -k)
+    st._grow_all(100)
+    assert [len(r) for r in st._table_host] == [7, 7] and len(set(sum(st._table_host, []))) == 14
+    for b in range(2):
+        assert st.block_table[b, :7].tolist() == st._table_host[b]
