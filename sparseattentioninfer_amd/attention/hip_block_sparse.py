@@ -135,9 +135,13 @@ class HipBlockSparseBackend(AttentionBackend):
             else:
                 raise ValueError("hip_block_sparse needs block_pairs/block_pair_offsets or kv_block_list")
             return pairs, offsets, bs
-        raise NotImplementedError(
-            f"hip_block_sparse does not run pattern kind {pattern.kind!r} (data-dependent top-k "
-            "selection is not a block schedule)")
+        raise NotImplementedError(f"hip_block_sparse does not run {self._not_a_schedule(pattern.kind)}")
+
+    @staticmethod
+    def _not_a_schedule(kind: str) -> str:
+        if kind == "block_topk":
+            return "pattern kind 'block_topk' over contiguous K/V (forward_packed runs it over a paged store)"
+        return f"pattern kind {kind!r} (data-dependent top-k selection is not a block schedule)"
 
     @staticmethod
     def unsupported_reason(q: torch.Tensor, pattern: PatternMetadata):
@@ -156,7 +160,7 @@ class HipBlockSparseBackend(AttentionBackend):
             if (pattern.block_pairs is None or pattern.block_pair_offsets is None) and pattern.kv_block_list is None:
                 return "no block schedule (block_pairs/block_pair_offsets or kv_block_list)"
         elif pattern.kind != "dense":
-            return f"pattern kind {pattern.kind!r} (data-dependent top-k selection is not a block schedule)"
+            return HipBlockSparseBackend._not_a_schedule(pattern.kind)
         return None
 
     def _run_fallback(self, q, k, v, pattern, reason: str) -> torch.Tensor:

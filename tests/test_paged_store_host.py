@@ -55,3 +55,12 @@ def test_sequences_with_unequal_page_counts_grow_into_their_own_pages():
     assert [len(r) for r in st._table_host] == [7, 7] and len(set(sum(st._table_host, []))) == 14
     for b in range(2):
         assert st.block_table[b, :7].tolist() == st._table_host[b]
+
+
+def test_a_block_topk_caller_is_told_where_it_runs():
+    be = get_backend("hip_block_sparse")
+    pattern = BlockTopKPattern(4).build(torch.zeros(1, 1, 1, 64), torch.zeros(1, 1, 1, 64))
+    q = SimpleNamespace(is_cuda=True, dtype=BF, size=lambda d: 64)
+    assert "forward_packed" in be.unsupported_reason(q, pattern)
+    with pytest.raises(NotImplementedError, match="forward_packed"):
+        be._schedule(1, 64, 1, "cpu", pattern)
