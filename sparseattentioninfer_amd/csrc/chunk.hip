@@ -1203,7 +1203,9 @@ extern "C" int sa_paged_chunk_attn(int dtype, const void* q, int64_t q_st, int64
     return set_error(SA_E_SHAPE, "%s: a selection needs offsets and %lld rows, got %d", name,
                      (long long)N / CK_BLOCK + B, sel_rows);
   if (N == 0 || B == 0) return 0;
-  if (!q || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || !o || (selected && sel_width && !sel))
+  // A table without columns and pools without pages are never read.
+  if (!q || (num_pages && (!k_pages || !v_pages)) || (max_blocks && !block_table) || !cu_seqlens || !kv_lens || !o ||
+      (selected && sel_width && !sel))
     return set_error(SA_E_NULL, "%s: NULL pointer", name);
   if (bad_ptr(q) || bad_ptr(k_pages) || bad_ptr(v_pages) || bad_ptr(o) || bad_ptr(workspace) ||
       (q_st | q_sh | pages_sp | pages_sh | pages_st | o_st | o_sh) % 8)

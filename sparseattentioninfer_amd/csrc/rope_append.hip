@@ -459,7 +459,9 @@ static int append(const char* name, int dtype, const void* q, int64_t q_st, int6
     return set_error(SA_E_SHAPE, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages",
                      name, N, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages);
   if (N == 0 || B == 0) return 0;
-  if (!k || !v || !k_pages || !v_pages || !block_table || !cu_seqlens || !kv_lens || (Hq && (!q || !q_out)))
+  // A table without columns and pools without pages are neither read nor written.
+  if (!k || !v || (num_pages && (!k_pages || !v_pages)) || (max_blocks && !block_table) || !cu_seqlens || !kv_lens ||
+      (Hq && (!q || !q_out)))
     return set_error(SA_E_NULL, "%s: NULL pointer", name);
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out) || misaligned(q_weight) ||
       misaligned(k_weight) || misaligned(k_pages) || misaligned(v_pages) || misaligned(k_bounds) ||

@@ -450,7 +450,8 @@ extern "C" int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int
     return set_error(SA_E_SHAPE, "%s: lists [%d, Hkv, %d], needed [%lld, Hkv, %d]", name, rows, width, (long long)need_rows,
                      sink + top_k + recent - 1 + span);
   if (rows == 0) return 0;
-  if ((N && !q) || !k_bounds || !block_table || !kv_lens || !sel || !sel_off) return set_error(SA_E_NULL, "%s: NULL pointer", name);
+  // A table without columns and bounds of no page are never read.
+  if ((N && !q) || (num_pages && !k_bounds) || (max_blocks && !block_table) || !kv_lens || !sel || !sel_off) return set_error(SA_E_NULL, "%s: NULL pointer", name);
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_bounds) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (q_st | q_sh | bounds_sp | bounds_sh) % 8)
     return set_error(SA_E_ALIGN, "%s: rows must be 16-byte aligned", name);

@@ -47,3 +47,10 @@ def test_append_at_refusals(lib, change, code, text):
 
 def test_append_at_nothing_to_do(lib):
     assert _append_at(lib, N=0, k=None, pos=None) == 0 and _append_at(lib, B=0) == 0
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(kp=None), -6, b"NULL"), (dict(table=None), -6, b"NULL"), (dict(kp=None, table=None, mb=0), -6, b"NULL"),
+    (dict(kp=None, table=None, pages=0), -6, b"NULL")])
+def test_a_table_with_columns_and_a_pool_with_pages_are_needed(lib, change, code, text):
+    assert _chunk(lib, **change) == code and text in lib.sa_last_error()

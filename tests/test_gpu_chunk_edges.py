@@ -124,3 +124,24 @@ def test_select_nan_queries_leave_the_lowest_pages():
     same = torch.ones(got.shape[:2], dtype=torch.bool)
     same[0, 1] = same[2, 0] = False
     assert torch.equal(got[same], clean[same])
+
+
+@pytest.mark.parametrize("what", ["table", "pool"])
+def test_tables_without_columns_and_pools_without_pages(what):
+    """Nothing can be read or written: outputs are 0, lists hold no page that is not there, the pools stay."""
+    _say("empty", what)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cols, pages = (0, 3) if what == "table" else (2, 0)
+    table = torch.zeros(2, cols, dtype=torch.int32, device="cuda")
+    kp, vp = (torch.full((pages, 2, 64, 64), 5.0, dtype=BF, device="cuda") for _ in range(2))
+    bd = torch.full((pages, 2, 2, 64), 5.0, dtype=BF, device="cuda")
+    cu, lens = i32(0, 70, 71), i32(100, 30)
+    q, k = randn(71, 4, 64, seed=440).cuda(), randn(71, 2, 64, seed=441).cuda()
+    qo = ops.paged_append(k, k, kp, vp, table, cu, lens, q=q, k_bounds=bd)
+    assert torch.equal(qo, q) and (kp == 5.0).all() and (vp == 5.0).all() and (bd == 5.0).all()
+    assert not ops.paged_chunk_attn(q, kp, vp, table, cu, lens).any()
+    sel, off = ops.paged_block_select(q, bd, table, lens, page=64, top_k=1, cu_seqlens=cu)
+    assert sel.max() < max(cols, 1) and off.max() <= cols
+    assert not ops.paged_chunk_attn(q, kp, vp, table, cu, lens, sel=sel, sel_off=off).any()
+    sel, off = ops.paged_block_select(q[:2], bd, table, lens, page=64, top_k=1)
+    assert sel.max() < max(cols, 1) and off.max() <= cols
