@@ -18,6 +18,7 @@ number differs from sequence to sequence.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from itertools import accumulate
 
 import torch
 
@@ -192,8 +193,13 @@ class PagedKVStore:
     def _upload_table(self, first: int, last: int) -> None:
         """Brings columns ``first .. last - 1`` of the device's table up to date; 0 where a sequence has no page."""
         cols = [row[first:last] + [0] * (last - max(first, len(row))) for row in self._table_host]
-        self.block_table[:, first:last] = torch.tensor(cols, dtype=torch.int32).to(self.block_table.device)
+        self.block_table[:, first:last] = self._upload(cols)
         self._page_cols.clear()
+
+    def _upload(self, values) -> torch.Tensor:
+        """int32 values on the store's device; from pinned memory, as a copy from other memory waits for the stream."""
+        dev = self.kv_lens.device
+        return torch.tensor(values, dtype=torch.int32, pin_memory=dev.type == "cuda").to(dev, non_blocking=True)
 
     def _uniform_len(self, what: str) -> int:
         if any(n != self.lens[0] for n in self.lens):
@@ -208,7 +214,10 @@ class PagedKVStore:
         Keys are normed (``k_weight``) and rotated (``inv_freq``, by their places in the cache or by ``positions``
         int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them
         (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).  A call that is refused leaves the store as it was.
+        Nothing here waits for the GPU.  The lengths are kept on the host, so the call cannot be captured into a graph.
         """
+        if self.kv_lens.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVStore.append advances lengths on the host; a captured graph would not")
         counts = tuple(int(n) for n in counts)
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k_new.size(0):
             raise ValueError(f"counts {counts} do not split {k_new.size(0)} tokens over {self.batch} sequences")
@@ -216,11 +225,14 @@ class PagedKVStore:
         blocks = [len(row) for row in self._table_host]
         self._grow_each(new_lens)
         try:
-            cu = [0]
-            for t in counts:
-                cu.append(cu[-1] + t)
-            cu = torch.tensor(cu, dtype=torch.int32).to(self.kv_lens.device)
-            self.kv_lens.copy_(torch.tensor(new_lens, dtype=torch.int32))
+            if min(counts) == max(counts) > 0:
+                cu = torch.arange(0, k_new.size(0) + 1, counts[0], dtype=torch.int32, device=self.kv_lens.device)
+            else:
+                cu = self._upload([0, *accumulate(counts)])
+            if min(new_lens) == max(new_lens):
+                self.kv_lens.fill_(new_lens[0])
+            else:
+                self.kv_lens.copy_(self._upload(new_lens))
             q_out = ops.paged_append(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
                                      inv_freq=inv_freq, positions=positions, k_weight=k_weight, eps=eps,
                                      k_bounds=self.k_bounds, q=q, q_weight=q_weight)

@@ -94,6 +94,48 @@ def test_appends_from_many_refusals_go_on_where_they_were():
     assert torch.equal(r.cached(r.k_pages, 1, 31), torch.cat([k[20:21], k[30:]]).cpu().double().transpose(0, 1))
 
 
+def test_appends_do_not_wait_for_the_stream():
+    """Uniform and ragged counts, with new pages and without, and a write that keeps bounds."""
+    _say("no waits")
+    st = PagedKVStore(2, 2, 64, 900, page=16, bounds=True)
+    k = randn(80, 2, 64, seed=630).cuda()
+    w = randn(2, 2, 3, 64, seed=631).cuda()
+    want, steps = [0, 0], ([40, 40], [1, 1], [0, 33], [5, 0], [1, 1], [0, 0])
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        chunks = [st.append(k[:sum(c)], k[:sum(c)], c) for c in steps]
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    for c, chunk in zip(steps, chunks):
+        want = [a + b for a, b in zip(want, c)]
+        assert chunk.cu_seqlens.tolist() == [0, c[0], sum(c)] and chunk.cu_seqlens.dtype == torch.int32
+    assert st.lens == want == st.kv_lens.tolist()
+    st.reset()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(7):
+            st.write(w, w)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert st.lens == [21, 21] == st.kv_lens.tolist()
+    r = _view(st)
+    pages = r.table[:, :2].flatten().long()
+    assert torch.equal(st.k_bounds.cpu()[pages], bounds_of(r)[pages])
+    assert torch.equal(st.gather()[0], w.repeat(1, 1, 7, 1))
+
+
+def test_an_append_under_capture_is_refused(monkeypatch):
+    """Host lengths would not advance on a replay."""
+    st = PagedKVStore(1, 1, 64, 64, page=16)
+    k = randn(3, 1, 64, seed=635).cuda()
+    before = _state(st)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        st.append(k, k, [3])
+    assert _state(st) == before
+
+
 def _model(pattern="block_topk", block_size=32):
     cfg = qwen3_config(pattern=pattern, block_size=block_size, vocab_size=512, hidden_size=256, intermediate_size=256,
                        num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=128)
