@@ -17,6 +17,7 @@ number differs from sequence to sequence.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from itertools import accumulate
 
@@ -242,6 +243,20 @@ class PagedKVStore:
             raise
         self.lens = new_lens
         return PagedChunk(cu, counts, q_out)
+
+    def refresh_bounds(self, start: int) -> None:
+        """Key bounds of the pages that hold the tokens from position ``start`` on, from their keys: for those who write
+        pages themselves, as a captured decode does (``append`` and ``write`` keep the bounds)."""
+        n = self._uniform_len("refresh_bounds")
+        first, last = start // self.page, -(-n // self.page)
+        if self.k_bounds is None or first >= last:
+            return
+        pages = self.block_table[:, first:last].long()                         # [B, nb]
+        k = self.k_pages[pages]                                                 # [B, nb, H, page, D]
+        pos = torch.arange(first * self.page, last * self.page, device=k.device).view(-1, 1, self.page, 1)
+        held = (pos < n) & ~k.isnan()
+        lo, hi = torch.where(held, k, math.inf).amin(3), torch.where(held, k, -math.inf).amax(3)
+        self.k_bounds[pages] = torch.stack([lo, hi], dim=3)
 
     def _page_col(self, lb: int) -> torch.Tensor:
         """Pages of logical block ``lb`` for every sequence, as a device index tensor (cached)."""

@@ -350,8 +350,9 @@ class GraphDecoder:
         return self.ids
 
     def finish(self) -> None:
-        """Brings the stores' lengths up to date (graph replays advance only the device state)."""
+        """Brings the stores' lengths and key bounds up to date (graph replays advance only the device state)."""
         n = self.position
         for s in self.stores:
             s.lens = [n] * s.batch
             s.kv_lens.fill_(n)
+            s.refresh_bounds(self.start)

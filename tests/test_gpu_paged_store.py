@@ -199,3 +199,23 @@ def test_qwen3_block_topk_refuses_a_page_that_is_not_its_block_before_it_appends
     with pytest.raises(ValueError, match="page"):
         model(input_ids=torch.zeros(1, 40, dtype=torch.long, device="cuda"), past_key_values=cache, use_cache=True)
     assert cache.get_seq_length() == 0
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("fused", [True, False])
+def test_a_captured_decode_leaves_key_bounds_of_what_it_wrote(fused):
+    """Its steps write keys without the append kernel; ``finish`` brings the pages' bounds up to date."""
+    _say("bounds after GraphDecoder", fused)
+    model = _model("dense", 64)
+    cache = PagedKVCache(2, 200, page=64, shuffle_seed=5, bounds=True)
+    ids = torch.randint(0, 512, (2, 90), generator=torch.Generator().manual_seed(9)).cuda()
+    out = model(input_ids=ids, past_key_values=cache, use_cache=True, logits_to_keep=1)
+    dec = GraphDecoder(model, cache, out.logits[:, -1].argmax(-1), 140, fused=fused)
+    for _ in range(12):
+        dec.step()
+    dec.finish()
+    for layer in cache.layers:
+        r = _view(layer.store)
+        assert r.lens == [102, 102]
+        pages = r.table[:, :2].flatten().long()
+        assert torch.equal(layer.store.k_bounds.cpu()[pages], bounds_of(r)[pages])
