@@ -147,8 +147,6 @@ class GraphDecoder:
         if max_len > st0.max_blocks * self.page:
             raise ValueError(f"max_len {max_len} exceeds the cache capacity {st0.max_blocks * self.page}")
         self.max_len = max_len
-        for s in self.stores:
-            s._grow_all(max_len)
         self.head_dim = cfg.head_dim
         V = cfg.vocab_size
         self.chunk = _argmax_chunk(V)
@@ -159,6 +157,8 @@ class GraphDecoder:
                 raise ValueError("GraphDecoder builds its selections before the run; block_topk selects at every step")
             if not hasattr(layer.self_attn.sparse_backend, "forward_paged"):
                 raise ValueError("GraphDecoder needs a backend with paged decode (hip_block_sparse)")
+        for s in self.stores:
+            s._grow_all(max_len)
         # one selection table per distinct pattern (dense causal layers all share one)
         sched: dict = {}
         self.sched = []
