@@ -414,7 +414,7 @@ struct ChunkWindow {
 
 // 32 rows to a workgroup: its first four waves hold the same rows and divide the keys, each with tiles of its own in
 // LDS and no barrier before they merge.  Bound by the keys' bytes: a wave keeps 32 KB of loads in flight.  8 sequences of
-// 4 new tokens over 4,096 keys, 32/8 heads, bf16, D = 128: 31 us with the merge, 134 MB.
+// 4 new tokens over 4,001 to 4,096 keys, 32/8 heads, bf16, D = 128: 34 us for 132 MB, and 4 to 5 for the merge.
 template <bool BF16, int D>
 struct ChunkNarrow : StagedTile {
   using E = Elem<BF16>;
@@ -663,7 +663,9 @@ struct ChunkNarrow : StagedTile {
 // A row's reference is the maximum of its first tile and is raised only when its probabilities would pass the
 // element type's range (REFIT_SUM), so the common step never touches O with vector instructions.
 // Bound by the step: 1.75 us of it per tile at D = 128 with the chip full, 1.35 at D = 64 (exponentials).  8K new tokens
-// over 32K keys, 32/8 heads, bf16, take 3.2 ms, 1.20 PFLOP/s where a large matrix product reaches 1.44.
+// over 32K keys, 32/8 heads, bf16, take 3.1 to 3.3 ms on different cards, 1.16 to 1.24 PFLOP/s
+// where a large matrix product reaches 1.44.  Over a selection an item holds rows of one block of 64 tokens only: all 256
+// are in use for groups of 4 and 8, 64 for groups of one, 128 for 2, 320 of 512 for 5.
 template <bool BF16, int D>
 struct ChunkWide : StagedTile {
   using E = Elem<BF16>;

@@ -21,8 +21,9 @@
 // tokens before, else written fresh.  Min and max are exact and have no order, so the result has none either.
 //
 // Measured, bf16, D = 128, 32 + 8 heads: 32K tokens unpaged 136 us, 4.9 TB/s (a copy reaches 5.4); 8K tokens in 8
-// sequences into pages of 16 with bounds 50 us, 4.0 TB/s, of which the kernel takes 45 to 47; 64 single tokens 7.3 us,
-// the latency of four dependent reads (lengths, table, rows, bounds).
+// sequences into pages of 16 with bounds 51 us, 3.9 TB/s, of which the kernel takes 45 to 47; 64 single tokens 7.3 to 7.6 us,
+// the latency of four dependent reads (lengths, table, rows, bounds).  Angles of given positions, one 8-byte read a token,
+// cost 1 % of the former (41.1 against 40.7, replayed) and nothing of the latter.
 #include <algorithm>
 
 #include "lds_tile.h"
