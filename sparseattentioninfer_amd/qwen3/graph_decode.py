@@ -157,8 +157,6 @@ class GraphDecoder:
                 raise ValueError("GraphDecoder builds its selections before the run; block_topk selects at every step")
             if not hasattr(layer.self_attn.sparse_backend, "forward_paged"):
                 raise ValueError("GraphDecoder needs a backend with paged decode (hip_block_sparse)")
-        for s in self.stores:
-            s._grow_all(max_len)
         # one selection table per distinct pattern (dense causal layers all share one)
         sched: dict = {}
         self.sched = []
@@ -182,6 +180,8 @@ class GraphDecoder:
         self.fused = fused
         if fused:
             self._init_fused(cfg)
+        for s in self.stores:
+            s._grow_all(max_len)
 
     @property
     def position(self) -> int:

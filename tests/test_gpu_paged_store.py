@@ -222,13 +222,14 @@ def test_a_captured_decode_leaves_key_bounds_of_what_it_wrote(fused):
 
 
 @torch.no_grad()
-def test_a_refused_graph_decoder_takes_no_pages():
-    _say("refused GraphDecoder")
-    model = _model("block_topk")
-    cache = PagedKVCache(2, 200, page=32, bounds=True)
+@pytest.mark.parametrize("pattern,page,text", [("block_topk", 32, "block_topk"), ("dense", 32, "page 32")])
+def test_a_refused_graph_decoder_takes_no_pages(pattern, page, text):
+    _say("refused GraphDecoder", pattern)
+    model = _model(pattern)
+    cache = PagedKVCache(2, 200, page=page, bounds=True)
     ids = torch.randint(0, 512, (2, 40), generator=torch.Generator().manual_seed(10)).cuda()
     model(input_ids=ids, past_key_values=cache, use_cache=True, logits_to_keep=1)
     before = [_state(layer.store) for layer in cache.layers]
-    with pytest.raises(ValueError, match="block_topk"):
+    with pytest.raises(ValueError, match=text):
         GraphDecoder(model, cache, ids[:, -1], 180)
     assert [_state(layer.store) for layer in cache.layers] == before
