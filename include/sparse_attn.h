@@ -573,6 +573,47 @@ int sa_paged_block_select(int dtype, const void* q, int64_t q_st, int64_t q_sh,
                           void* workspace, int64_t workspace_bytes, void* stream);
 int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks);
 
+/*
+ * The same operators over a cache held in 4 bits: 3.2 times fewer bytes than in 16.  No counterpart in the reference.
+ *
+ * A pool is [num_pages, Hkv] blocks of page * D * 5 / 8 bytes (strides of pages and heads in bytes, blocks 16-byte aligned),
+ * written for one element type T, the dtype of the calls that read it.  32 dims of one token's head are a group, held as
+ * m + s c: m = min x, s = (max x - min x) / 15 toward zero to T (a scale below 2^-126 is 0), c = floor((x - m) / s + 1/2)
+ * and at most 15, 0 where s is.  x is of type T, so a value is off by at most s / 2 (the group's largest by at most what
+ * cutting s takes from 15 s: 0.12 s in bf16).  A group with a NaN or an infinity reads back as NaN.  In a block, first the codes:
+ *   keys    word (D / 32) q + g of a token's D / 2 bytes: dims 32 g + 8 q + e at bit 8 (e % 4) + 4 (e / 4), e < 8
+ *   values  byte t % 4 of word (D / 32) i + g of the 2 D bytes that tokens t with one t / 4 share: dims 32 g + i (low four
+ *           bits) and 32 g + 16 + i (high), i < 16
+ * then the pairs (s, m) of type T, [D / 32][page].
+ *
+ * What a slot holds that no token was written to is never used, whatever its bytes.
+ */
+
+/*
+ * sa_paged_append into such pools: norms and rotation as there, rounded to T, then quantised.  positions (device int64,
+ * stride pos_st; with inv_freq) or NULL as for sa_paged_append_at.  k_bounds are those of the keys as they are read back.
+ */
+int sa_paged_append_q4(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                       const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                       const void* q_weight, const void* k_weight, const float* inv_freq,
+                       const int64_t* positions, int64_t pos_st,
+                       void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,
+                       void* k_bounds, int64_t bounds_sp, int64_t bounds_sh,
+                       const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                       const int32_t* cu_seqlens, const int32_t* kv_lens,
+                       int N, int B, int Hq, int Hkv, int D, int page, float eps, void* stream);
+
+/*
+ * Reads such pools back: packed row cu_seqlens[b] + i of k_out and v_out [N, Hkv, D] (strides in elements) receives token
+ * kv_lens[b] - n + i of sequence b, n = cu_seqlens[b + 1] - cu_seqlens[b] of them; m + s c in fp32, rounded once.  Rows of
+ * no sequence are left as they were; tokens without a page (past the table, ids outside the pool) are zeros.
+ */
+int sa_paged_read_q4(int dtype, const void* k_pages, const void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,
+                     const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                     const int32_t* cu_seqlens, const int32_t* kv_lens,
+                     void* k_out, int64_t ko_st, int64_t ko_sh, void* v_out, int64_t vo_st, int64_t vo_sh,
+                     int N, int B, int Hkv, int D, int page, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -204,6 +204,19 @@ SIGNATURES = {
         _vp, _i64, _vp,
     ]),
     "sa_paged_block_select_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "sa_paged_append_q4": (_i32, [
+        _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+        _vp, _i64,                                        # positions
+        _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64,      # pools, bounds
+        _vp, _i64, _i32, _vp, _vp,
+        _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp,
+    ]),
+    "sa_paged_read_q4": (_i32, [
+        _i32, _vp, _vp, _i64, _i64, _i32,                 # pools
+        _vp, _i64, _i32, _vp, _vp,
+        _vp, _i64, _i64, _vp, _i64, _i64,                 # k_out, v_out
+        _i32, _i32, _i32, _i32, _i32, _vp,
+    ]),
 }
 
 

@@ -26,6 +26,7 @@
 // cost 1 % of the former (41.1 against 40.7, replayed) and nothing of the latter.
 #include <algorithm>
 
+#include "kv4.h"
 #include "lds_tile.h"
 #include "ragged.h"
 
@@ -62,7 +63,13 @@ struct RopeArgs {
   const int32_t* table;
   int64_t table_stride;
   int max_blocks, num_pages, page;
+  // paged, in 4 bits: pools of blocks (kv4.h), strides in bytes
+  uint8_t *k4, *v4;
+  int64_t p4_sp, p4_sh;
 };
+
+// What heads are written to: rows, pages, or pages held in 4 bits.
+enum : int { TO_ROWS = 0, TO_PAGES = 1, TO_PAGES_4BIT = 2 };
 
 template <bool BF16>
 __device__ __forceinline__ void unpack8(u32x4 v, float* f) {
@@ -80,8 +87,60 @@ __device__ __forceinline__ u32x4 pack8(const float* f) {
   return v;
 }
 
-template <bool BF16, int D, bool PAGED>
+// Codes of one group's 32 dims, of which each of four neighbouring lanes holds 8: `lo` and `hi` the lane's codes of dims
+// 0..3 and 4..7, a byte each; the group's pair, as stored.
+template <bool BF16>
+struct Group4 {
+  uint32_t lo, hi, pair;
+
+  __device__ __forceinline__ explicit Group4(const float* x) {
+    float mn = x[0], mx = x[0], odd = 0.f * x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+      mn = fminf(mn, x[e]);
+      mx = fmaxf(mx, x[e]);
+      odd = fmaf(x[e], 0.f, odd);              // NaN if one of them is no finite number
+    }
+    mn = fminf(mn, dpp<0xB1>(mn));
+    mx = fmaxf(mx, dpp<0xB1>(mx));
+    odd += dpp<0xB1>(odd);
+    mn = fminf(mn, dpp<0x4E>(mn));
+    mx = fmaxf(mx, dpp<0x4E>(mx));
+    odd += dpp<0x4E>(odd);
+    // Halves: the range of large bf16 values passes fp32's.
+    const float half = 0.5f * mn;
+    float s = cut(fmaf(0.5f, mx, -half) / 7.5f);
+    s = s < 1.17549435e-38f ? 0.f : s;
+    // 2 / s, and so much more that the rounded products below never bring a tie under the code it goes up to: 2^-22
+    // against 2^-24 each of the quotient and the product.
+    const float r = s > 0.f ? 2.f / s * 1.0000002384185791f : 0.f;
+    uint32_t c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = (uint32_t)fminf(fmaf(fmaf(0.5f, x[e], -half), r, 0.5f), 15.f);
+    lo = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+    hi = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
+    const uint32_t nan = BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+    pair = odd == 0.f ? (uint32_t)Elem<BF16>::from_f32(s) | (uint32_t)Elem<BF16>::from_f32(mn) << 16 : nan;
+  }
+  // Toward zero to the element type.
+  static __device__ __forceinline__ float cut(float s) {
+    if constexpr (BF16) return __uint_as_float(__float_as_uint(s) & 0xffff0000u);
+    const float t = Elem<false>::to_f32(Elem<false>::from_f32(s));
+    return t > s ? Elem<false>::to_f32((elem_t)(Elem<false>::from_f32(s) - 1)) : t;
+  }
+  // The lane's 8 values as they are read back.
+  __device__ __forceinline__ u32x4 values() const {
+    const float s = q4_scale<BF16>(pair), m = q4_min<BF16>(pair);
+    return u32x4{Elem<BF16>::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
+                 Elem<BF16>::pack2f(fmaf(q4_code<2>(lo), s, m), fmaf(q4_code<3>(lo), s, m)),
+                 Elem<BF16>::pack2f(fmaf(q4_code<0>(hi), s, m), fmaf(q4_code<1>(hi), s, m)),
+                 Elem<BF16>::pack2f(fmaf(q4_code<2>(hi), s, m), fmaf(q4_code<3>(hi), s, m))};
+  }
+};
+
+template <bool BF16, int D, int TO>
 struct RopeAppend {
+  static constexpr bool PAGED = TO != TO_ROWS;
   static constexpr int LPR = D / 16;            // lanes of one token's head
   static constexpr int RPI = 64 / LPR;          // tokens of a wave's pass
   static constexpr int HALF = D / 2;
@@ -282,7 +341,10 @@ struct RopeAppend {
         vl = pack8<BF16>(l);
         vh = pack8<BF16>(r);
       }
-      if (live) {
+      if (TO == TO_PAGES_4BIT && cur.kind) {
+        const int pg = live ? s_page[slot / RA_CHUNK] : -1;
+        store4(a, w, cur.kind, cur.hh, vl, vh, c, g, slot, pg, live ? s_slot[slot / RA_CHUNK] + slot % RA_CHUNK : 0);
+      } else if (live) {
         elem_t* d = nullptr;
         if (!PAGED || cur.kind == 0) {
           d = cur.dst + row_at(a, w.row0 + slot, cur.d_sb, cur.d_st) + 8 * c;
@@ -315,6 +377,67 @@ struct RopeAppend {
       }
       if (h >= h_end) break;
     }
+  }
+
+  // Writes a pass's heads in 4 bits: the lane's dims 8 c .. + 7 (vl) and D / 2 + 8 c .. + 7 (vh) of the token at `slot`
+  // of the window, `at` of page `pg` (-1: not written).  vl and vh are left as they are read back.
+  static __device__ __forceinline__ void store4(const RopeArgs& a, const Window& w, int kind, int hh, u32x4& vl, u32x4& vh,
+                                                int c, int g, int slot, int pg, int at) {
+    using F = Kv4<D>;
+    float x[16];
+    unpack8<BF16>(vl, x);
+    unpack8<BF16>(vh, x + 8);
+    const Group4<BF16> l(x), h(x + 8);
+    const int q = c & 3, gl = c >> 2, gh = D / 64 + gl;
+    uint8_t* block = nullptr;
+    if (pg >= 0) block = (kind == 1 ? a.k4 : a.v4) + pg * a.p4_sp + hh * a.p4_sh;
+    if (pg >= 0 && q == 0) {
+      uint32_t* st = reinterpret_cast<uint32_t*>(block + F::stats_at(a.page)) + at;
+      st[gl * a.page] = l.pair;
+      st[gh * a.page] = h.pair;
+    }
+    if (kind == 1) {
+      if (pg >= 0) {
+        uint32_t* row = reinterpret_cast<uint32_t*>(block + at * F::ROW) + F::NG * q;
+        row[gl] = l.lo | l.hi << 4;
+        row[gh] = h.lo | h.hi << 4;
+      }
+      if (a.bounds) {
+        vl = l.values();
+        vh = h.values();
+      }
+      return;
+    }
+    // Lanes q and q ^ 2 hold dims i and i + 16 of a group: the first takes both halves of the lower group's bytes, the
+    // second of the upper's, 8 dims i each.
+    const bool up = q & 2;
+    const uint32_t x0 = quad2(up ? l.lo : h.lo), x1 = quad2(up ? l.hi : h.hi);
+    const uint32_t b0 = up ? x0 | h.lo << 4 : l.lo | x0 << 4, b1 = up ? x1 | h.hi << 4 : l.hi | x1 << 4;
+    const int group = up ? gh : gl, i0 = 8 * (q & 1), r = g & 3;
+    // Four tokens' bytes of one dim make a word: two exchanges between the lanes of tokens r ^ 1 and r ^ 2, after which a
+    // lane holds the words of two dims.
+    const bool odd = r & 1, high = r & 2;
+    const uint32_t y = __shfl_xor(odd ? b0 : b1, LPR, 64);
+    const uint32_t te = odd ? y : b0, to = odd ? b1 : y;
+    const uint32_t p0 = __builtin_amdgcn_perm(to, te, 0x05010400), p1 = __builtin_amdgcn_perm(to, te, 0x07030602);
+    const uint32_t z = __shfl_xor(high ? p0 : p1, 2 * LPR, 64);
+    const uint32_t f0 = high ? z : p0, f1 = high ? p1 : z;
+    if (pg < 0) return;
+    uint8_t* quad = block + (at >> 2) * F::QUAD + 4 * group;
+    const int s4 = slot & ~3;
+    if (s4 >= w.lo && s4 + 4 <= w.hi) {
+      uint8_t* p = quad + (i0 + 4 * (r & 1) + (r & 2)) * (D / 8);
+      *reinterpret_cast<uint32_t*>(p) = __builtin_amdgcn_perm(f1, f0, 0x05040100);
+      *reinterpret_cast<uint32_t*>(p + D / 8) = __builtin_amdgcn_perm(f1, f0, 0x07060302);
+    } else {                                   // not all four of them are here: byte by byte
+#pragma unroll
+      for (int j = 0; j < 8; ++j) quad[(i0 + j) * (D / 8) + r] = (uint8_t)((j < 4 ? b0 : b1) >> (8 * (j & 3)));
+    }
+  }
+
+  // The value of lane l ^ 2.
+  static __device__ __forceinline__ uint32_t quad2(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true);
   }
 
   // Sum over the LPR (4 or 8) lanes of a token's head, in every one.
@@ -361,23 +484,23 @@ struct RopeAppend {
   }
 };
 
-template <bool BF16, int D, bool PAGED>
+template <bool BF16, int D, int TO>
 __global__ __launch_bounds__(RA_THREADS) void rope_append_kernel(const RopeArgs a) {
-  RopeAppend<BF16, D, PAGED>::run(a);
+  RopeAppend<BF16, D, TO>::run(a);
 }
 
-template <bool PAGED>
+template <int TO>
 static int launch_rope(const char* name, int dtype, int D, const RopeArgs& a, dim3 grid, hipStream_t s) {
   const dim3 block(RA_THREADS);
   const size_t lds = a.inv_freq ? (size_t)a.window * (D + 4) * sizeof(float) : 0;
   if (dtype == SA_DTYPE_BF16 && D == 128)
-    hipLaunchKernelGGL((rope_append_kernel<true, 128, PAGED>), grid, block, lds, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<true, 128, TO>), grid, block, lds, s, a);
   else if (dtype == SA_DTYPE_BF16)
-    hipLaunchKernelGGL((rope_append_kernel<true, 64, PAGED>), grid, block, lds, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<true, 64, TO>), grid, block, lds, s, a);
   else if (D == 128)
-    hipLaunchKernelGGL((rope_append_kernel<false, 128, PAGED>), grid, block, lds, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<false, 128, TO>), grid, block, lds, s, a);
   else
-    hipLaunchKernelGGL((rope_append_kernel<false, 64, PAGED>), grid, block, lds, s, a);
+    hipLaunchKernelGGL((rope_append_kernel<false, 64, TO>), grid, block, lds, s, a);
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "%s: launch failed: %s", name, hipGetErrorString(err));
 }
@@ -440,10 +563,11 @@ extern "C" int sa_qk_norm_rope(int dtype, const void* q, int64_t q_sb, int64_t q
   if (windows > MAX_WORKGROUPS) return set_error(SA_E_SHAPE, "%s: %lld tokens are too many", name, (long long)a.N);
   a.heads_per_part = heads_per_part(windows, Hq + Hkv, RA_TARGET);
   const int parts = (Hq + Hkv + a.heads_per_part - 1) / a.heads_per_part;
-  return launch_rope<false>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
+  return launch_rope<TO_ROWS>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
 }
 
-static int append(const char* name, int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+// four: pools of 4-bit blocks, strides of pages and heads in bytes.
+static int append(const char* name, bool four, int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
                   int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
                   const void* q_weight, const void* k_weight, const float* inv_freq, const int64_t* positions,
                   int64_t pos_st, void* k_pages, void* v_pages, int64_t pages_sp, int64_t pages_sh, int64_t pages_st,
@@ -466,8 +590,9 @@ static int append(const char* name, int dtype, const void* q, int64_t q_st, int6
     return set_error(SA_E_NULL, "%s: NULL pointer", name);
   if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out) || misaligned(q_weight) ||
       misaligned(k_weight) || misaligned(k_pages) || misaligned(v_pages) || misaligned(k_bounds) ||
-      (q_st | q_sh | k_st | k_sh | v_st | v_sh | qo_st | qo_sh | pages_sp | pages_sh | pages_st | bounds_sp | bounds_sh) % 8)
-    return set_error(SA_E_ALIGN, "%s: head rows must be 16-byte aligned", name);
+      (q_st | q_sh | k_st | k_sh | v_st | v_sh | qo_st | qo_sh | pages_sp | pages_sh | pages_st | bounds_sp | bounds_sh) % 8 ||
+      (four && (pages_sp | pages_sh) % 16))
+    return set_error(SA_E_ALIGN, "%s: head rows%s must be 16-byte aligned", name, four ? " and blocks" : "");
   RopeArgs a = {};
   a.q = static_cast<const elem_t*>(q);
   a.k = static_cast<const elem_t*>(k);
@@ -483,9 +608,15 @@ static int append(const char* name, int dtype, const void* q, int64_t q_st, int6
   a.N = N;
   a.Hq = Hq, a.Hkv = Hkv, a.eps = eps;
   a.seqs = Ragged{cu_seqlens, kv_lens, B, N};
-  a.k_pages = static_cast<elem_t*>(k_pages);
-  a.v_pages = static_cast<elem_t*>(v_pages);
-  a.pg_sp = pages_sp, a.pg_sh = pages_sh, a.pg_st = pages_st;
+  if (four) {
+    a.k4 = static_cast<uint8_t*>(k_pages);
+    a.v4 = static_cast<uint8_t*>(v_pages);
+    a.p4_sp = pages_sp, a.p4_sh = pages_sh;
+  } else {
+    a.k_pages = static_cast<elem_t*>(k_pages);
+    a.v_pages = static_cast<elem_t*>(v_pages);
+    a.pg_sp = pages_sp, a.pg_sh = pages_sh, a.pg_st = pages_st;
+  }
   a.bounds = static_cast<elem_t*>(k_bounds);
   a.bd_sp = bounds_sp, a.bd_sh = bounds_sh;
   a.table = block_table;
@@ -501,7 +632,9 @@ static int append(const char* name, int dtype, const void* q, int64_t q_st, int6
   const int heads = Hq + 2 * Hkv;
   a.heads_per_part = heads_per_part(windows, heads, RA_TARGET_PAGED);
   const int parts = (heads + a.heads_per_part - 1) / a.heads_per_part;
-  return launch_rope<true>(name, dtype, D, a, dim3((unsigned)windows, parts), static_cast<hipStream_t>(stream));
+  const dim3 grid((unsigned)windows, parts);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return four ? launch_rope<TO_PAGES_4BIT>(name, dtype, D, a, grid, st) : launch_rope<TO_PAGES>(name, dtype, D, a, grid, st);
 }
 
 extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
@@ -513,7 +646,7 @@ extern "C" int sa_paged_append(int dtype, const void* q, int64_t q_st, int64_t q
                                const int32_t* cu_seqlens, const int32_t* kv_lens, int N, int B, int Hq, int Hkv,
                                int D, int page, float eps, void* stream) {
   clear_error();
-  return append("sa_paged_append", dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight,
+  return append("sa_paged_append", false, dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight,
                 k_weight, inv_freq, nullptr, 0, k_pages, v_pages, pages_sp, pages_sh, pages_st, num_pages, k_bounds,
                 bounds_sp, bounds_sh, block_table, block_table_stride, max_blocks, cu_seqlens, kv_lens, N, B, Hq, Hkv, D,
                 page, eps, stream);
@@ -532,8 +665,26 @@ extern "C" int sa_paged_append_at(int dtype, const void* q, int64_t q_st, int64_
   const char* name = "sa_paged_append_at";
   if (N > 0 && B > 0 && (!inv_freq || !positions)) return set_error(SA_E_NULL, "%s: NULL inv_freq or positions", name);
   if (pos_st < 0) return set_error(SA_E_SHAPE, "%s: positions of stride %lld", name, (long long)pos_st);
-  return append(name, dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight, k_weight,
+  return append(name, false, dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight, k_weight,
                 inv_freq, positions, pos_st, k_pages, v_pages, pages_sp, pages_sh, pages_st, num_pages, k_bounds,
                 bounds_sp, bounds_sh, block_table, block_table_stride, max_blocks, cu_seqlens, kv_lens, N, B, Hq, Hkv, D,
                 page, eps, stream);
+}
+
+extern "C" int sa_paged_append_q4(int dtype, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, void* q_out, int64_t qo_st,
+                                  int64_t qo_sh, const void* q_weight, const void* k_weight, const float* inv_freq,
+                                  const int64_t* positions, int64_t pos_st, void* k_pages, void* v_pages,
+                                  int64_t pages_sp, int64_t pages_sh, int num_pages, void* k_bounds, int64_t bounds_sp,
+                                  int64_t bounds_sh, const int32_t* block_table, int64_t block_table_stride,
+                                  int max_blocks, const int32_t* cu_seqlens, const int32_t* kv_lens, int N, int B, int Hq,
+                                  int Hkv, int D, int page, float eps, void* stream) {
+  clear_error();
+  const char* name = "sa_paged_append_q4";
+  if (positions && !inv_freq) return set_error(SA_E_NULL, "%s: positions without inv_freq", name);
+  if (positions && pos_st < 0) return set_error(SA_E_SHAPE, "%s: positions of stride %lld", name, (long long)pos_st);
+  return append(name, true, dtype, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, q_out, qo_st, qo_sh, q_weight, k_weight,
+                inv_freq, positions, pos_st, k_pages, v_pages, pages_sp, pages_sh, 0, num_pages, k_bounds, bounds_sp,
+                bounds_sh, block_table, block_table_stride, max_blocks, cu_seqlens, kv_lens, N, B, Hq, Hkv, D, page, eps,
+                stream);
 }

@@ -11,8 +11,10 @@ may hold one row per KV group.
 ``paged_sparse_decode`` is new: one query token per sequence over a paged
 cache.  So are the operators of a chunk of new tokens over a paged cache, for
 sequences of different lengths: ``qk_norm_rope``, ``paged_append``,
-``paged_chunk_attn`` and ``paged_block_select``.  All work is enqueued on the
-current HIP stream; nothing synchronises.
+``paged_chunk_attn`` and ``paged_block_select``, and those of a cache held in
+4 bits: ``paged_append_q4``, ``paged_read_q4``, ``paged_chunk_attn_q4`` and
+``paged_sparse_decode_q4``.  All work is enqueued on the current HIP stream;
+nothing synchronises.
 """
 from __future__ import annotations
 
@@ -1099,3 +1101,140 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, block_table: tor
           top_k, sink, recent, sel.data_ptr(), Hkv * width, width, rows, width, sel_off.data_ptr(),
           None if ws is None else ws.data_ptr(), need)
     return sel, sel_off
+
+
+# ---- the paged cache in 4 bits -------------------------------------------------------------------
+
+Q4_GROUP = 32       # dims of a token's head that share a scale and a minimum (include/sparse_attn.h)
+
+
+def q4_block_bytes(page: int, head_dim: int) -> int:
+    """Bytes of one page of one KV head in a 4-bit pool: ``page * head_dim * 5 / 8``."""
+    _require(page % 16 == 0 and 16 <= page <= 128, f"q4_block_bytes: page {page} is not a multiple of 16 in [16, 128]")
+    _require(head_dim in (64, 128), f"q4_block_bytes: head_dim {head_dim} is not 64 or 128")
+    return page * head_dim * 5 // 8
+
+
+def _q4_page(nbytes: int, D: int) -> int:
+    """Tokens of a page whose block has ``nbytes``, 0 if no page has."""
+    page, odd = divmod(nbytes * 8, 5 * D) if D > 0 else (0, 1)
+    return 0 if odd or page % 16 or not 16 <= page <= 128 else page
+
+
+def _q4_pools_ok(kp: torch.Tensor, vp: torch.Tensor, dev) -> bool:
+    return (kp.dtype == torch.uint8 and vp.dtype == torch.uint8 and kp.device == dev and vp.device == dev and kp.dim() == 3
+            and kp.shape == vp.shape and kp.stride() == vp.stride() and kp.stride(2) == 1)
+
+
+def _refuse_q4(name: str, like: torch.Tensor, dtype, D: int, kp: torch.Tensor, vp: torch.Tensor, *, heads: dict, index: dict,
+               other: str) -> None:
+    """Says what is wrong with a call on 4-bit pools whose one test of everything has failed."""
+    dev = like.device
+    _require(like.is_cuda and dtype in _DTYPES, f"{name}: the element type must be fp16 or bf16 on the GPU, got {dtype} on {dev}")
+    for label, t in (("k_pages", kp), ("v_pages", vp)):
+        _require(t.dtype == torch.uint8 and t.device == dev, f"{name}: {label} must be a uint8 pool on {dev}, got {t.dtype} on {t.device}")
+        _require(t.dim() == 3 and t.stride(2) == 1,
+                 f"{name}: {label} must be [P, Hkv, block bytes] with contiguous blocks, got {tuple(t.shape)}")
+    _require(kp.shape == vp.shape and kp.stride() == vp.stride(), f"{name}: k and v pools must share shape and strides")
+    _require(_q4_page(kp.size(2), D) > 0, f"{name}: blocks of {kp.size(2)} bytes hold no page of head dim {D} (q4_block_bytes)")
+    _refuse(name, like, heads=heads, index=index, B=index["block_table"].size(0) if index["block_table"].dim() else 0, other=other)
+
+
+def paged_append_q4(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *,
+                    inv_freq: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                    k_weight: torch.Tensor | None = None, eps: float = 1e-6, k_bounds: torch.Tensor | None = None,
+                    q: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                    q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """:func:`paged_append` into a cache held in 4 bits: norms, rotation, quantisation and page writes in one launch.
+
+    ``k_pages, v_pages [P, Hkv, q4_block_bytes(page, D)]`` uint8; everything else is as for :func:`paged_append`, and
+    the pools belong to the element type of ``k``.  Each group of 32 dims of a token's head keeps its minimum and a
+    fifteenth of its range, so a value is off by at most half of that step.  ``k_bounds [P, Hkv, 2, D]`` holds the
+    smallest and largest key per dim as they are read back.
+    """
+    name = "paged_append_q4"
+    dt, dev, ks, ps, B = k.dtype, k.device, k.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    kst, vst = k.stride(), v.stride()
+    page = _q4_page(ps[2], ks[2]) if len(ps) == 3 and len(ks) == 3 else 0
+    ok = (k.is_cuda and dt in _DTYPES and len(ks) == 3 and v.shape == ks and v.dtype == dt and v.device == dev
+          and kst[2] == 1 and vst[2] == 1 and _q4_pools_ok(k_pages, v_pages, dev) and ps[1] == ks[1] and page > 0
+          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
+          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
+          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+          and (k_weight is None or (k_weight.shape == (ks[2],) and k_weight.dtype == dt and k_weight.device == dev
+                                    and k_weight.is_contiguous()))
+          and (inv_freq is None or (inv_freq.dtype == torch.float32 and inv_freq.shape == (ks[2] // 2,)
+                                    and inv_freq.is_contiguous() and inv_freq.device == dev))
+          and (positions is None or (inv_freq is not None and positions.dtype == torch.int64 and positions.device == dev
+                                     and positions.shape == (ks[0],))))
+    if ok and k_bounds is not None:
+        ok = (k_bounds.shape == (ps[0], ps[1], 2, ks[2]) and k_bounds.dtype == dt and k_bounds.device == dev
+              and k_bounds.stride(3) == 1 and k_bounds.stride(2) == ks[2])
+    qargs, oargs, Hq = (None, 0, 0), (None, 0, 0), 0
+    if q is None:
+        ok = ok and q_out is None and q_weight is None
+    elif ok:
+        if q_out is None:
+            q_out = _empty_like(q)
+        qs, qst, ost = q.shape, q.stride(), q_out.stride()
+        ok = (len(qs) == 3 and qs[0] == ks[0] and qs[2] == ks[2] and q.dtype == dt and q.device == dev and qst[2] == 1
+              and q_out.shape == qs and q_out.dtype == dt and q_out.device == dev and ost[2] == 1
+              and (q_weight is None or (q_weight.shape == (ks[2],) and q_weight.dtype == dt and q_weight.device == dev
+                                        and q_weight.is_contiguous())))
+        if ok:
+            qargs, oargs, Hq = (q.data_ptr(), qst[0], qst[1]), (q_out.data_ptr(), ost[0], ost[1]), qs[1]
+    if not ok:
+        _refuse_q4(name, k, dt, ks[-1] if len(ks) else 0, k_pages, v_pages,
+                   heads=dict(k=k, v=v, q=q, q_out=q_out, k_bounds=k_bounds, q_weight=q_weight, k_weight=k_weight),
+                   index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens),
+                   other="k and v must be [N, Hkv, D], q [N, Hq, D] (q_out and q_weight need it), norm weights [D], inv_freq "
+                         "float32 [D/2], pools of Hkv heads, k_bounds [P, Hkv, 2, D] with contiguous [2, D], positions (with "
+                         "inv_freq) int64 [N]")
+    bargs = (None, 0, 0) if k_bounds is None else (k_bounds.data_ptr(), k_bounds.stride(0), k_bounds.stride(1))
+    at = (None, 0) if positions is None else (positions.data_ptr(), positions.stride(0))
+    _call("sa_paged_append_q4", dev.index, _DTYPES[dt], *qargs, k.data_ptr(), kst[0], kst[1], v.data_ptr(), vst[0], vst[1],
+          *oargs, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+          None if inv_freq is None else inv_freq.data_ptr(), *at, k_pages.data_ptr(), v_pages.data_ptr(),
+          k_pages.stride(0), k_pages.stride(1), ps[0], *bargs, block_table.data_ptr(), block_table.stride(0),
+          block_table.size(1), cu_seqlens.data_ptr(), kv_lens.data_ptr(), ks[0], B, Hq, ks[1], ks[2], page, eps)
+    return q_out
+
+
+def paged_read_q4(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                  kv_lens: torch.Tensor, *, rows: int, head_dim: int, dtype: torch.dtype,
+                  k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of a 4-bit cache as ``[rows, Hkv, head_dim]`` tensors of ``dtype``, the type the pools were written for.
+
+    The last ``cu_seqlens[b + 1] - cu_seqlens[b]`` tokens of the ``kv_lens[b]`` of each sequence b, packed as
+    :func:`paged_append_q4` takes them; whole sequences where those are its length.  ``rows`` is the packed tensors' (the
+    lengths are on the device).  Rows of given outputs that belong to no sequence are left as they are.
+    """
+    name = "paged_read_q4"
+    dev, ps, B = k_pages.device, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    page = _q4_page(ps[2], head_dim) if len(ps) == 3 else 0
+    ok = (k_pages.is_cuda and dtype in _DTYPES and _q4_pools_ok(k_pages, v_pages, dev) and page > 0 and rows >= 0
+          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
+          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
+          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous())
+    shape = (rows, ps[1] if len(ps) == 3 else 0, head_dim)
+    for out in (k_out, v_out):
+        ok = ok and (out is None or (out.shape == shape and out.dtype == dtype and out.device == dev and out.stride(2) == 1))
+    if not ok:
+        outs = {label: t for label, t in (("k_out", k_out), ("v_out", v_out)) if t is not None}
+        like = next(iter(outs.values()), torch.empty(0, dtype=dtype, device=dev)) if k_pages.is_cuda else k_pages
+        _refuse_q4(name, like, dtype, head_dim, k_pages, v_pages, heads=outs,
+                   index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens),
+                   other=f"outputs must be [rows={rows}, Hkv, head_dim={head_dim}] of {dtype} on {dev}")
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=dev)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=dtype, device=dev)
+    kst, vst = k_out.stride(), v_out.stride()
+    _call("sa_paged_read_q4", dev.index, _DTYPES[dtype], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0),
+          k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
+          kv_lens.data_ptr(), k_out.data_ptr(), kst[0], kst[1], v_out.data_ptr(), vst[0], vst[1], rows, B, ps[1], head_dim, page)
+    return k_out, v_out

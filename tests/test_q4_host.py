@@ -1,0 +1,95 @@
+"""The 4-bit cache on the CPU: the byte form of its reference, and what the operators refuse before any device access."""
+import pytest
+import torch
+
+from sparseattentioninfer_amd import _lib, ops
+from tests.q4_reference import codes_of, pack, places, quantise, unpack, value_of
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,D", [(16, 64), (48, 128), (64, 128)])
+def test_form(dtype, page, D):
+    x = torch.randn(2, 3, page, D, generator=torch.Generator().manual_seed(1)).to(dtype)
+    code, s, m = quantise(x)
+    for values in (False, True):
+        byte, shift = places(page, D, values)
+        assert sorted((byte * 8 + shift).flatten().tolist()) == list(range(0, page * D // 2 * 8, 4))   # every nibble once
+        pool = pack(x, values)
+        assert pool.shape == (2, 3, ops.q4_block_bytes(page, D))
+        assert torch.equal(codes_of(pool, page, D, values), code)
+        assert torch.equal(unpack(pool, page, D, dtype, values), value_of(code, s, m))
+    err = (value_of(code, s, m) - x.double()).abs().unflatten(-1, (-1, 32))
+    assert (err <= s.double()[..., None] / 2).all()
+    assert (value_of(code, s, m).unflatten(-1, (-1, 32)).amax(-1) <= x.double().unflatten(-1, (-1, 32)).amax(-1)).all()
+
+
+def test_block_bytes():
+    assert ops.q4_block_bytes(64, 128) == 5120 and ops.q4_block_bytes(16, 64) == 640
+    for page, D in ((8, 128), (40, 128), (144, 128), (64, 96)):
+        with pytest.raises(AssertionError):
+            ops.q4_block_bytes(page, D)
+
+
+def test_calls_refuse_cpu_tensors():
+    pool = torch.zeros(2, 1, 5120, dtype=torch.uint8)
+    i = lambda *n: torch.tensor(n, dtype=torch.int32)
+    x = torch.zeros(1, 1, 128, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="on the GPU"):
+        ops.paged_append_q4(x, x, pool, pool, i(0)[None], i(0, 1), i(1))
+    with pytest.raises(AssertionError, match="on the GPU"):
+        ops.paged_read_q4(pool, pool, i(0)[None], i(0, 1), i(1), rows=1, head_dim=128, dtype=torch.bfloat16)
+
+
+FAKE = 1 << 12      # a 16-byte aligned stand-in address
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.library_path().exists():
+        from sparseattentioninfer_amd import _build
+        _build.build(verbose=False)
+    return _lib.load()
+
+
+def _append(lib, **o):
+    a = dict(dtype=0, k=FAKE, kp=FAKE, sp=10240, inv=FAKE, pos=None, pos_st=1, N=4, B=2, D=128, page=64, pages=8, mb=4, st=4,
+             table=FAKE, Hkv=2, Hq=0, q=None)
+    a.update(o)
+    return lib.sa_paged_append_q4(a["dtype"], a["q"], 1024, 128, a["k"], 1024, 128, FAKE, 1024, 128, None, 0, 0, None, None,
+                                  a["inv"], a["pos"], a["pos_st"], a["kp"], FAKE, a["sp"], 5120, a["pages"], None, 0, 0,
+                                  a["table"], a["st"], a["mb"], FAKE, FAKE, a["N"], a["B"], a["Hq"], a["Hkv"], a["D"],
+                                  a["page"], 1e-6, None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=5), -1, b"dtype 5"), (dict(D=96), -3, b"head dim 96"), (dict(page=24), -4, b"page 24"),
+    (dict(page=144), -4, b"page 144"), (dict(N=-1), -2, b"bad sizes"), (dict(mb=8), -2, b"8 columns"),
+    (dict(k=None), -6, b"NULL"), (dict(kp=None), -6, b"NULL"), (dict(table=None), -6, b"NULL"), (dict(Hq=4), -6, b"NULL"),
+    (dict(kp=FAKE + 8), -8, b"aligned"), (dict(sp=10248), -8, b"aligned"), (dict(k=FAKE + 2), -8, b"aligned"),
+    (dict(pos=FAKE, inv=None), -6, b"inv_freq"), (dict(pos=FAKE, pos_st=-1), -2, b"stride -1")])
+def test_append_refusals(lib, change, code, text):
+    assert _append(lib, **change) == code and b"sa_paged_append_q4" in lib.sa_last_error() and text in lib.sa_last_error()
+
+
+def test_append_nothing_to_do(lib):
+    assert _append(lib, N=0, k=None) == 0 and _append(lib, B=0) == 0
+
+
+def _read(lib, **o):
+    a = dict(dtype=0, kp=FAKE, sp=10240, N=4, B=2, D=128, page=64, pages=8, mb=4, table=FAKE, Hkv=2, ko=FAKE, ko_st=256)
+    a.update(o)
+    return lib.sa_paged_read_q4(a["dtype"], a["kp"], FAKE, a["sp"], 5120, a["pages"], a["table"], 4, a["mb"], FAKE, FAKE,
+                                a["ko"], a["ko_st"], 128, FAKE, 256, 128, a["N"], a["B"], a["Hkv"], a["D"], a["page"], None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=2), -1, b"dtype 2"), (dict(D=256), -3, b"head dim 256"), (dict(page=0), -4, b"page 0"),
+    (dict(Hkv=0), -2, b"bad sizes"), (dict(mb=5), -2, b"5 columns"), (dict(kp=None), -6, b"NULL"),
+    (dict(ko=None), -6, b"NULL"), (dict(table=None), -6, b"NULL"), (dict(kp=FAKE + 4), -8, b"aligned"),
+    (dict(ko=FAKE + 2), -8, b"aligned"), (dict(ko_st=260), -8, b"aligned"), (dict(N=1 << 30, B=1 << 26), -2, b"too many")])
+def test_read_refusals(lib, change, code, text):
+    assert _read(lib, **change) == code and b"sa_paged_read_q4" in lib.sa_last_error() and text in lib.sa_last_error()
+
+
+def test_read_nothing_to_do(lib):
+    assert _read(lib, N=0, ko=None) == 0 and _read(lib, B=0) == 0
