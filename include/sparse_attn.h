@@ -614,6 +614,37 @@ int sa_paged_read_q4(int dtype, const void* k_pages, const void* v_pages, int64_
                      void* k_out, int64_t ko_st, int64_t ko_sh, void* v_out, int64_t vo_st, int64_t vo_sh,
                      int N, int B, int Hkv, int D, int page, void* stream);
 
+/*
+ * sa_paged_chunk_attn over such pools: causal attention of the new tokens, over every page or a selection's, with the
+ * division of keys, the workspace (sa_paged_chunk_workspace_bytes) and the rules for rows and pages given there.
+ */
+int sa_paged_chunk_attn_q4(int dtype, const void* q, int64_t q_st, int64_t q_sh,
+                           const void* k_pages, const void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,
+                           const int32_t* block_table, int64_t block_table_stride, int max_blocks,
+                           const int32_t* cu_seqlens, const int32_t* kv_lens,
+                           const int32_t* sel, int64_t sel_sr, int64_t sel_sh, int sel_rows, int sel_width,
+                           const int32_t* sel_off, int64_t off_sr, int64_t off_sh,
+                           void* o, int64_t o_st, int64_t o_sh,
+                           int N, int B, int Hq, int Hkv, int D, int page, float sm_scale,
+                           int num_splits, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * One new token per sequence over such pools: q and o [B, Hq, D].  sel with sel_off (both NULL: every page) as for sa_decode,
+ * [B, sel_rows] lists (sel_rows Hq or Hkv; strides of the batch may be 0) whose offsets are clamped to sel_width entries; a listed page that
+ * is past the table, outside the pool or past kv_lens[b] adds no key.  A sequence without keys gets zeros.  num_splits
+ * (1..64): the longest list that the sizes allow (sel_width pages, or max_blocks) is shared by that many workgroups, and
+ * every list by as many as its own length needs of the same share; more than 1 needs
+ * sa_decode_q4_workspace_bytes(B, Hq, D, num_splits) bytes, 16-byte aligned, which concurrent calls must not share.
+ */
+int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh,
+                 const void* k_pages, const void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,
+                 const int32_t* block_table, int64_t block_table_stride, int max_blocks, const int32_t* kv_lens,
+                 const int32_t* sel, int64_t sel_sb, int64_t sel_sr, int sel_width,
+                 const int32_t* sel_off, int64_t off_sb, int64_t off_sr, int sel_rows,
+                 void* o, int64_t o_sb, int64_t o_sh, int B, int Hq, int Hkv, int D, int page, float sm_scale,
+                 int num_splits, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sa_decode_q4_workspace_bytes(int B, int Hq, int D, int num_splits);
+
 #ifdef __cplusplus
 }
 #endif

@@ -217,6 +217,23 @@ SIGNATURES = {
         _vp, _i64, _i64, _vp, _i64, _i64,                 # k_out, v_out
         _i32, _i32, _i32, _i32, _i32, _vp,
     ]),
+    "sa_paged_chunk_attn_q4": (_i32, [
+        _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i32,    # q, pools
+        _vp, _i64, _i32, _vp, _vp,
+        _vp, _i64, _i64, _i32, _i32, _vp, _i64, _i64,         # sel, sel_off
+        _vp, _i64, _i64,
+        _i32, _i32, _i32, _i32, _i32, _i32, _f32,
+        _i32, _vp, _i64, _vp,
+    ]),
+    "sa_decode_q4": (_i32, [
+        _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i32,    # q, pools
+        _vp, _i64, _i32, _vp,
+        _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32,         # sel, sel_off
+        _vp, _i64, _i64,
+        _i32, _i32, _i32, _i32, _i32, _f32,
+        _i32, _vp, _i64, _vp,
+    ]),
+    "sa_decode_q4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
 }
 
 

@@ -1238,3 +1238,115 @@ def paged_read_q4(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: tor
           k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
           kv_lens.data_ptr(), k_out.data_ptr(), kst[0], kst[1], v_out.data_ptr(), vst[0], vst[1], rows, B, ps[1], head_dim, page)
     return k_out, v_out
+
+
+def paged_chunk_attn_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                        cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *, sel: torch.Tensor | None = None,
+                        sel_off: torch.Tensor | None = None, sm_scale: float | None = None, num_splits: int = 0,
+                        workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_chunk_attn` over a cache held in 4 bits; returns ``[N, Hq, D]``.
+
+    ``k_pages, v_pages [P, Hkv, q4_block_bytes(page, D)]`` uint8 as :func:`paged_append_q4` writes them for the type of ``q``;
+    everything else is as for :func:`paged_chunk_attn`.
+    """
+    name = "paged_chunk_attn_q4"
+    dt, dev, qs, ps, B = q.dtype, q.device, q.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    qst = q.stride()
+    page = _q4_page(ps[2], qs[2]) if len(ps) == 3 and len(qs) == 3 else 0
+    ok = (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and _q4_pools_ok(k_pages, v_pages, dev) and page > 0
+          and ps[1] > 0 and qs[1] % ps[1] == 0
+          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
+          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
+          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+          and (sel is None) == (sel_off is None))
+    if out is None:
+        out = _empty_like(q)
+    elif ok:
+        ok = out.shape == qs and out.dtype == dt and out.device == dev and out.stride(2) == 1
+    sargs = (None, 0, 0, 0, 0, None, 0, 0)
+    max_blocks = block_table.size(-1) if ok else 0
+    keys = max_blocks
+    if ok and sel is not None:
+        ss, sst = sel.shape, sel.stride()
+        ok = (sel.dtype == torch.int32 and sel_off.dtype == torch.int32 and sel.device == dev and sel_off.device == dev
+              and len(ss) == 3 and ss[0] >= qs[0] // CHUNK_BLOCK + B and ss[1] == ps[1]
+              and sel_off.shape == (ss[0], ss[1], 2) and (ss[2] <= 1 or sst[2] == 1) and sel_off.stride(2) == 1)
+        if ok:
+            sargs = (sel.data_ptr(), sst[0], sst[1], ss[0], ss[2], sel_off.data_ptr(), sel_off.stride(0), sel_off.stride(1))
+            keys = min(keys, ss[2])
+    if not ok:
+        _refuse_q4(name, q, dt, qs[-1] if len(qs) else 0, k_pages, v_pages, heads=dict(q=q, out=out),
+                   index=dict(block_table=block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens, sel=sel, sel_off=sel_off),
+                   other="q and out must be [N, Hq, D] with Hq a multiple of the pools' heads, sel and sel_off "
+                         f"(both or neither) [at least N // {CHUNK_BLOCK} + B rows, Hkv, width] and [rows, Hkv, 2]")
+    N, Hq, D = qs
+    ost = out.stride()
+    ws = _workspace(name, workspace, _lib.load().sa_paged_chunk_workspace_bytes(
+        N, B, Hq, ps[1], D, min(keys * page, 1 << 30), num_splits), dev)
+    _call("sa_paged_chunk_attn_q4", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_pages.data_ptr(),
+          v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0),
+          max_blocks, cu_seqlens.data_ptr(), kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], N, B, Hq, ps[1], D,
+          page, D ** -0.5 if sm_scale is None else sm_scale, num_splits, *_ws_bytes(ws))
+    return out
+
+
+def decode_q4_splits(B: int, rows: int, steps: int) -> int:
+    """Workgroups that share the longest list of a :func:`paged_sparse_decode_q4` call, ``steps`` steps of 32 keys, where it
+    has ``B * rows`` lists."""
+    return max(1, min(64, -(-1024 // max(1, B * rows)), steps // 8))
+
+
+def paged_sparse_decode_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                           kv_lens: torch.Tensor, sel: torch.Tensor | None = None, sel_off: torch.Tensor | None = None, *,
+                           num_splits: int = 0, workspace: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`paged_sparse_decode` over a cache held in 4 bits: one token per sequence, retained blocks or every block.
+
+    ``q [B, Hq, D]`` (or ``[B, Hq, 1, D]``); ``k_pages, v_pages [P, Hkv, q4_block_bytes(page, D)]`` uint8 as
+    :func:`paged_append_q4` writes them for the type of ``q``; ``block_table [B, max_blocks]``, ``kv_lens [B]``, ``sel
+    [B, R, max_sel]`` and ``sel_off [B, R, 2]`` (R = Hq or Hkv) int32 as for :func:`paged_sparse_decode`; without ``sel`` and
+    ``sel_off`` the whole cache is attended.  ``num_splits`` workgroups (at most 64) share the longest list that the sizes allow
+    and other lists as many as their lengths need of the same share; ``0`` picks the number from the sizes
+    (:func:`decode_q4_splits`).  More than one takes a byte workspace of ``sa_decode_q4_workspace_bytes`` (allocated if
+    omitted), which concurrent calls must not share.  A sequence without keys gets zeros.
+    """
+    name = "paged_sparse_decode_q4"
+    q3 = q.reshape(q.shape[0], q.shape[1], q.shape[-1]) if q.dim() == 4 else q
+    dt, dev, qs, ps = q3.dtype, q3.device, q3.shape, k_pages.shape
+    qst = q3.stride()
+    B = qs[0] if len(qs) == 3 else 0
+    page = _q4_page(ps[2], qs[2]) if len(ps) == 3 and len(qs) == 3 else 0
+    ok = (q3.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and _q4_pools_ok(k_pages, v_pages, dev) and page > 0
+          and ps[1] > 0 and qs[1] % ps[1] == 0 and block_table.dtype == torch.int32 and kv_lens.dtype == torch.int32
+          and block_table.device == dev and kv_lens.device == dev and block_table.dim() == 2 and block_table.size(0) == B
+          and (block_table.size(1) <= 1 or block_table.stride(1) == 1) and kv_lens.shape == (B,) and kv_lens.is_contiguous()
+          and (sel is None) == (sel_off is None))
+    if out is None:
+        out = _empty_like(q3)
+    elif ok:
+        ok = out.shape == qs and out.dtype == dt and out.device == dev and out.stride(2) == 1
+    sargs, R, width = (None, 0, 0, 0, None, 0, 0, 0), ps[1] if len(ps) == 3 else 1, block_table.size(-1) if ok else 0
+    if ok and sel is not None:
+        ss, sst = sel.shape, sel.stride()
+        ok = (sel.dtype == torch.int32 and sel_off.dtype == torch.int32 and sel.device == dev and sel_off.device == dev
+              and len(ss) == 3 and ss[0] == B and (ss[1] == qs[1] or ss[1] == ps[1]) and sel_off.shape == (B, ss[1], 2)
+              and (ss[2] <= 1 or sst[2] == 1) and sel_off.stride(2) == 1)
+        if ok:
+            R, width = ss[1], ss[2]
+            sargs = (sel.data_ptr(), sst[0], sst[1], width, sel_off.data_ptr(), sel_off.stride(0), sel_off.stride(1), R)
+    if not ok:
+        _refuse_q4(name, q3, dt, qs[-1] if len(qs) else 0, k_pages, v_pages, heads=dict(q=q3, out=out),
+                   index=dict(block_table=block_table, kv_lens=kv_lens, sel=sel, sel_off=sel_off, cu_seqlens=None),
+                   other="q and out must be [B, Hq, D] with Hq a multiple of the pools' heads, block_table [B, max_blocks], "
+                         "sel and sel_off (both or neither) [B, Hq or Hkv, width] and [B, Hq or Hkv, 2]")
+    Hq, D = qs[1], qs[2]
+    if num_splits == 0:
+        num_splits = decode_q4_splits(B, R, -(-width * page // 32))
+    ws = _workspace(name, workspace, _lib.load().sa_decode_q4_workspace_bytes(B, Hq, D, num_splits), dev)
+    ost = out.stride()
+    _call("sa_decode_q4", dev.index, _DTYPES[dt], q3.data_ptr(), qst[0], qst[1], k_pages.data_ptr(), v_pages.data_ptr(),
+          k_pages.stride(0), k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0), block_table.size(1),
+          kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], B, Hq, ps[1], D, page, D ** -0.5, num_splits,
+          *_ws_bytes(ws))
+    return out.reshape(q.shape) if q.dim() == 4 else out

@@ -1,9 +1,11 @@
 """The 4-bit form of a paged cache, byte by byte in float64 on the CPU, and ragged inputs held in it."""
 from __future__ import annotations
 
+import copy
+
 import torch
 
-from tests.chunk_reference import Ragged
+from tests.chunk_reference import Ragged, attention
 
 GROUP = 32
 
@@ -92,3 +94,44 @@ class Q4Ragged(Ragged):
             for p, t in (~self.held).nonzero().tolist():
                 pool[p, :, bytes_of[t]] = 0xFF
         self.k_pages, self.v_pages = (unpack(p, page, D, dtype, v) for p, v in ((self.k4, False), (self.v4, True)))
+
+
+def rounded(r: Q4Ragged) -> Q4Ragged:
+    """The same cache with its keys and values rounded to the element type, as kernels that multiply those take them."""
+    out = copy.copy(r)
+    out.k_pages, out.v_pages = (x.float().to(r.dtype).double() for x in (r.k_pages, r.v_pages))
+    return out
+
+
+def assert_attention(got, r: Q4Ragged, q, sel=None, sel_off=None, what="", scores=0.0):
+    """Rows of attention over a 4-bit cache against float64: over m + s c, or over that rounded to the element type.
+    ``scores``: the largest sum |q k| scale where that passes the 16 that attention()'s bound counts; a score is off by
+    D 2^-24 of it, a probability by twice that."""
+    got = got.double().cpu()
+    worst, ok = None, None
+    for form in (r, rounded(r)):
+        want, tol, live = attention(form, q, sel, sel_off)
+        tol = tol + q4_slack(r, q) + 2 * r.D * 2.0 ** -24 * scores * form.v_pages.nan_to_num(0.0).abs().max()
+        over = ((got - want).abs() - tol).nan_to_num(float("inf")).amax(-1)     # [N, Hq]
+        good = over <= 0
+        ok = good if ok is None else ok | good
+        worst = over if worst is None else torch.minimum(worst, over)
+    assert ok[live].all(), f"{what}: {int((~ok[live]).sum())} of {ok[live].numel()} rows, worst {worst[live].max():.3e} past the bound"
+    return live
+
+
+def q4_slack(r: Q4Ragged, q) -> float:
+    """What kernels that multiply codes and scale the sums add to attention()'s bound.  A probability times its scale is
+    rounded to bf16 once and meets |c - 7.5| <= 7.5: half a step of s 7.5, with s the largest.  A score is the fp32 sum of
+    s sum q c and m sum q over the groups: at most D 2^-24 of sum |q| (15 s + |m|) scale, twice that in a probability, of
+    values no larger than the largest."""
+    held = r.held[:, None, :, None].expand(-1, r.Hkv, -1, r.D // GROUP)
+    smax, mmax, vmax = 0.0, 0.0, 0.0
+    for pool in (r.k4, r.v4):
+        s, m = stats_of(pool, r.page, r.D, r.dtype)
+        if held.any():
+            smax, mmax = s[held].double().max().item(), m[held].double().abs().max().item()
+    if held.any():
+        vmax = r.v_pages[r.held[:, None, :, None].expand_as(r.v_pages)].abs().max().item()
+    qsum = q.double().abs().sum(-1).max().item() / r.D ** 0.5
+    return 7.5 * smax * 2.0 ** -9 + 2 * r.D * 2.0 ** -24 * qsum * (15 * smax + mmax) * vmax

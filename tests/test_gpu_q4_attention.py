@@ -1,0 +1,353 @@
+"""Attention over the 4-bit paged cache (``paged_chunk_attn_q4``, ``paged_sparse_decode_q4``) against float64 over what the cache
+holds: lengths, pages, groups and lists where it can go wrong.  Slots without a token hold NaN scales."""
+import pytest
+import torch
+
+from sparseattentioninfer_amd import ops
+from tests.chunk_reference import randn
+from tests.q4_reference import Q4Ragged, assert_attention, pack, unpack
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _say(*msg):
+    print("[q4-attention]", *msg, flush=True)
+
+
+def _cache(r):
+    return r.gpu("k4", "v4", "table")
+
+
+def _chunk(q_lens, kv_lens, page, Hq, Hkv, D, dtype, *, pad=0, seed=1, splits=0, offset=0.0, lists=None):
+    r = Q4Ragged(q_lens, kv_lens, page=page, Hkv=Hkv, D=D, dtype=dtype, seed=seed, pad_rows=pad, offset=offset)
+    q = randn(r.N, Hq, D, seed=seed + 7, dtype=dtype)
+    out = torch.full((r.N, Hq, D), 7.0, dtype=dtype, device="cuda")
+    sel = off = None
+    if lists:
+        sel, off = lists(r)
+    g = lambda t: None if t is None else t.cuda()
+    got = ops.paged_chunk_attn_q4(q.cuda(), *_cache(r), *r.gpu("cu", "kv_lens"), sel=g(sel), sel_off=g(off), num_splits=splits,
+                                  out=out)
+    assert got is out
+    live = assert_attention(out, r, q, sel, off, f"{q_lens} {kv_lens}")
+    assert (out[~live.cuda()] == 7.0).all()
+    return r, q, out
+
+
+def _random_lists(r, width, seed=3):
+    """Lists of up to `width` pages for each block of 64 queries and head, some empty, offsets inside the row."""
+    g = torch.Generator().manual_seed(seed)
+    rows = r.N // 64 + len(r.q_lens)
+    sel = torch.zeros(rows, r.Hkv, width, dtype=torch.int32)
+    off = torch.zeros(rows, r.Hkv, 2, dtype=torch.int32)
+    at = 0
+    for b, _, t, n in r.rows():
+        for i in range(-(-t // 64)):
+            last = n - t + min(t, 64 * (i + 1)) - 1
+            for h in range(r.Hkv):
+                pages = torch.randperm(max(0, last // r.page + 1), generator=g)[:int(torch.randint(0, width, (1,), generator=g))]
+                e0 = int(torch.randint(0, width - pages.numel() + 1, (1,), generator=g))
+                sel[at, h, e0:e0 + pages.numel()] = pages.sort().values.to(torch.int32)
+                off[at, h] = torch.tensor([e0, e0 + pages.numel()])
+            at += 1
+    return sel, off
+
+
+# ---- chunks ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 80, 128])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF), (128, HF), (64, BF)])
+def test_chunk_ragged(page, D, dtype):
+    _say("chunk", page, D, dtype)
+    _chunk([70, 0, 1, 33, 16, 5, 3], [130, 40, 90, 33, 16, 431, 3], page, 8, 2, D, dtype, pad=5)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (6, 2), (7, 1), (8, 1), (14, 2), (16, 1), (40, 8), (33, 1)])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+def test_chunk_groups(Hq, Hkv, D, dtype):
+    _say("chunk groups", Hq, Hkv, D)
+    _chunk([1, 2, 9, 66], [200, 65, 100, 150], 32, Hq, Hkv, D, dtype, seed=Hq)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5, 64])
+def test_chunk_splits(splits):
+    _say("chunk splits", splits)
+    for D, dtype in ((128, BF), (64, HF)):
+        _chunk([1, 3, 80, 1], [2000, 700, 1500, 1], 64, 8, 2, D, dtype, splits=splits)
+
+
+def test_chunk_planned_division():
+    """Long keys and few rows, so that the launch divides the keys by itself."""
+    _say("chunk planned")
+    _chunk([1, 4], [5000, 3001], 64, 8, 2, 128, BF)
+    _chunk([100], [3000], 16, 4, 1, 64, HF)
+
+
+def test_chunk_offset_values():
+    """Groups whose range is small against their values."""
+    _say("chunk offset")
+    _chunk([1, 40, 90], [300, 400, 90], 64, 8, 2, 128, BF, offset=6.0)
+    _chunk([1, 40, 90], [300, 400, 90], 64, 8, 2, 64, HF, offset=6.0)
+
+
+@pytest.mark.parametrize("page,width", [(16, 9), (64, 5), (48, 4)])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+def test_chunk_selected(page, width, D, dtype):
+    _say("chunk selected", page, width, D)
+    _chunk([130, 1, 0, 64, 7], [330, 200, 9, 64, 300], page, 8, 2, D, dtype, pad=3, lists=lambda r: _random_lists(r, width))
+
+
+def test_chunk_of_nothing():
+    _say("chunk of nothing")
+    r = Q4Ragged([0, 0], [5, 0], page=16, Hkv=1, D=64, dtype=HF)
+    q = torch.zeros(0, 2, 64, dtype=HF, device="cuda")
+    assert ops.paged_chunk_attn_q4(q, *_cache(r), *r.gpu("cu", "kv_lens")).shape == (0, 2, 64)
+    # rows of a sequence without a key, tables without columns, pools without pages: zeros
+    q = randn(3, 2, 64, seed=1, dtype=HF).cuda()
+    one = lambda *n: torch.tensor(n, dtype=torch.int32, device="cuda")
+    out = ops.paged_chunk_attn_q4(q, *_cache(r)[:2], torch.zeros(2, 0, dtype=torch.int32, device="cuda"), one(0, 2, 3), one(2, 1))
+    assert not out.any()
+    none = torch.zeros(0, 1, ops.q4_block_bytes(16, 64), dtype=torch.uint8, device="cuda")
+    assert not ops.paged_chunk_attn_q4(q, none, none, one(0, 0)[:, None], one(0, 2, 3), one(2, 1)).any()
+    assert not ops.paged_chunk_attn_q4(q, *_cache(r)[:2], one(-1, 99)[:, None], one(0, 2, 3), one(2, 1)).any()
+    assert not ops.paged_chunk_attn_q4(q, *_cache(r)[:2], one(0, 0)[:, None], one(0, 2, 3), one(0, 0)).any()
+
+
+def test_chunk_strided_and_scaled():
+    """Queries inside a projection row, pools with gaps between pages, an output inside a wider tensor, another scale."""
+    _say("chunk strided")
+    r = Q4Ragged([3, 70], [90, 200], page=32, Hkv=2, D=128, seed=5)
+    row = randn(r.N, 12 * 128, seed=6)
+    q = row.unflatten(1, (12, 128))[:, 2:10]
+    wide = torch.full((r.N, 8, 256), 7.0, dtype=BF, device="cuda")
+    pools = [torch.zeros(p.size(0), 3, p.size(1), p.size(2), dtype=torch.uint8, device="cuda") for p in (r.k4, r.v4)]
+    for p, src in zip(pools, (r.k4, r.v4)):
+        p[:, 1] = src.cuda()
+    ops.paged_chunk_attn_q4((row.cuda().unflatten(1, (12, 128)) * 2)[:, 2:10], pools[0][:, 1], pools[1][:, 1],
+                            *r.gpu("table", "cu", "kv_lens"), sm_scale=0.5 * 128 ** -0.5, out=wide[:, :, 128:])
+    assert_attention(wide[:, :, 128:], r, q, what="strided")
+    assert (wide[:, :, :128] == 7.0).all()
+
+
+# ---- single tokens -----------------------------------------------------------------------------
+
+def _decode(kv_lens, page, Hq, Hkv, D, dtype, *, rows=None, width=0, splits=0, seed=1, offset=0.0, shared=False):
+    """rows: Hq or Hkv lists of each sequence, up to `width` pages long (the last page among them, empty for some)."""
+    B = len(kv_lens)
+    r = Q4Ragged([1] * B, kv_lens, page=page, Hkv=Hkv, D=D, dtype=dtype, seed=seed, offset=offset)
+    q = randn(B, Hq, D, seed=seed + 9, dtype=dtype)
+    sel = off = None
+    args, keep = (), None
+    if rows:
+        g = torch.Generator().manual_seed(seed)
+        sel = torch.zeros(B, rows, width, dtype=torch.int32)
+        off = torch.zeros(B, rows, 2, dtype=torch.int32)
+        for b, n in enumerate(kv_lens):
+            for h in range(rows):
+                pages = torch.randperm(-(-n // page), generator=g)[:int(torch.randint(0, width + 1, (1,), generator=g))].sort().values
+                sel[b, h, :pages.numel()] = pages.to(torch.int32)
+                off[b, h, 1] = pages.numel()
+        args = (sel.cuda(), off.cuda())
+        if shared:
+            sel, off = sel[:1].expand(B, -1, -1), off[:1].expand(B, -1, -1)
+            args = (args[0][:1].expand(B, -1, -1), args[1][:1].expand(B, -1, -1))
+    out = ops.paged_sparse_decode_q4(q.cuda(), *_cache(r), r.kv_lens.cuda(), *args, num_splits=splits)
+    G = Hq // Hkv
+    if rows == Hq and G > 1:      # a list per query head: each head by itself over its KV head
+        for h in range(Hq):
+            one = Q4Ragged.__new__(Q4Ragged)
+            one.__dict__ = dict(r.__dict__, Hkv=1)
+            for x in ("k_pages", "v_pages", "k4", "v4"):
+                setattr(one, x, getattr(r, x)[:, h // G:h // G + 1])
+            assert_attention(out[:, h:h + 1], one, q[:, h:h + 1], sel[:, h:h + 1], off[:, h:h + 1], f"head {h}")
+    else:
+        assert_attention(out, r, q, sel, off, f"{kv_lens}")
+    return r, q, args, out
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 80, 128])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF), (128, HF), (64, BF)])
+def test_decode_whole(page, D, dtype):
+    _say("decode", page, D, dtype)
+    _decode([1, 0, 15, 16, 17, 130, 700, 33], page, 8, 2, D, dtype)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (6, 2), (7, 1), (8, 1), (14, 2), (16, 1), (40, 8), (33, 1), (9, 3)])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+def test_decode_groups(Hq, Hkv, D, dtype):
+    _say("decode groups", Hq, Hkv, D)
+    _decode([300, 65, 1], 32, Hq, Hkv, D, dtype, seed=Hq)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 2, 5, 64])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+def test_decode_splits(splits, D, dtype):
+    _say("decode splits", splits, D)
+    _decode([5000, 700, 1, 0, 2048], 64, 8, 2, D, dtype, splits=splits)
+
+
+@pytest.mark.parametrize("rows", [2, 8])
+@pytest.mark.parametrize("splits", [0, 3])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+def test_decode_lists(rows, splits, D, dtype):
+    _say("decode lists", rows, splits, D)
+    _decode([500, 333, 64, 1, 0, 900], 32, 8, 2, D, dtype, rows=rows, width=9, splits=splits)
+
+
+def test_decode_shared_lists():
+    _say("decode shared lists")
+    _decode([333, 500, 500], 32, 8, 2, 128, BF, rows=2, width=9, shared=True)
+
+
+@pytest.mark.parametrize("offset", [6.0, -40.0])
+def test_decode_offset_values(offset):
+    _say("decode offset", offset)
+    _decode([300, 100], 64, 8, 2, 128, BF, offset=offset)
+    _decode([300, 100], 64, 8, 2, 64, HF, offset=offset)
+
+
+@pytest.mark.parametrize("scale", [1e-4, 30.0])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_scaled_values(scale, dtype):
+    """Values far from 1: the scales of the groups with them."""
+    _say("decode scaled", scale, dtype)
+    r = Q4Ragged([1, 1], [300, 77], page=64, Hkv=2, D=128, dtype=dtype, seed=4)
+    r.v4 = pack((randn(*r.v_pages.shape, seed=8, dtype=dtype).float() * scale).to(dtype), True)
+    r.v_pages = unpack(r.v4, 64, 128, dtype, True)
+    q = randn(2, 8, 128, seed=9, dtype=dtype)
+    out = ops.paged_sparse_decode_q4(q.cuda(), *_cache(r), r.kv_lens.cuda())
+    assert_attention(out, r, q, what=f"scale {scale}")
+
+
+def test_decode_large_scores():
+    """Scores far apart and rising along the keys, so that the reference of a row is raised again and again."""
+    _say("decode large scores")
+    for D, dtype in ((128, BF), (64, HF)):
+        r = Q4Ragged([1], [600], page=16, Hkv=1, D=D, dtype=dtype, seed=2)
+        ramp = torch.zeros(r.k_pages.shape)
+        order = r.table[0, :38].long()
+        for lb in range(38):
+            ramp[order[lb]] = (torch.arange(16) + 16 * lb)[None, :, None] / 60.0
+        r.k4 = pack((ramp + 0.3 * randn(*ramp.shape, seed=3).float()).to(dtype), False)
+        r.k_pages = unpack(r.k4, 16, D, dtype, False)
+        q = (randn(1, 4, D, seed=4, dtype=dtype).float().abs() * 1.2).to(dtype)
+        out = ops.paged_sparse_decode_q4(q.cuda(), *_cache(r), r.kv_lens.cuda())
+        # |k| <= 10.1 + 0.3 * 5 and sum |q| <= D * 1.2 * 4.5
+        assert_attention(out, r, q, what=f"D {D}", scores=11.6 * q.double().abs().sum(-1).max().item() / D ** 0.5)
+
+
+def test_decode_missing_pages():
+    """Ids outside the pool, columns past the table, listed pages past the sequence: no keys from them."""
+    _say("decode missing pages")
+    r = Q4Ragged([1, 1], [100, 100], page=32, Hkv=1, D=128, seed=3, extra_cols=0)
+    q = randn(2, 4, 128, seed=4)
+    sel = torch.tensor([[[0, 1, 3, 9, 0]], [[2, -5, 1 << 29, 0, 0]]], dtype=torch.int32)
+    off = torch.tensor([[[0, 4]], [[0, 3]]], dtype=torch.int32)
+    bad = r.table.clone()
+    bad[0, 1] = 77
+    out = ops.paged_sparse_decode_q4(q.cuda(), *r.gpu("k4", "v4"), bad.cuda(), r.kv_lens.cuda(), sel.cuda(), off.cuda())
+    seen, noff = torch.tensor([[[0, 3]], [[2, 0]]], dtype=torch.int32), torch.tensor([[[0, 2]], [[0, 1]]], dtype=torch.int32)
+    assert_attention(out, r, q, seen, noff, "missing")
+    # offsets outside the row are clamped to it
+    off[0, 0] = torch.tensor([-3, 2])
+    out = ops.paged_sparse_decode_q4(q.cuda(), *_cache(r), r.kv_lens.cuda(), sel.cuda(), off.cuda())
+    noff[0, 0] = torch.tensor([0, 2])
+    seen[0, 0] = torch.tensor([0, 1])
+    assert_attention(out, r, q, seen, noff, "clamped")
+
+
+def test_decode_nothing():
+    _say("decode nothing")
+    r = Q4Ragged([0, 0], [5, 0], page=16, Hkv=1, D=64, dtype=HF)
+    one = lambda *n: torch.tensor(n, dtype=torch.int32, device="cuda")
+    q = randn(2, 2, 64, seed=1, dtype=HF).cuda()
+    none = torch.zeros(0, 1, ops.q4_block_bytes(16, 64), dtype=torch.uint8, device="cuda")
+    assert not ops.paged_sparse_decode_q4(q, none, none, one(0, 0)[:, None], one(5, 5)).any()
+    assert not ops.paged_sparse_decode_q4(q, *_cache(r)[:2], torch.zeros(2, 0, dtype=torch.int32, device="cuda"), one(5, 5)).any()
+    empty = torch.zeros(2, 1, 0, dtype=torch.int32, device="cuda")
+    assert not ops.paged_sparse_decode_q4(q, *_cache(r)[:2], one(0, 0)[:, None], one(5, 5), empty,
+                                          torch.zeros(2, 1, 2, dtype=torch.int32, device="cuda")).any()
+    q0 = torch.zeros(0, 2, 64, dtype=HF, device="cuda")
+    assert ops.paged_sparse_decode_q4(q0, *_cache(r)[:2], torch.zeros(0, 3, dtype=torch.int32, device="cuda"), one(0)[:0]).shape == q0.shape
+
+
+def test_nan_tokens_reach_their_rows_only():
+    """A token whose group is NaN makes NaN of the rows that see it, whatever else shares its tile or workgroup."""
+    _say("nan tokens")
+    r = Q4Ragged([1, 1], [200, 200], page=32, Hkv=2, D=128, seed=3)
+    q = randn(2, 8, 128, seed=4).cuda()
+    want = ops.paged_sparse_decode_q4(q, *_cache(r), r.kv_lens.cuda())
+    pg = r.table[1, 2].item()
+    k4 = r.k4.clone()
+    k4[pg, 1, 32 * 64 + 4 * 5:32 * 64 + 4 * 5 + 4] = 0xFF               # group 0 of token 64 + 5, KV head 1
+    got = ops.paged_sparse_decode_q4(q, k4.cuda(), r.v4.cuda(), r.table.cuda(), r.kv_lens.cuda())
+    assert got[1, 4:].isnan().all()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, :4], want[1, :4])
+
+
+# ---- streams, graphs, workspaces ---------------------------------------------------------------
+
+def test_other_stream_and_workspaces():
+    _say("stream, workspace")
+    r = Q4Ragged([1, 1], [3000, 500], page=64, Hkv=2, D=128, seed=6)
+    q = randn(2, 8, 128, seed=7)
+    args = (q.cuda(), *_cache(r), r.kv_lens.cuda())
+    want = ops.paged_sparse_decode_q4(*args, num_splits=7)
+    ws = torch.full((int(2 * 8 * 130 * 4 * 7),), 255, dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.paged_sparse_decode_q4(*args, num_splits=7, workspace=ws)
+    s.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(AssertionError, match="workspace"):
+        ops.paged_sparse_decode_q4(*args, num_splits=7, workspace=ws[:-4])
+
+
+def test_graph_of_append_attention_and_read():
+    """One captured step on a 4-bit cache, append, attention, decode over lists, read back, replayed with other lengths and
+    inputs, with eager work between the replays; every replay equals the eager calls on a cache of its own."""
+    _say("graph")
+    B, Hq, Hkv, D, page = 3, 8, 2, 128, 32
+    dev = "cuda"
+    table = torch.arange(B * 40, dtype=torch.int32, device=dev).view(B, 40)
+    pools = [[torch.zeros(B * 40, Hkv, ops.q4_block_bytes(page, D), dtype=torch.uint8, device=dev) for _ in "kv"] for _ in range(2)]
+    bounds = [torch.zeros(B * 40, Hkv, 2, D, dtype=BF, device=dev) for _ in range(2)]
+    cu = torch.arange(B + 1, dtype=torch.int32, device=dev)
+    lens = torch.zeros(B, dtype=torch.int32, device=dev)
+    row = torch.zeros(B, (Hq + 2 * Hkv) * D, dtype=BF, device=dev)
+    inv = (1.0 / 1e6 ** (torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(dev)
+
+    def step(i):
+        q, k, v = (x.unflatten(1, (-1, D)) for x in row.split([Hq * D, Hkv * D, Hkv * D], dim=1))
+        cache = (*pools[i], table)
+        q = ops.paged_append_q4(k, v, *cache, cu, lens, inv_freq=inv, q=q, k_bounds=bounds[i])
+        sel, off = ops.paged_block_select(q, bounds[i], table, lens, page=page, top_k=3)
+        return (ops.paged_chunk_attn_q4(q, *cache, cu, lens), ops.paged_sparse_decode_q4(q, *cache, lens),
+                ops.paged_sparse_decode_q4(q, *cache, lens, sel, off), *ops.paged_read_q4(*cache, cu, lens, rows=B, head_dim=D, dtype=BF))
+
+    # a cache of some tokens, the same in both
+    first = randn(B * 1000, Hkv, D, seed=3).to(dev)
+    for i in range(2):
+        ops.paged_append_q4(first, first, *pools[i], table, 1000 * cu, torch.full((B,), 1000, dtype=torch.int32, device=dev),
+                            k_bounds=bounds[i])
+    lens.fill_(1000)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(0)
+    step(1)                                     # it has written a token
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(0)
+    for n in range(5):
+        lens.copy_(torch.tensor([1001 + n, 1001 + 2 * n, 1001], dtype=torch.int32))
+        row.copy_(randn(*row.shape, seed=20 + n))
+        graph.replay()
+        want = step(1)
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b), n
+    assert all(torch.equal(a, b) for a, b in zip(pools[0], pools[1])) and torch.equal(*bounds)

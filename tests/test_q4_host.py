@@ -93,3 +93,64 @@ def test_read_refusals(lib, change, code, text):
 
 def test_read_nothing_to_do(lib):
     assert _read(lib, N=0, ko=None) == 0 and _read(lib, B=0) == 0
+
+
+def _chunk(lib, **o):
+    a = dict(dtype=0, kp=FAKE, sp=10240, pages=8, table=FAKE, mb=4, sel=None, rows=0, width=0, off=None, N=4, Hq=8, D=128, page=64,
+             scale=0.1, splits=1, ws=None, q=FAKE)
+    a.update(o)
+    return lib.sa_paged_chunk_attn_q4(a["dtype"], a["q"], 1024, 128, a["kp"], a["kp"], a["sp"], 5120, a["pages"], a["table"],
+                                      4, a["mb"], FAKE, FAKE, a["sel"], 8, 4, a["rows"], a["width"], a["off"], 8, 4, FAKE,
+                                      1024, 128, a["N"], 2, a["Hq"], 2, a["D"], a["page"], a["scale"], a["splits"], a["ws"], 0,
+                                      None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=7), -1, b"dtype 7"), (dict(D=80), -3, b"head dim 80"), (dict(page=20), -4, b"page 20"),
+    (dict(Hq=9), -2, b"Hq=9"), (dict(mb=5), -2, b"5 columns"), (dict(splits=65), -2, b"65 splits"), (dict(scale=0.0), -2, b"scale"),
+    (dict(q=None), -6, b"NULL"), (dict(kp=None), -6, b"NULL"), (dict(table=None), -6, b"NULL"),
+    (dict(off=FAKE, rows=2, width=4), -6, b"NULL"), (dict(off=FAKE, rows=1, width=0), -2, b"selection"),
+    (dict(sel=FAKE, rows=2, width=4), -2, b"selection"), (dict(kp=FAKE + 8), -8, b"aligned"), (dict(sp=10241), -8, b"aligned"),
+    (dict(q=FAKE + 2), -8, b"aligned"), (dict(splits=2), -7, b"workspace")])
+def test_chunk_refusals(lib, change, code, text):
+    assert _chunk(lib, **change) == code and b"sa_paged_chunk_attn_q4" in lib.sa_last_error() and text in lib.sa_last_error()
+
+
+def test_chunk_nothing_to_do(lib):
+    assert _chunk(lib, N=0, q=None) == 0
+
+
+def _decode(lib, **o):
+    a = dict(dtype=0, kp=FAKE, sp=10240, pages=8, table=FAKE, mb=4, sel=None, rows=0, width=0, off=None, B=4, Hq=8, D=128, page=64,
+             scale=0.1, splits=1, ws=None, q=FAKE, lens=FAKE)
+    a.update(o)
+    return lib.sa_decode_q4(a["dtype"], a["q"], 1024, 128, a["kp"], a["kp"], a["sp"], 5120, a["pages"], a["table"], 4, a["mb"],
+                            a["lens"], a["sel"], 8, 4, a["width"], a["off"], 8, 4, a["rows"], FAKE, 1024, 128, a["B"], a["Hq"],
+                            2, a["D"], a["page"], a["scale"], a["splits"], a["ws"], 0, None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=7), -1, b"dtype 7"), (dict(D=32), -3, b"head dim 32"), (dict(page=136), -4, b"page 136"),
+    (dict(Hq=9), -2, b"Hq=9"), (dict(mb=5), -2, b"5 columns"), (dict(splits=65), -2, b"65 splits"), (dict(splits=0), -2, b"0 splits"),
+    (dict(scale=-1.0), -2, b"scale"), (dict(off=FAKE, sel=FAKE, rows=3, width=4), -5, b"sel_rows=3"),
+    (dict(sel=FAKE), -2, b"selection"), (dict(off=FAKE, sel=FAKE, rows=2, width=-1), -2, b"selection"),
+    (dict(off=FAKE, rows=2, width=4), -6, b"NULL"), (dict(lens=None), -6, b"NULL"), (dict(kp=None), -6, b"NULL"),
+    (dict(kp=FAKE + 4), -8, b"aligned"), (dict(sp=8), -8, b"aligned"), (dict(splits=4), -7, b"workspace")])
+def test_decode_refusals(lib, change, code, text):
+    assert _decode(lib, **change) == code and b"sa_decode_q4" in lib.sa_last_error() and text in lib.sa_last_error()
+
+
+def test_decode_nothing_to_do(lib):
+    assert _decode(lib, B=0, q=None) == 0
+    assert lib.sa_decode_q4_workspace_bytes(2, 4, 128, 3) == 3 * 2 * 4 * 130 * 4
+    assert lib.sa_decode_q4_workspace_bytes(2, 4, 128, 1) == 0
+
+
+def test_attention_refuses_cpu_tensors():
+    pool = torch.zeros(2, 1, 5120, dtype=torch.uint8)
+    i = lambda *n: torch.tensor(n, dtype=torch.int32)
+    x = torch.zeros(1, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="on the GPU"):
+        ops.paged_chunk_attn_q4(x, pool, pool, i(0)[None], i(0, 1), i(1))
+    with pytest.raises(AssertionError, match="on the GPU"):
+        ops.paged_sparse_decode_q4(x, pool, pool, i(0)[None], i(1))
