@@ -87,7 +87,8 @@ struct Q4Window {
   }
 };
 
-// Row references are raised when a lane's probabilities of a step sum past this: no probability then exceeds 2^16 in
+// What a wave's 32-key steps leave: fp32 accumulators of rows of queries against row references (base 2), and the sums of
+// their probabilities.  Row references are raised when a lane's probabilities of a step sum past this: no probability then exceeds 2^16 in
 // bf16 (2^15 in fp16, whose largest is 65,504).
 template <bool BF16>
 constexpr float Q4_REFIT = BF16 ? 65536.f : 32768.f;
@@ -248,29 +249,258 @@ struct Q4Dequant {
       }
     }
   }
+};
 
-  // All steps of the wave; the loads of the next are in flight during one.
-  __device__ __forceinline__ void run(const Q4Keys& ks, float scale) {
-    const int ns = ks.steps();
-    if (ns == 0) return;
-    Q4Window w;
-    w.fill(ks, 0);
-    Chunk a[2], b[2];
-    auto fetch = [&](Chunk (&ch)[2], int s) {
-      if (s - w.base >= 32) w.fill(ks, s);
-      load(ch[0], ks, w, s, 0);
-      load(ch[1], ks, w, s, 1);
+// Few rows, codes multiplied as they are: with the groups g of the dims and c the codes,
+//   q . k_t = sum_g s[t,g] (sum_{d in g} q_d c[t,d]) + m[t,g] sum_{d in g} q_d
+//   o_d     = sum_t (p_t s[t,g]) c[t,d] + sum_t p_t m[t,g]              (d in g)
+// so neither keys nor values are scaled one by one, and q c is exact.  The columns of the products are (group, row) pairs:
+// the operand of column (g, r) is row r of the queries in group g and 0 in the others, so that one accumulator holds the
+// partial scores of all groups, each lane needs the pairs of one group only, and a rotation over 16 lanes adds them up.  In
+// the second product column (g, r) is p s[., g], of use in the dims of g.
+// What rounds: p s, once, to bf16.  Codes lie in 0 .. 15, so that would weigh with up to 15 s where half of it is the
+// values' own; sum_t (p s) 7.5, of the rounded products (a row of ones more in the matrix product), is taken out
+// and put back from the unrounded ones.  For fp16 the product is split in two bf16 parts instead, 16 bits in all.
+template <bool BF16, int D, int NQ>
+struct Q4Fold {
+  using E = Elem<BF16>;
+  using F = Kv4<D>;
+  static constexpr int NG = F::NG, NE = D / 16;
+  static constexpr int RPS = 16 / NG;              // rows of a column set
+  static constexpr int ROWS = RPS * NQ;
+  static constexpr float REFIT = 65536.f;
+
+  struct Chunk {
+    Words<NG> k, v;
+    u32x4 ks, vs;                                  // pairs of the lane's group, keys 4 q .. + 3
+    int key;
+  };
+
+  u32x4 qz[NQ][NG];
+  float qsum[NQ];                                  // of the lane's group and row
+  int pos[NQ];                                     // position of the lane's row
+  int pos_min;                                     // of all rows
+  f32x4 O[NQ][NE], ones[NQ];
+  float base[NQ];                                  // sum p m (+ 7.5 p s in bf16) of the lane's keys
+  float m_ref[NQ], l_run[NQ];
+  bool ref_ok;
+
+  static __device__ __forceinline__ int group_of(int lane) { return (lane & 15) / RPS; }
+  static __device__ __forceinline__ int row_of(int lane) { return (lane & 15) % RPS; }
+
+  static __device__ __forceinline__ void load(Chunk& c, const Q4Keys& ks, const Q4Window& w, int step, int h) {
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int slot = w.slot_of(step, h);
+    const int64_t off = w.off_of(step, h);
+    c.key = w.key_of(step, h);
+    const uint8_t *kb = ks.k + off, *vb = ks.v + off;
+    c.k.load(kb + slot * F::ROW + (i * F::ROW + 4 * NG * q));
+    c.v.load(vb + slot * F::ROW + (q * F::QUAD + 4 * NG * i));
+    const int st = F::stats_at(ks.page) + 4 * slot, of_lane = 4 * group_of(lane) * ks.page + 16 * q;
+    c.ks = *reinterpret_cast<const u32x4*>(kb + st + of_lane);
+    c.vs = *reinterpret_cast<const u32x4*>(vb + st + of_lane);
+  }
+
+  // The lane's row of set x: its query from element 0 on, and its position.
+  __device__ __forceinline__ void set_query(int x, const elem_t* row, int position) {
+    const int lane = threadIdx.x & 63, g = group_of(lane);
+    const u32x4 v = *reinterpret_cast<const u32x4*>(row + 32 * g + 8 * (lane >> 4));
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += E::to_f32((elem_t)(v[e] & 0xffffu)) + E::to_f32((elem_t)(v[e] >> 16));
+    qsum[x] = quarters_sum(sum);
+    pos[x] = position;
+#pragma unroll
+    for (int y = 0; y < NG; ++y) qz[x][y] = y == g ? v : u32x4{0u, 0u, 0u, 0u};
+  }
+
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+#pragma unroll
+      for (int e = 0; e < NE; ++e) O[x][e] = f32x4{};
+      ones[x] = f32x4{};
+      base[x] = l_run[x] = 0.f;
+      m_ref[x] = -__builtin_inff();
+    }
+    ref_ok = false;
+  }
+
+  __device__ __forceinline__ void raise(const f32x4 (&S)[NQ][2], float scale) {
+    ref_ok = true;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      float mx = S[x][0][0];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, S[x][h][j]);
+      // The lanes of a row's groups have its scores from sums in different orders: one reference for all of them.
+      mx = over_groups<MAX>(mx);
+      const float m_new = fmaxf(m_ref[x], quarters_max(mx) * scale);   // -inf stays -inf (scale > 0)
+      const float alpha = m_ref[x] == -__builtin_inff() ? 1.f : fast_exp2(m_ref[x] - m_new);
+      l_run[x] *= alpha;
+      base[x] *= alpha;
+      ones[x] *= alpha;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) O[x][e] *= alpha;
+      m_ref[x] = m_new;
+      ref_ok = ref_ok && !__any(m_new == -__builtin_inff());
+    }
+  }
+
+  // Sum or maximum over the lanes of a row's groups, in every one.
+  template <int OP>
+  static __device__ __forceinline__ float over_groups(float x) {
+    auto op = [](float a, float b) { return OP == MAX ? fmaxf(a, b) : a + b; };
+    if constexpr (NG == 4) x = op(x, dpp<0x124>(x));   // row_ror:4
+    return op(x, dpp<0x128>(x));                       // row_ror:8
+  }
+
+  __device__ __forceinline__ void step(const Chunk (&ch)[2], int end, float scale) {
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    f32x4 S[NQ][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) S[x][h] = f32x4{};
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t lo = q4_low(ch[h].k.w[g]), hi = q4_high(ch[h].k.w[g]);
+        const u32x4 kf = BF16 ? u32x4{q4_pair_bf16<false>(lo), q4_pair_bf16<true>(lo), q4_pair_bf16<false>(hi), q4_pair_bf16<true>(hi)}
+                              : u32x4{q4_pair_f16<false>(lo), q4_pair_f16<true>(lo), q4_pair_f16<false>(hi), q4_pair_f16<true>(hi)};
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) S[x][h] = E::mfma16(kf, qz[x][g], S[x][h]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = q4_scale<BF16>(ch[h].ks[j]), m = q4_min<BF16>(ch[h].ks[j]);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) S[x][h][j] = over_groups<SUM>(fmaf(s, S[x][h][j], m * qsum[x]));
+      }
+      if (ch[h].key + 15 > pos_min) {              // keys past a row's position
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          const int lim = pos[x] - ch[h].key - 4 * q;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) S[x][h][j] = j > lim ? -__builtin_inff() : S[x][h][j];
+        }
+      }
+    }
+    float p[NQ][8];
+    auto probs = [&](int x) {
+      const float neg = m_ref[x] == -__builtin_inff() ? 0.f : -m_ref[x];
+      float ls = 0.f;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        p[x][y] = fast_exp2(fmaf(S[x][y >> 2][y & 3], scale, neg));
+        ls += p[x][y];
+      }
+      return ls;
     };
-    fetch(a, 0);
-#pragma unroll 1
-    for (int s = 0; s < ns; s += 2) {
-      if (s + 1 < ns) fetch(b, s + 1);
-      step(a, ks.end, scale);
-      if (s + 1 >= ns) break;
-      if (s + 2 < ns) fetch(a, s + 2);
-      step(b, ks.end, scale);
+    if (!ref_ok) raise(S, scale);
+    float ls[NQ];
+    bool over = false;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      ls[x] = probs(x);
+      over = over || !(ls[x] <= REFIT);
+    }
+    if (__any(over)) {
+      raise(S, scale);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) ls[x] = probs(x);
+    }
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) l_run[x] += ls[x];
+    // p s of the lane's group in the order of the operand, and p m.
+    u32x4 P[NQ], R[NQ];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 vs = ch[h].vs;
+      if (ch[h].key + 16 > end) {                  // 0 times what a slot without a token holds is 0
+        const int live = end - ch[h].key - 4 * q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vs[j] = j < live ? vs[j] : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const float s0 = q4_scale<BF16>(vs[j]), s1 = q4_scale<BF16>(vs[j + 1]);
+        const float m0 = q4_min<BF16>(vs[j]), m1 = q4_min<BF16>(vs[j + 1]);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          const float p0 = p[x][4 * h + j], p1 = p[x][4 * h + j + 1];
+          const float y0 = p0 * s0, y1 = p1 * s1;
+          base[x] = fmaf(p0, m0, fmaf(p1, m1, base[x]));
+          const uint32_t w = Elem<true>::pack2f(y0, y1);
+          P[x][2 * h + (j >> 1)] = w;
+          if constexpr (BF16)
+            base[x] = fmaf(y0, 7.5f, fmaf(y1, 7.5f, base[x]));
+          else
+            R[x][2 * h + (j >> 1)] = Elem<true>::pack2f(y0 - __uint_as_float(w << 16), y1 - __uint_as_float(w & 0xffff0000u));
+        }
+      }
+    }
+    constexpr uint32_t ONE2 = 0x3f803f80u;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x)
+      if constexpr (BF16) ones[x] = Elem<true>::mfma16(u32x4{ONE2, ONE2, ONE2, ONE2}, P[x], ones[x]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {       // dims 32 g + 16 half + 0..15
+        u32x4 vf;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t c = half ? q4_high(ch[h].v.w[g]) : q4_low(ch[h].v.w[g]);
+          vf[2 * h] = q4_pair_bf16<false>(c);
+          vf[2 * h + 1] = q4_pair_bf16<true>(c);
+        }
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          O[x][2 * g + half] = Elem<true>::mfma16(vf, P[x], O[x][2 * g + half]);
+          if constexpr (!BF16) O[x][2 * g + half] = Elem<true>::mfma16(vf, R[x], O[x][2 * g + half]);
+        }
+      }
+  }
+
+  // Dims 32 g + 16 half + 4 q .. + 3 of the lane's group g and row of set x.
+  __device__ __forceinline__ void result(int x, f32x4 (&out)[2]) const {
+    const int g = group_of(threadIdx.x & 63);
+    const float b = quarters_sum(base[x]);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      out[half] = O[x][half];
+#pragma unroll
+      for (int y = 1; y < NG; ++y) out[half] = y == g ? O[x][2 * y + half] : out[half];
+      if constexpr (BF16) out[half] = out[half] - 7.5f * ones[x] + b;
+      else out[half] = out[half] + b;
     }
   }
 };
+
+// All steps of the wave; the loads of the next are in flight during one.
+template <class W>
+__device__ __forceinline__ void q4_run(W& wave, const Q4Keys& ks, float scale) {
+  const int ns = ks.steps();
+  if (ns == 0) return;
+  Q4Window w;
+  w.fill(ks, 0);
+  typename W::Chunk a[2], b[2];
+  auto fetch = [&](typename W::Chunk (&ch)[2], int s) {
+    if (s - w.base >= 32) w.fill(ks, s);
+    W::load(ch[0], ks, w, s, 0);
+    W::load(ch[1], ks, w, s, 1);
+  };
+  fetch(a, 0);
+#pragma unroll 1
+  for (int s = 0; s < ns; s += 2) {
+    if (s + 1 < ns) fetch(b, s + 1);
+    wave.step(a, ks.end, scale);
+    if (s + 1 >= ns) break;
+    if (s + 2 < ns) fetch(a, s + 2);
+    wave.step(b, ks.end, scale);
+  }
+}
 
 }  // namespace sa

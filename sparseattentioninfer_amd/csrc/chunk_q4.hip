@@ -59,7 +59,7 @@ struct ChunkQ4 {
     w.start();
     Q4Keys ks = keys_of(a, it);
     ks.wave = wave, ks.waves = NW;
-    w.run(ks, a.c.scale_log2);
+    q4_run(w, ks, a.c.scale_log2);
     // Merge in fp32: accumulator row r is D floats at r * 4 D, its 16-byte chunk x at position x ^ (r % (D / 4)).
     constexpr int NC4 = D / 4;
     char* acc = s_acc + wave * ACC;
@@ -125,7 +125,7 @@ struct ChunkQ4 {
     Rows32 w;
     queries(a, it, w, row0);
     w.start();
-    w.run(keys_of(a, it), a.c.scale_log2);
+    q4_run(w, keys_of(a, it), a.c.scale_log2);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int row = row0 + 16 * c + (lane & 15);

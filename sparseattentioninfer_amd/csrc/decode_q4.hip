@@ -3,7 +3,7 @@
 //
 //   o = sum_j softmax_j(q . k_j * scale) v_j over the kept keys below kv_len; fp32 statistics and accumulators
 //
-// A workgroup has the query heads of one list (up to 16) and `unit` steps of 32 keys of it, which its four waves take in
+// A workgroup has the query heads of one list (up to 8 at D = 128, 16 at 64) and `unit` steps of 32 keys of it, which its four waves take in
 // turn; a longer list is shared by workgroups whose fp32 partials a second kernel merges.  The unit is the same for every
 // sequence, so the workgroups' loads are even whatever the lengths, and those past a sequence's end leave at once.
 #include <algorithm>
@@ -13,7 +13,6 @@
 namespace sa {
 
 constexpr int DQ_WAVES = 4;
-constexpr int DQ_ROWS = 16;
 
 struct DecodeQ4Args {
   const elem_t* q;
@@ -56,14 +55,15 @@ struct DecodeQ4Args {
   }
 };
 
-template <bool BF16, int D>
+template <bool BF16, int D, int NQ>
 struct DecodeQ4 {
   using E = Elem<BF16>;
-  using Rows = Q4Dequant<BF16, D, 1>;
-  static constexpr int ACC = DQ_ROWS * D * 4;
+  using Rows = Q4Fold<BF16, D, NQ>;
+  static constexpr int ROWS = Rows::ROWS;
+  static constexpr int ACC = ROWS * D * 4;
 
   static __device__ void run(const DecodeQ4Args& a, char* s_acc, float* s_ml) {
-    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int x = blockIdx.x;
     const int tile = x % a.tiles;
@@ -76,14 +76,12 @@ struct DecodeQ4 {
     const int chunks = a.chunks(b, row, list, len);
     const int n = a.splits_of(chunks);
     if (split >= n) return;
-    const int head0 = row * a.heads + tile * DQ_ROWS, live = min(DQ_ROWS, a.heads - tile * DQ_ROWS);
+    const int head0 = row * a.heads + tile * ROWS, live = min(ROWS, a.heads - tile * ROWS);
     Rows w;
-    {
-      const elem_t* qs = a.q + b * a.q_sb + (head0 + min(i, live - 1)) * a.q_sh + 8 * q;
 #pragma unroll
-      for (int g = 0; g < Rows::NG; ++g) w.qf[0][g] = *reinterpret_cast<const u32x4*>(qs + 32 * g);
-    }
-    w.pos[0] = w.pos_min = len - 1;
+    for (int x = 0; x < NQ; ++x)
+      w.set_query(x, a.q + b * a.q_sb + (head0 + min(x * Rows::RPS + Rows::row_of(lane), live - 1)) * a.q_sh, len - 1);
+    w.pos_min = len - 1;
     w.start();
     Q4Keys ks;
     const int kvh = row / a.group;
@@ -98,16 +96,22 @@ struct DecodeQ4 {
     ks.c1 = min(chunks, ks.c0 + 2 * a.unit);
     ks.end = len, ks.pos_max = len - 1;
     ks.wave = wave, ks.waves = DQ_WAVES;
-    w.run(ks, a.scale_log2);
+    q4_run(w, ks, a.scale_log2);
     // Merge in fp32: row r is D floats at r * 4 D, its 16-byte chunk x at position x ^ (r % (D / 4)).
     constexpr int NC4 = D / 4, OC = D / 8;
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e)
-      *reinterpret_cast<f32x4*>(s_acc + wave * ACC + i * 4 * D + 16 * ((4 * e + q) ^ (i & (NC4 - 1)))) = w.O[0][e];
-    const float l = quarters_sum(w.l_run[0]);
-    if (lane < 16) {
-      s_ml[2 * (wave * DQ_ROWS + lane)] = w.m_ref[0];
-      s_ml[2 * (wave * DQ_ROWS + lane) + 1] = l;
+    for (int x = 0; x < NQ; ++x) {
+      const int r = x * Rows::RPS + Rows::row_of(lane), g = Rows::group_of(lane);
+      f32x4 out[2];
+      w.result(x, out);
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        *reinterpret_cast<f32x4*>(s_acc + wave * ACC + r * 4 * D + 16 * ((8 * g + 4 * half + (lane >> 4)) ^ (r & (NC4 - 1)))) = out[half];
+      const float l = quarters_sum(w.l_run[x]);
+      if (lane < Rows::RPS) {
+        s_ml[2 * (wave * ROWS + r)] = w.m_ref[x];
+        s_ml[2 * (wave * ROWS + r) + 1] = l;
+      }
     }
     __syncthreads();
     for (int y = threadIdx.x; y < live * OC; y += 64 * DQ_WAVES) {
@@ -115,7 +119,7 @@ struct DecodeQ4 {
       float m[DQ_WAVES], l = 0.f, M = -__builtin_inff();
 #pragma unroll
       for (int s = 0; s < DQ_WAVES; ++s) {
-        m[s] = s_ml[2 * (s * DQ_ROWS + r)];
+        m[s] = s_ml[2 * (s * ROWS + r)];
         M = fmaxf(M, m[s]);
       }
       const float Mu = M == -__builtin_inff() ? 0.f : M;
@@ -123,7 +127,7 @@ struct DecodeQ4 {
 #pragma unroll
       for (int s = 0; s < DQ_WAVES; ++s) {
         const float fs = fast_exp2(m[s] - Mu);
-        l += fs * s_ml[2 * (s * DQ_ROWS + r) + 1];
+        l += fs * s_ml[2 * (s * ROWS + r) + 1];
         const char* p = s_acc + s * ACC + r * 4 * D;
         lo += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc) ^ (r & (NC4 - 1))));
         hi += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc + 1) ^ (r & (NC4 - 1))));
@@ -149,11 +153,11 @@ struct DecodeQ4 {
   }
 };
 
-template <bool BF16, int D>
-static __global__ __launch_bounds__(64 * DQ_WAVES) void decode_q4_kernel(const DecodeQ4Args a) {
-  using K = DecodeQ4<BF16, D>;
+template <bool BF16, int D, int NQ>
+static __global__ __launch_bounds__(64 * DQ_WAVES, NQ == 1 ? 3 : 2) void decode_q4_kernel(const DecodeQ4Args a) {
+  using K = DecodeQ4<BF16, D, NQ>;
   __shared__ __attribute__((aligned(16))) char s_acc[DQ_WAVES * K::ACC];
-  __shared__ float s_ml[2 * DQ_WAVES * DQ_ROWS];
+  __shared__ float s_ml[2 * DQ_WAVES * K::ROWS];
   K::run(a, s_acc, s_ml);
 }
 
@@ -211,8 +215,11 @@ static __global__ __launch_bounds__(256) void decode_q4_combine_kernel(const Dec
 }
 
 template <bool BF16, int D>
-static int launch_decode_q4(const DecodeQ4Args& a, int64_t groups, hipStream_t s) {
-  hipLaunchKernelGGL((decode_q4_kernel<BF16, D>), dim3((unsigned)groups), dim3(64 * DQ_WAVES), 0, s, a);
+static int launch_decode_q4(const DecodeQ4Args& a, int64_t groups, int sets, hipStream_t s) {
+  if (sets == 1)
+    hipLaunchKernelGGL((decode_q4_kernel<BF16, D, 1>), dim3((unsigned)groups), dim3(64 * DQ_WAVES), 0, s, a);
+  else
+    hipLaunchKernelGGL((decode_q4_kernel<BF16, D, 2>), dim3((unsigned)groups), dim3(64 * DQ_WAVES), 0, s, a);
   if (a.splits > 1) {
     const int per = 256 / (D / 8);
     hipLaunchKernelGGL((decode_q4_combine_kernel<BF16, D>), dim3((unsigned)((a.B * a.Hq + per - 1) / per)), dim3(256), 0, s, a);
@@ -291,7 +298,9 @@ extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh
   a.rows = sel_off ? sel_rows : Hkv;
   a.heads = Hq / a.rows;
   a.group = a.rows / Hkv;
-  a.tiles = (a.heads + DQ_ROWS - 1) / DQ_ROWS;
+  // Query heads of a workgroup: one column set, or two.
+  const int per_set = 16 / (D / 32), sets = a.heads > per_set ? 2 : 1;
+  a.tiles = (a.heads + sets * per_set - 1) / (sets * per_set);
   a.o = static_cast<elem_t*>(o);
   a.o_sb = o_sb, a.o_sh = o_sh;
   a.B = B, a.Hq = Hq;
@@ -302,6 +311,6 @@ extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh
     return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == SA_DTYPE_BF16)
-    return D == 128 ? launch_decode_q4<true, 128>(a, groups, s) : launch_decode_q4<true, 64>(a, groups, s);
-  return D == 128 ? launch_decode_q4<false, 128>(a, groups, s) : launch_decode_q4<false, 64>(a, groups, s);
+    return D == 128 ? launch_decode_q4<true, 128>(a, groups, sets, s) : launch_decode_q4<true, 64>(a, groups, sets, s);
+  return D == 128 ? launch_decode_q4<false, 128>(a, groups, sets, s) : launch_decode_q4<false, 64>(a, groups, sets, s);
 }

@@ -65,4 +65,15 @@ __device__ __forceinline__ uint32_t q4_high(uint32_t w) { return (w >> 4) & 0x0f
 template <int E>
 __device__ __forceinline__ float q4_code(uint32_t codes) { return (float)((codes >> (8 * E)) & 0xffu); }
 
+// Two of four codes as numbers of 16 bits, exact: a code in a byte is an e4m3 number of that many 2^-9, subnormals and the
+// first binade together, so the conversion scales by 2^9.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t q4_pair_bf16(uint32_t codes) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)codes, 512.f, HIGH));
+}
+template <bool HIGH>
+__device__ __forceinline__ uint32_t q4_pair_f16(uint32_t codes) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)codes, 512.f, HIGH));
+}
+
 }  // namespace sa
