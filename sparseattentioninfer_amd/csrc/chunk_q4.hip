@@ -115,40 +115,421 @@ struct ChunkQ4 {
       }
     }
   }
+};
 
-  // 256 rows, 32 to a wave.
-  static __device__ void wide(const ChunkQ4Args& a, const ChunkItem& it) {
+// 256 rows to a workgroup: eight waves of 32 rows share every key tile.  Each wave brings an eighth of a tile's codes into
+// registers a step ahead, scales them to the element type and writes them to LDS: keys as rows (lds_tile.h), values
+// transposed, [D][64], so that both products read their fragments with 16-byte reads.  One step per tile and one barrier per
+// step.  Block A of a step runs S^T = K Q^T of the next tile on the matrix cores under the exponentials of this one, block
+// B O^T += V^T P^T.  Waves 0..3 run A(i), B(i) in step i and waves 4..7, one on each SIMD beside them, B(i - 1), A(i), so
+// that the two waves of a SIMD run the vector-heavy A and the matrix-only B at the same time.  In step i the waves
+// read K(i + 1), V(i) and V(i - 1) and write K(i + 2) and V(i + 1): two K and three V buffers.
+// A row's reference is the maximum of its first tile and is raised only when its probabilities would pass the
+// element type's range (REFIT_SUM), so the common step never touches O with vector instructions.
+template <bool BF16, int D>
+struct ChunkQ4Wide : StagedTile {
+  using E = Elem<BF16>;
+  using F = Kv4<D>;
+  static constexpr int NW = 8;
+  static_assert(NW * CK_ROWS == CK_WIDE_ROWS, "rows of a wide item");
+  static constexpr int NCG = D / 32;
+  static constexpr int NWD = D / 64;               // words of a tile's keys (and of its values) that a lane scales
+  static constexpr int TILE_BYTES = CK_KT * D * 2;
+  static constexpr int NBK = 2, NBV = 3;
+  static constexpr int STAGE = CK_ROWS * D * 2;    // a wave's share of O
+  static constexpr int LDS_BYTES = (NBK + NBV) * TILE_BYTES;
+  static constexpr int KEYS = NW * 4 * 64;         // ints of LDS for the tiles' first keys
+  static_assert(NW * STAGE <= LDS_BYTES, "O is staged in the K/V buffers");
+  static constexpr float REFIT_SUM = BF16 ? 65536.f : 32768.f;
+
+  // 64 tiles looked up at once: lane i holds, for tile base + i, the place and first key of the chunk of which this
+  // wave scales half, and the tile's largest key; the first keys of its four chunks go to LDS, for the tiles that need
+  // a mask.  Tiles are looked up three ahead of the one whose mask is due, so a window starts three tiles back.
+  static constexpr int AHEAD = 3;
+  struct Window {
+    int base;
+    int64_t off;
+    int key, slot, last;
+
+    __device__ __forceinline__ void fill(const ChunkArgs& a, const ChunkItem& it, int64_t sp, int first, int rb, int* s_keys) {
+      base = first;
+      const int lane = threadIdx.x & 63;
+      key = CK_NO_KEY;
+      off = 0;
+      slot = 0;
+      last = -1;
+      int keys[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int c = it.c0 + 4 * (first + lane) + x;
+        keys[x] = CK_NO_KEY;
+        if (c < it.c1) {
+          int lb, s;
+          if (it.list) {
+            const int e = (int)fast_div((uint32_t)c, (uint32_t)(a.page / 16), a.mul_ppc);
+            lb = it.list[e];
+            s = (c - e * (a.page / 16)) * 16;
+          } else {
+            lb = (int)fast_div((uint32_t)(16 * c), (uint32_t)a.page, a.mul_page);
+            s = 16 * c - lb * a.page;
+          }
+          // (a page whose first key no row sees is not looked up; neither are ids that are no column)
+          if (lb >= 0 && lb < a.max_blocks && (int64_t)lb * a.page + s <= it.pos_max) {
+            const int pg = a.table[it.b * a.table_stride + lb];
+            if (pg >= 0 && pg < a.num_pages) {
+              keys[x] = lb * a.page + s;
+              if (x == rb) {
+                off = (int64_t)pg * sp;
+                key = keys[x];
+                slot = s;
+              }
+            }
+          }
+        }
+        last = max(last, keys[x] + 15);
+      }
+      *reinterpret_cast<int4*>(s_keys + 4 * lane) = int4{keys[0], keys[1], keys[2], keys[3]};
+    }
+    __device__ __forceinline__ int key_of(int t) const { return __builtin_amdgcn_readlane(key, t - base); }
+    __device__ __forceinline__ int slot_of(int t) const { return __builtin_amdgcn_readlane(slot, t - base); }
+    __device__ __forceinline__ int last_of(int t) const { return __builtin_amdgcn_readlane(last, t - base); }
+    __device__ __forceinline__ int64_t off_of(int t) const {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uint64_t)off, t - base);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)off >> 32), t - base);
+      return (int64_t)(((uint64_t)hi << 32) | lo);
+    }
+  };
+
+  // A lane's words of a tile and their pairs.  Keys: token 8 (wave % 2) + l / 4 % 8 of the wave's chunk, words NWD p + u of
+  // quarter l % 4, p = l / 32.  Values: tokens 8 (wave % 2) + 4 (l % 2) .. + 3, dims l / 2 % 16 of the groups NWD p + u.
+  struct KeyWords {
+    uint32_t w[NWD], st[NWD];
+  };
+  struct ValueWords {
+    uint32_t w[NWD];
+    u32x4 st[NWD];
+  };
+
+  static __device__ __forceinline__ void load_words(uint32_t (&w)[NWD], const uint8_t* p) {
+    if constexpr (NWD == 2) {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+      w[0] = v[0], w[1] = v[1];
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
+
+  // A operand of O^T = V^T P^T: lane l holds d = 32 dt + l % 32 of keys 32 j + 16 h + 8 (l / 32) + 0..7.
+  static __device__ __forceinline__ u32x4 vtfrag(const char* cV, int v0, int swz, int j, int h, int dt) {
+    return *reinterpret_cast<const u32x4*>(cV + 4096 * dt + v0 + ((16 * (4 * j + 2 * h)) ^ swz));
+  }
+
+  static __device__ void run(const ChunkQ4Args& x, const ChunkItem& it, char* s_kv, int* s_all_keys) {
+    const ChunkArgs& a = x.c;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row0 = it.row0 + CK_ROWS * wave;
-    if (row0 >= it.row_end) return;
-    Rows32 w;
-    queries(a, it, w, row0);
-    w.start();
-    q4_run(w, keys_of(a, it), a.c.scale_log2);
+    const int g = lane >> 5, l32 = lane & 31;
+    int* s_keys = s_all_keys + 4 * 64 * wave;
+    char* sK = s_kv;
+    char* sV = s_kv + NBK * TILE_BYTES;
+
+    const int row0 = min(it.row0 + CK_ROWS * wave, it.row_end - 1);   // a wave past the rows repeats the last one
+    const int row = min(row0 + l32, it.row_end - 1);
+    const int token = (int)fast_div((uint32_t)row, (uint32_t)a.G, a.mul_G);
+    const int pos_min = it.start + (int)fast_div((uint32_t)row0, (uint32_t)a.G, a.mul_G);
+    const int pos8 = it.start + token - 8 * g;   // a key at offset e of a chunk's lane half is seen if e <= pos8 - key
+    u32x4 Qr[D / 16];
+    {
+      const elem_t* qs = a.q + (int64_t)(it.tok0 + token) * a.q_st + (it.kvh * a.G + row - token * a.G) * a.q_sh + 8 * g;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int row = row0 + 16 * c + (lane & 15);
-      const float l = quarters_sum(w.l_run[c]);
-      if (row >= it.row_end) continue;
-      const int tk = (int)fast_div((uint32_t)row, (uint32_t)a.c.G, a.c.mul_G);
-      const int h = it.kvh * a.c.G + row - tk * a.c.G, q = lane >> 4;
-      if (it.splits > 1) {
-        const int64_t at = it.part_row(a.c, tk, h);
+      for (int c = 0; c < D / 16; ++c) Qr[c] = *reinterpret_cast<const u32x4*>(qs + 16 * c);
+    }
+    const Frag f(lane);
+    const int v0 = l32 * 128, vswz = 16 * (g ^ (l32 & 7));
+    const float c = a.scale_log2;
+    const int nt = (it.c1 - it.c0 + 3) / 4;
+
+    // This wave's eighth of a tile: half of chunk rb.
+    const int rb = wave >> 1;
+    const uint8_t* kh = x.k + it.kvh * x.sh;
+    const uint8_t* vh = x.v + it.kvh * x.sh;
+    const int ktok = 8 * (wave & 1) + ((lane >> 2) & 7), kq = lane & 3, p = lane >> 5;
+    const int vtok = 8 * (wave & 1) + 4 * (lane & 1), vi = (lane >> 1) & 15;
+    const int k_at = ktok * F::ROW + 4 * F::NG * kq + 4 * NWD * p;
+    const int v_at = (vtok >> 2) * F::QUAD + 4 * F::NG * vi + 4 * NWD * p;
+    const int stats = F::stats_at(a.page);
+    const int krow16 = krow(ktok);
+    char* const lds_k = sK + rb * 1024 + krow16 * 64 + 16 * (kq ^ ((krow16 >> 2) & 3)) + 4096 * NWD * p;
+    char* const lds_v = sV + (32 * NWD * p + vi) * 128 + 16 * (wave ^ (vi & 7)) + 8 * (lane & 1);
+    Window w;
+    KeyWords kw;
+    ValueWords vw;
+    auto load_k = [&](int t) {
+      if (t - w.base >= 64) w.fill(a, it, x.sp, t - AHEAD, rb, s_keys);
+      const uint8_t* b = kh + w.off_of(t);
+      const int slot = w.slot_of(t), key = w.key_of(t);
+      load_words(kw.w, b + slot * F::ROW + k_at);
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e)
-          *reinterpret_cast<f32x4*>(a.c.part_acc + at * D + 16 * e + 4 * q) = w.O[c][e];
-        if (q == 0) {
-          a.c.part_ml[2 * at] = w.m_ref[c];
-          a.c.part_ml[2 * at + 1] = l;
+      for (int u = 0; u < NWD; ++u)
+        kw.st[u] = *reinterpret_cast<const uint32_t*>(b + stats + 4 * slot + 4 * ((NWD * p + u) * a.page + ktok));
+      if (key + 16 > it.end) {       // keys that are not there are zeros
+#pragma unroll
+        for (int u = 0; u < NWD; ++u) kw.st[u] = key + ktok < it.end ? kw.st[u] : 0u;
+      }
+    };
+    auto load_v = [&](int t) {
+      const uint8_t* b = vh + w.off_of(t);
+      const int slot = w.slot_of(t), key = w.key_of(t);
+      load_words(vw.w, b + slot * F::ROW + v_at);
+#pragma unroll
+      for (int u = 0; u < NWD; ++u)
+        vw.st[u] = *reinterpret_cast<const u32x4*>(b + stats + 4 * slot + 4 * ((NWD * p + u) * a.page + vtok));
+      if (key + 16 > it.end) {
+#pragma unroll
+        for (int u = 0; u < NWD; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vw.st[u][j] = key + vtok + j < it.end ? vw.st[u][j] : 0u;
+      }
+    };
+    // Scales the loaded words into buffer kb / vb.
+    auto put_k = [&](int kb) {
+#pragma unroll
+      for (int u = 0; u < NWD; ++u) {
+        const float s = q4_scale<BF16>(kw.st[u]), m = q4_min<BF16>(kw.st[u]);
+        const uint32_t lo = q4_low(kw.w[u]), hi = q4_high(kw.w[u]);
+        *reinterpret_cast<u32x4*>(lds_k + kb * TILE_BYTES + 4096 * u) =
+            u32x4{E::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
+                  E::pack2f(fmaf(q4_code<2>(lo), s, m), fmaf(q4_code<3>(lo), s, m)),
+                  E::pack2f(fmaf(q4_code<0>(hi), s, m), fmaf(q4_code<1>(hi), s, m)),
+                  E::pack2f(fmaf(q4_code<2>(hi), s, m), fmaf(q4_code<3>(hi), s, m))};
+      }
+    };
+    auto put_v = [&](int vb) {
+#pragma unroll
+      for (int u = 0; u < NWD; ++u) {
+        float s[4], m[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = q4_scale<BF16>(vw.st[u][j]), m[j] = q4_min<BF16>(vw.st[u][j]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t cs = half ? q4_high(vw.w[u]) : q4_low(vw.w[u]);
+          *reinterpret_cast<u32x2*>(lds_v + vb * TILE_BYTES + 4096 * u + 2048 * half) =
+              u32x2{E::pack2f(fmaf(q4_code<0>(cs), s[0], m[0]), fmaf(q4_code<1>(cs), s[1], m[1])),
+                    E::pack2f(fmaf(q4_code<2>(cs), s[2], m[2]), fmaf(q4_code<3>(cs), s[3], m[3]))};
         }
-      } else {
-        const float inv = l > 0.f ? 1.f / l : 1.f;
-        elem_t* o = a.c.o + (int64_t)(it.tok0 + tk) * a.c.o_st + h * a.c.o_sh + 4 * q;
+      }
+    };
+    // Scores of tile t past a row's position become -inf.
+    auto mask = [&](f32x16 (&S)[2], int t) {
+      if (w.last_of(t) <= pos_min) return;
+      const int4 keys = *reinterpret_cast<const int4*>(&s_keys[4 * (t - w.base)]);
+      const int lim[4] = {pos8 - keys.x, pos8 - keys.y, pos8 - keys.z, pos8 - keys.w};
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e)
-          *reinterpret_cast<u32x2*>(o + 16 * e) = u32x2{E::pack2f(w.O[c][e][0] * inv, w.O[c][e][1] * inv),
-                                                         E::pack2f(w.O[c][e][2] * inv, w.O[c][e][3] * inv)};
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            S[j][8 * h + e] = e > lim[2 * j + h] ? -__builtin_inff() : S[j][8 * h + e];
+    };
+
+    f32x16 O[NCG];
+#pragma unroll
+    for (int dt = 0; dt < NCG; ++dt) O[dt] = f32x16{};
+    float m_ref = -__builtin_inff(), l_run = 0.f;
+    f32x16 S[2] = {f32x16{}, f32x16{}};
+    if (nt > 0) {
+      w.fill(a, it, x.sp, 0, rb, s_keys);
+      load_k(0);
+      load_v(0);
+      put_k(0);
+      put_v(0);
+      if (nt > 1) {
+        load_k(1);
+        put_k(1);
+      }
+      if (nt > 2) load_k(2);
+      if (nt > 1) load_v(1);
+      __syncthreads();
+#pragma unroll
+      for (int cc = 0; cc < D / 16; ++cc)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) S[j] = E::mfma32(kfrag(sK, f, j, cc), Qr[cc], S[j]);
+      mask(S, 0);
+      float mx = S[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[j][r]);
+      m_ref = halves_max(mx) * c;   // -inf stays -inf (c > 0)
+      __syncthreads();              // K of tile 0 has been read
+    }
+    float neg_m = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+    bool ref_ok = !__any(m_ref == -__builtin_inff());
+
+    const bool lag = wave >= NW / 2;
+    int vb_cur = 0, kb_cur = 0;   // buffers of the current tile
+    bool pending = false;
+    auto ring = [](int y, int n) { return y >= n ? y - n : y; };
+    u32x4 P[2][2];
+    constexpr int NQ = D / 8;    // QK MFMAs of a tile: i -> (key half i % 2, cc = i / 2)
+    constexpr int PE = 32 / NQ;  // probabilities per QK MFMA
+    constexpr int NP = D / 8;    // PV MFMAs: i -> (dt = i % NCG, h, j)
+
+    auto block_b = [&](const char* cV) {
+      auto vfr = [&](int i) { return vtfrag(cV, v0, vswz, i / (2 * NCG), (i / NCG) & 1, i % NCG); };
+      u32x4 vf[2] = {vfr(0), vfr(1)};
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        O[i % NCG] = E::mfma32(vf[i & 1], P[i / (2 * NCG)][(i / NCG) & 1], O[i % NCG]);
+        if (i + 2 < NP) vf[i & 1] = vfr(i + 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto probs = [&](const f32x16 (&Sc)[2], float& ls) {
+      ls = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = fast_exp2(fmaf(Sc[j][8 * h + 2 * e], c, neg_m));
+            const float p1 = fast_exp2(fmaf(Sc[j][8 * h + 2 * e + 1], c, neg_m));
+            ls += p0 + p1;
+            P[j][h][e] = E::pack2f(p0, p1);
+          }
+    };
+    // Rare: a row without a reference yet, or probabilities past REFIT_SUM.
+    auto raise = [&](const f32x16 (&Sc)[2], float& ls) {
+      float mx = Sc[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, Sc[j][r]);
+      const float m_new = fmaxf(m_ref, halves_max(mx) * c);
+      const float alpha = m_ref == -__builtin_inff() ? 1.f : fast_exp2(m_ref - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NCG; ++dt) O[dt] *= alpha;
+      m_ref = m_new;
+      neg_m = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+      ref_ok = !__any(m_ref == -__builtin_inff());
+      probs(Sc, ls);
+    };
+
+    // One step on tile t, whose scores are in Sc; fills Sx with the next tile's.
+    auto step = [&](int t, f32x16 (&Sc)[2], f32x16 (&Sx)[2]) {
+      if (t + 2 < nt) put_k(kb_cur);
+      put_v(ring(vb_cur + 1, NBV));            // of tile t + 1: there is one
+      if (t + 3 < nt) load_k(t + 3);
+      if (t + 2 < nt) load_v(t + 2);
+      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES);
+      const char* cK = sK + (kb_cur ^ 1) * TILE_BYTES;
+      auto kfr = [&](int i) { return kfrag(cK, f, i & 1, i >> 1); };
+      u32x4 kf[3] = {kfr(0), kfr(1), kfr(2)};
+      Sx[0] = f32x16{};
+      Sx[1] = f32x16{};
+      float ls = 0.f;
+      uint32_t pw[2][2][4];
+      __builtin_amdgcn_s_setprio(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        Sx[i & 1] = E::mfma32(kf[i % 3], Qr[i >> 1], Sx[i & 1]);
+        if (i + 3 < NQ) kf[i % 3] = kfr(i + 3);
+#pragma unroll
+        for (int u = 0; u < PE; u += 2) {
+          const int y = PE * i + u, j = y >> 4, rr = y & 15;
+          const float p0 = fast_exp2(fmaf(Sc[j][rr], c, neg_m));
+          const float p1 = fast_exp2(fmaf(Sc[j][rr + 1], c, neg_m));
+          ls += p0 + p1;
+          uint32_t pk = E::pack2f(p0, p1);
+          asm volatile("" : "+v"(pk), "+v"(ls));   // computed here, not sunk to its use in block B
+          pw[j][rr >> 3][(rr & 7) >> 1] = pk;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) P[j][h] = u32x4{pw[j][h][0], pw[j][h][1], pw[j][h][2], pw[j][h][3]};
+      if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(Sc, ls);
+      l_run += ls;
+      mask(Sx, t + 1);
+      if (!lag) block_b(sV + vb_cur * TILE_BYTES);
+      pending = true;
+      __syncthreads();
+      vb_cur = ring(vb_cur + 1, NBV);
+      kb_cur ^= 1;
+    };
+    if (nt > 0) {
+      f32x16 Sn[2];
+      int t = 0;
+      while (t + 2 < nt) {
+        step(t, S, Sn);
+        step(t + 1, Sn, S);
+        t += 2;
+      }
+      if (t + 1 < nt) {
+        step(t, S, Sn);
+        S[0] = Sn[0];
+        S[1] = Sn[1];
+      }
+      // The last tile: no next one, nothing to load.
+      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES);
+      float ls;
+      probs(S, ls);
+      if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(S, ls);
+      l_run += ls;
+      block_b(sV + vb_cur * TILE_BYTES);
+    }
+    __syncthreads();   // the K/V buffers are free
+    const float lt = halves_sum(l_run);
+    if (it.splits > 1) {
+      if (it.row0 + CK_ROWS * wave + l32 < it.row_end) {
+        const int64_t at = it.part_row(a, token, it.kvh * a.G + row - token * a.G);
+#pragma unroll
+        for (int dt = 0; dt < NCG; ++dt)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq)
+            *reinterpret_cast<f32x4*>(a.part_acc + at * D + 32 * dt + 8 * rq + 4 * g) =
+                f32x4{O[dt][4 * rq], O[dt][4 * rq + 1], O[dt][4 * rq + 2], O[dt][4 * rq + 3]};
+        if (g == 0) {
+          a.part_ml[2 * at] = m_ref;
+          a.part_ml[2 * at + 1] = lt;
+        }
+      }
+      return;
+    }
+    // O / l through this wave's 32 x D staging area: 16-byte chunk x of row r at position x ^ (r % (D / 8)); each
+    // store instruction then writes whole rows.
+    constexpr int NCH = D / 8, RPI = 64 / NCH;
+    const float inv = lt > 0.f ? 1.f / lt : 1.f;
+    char* stage = s_kv + wave * STAGE;
+#pragma unroll
+    for (int dt = 0; dt < NCG; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int y = 4 * dt + rq;
+        *reinterpret_cast<u32x2*>(stage + l32 * 2 * D + 16 * (y ^ (l32 & (NCH - 1))) + 8 * g) =
+            u32x2{E::pack2f(O[dt][4 * rq] * inv, O[dt][4 * rq + 1] * inv),
+                  E::pack2f(O[dt][4 * rq + 2] * inv, O[dt][4 * rq + 3] * inv)};
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave reads back what its own lanes wrote
+    const int pc = lane % NCH;
+#pragma unroll
+    for (int k = 0; k < CK_ROWS / RPI; ++k) {
+      const int r = RPI * k + lane / NCH;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * 2 * D + 16 * pc);
+      const int fr = it.row0 + CK_ROWS * wave + r;
+      if (fr < it.row_end) {
+        const int tk = (int)fast_div((uint32_t)fr, (uint32_t)a.G, a.mul_G);
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(a.o + (int64_t)(it.tok0 + tk) * a.o_st +
+                                                                 (it.kvh * a.G + fr - tk * a.G) * a.o_sh +
+                                                                 8 * (pc ^ (r & (NCH - 1)))));
       }
     }
   }
@@ -156,15 +537,17 @@ struct ChunkQ4 {
 
 template <bool BF16, int D>
 static __global__ __launch_bounds__(512, 2) void chunk_q4_kernel(const ChunkQ4Args a) {
-  using K = ChunkQ4<BF16, D>;
-  __shared__ __attribute__((aligned(16))) char s_acc[K::LDS_BYTES];
-  __shared__ float s_ml[2 * K::NW * CK_ROWS];
+  using N = ChunkQ4<BF16, D>;
+  using W = ChunkQ4Wide<BF16, D>;
+  __shared__ __attribute__((aligned(16))) char s_kv[W::LDS_BYTES > N::LDS_BYTES ? W::LDS_BYTES : N::LDS_BYTES];
+  __shared__ __attribute__((aligned(16))) int s_aux[W::KEYS];
+  static_assert(W::KEYS >= 2 * N::NW * CK_ROWS, "row references and sums of the narrow items' waves");
   ChunkItem it;
   if (!find_chunk_item(a.c, blockIdx.x, it)) return;
   if (it.narrow)
-    K::narrow(a, it, s_acc, s_ml);
+    N::narrow(a, it, s_kv, reinterpret_cast<float*>(s_aux));
   else
-    K::wide(a, it);
+    W::run(a, it, s_kv, s_aux);
 }
 
 template <bool BF16, int D>
