@@ -100,13 +100,15 @@ struct Q4Dequant {
   using F = Kv4<D>;
   static constexpr int NG = F::NG, NE = D / 16;
 
+  static constexpr int LDS_WORDS = 4 * 16 * NG;    // of a wave: pairs of a step's keys and values, [chunk][NG][16] each
+
   struct Chunk {
     Words<NG> k, v;
-    uint32_t ks[NG];
-    u32x4 vs[NG];
+    uint32_t ks, vs;               // the pair of key l % 16 and group l / 16 (those that there are)
     int key;
   };
 
+  uint32_t* pairs;                 // LDS_WORDS of LDS of the wave's own
   u32x4 qf[NC][NG];
   int pos[NC];                     // position of the lane's row
   int pos_min;                     // of all rows
@@ -122,12 +124,9 @@ struct Q4Dequant {
     const uint8_t *kb = ks.k + off, *vb = ks.v + off;
     c.k.load(kb + slot * F::ROW + (i * F::ROW + 4 * NG * q));
     c.v.load(vb + slot * F::ROW + (q * F::QUAD + 4 * NG * i));
-    const int st = F::stats_at(ks.page) + 4 * slot;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      c.ks[g] = *reinterpret_cast<const uint32_t*>(kb + st + 4 * g * ks.page + 4 * i);
-      c.vs[g] = *reinterpret_cast<const u32x4*>(vb + st + 4 * g * ks.page + 16 * q);
-    }
+    const int st = F::stats_at(ks.page) + 4 * slot + 4 * (min(q, NG - 1) * ks.page + i);
+    c.ks = *reinterpret_cast<const uint32_t*>(kb + st);
+    c.vs = *reinterpret_cast<const uint32_t*>(vb + st);
   }
 
   __device__ __forceinline__ void start() {
@@ -161,7 +160,15 @@ struct Q4Dequant {
   }
 
   __device__ __forceinline__ void step(const Chunk (&ch)[2], int end, float scale) {
-    const int lane = threadIdx.x & 63, q = lane >> 4;
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    // The pairs change lanes through LDS, whose accesses by one wave run in order.
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (q < NG) {
+        const bool live = ch[h].key + i < end;     // 0 times what a slot without a token holds is 0
+        pairs[(16 * NG) * h + lane] = ch[h].ks;
+        pairs[(16 * NG) * (2 + h) + lane] = live ? ch[h].vs : 0u;
+      }
     f32x4 S[NC][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -169,7 +176,8 @@ struct Q4Dequant {
       for (int c = 0; c < NC; ++c) S[c][h] = f32x4{};
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float s = q4_scale<BF16>(ch[h].ks[g]), m = q4_min<BF16>(ch[h].ks[g]);
+        const uint32_t st = pairs[(16 * NG) * h + 16 * g + i];
+        const float s = q4_scale<BF16>(st), m = q4_min<BF16>(st);
         const uint32_t lo = q4_low(ch[h].k.w[g]), hi = q4_high(ch[h].k.w[g]);
         const u32x4 kf = {E::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
                           E::pack2f(fmaf(q4_code<2>(lo), s, m), fmaf(q4_code<3>(lo), s, m)),
@@ -215,26 +223,15 @@ struct Q4Dequant {
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) l_run[c] += ls[c];
-    u32x4 vs[2][NG];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int live = end - ch[h].key - 4 * q;    // of the lane's four keys, those that are there
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        vs[h][g] = ch[h].vs[g];
-        if (ch[h].key + 16 > end) {                // 0 times what a slot without a token holds is 0
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vs[h][g][j] = j < live ? vs[h][g][j] : 0u;
-        }
-      }
-    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float s[2][4], m[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const u32x4 st = *reinterpret_cast<const u32x4*>(pairs + (16 * NG) * (2 + h) + 16 * g + 4 * q);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[h][j] = q4_scale<BF16>(vs[h][g][j]), m[h][j] = q4_min<BF16>(vs[h][g][j]);
+        for (int j = 0; j < 4; ++j) s[h][j] = q4_scale<BF16>(st[j]), m[h][j] = q4_min<BF16>(st[j]);
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {       // dims 32 g + 16 half + 0..15
         u32x4 vf;

@@ -17,7 +17,6 @@ struct ChunkQ4 {
   static constexpr int NW = 8;
   static constexpr int ACC = CK_ROWS * D * 4;
   static constexpr int LDS_BYTES = NW * ACC;
-  using Rows32 = Q4Dequant<BF16, D, 2>;
 
   static __device__ __forceinline__ Q4Keys keys_of(const ChunkQ4Args& a, const ChunkItem& it) {
     Q4Keys ks;
@@ -34,52 +33,107 @@ struct ChunkQ4 {
     return ks;
   }
 
-  // Flattened rows row0 .. row0 + 31 of the item's sequence, those at or past `row_end` repeats of the last.
-  static __device__ __forceinline__ void queries(const ChunkQ4Args& a, const ChunkItem& it, Rows32& w, int row0) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int row = min(row0 + 16 * c + (lane & 15), it.row_end - 1);
-      const int token = (int)fast_div((uint32_t)row, (uint32_t)a.c.G, a.c.mul_G);
-      w.pos[c] = it.start + token;
-      const elem_t* qs = a.c.q + (int64_t)(it.tok0 + token) * a.c.q_st + (it.kvh * a.c.G + row - token * a.c.G) * a.c.q_sh +
-                         8 * (lane >> 4);
-#pragma unroll
-      for (int g = 0; g < Rows32::NG; ++g) w.qf[c][g] = *reinterpret_cast<const u32x4*>(qs + 32 * g);
-    }
-    w.pos_min = it.start + (int)fast_div((uint32_t)min(row0, it.row_end - 1), (uint32_t)a.c.G, a.c.mul_G);
+  // Query row r of the item (a repeat of its last past the end), its position.
+  static __device__ __forceinline__ const elem_t* query(const ChunkQ4Args& a, const ChunkItem& it, int r, int& pos) {
+    const int row = min(it.row0 + r, it.row_end - 1);
+    const int token = (int)fast_div((uint32_t)row, (uint32_t)a.c.G, a.c.mul_G);
+    pos = it.start + token;
+    return a.c.q + (int64_t)(it.tok0 + token) * a.c.q_st + (it.kvh * a.c.G + row - token * a.c.G) * a.c.q_sh;
   }
 
-  // 32 rows whose keys the waves divide.
-  static __device__ void narrow(const ChunkQ4Args& a, const ChunkItem& it, char* s_acc, float* s_ml) {
+  // Accumulator row r of a wave is D floats at r * 4 D, its 16-byte chunk x at position x ^ (r % (D / 4)).
+  static __device__ __forceinline__ f32x4* acc_at(char* acc, int r, int x) {
+    return reinterpret_cast<f32x4*>(acc + r * 4 * D + 16 * (x ^ (r & (D / 4 - 1))));
+  }
+
+  // Up to 16 NC rows, by scaled keys and values.
+  template <int NC>
+  static __device__ __forceinline__ void scaled(const ChunkQ4Args& a, const ChunkItem& it, const Q4Keys& ks, int pos_min,
+                                                char* acc, float* ml, uint32_t* pairs) {
+    using W = Q4Dequant<BF16, D, NC>;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Rows32 w;
-    queries(a, it, w, it.row0);
-    w.start();
-    Q4Keys ks = keys_of(a, it);
-    ks.wave = wave, ks.waves = NW;
-    q4_run(w, ks, a.c.scale_log2);
-    // Merge in fp32: accumulator row r is D floats at r * 4 D, its 16-byte chunk x at position x ^ (r % (D / 4)).
-    constexpr int NC4 = D / 4;
-    char* acc = s_acc + wave * ACC;
+    W w;
+    w.pairs = pairs;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < NC; ++c) {
+      const elem_t* qs = query(a, it, 16 * c + (lane & 15), w.pos[c]) + 8 * (lane >> 4);
+#pragma unroll
+      for (int g = 0; g < W::NG; ++g) w.qf[c][g] = *reinterpret_cast<const u32x4*>(qs + 32 * g);
+    }
+    w.pos_min = pos_min;
+    w.start();
+    q4_run(w, ks, a.c.scale_log2);
+    __syncthreads();               // the pairs lie where the accumulators go
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
       const int r = 16 * c + (lane & 15);
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e)
-        *reinterpret_cast<f32x4*>(acc + r * 4 * D + 16 * ((4 * e + (lane >> 4)) ^ (r & (NC4 - 1)))) = w.O[c][e];
+      for (int e = 0; e < D / 16; ++e) *acc_at(acc, r, 4 * e + (lane >> 4)) = w.O[c][e];
       const float l = quarters_sum(w.l_run[c]);
       if (lane < 16) {
-        s_ml[2 * (wave * CK_ROWS + r)] = w.m_ref[c];
-        s_ml[2 * (wave * CK_ROWS + r) + 1] = l;
+        ml[2 * r] = w.m_ref[c];
+        ml[2 * r + 1] = l;
       }
     }
+  }
+
+  // Up to Q4Fold::ROWS rows, by codes.
+  template <int NQ>
+  static __device__ __forceinline__ void folded(const ChunkQ4Args& a, const ChunkItem& it, const Q4Keys& ks, int pos_min,
+                                                char* acc, float* ml) {
+    using W = Q4Fold<BF16, D, NQ>;
+    const int lane = threadIdx.x & 63;
+    W w;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      int pos;
+      const elem_t* qs = query(a, it, x * W::RPS + W::row_of(lane), pos);
+      w.set_query(x, qs, pos);
+    }
+    w.pos_min = pos_min;
+    w.start();
+    q4_run(w, ks, a.c.scale_log2);
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      const int r = x * W::RPS + W::row_of(lane);
+      f32x4 out[2];
+      w.result(x, out);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) *acc_at(acc, r, 8 * W::group_of(lane) + 4 * half + (lane >> 4)) = out[half];
+      const float l = quarters_sum(w.l_run[x]);
+      if (lane < W::RPS) {
+        ml[2 * r] = w.m_ref[x];
+        ml[2 * r + 1] = l;
+      }
+    }
+  }
+
+  // 32 rows whose keys the waves divide.  Codes are multiplied as they are for up to two column sets of rows (8 at D = 128, 16
+  // at 64); more rows share the work of scaling them.
+  static __device__ void narrow(const ChunkQ4Args& a, const ChunkItem& it, char* s_acc, float* s_ml) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Q4Keys ks = keys_of(a, it);
+    ks.wave = wave, ks.waves = NW;
+    const int pos_min = it.start + (int)fast_div((uint32_t)it.row0, (uint32_t)a.c.G, a.c.mul_G);
+    const int rows = it.row_end - it.row0;
+    char* acc = s_acc + wave * ACC;
+    float* ml = s_ml + 2 * CK_ROWS * wave;
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(s_acc) + wave * Q4Dequant<BF16, D, 2>::LDS_WORDS;
+    constexpr int SET = Q4Fold<BF16, D, 1>::RPS;
+    if (rows <= SET) {
+      folded<1>(a, it, ks, pos_min, acc, ml);
+    } else if (rows <= 2 * SET) {
+      folded<2>(a, it, ks, pos_min, acc, ml);
+    } else if (2 * SET < 16 && rows <= 16) {
+      scaled<1>(a, it, ks, pos_min, acc, ml, pairs);
+    } else {
+      scaled<2>(a, it, ks, pos_min, acc, ml, pairs);
+    }
+    // Merge in fp32.
     __syncthreads();
     constexpr int OC = D / 8;
-    for (int x = threadIdx.x; x < CK_ROWS * OC; x += 64 * NW) {
+    for (int x = threadIdx.x; x < rows * OC; x += 64 * NW) {
       const int r = x / OC, oc = x % OC;
-      if (it.row0 + r >= it.row_end) continue;
       float m[NW], l = 0.f, M = -__builtin_inff();
 #pragma unroll
       for (int s = 0; s < NW; ++s) {
@@ -92,9 +146,8 @@ struct ChunkQ4 {
       for (int s = 0; s < NW; ++s) {
         const float fs = fast_exp2(m[s] - Mu);
         l += fs * s_ml[2 * (s * CK_ROWS + r) + 1];
-        const char* p = s_acc + s * ACC + r * 4 * D;
-        lo += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc) ^ (r & (NC4 - 1))));
-        hi += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc + 1) ^ (r & (NC4 - 1))));
+        lo += fs * *acc_at(s_acc + s * ACC, r, 2 * oc);
+        hi += fs * *acc_at(s_acc + s * ACC, r, 2 * oc + 1);
       }
       const int tk = (int)fast_div((uint32_t)(it.row0 + r), (uint32_t)a.c.G, a.c.mul_G);
       const int h = it.kvh * a.c.G + it.row0 + r - tk * a.c.G;
