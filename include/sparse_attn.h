@@ -631,10 +631,12 @@ int sa_paged_chunk_attn_q4(int dtype, const void* q, int64_t q_st, int64_t q_sh,
 /*
  * One new token per sequence over such pools: q and o [B, Hq, D].  sel with sel_off (both NULL: every page) as for sa_decode,
  * [B, sel_rows] lists (sel_rows Hq or Hkv; strides of the batch may be 0) whose offsets are clamped to sel_width entries; a listed page that
- * is past the table, outside the pool or past kv_lens[b] adds no key.  A sequence without keys gets zeros.  num_splits
- * (1..64): the longest list that the sizes allow (sel_width pages, or max_blocks) is shared by that many workgroups, and
- * every list by as many as its own length needs of the same share; more than 1 needs
- * sa_decode_q4_workspace_bytes(B, Hq, D, num_splits) bytes, 16-byte aligned, which concurrent calls must not share.
+ * is past the table, outside the pool or past kv_lens[b] adds no key.  A sequence without keys gets zeros.  num_splits: how
+ * many workgroups share the longest list that the sizes allow (sel_width pages, or max_blocks), and every list as many as
+ * its own length needs of the same share.  0: worked out, over whole caches on the device from the lengths; 1: one; up to
+ * 64.  Partial results take sa_decode_q4_workspace_bytes() bytes where that is not 0 (rows: sel_rows, or Hkv without lists;
+ * max_keys: sel_width or max_blocks times page, at most 2^30; selected: whether there are lists), 16-byte aligned, contents arbitrary,
+ * which calls that may run concurrently must not share.
  */
 int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh,
                  const void* k_pages, const void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,
@@ -643,7 +645,7 @@ int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh,
                  const int32_t* sel_off, int64_t off_sb, int64_t off_sr, int sel_rows,
                  void* o, int64_t o_sb, int64_t o_sh, int B, int Hq, int Hkv, int D, int page, float sm_scale,
                  int num_splits, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t sa_decode_q4_workspace_bytes(int B, int Hq, int D, int num_splits);
+int64_t sa_decode_q4_workspace_bytes(int B, int Hq, int rows, int D, int max_keys, int selected, int num_splits);
 
 #ifdef __cplusplus
 }

@@ -233,7 +233,7 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32, _f32,
         _i32, _vp, _i64, _vp,
     ]),
-    "sa_decode_q4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "sa_decode_q4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
 }
 
 

@@ -93,6 +93,49 @@ struct Q4Window {
 template <bool BF16>
 constexpr float Q4_REFIT = BF16 ? 65536.f : 32768.f;
 
+// The codes of a chunk's keys and values as they come from memory, and their pairs: those of key l % 16 and group l / 16
+// (of those that there are), which change lanes through LDS.
+template <int D>
+struct Q4Chunk {
+  using F = Kv4<D>;
+  static constexpr int NG = F::NG;
+  Words<NG> k, v;
+  uint32_t ks, vs;
+  int key;
+
+  __device__ __forceinline__ void load(const Q4Keys& keys, const Q4Window& w, int step, int h) {
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int slot = w.slot_of(step, h);
+    const int64_t off = w.off_of(step, h);
+    key = w.key_of(step, h);
+    const uint8_t *kb = keys.k + off, *vb = keys.v + off;
+    k.load(kb + slot * F::ROW + (i * F::ROW + 4 * NG * q));
+    v.load(vb + slot * F::ROW + (q * F::QUAD + 4 * NG * i));
+    const int st = F::stats_at(keys.page) + 4 * slot + 4 * (min(q, NG - 1) * keys.page + i);
+    ks = *reinterpret_cast<const uint32_t*>(kb + st);
+    vs = *reinterpret_cast<const uint32_t*>(vb + st);
+  }
+};
+
+// A step's pairs in a wave's own LDS, [keys, values][chunk][NG][16]; accesses of one wave run in order.
+template <int D>
+struct Q4Pairs {
+  static constexpr int NG = Kv4<D>::NG, WORDS = 4 * 16 * NG;
+  uint32_t* at;
+  __device__ __forceinline__ void put(const Q4Chunk<D> (&ch)[2], int end) const {
+    const int lane = threadIdx.x & 63;
+    if (lane < 16 * NG)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        at[16 * NG * h + lane] = ch[h].ks;
+        // 0 times what a slot without a token holds is 0
+        at[16 * NG * (2 + h) + lane] = ch[h].key + (lane & 15) < end ? ch[h].vs : 0u;
+      }
+  }
+  __device__ __forceinline__ const uint32_t* keys(int h, int g) const { return at + 16 * (NG * h + g); }
+  __device__ __forceinline__ const uint32_t* values(int h, int g) const { return at + 16 * (NG * (2 + h) + g); }
+};
+
 // 16 NC rows of queries.  Keys and values are brought to the element type in registers: m + s c in fp32, one rounding.
 template <bool BF16, int D, int NC>
 struct Q4Dequant {
@@ -100,34 +143,15 @@ struct Q4Dequant {
   using F = Kv4<D>;
   static constexpr int NG = F::NG, NE = D / 16;
 
-  static constexpr int LDS_WORDS = 4 * 16 * NG;    // of a wave: pairs of a step's keys and values, [chunk][NG][16] each
+  using Chunk = Q4Chunk<D>;
 
-  struct Chunk {
-    Words<NG> k, v;
-    uint32_t ks, vs;               // the pair of key l % 16 and group l / 16 (those that there are)
-    int key;
-  };
-
-  uint32_t* pairs;                 // LDS_WORDS of LDS of the wave's own
+  Q4Pairs<D> pairs;
   u32x4 qf[NC][NG];
   int pos[NC];                     // position of the lane's row
   int pos_min;                     // of all rows
   f32x4 O[NC][NE];
   float m_ref[NC], l_run[NC];      // base-2 reference; sum of the lane's probabilities
   bool ref_ok;
-
-  static __device__ __forceinline__ void load(Chunk& c, const Q4Keys& ks, const Q4Window& w, int step, int h) {
-    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    const int slot = w.slot_of(step, h);
-    const int64_t off = w.off_of(step, h);
-    c.key = w.key_of(step, h);
-    const uint8_t *kb = ks.k + off, *vb = ks.v + off;
-    c.k.load(kb + slot * F::ROW + (i * F::ROW + 4 * NG * q));
-    c.v.load(vb + slot * F::ROW + (q * F::QUAD + 4 * NG * i));
-    const int st = F::stats_at(ks.page) + 4 * slot + 4 * (min(q, NG - 1) * ks.page + i);
-    c.ks = *reinterpret_cast<const uint32_t*>(kb + st);
-    c.vs = *reinterpret_cast<const uint32_t*>(vb + st);
-  }
 
   __device__ __forceinline__ void start() {
 #pragma unroll
@@ -161,14 +185,7 @@ struct Q4Dequant {
 
   __device__ __forceinline__ void step(const Chunk (&ch)[2], int end, float scale) {
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    // The pairs change lanes through LDS, whose accesses by one wave run in order.
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (q < NG) {
-        const bool live = ch[h].key + i < end;     // 0 times what a slot without a token holds is 0
-        pairs[(16 * NG) * h + lane] = ch[h].ks;
-        pairs[(16 * NG) * (2 + h) + lane] = live ? ch[h].vs : 0u;
-      }
+    pairs.put(ch, end);
     f32x4 S[NC][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -176,7 +193,7 @@ struct Q4Dequant {
       for (int c = 0; c < NC; ++c) S[c][h] = f32x4{};
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t st = pairs[(16 * NG) * h + 16 * g + i];
+        const uint32_t st = pairs.keys(h, g)[i];
         const float s = q4_scale<BF16>(st), m = q4_min<BF16>(st);
         const uint32_t lo = q4_low(ch[h].k.w[g]), hi = q4_high(ch[h].k.w[g]);
         const u32x4 kf = {E::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
@@ -228,7 +245,7 @@ struct Q4Dequant {
       float s[2][4], m[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const u32x4 st = *reinterpret_cast<const u32x4*>(pairs + (16 * NG) * (2 + h) + 16 * g + 4 * q);
+        const u32x4 st = *reinterpret_cast<const u32x4*>(pairs.values(h, g) + 4 * q);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[h][j] = q4_scale<BF16>(st[j]), m[h][j] = q4_min<BF16>(st[j]);
       }
@@ -267,12 +284,9 @@ struct Q4Fold {
   static constexpr int ROWS = RPS * NQ;
   static constexpr float REFIT = 65536.f;
 
-  struct Chunk {
-    Words<NG> k, v;
-    u32x4 ks, vs;                                  // pairs of the lane's group, keys 4 q .. + 3
-    int key;
-  };
+  using Chunk = Q4Chunk<D>;
 
+  Q4Pairs<D> pairs;
   u32x4 qz[NQ][NG];
   float qsum[NQ];                                  // of the lane's group and row
   int pos[NQ];                                     // position of the lane's row
@@ -284,19 +298,6 @@ struct Q4Fold {
 
   static __device__ __forceinline__ int group_of(int lane) { return (lane & 15) / RPS; }
   static __device__ __forceinline__ int row_of(int lane) { return (lane & 15) % RPS; }
-
-  static __device__ __forceinline__ void load(Chunk& c, const Q4Keys& ks, const Q4Window& w, int step, int h) {
-    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    const int slot = w.slot_of(step, h);
-    const int64_t off = w.off_of(step, h);
-    c.key = w.key_of(step, h);
-    const uint8_t *kb = ks.k + off, *vb = ks.v + off;
-    c.k.load(kb + slot * F::ROW + (i * F::ROW + 4 * NG * q));
-    c.v.load(vb + slot * F::ROW + (q * F::QUAD + 4 * NG * i));
-    const int st = F::stats_at(ks.page) + 4 * slot, of_lane = 4 * group_of(lane) * ks.page + 16 * q;
-    c.ks = *reinterpret_cast<const u32x4*>(kb + st + of_lane);
-    c.vs = *reinterpret_cast<const u32x4*>(vb + st + of_lane);
-  }
 
   // The lane's row of set x: its query from element 0 on, and its position.
   __device__ __forceinline__ void set_query(int x, const elem_t* row, int position) {
@@ -355,7 +356,8 @@ struct Q4Fold {
   }
 
   __device__ __forceinline__ void step(const Chunk (&ch)[2], int end, float scale) {
-    const int lane = threadIdx.x & 63, q = lane >> 4;
+    const int lane = threadIdx.x & 63, q = lane >> 4, group = group_of(lane);
+    pairs.put(ch, end);
     f32x4 S[NQ][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -369,9 +371,10 @@ struct Q4Fold {
 #pragma unroll
         for (int x = 0; x < NQ; ++x) S[x][h] = E::mfma16(kf, qz[x][g], S[x][h]);
       }
+      const u32x4 ks = *reinterpret_cast<const u32x4*>(pairs.keys(h, group) + 4 * q);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float s = q4_scale<BF16>(ch[h].ks[j]), m = q4_min<BF16>(ch[h].ks[j]);
+        const float s = q4_scale<BF16>(ks[j]), m = q4_min<BF16>(ks[j]);
 #pragma unroll
         for (int x = 0; x < NQ; ++x) S[x][h][j] = over_groups<SUM>(fmaf(s, S[x][h][j], m * qsum[x]));
       }
@@ -414,12 +417,7 @@ struct Q4Fold {
     u32x4 P[NQ], R[NQ];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4 vs = ch[h].vs;
-      if (ch[h].key + 16 > end) {                  // 0 times what a slot without a token holds is 0
-        const int live = end - ch[h].key - 4 * q;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vs[j] = j < live ? vs[j] : 0u;
-      }
+      const u32x4 vs = *reinterpret_cast<const u32x4*>(pairs.values(h, group) + 4 * q);
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         const float s0 = q4_scale<BF16>(vs[j]), s1 = q4_scale<BF16>(vs[j + 1]);
@@ -486,8 +484,8 @@ __device__ __forceinline__ void q4_run(W& wave, const Q4Keys& ks, float scale) {
   typename W::Chunk a[2], b[2];
   auto fetch = [&](typename W::Chunk (&ch)[2], int s) {
     if (s - w.base >= 32) w.fill(ks, s);
-    W::load(ch[0], ks, w, s, 0);
-    W::load(ch[1], ks, w, s, 1);
+    ch[0].load(ks, w, s, 0);
+    ch[1].load(ks, w, s, 1);
   };
   fetch(a, 0);
 #pragma unroll 1

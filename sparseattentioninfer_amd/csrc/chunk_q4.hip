@@ -53,7 +53,7 @@ struct ChunkQ4 {
     using W = Q4Dequant<BF16, D, NC>;
     const int lane = threadIdx.x & 63;
     W w;
-    w.pairs = pairs;
+    w.pairs.at = pairs;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const elem_t* qs = query(a, it, 16 * c + (lane & 15), w.pos[c]) + 8 * (lane >> 4);
@@ -80,10 +80,11 @@ struct ChunkQ4 {
   // Up to Q4Fold::ROWS rows, by codes.
   template <int NQ>
   static __device__ __forceinline__ void folded(const ChunkQ4Args& a, const ChunkItem& it, const Q4Keys& ks, int pos_min,
-                                                char* acc, float* ml) {
+                                                char* acc, float* ml, uint32_t* pairs) {
     using W = Q4Fold<BF16, D, NQ>;
     const int lane = threadIdx.x & 63;
     W w;
+    w.pairs.at = pairs;
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       int pos;
@@ -93,6 +94,7 @@ struct ChunkQ4 {
     w.pos_min = pos_min;
     w.start();
     q4_run(w, ks, a.c.scale_log2);
+    __syncthreads();               // the pairs lie where the accumulators go
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const int r = x * W::RPS + W::row_of(lane);
@@ -118,12 +120,12 @@ struct ChunkQ4 {
     const int rows = it.row_end - it.row0;
     char* acc = s_acc + wave * ACC;
     float* ml = s_ml + 2 * CK_ROWS * wave;
-    uint32_t* pairs = reinterpret_cast<uint32_t*>(s_acc) + wave * Q4Dequant<BF16, D, 2>::LDS_WORDS;
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(s_acc) + wave * Q4Pairs<D>::WORDS;
     constexpr int SET = Q4Fold<BF16, D, 1>::RPS;
     if (rows <= SET) {
-      folded<1>(a, it, ks, pos_min, acc, ml);
+      folded<1>(a, it, ks, pos_min, acc, ml, pairs);
     } else if (rows <= 2 * SET) {
-      folded<2>(a, it, ks, pos_min, acc, ml);
+      folded<2>(a, it, ks, pos_min, acc, ml, pairs);
     } else if (2 * SET < 16 && rows <= 16) {
       scaled<1>(a, it, ks, pos_min, acc, ml, pairs);
     } else {

@@ -3,9 +3,11 @@
 //
 //   o = sum_j softmax_j(q . k_j * scale) v_j over the kept keys below kv_len; fp32 statistics and accumulators
 //
-// A workgroup has the query heads of one list (up to 8 at D = 128, 16 at 64) and `unit` steps of 32 keys of it, which its four waves take in
-// turn; a longer list is shared by workgroups whose fp32 partials a second kernel merges.  The unit is the same for every
-// sequence, so the workgroups' loads are even whatever the lengths, and those past a sequence's end leave at once.
+// A workgroup has the query heads of one list (up to 8 at D = 128, 16 at 64) and `unit` steps of 32 keys of it, which its
+// four waves take in turn; a longer list is shared by workgroups whose fp32 partials a second kernel merges.  The unit is
+// the same for all lists, so the workgroups' loads are even whatever the lengths.  Over whole caches every workgroup works
+// it out for itself, an even share of all steps for each of DQ_TARGET workgroups, and finds its list by a scan of the
+// lengths: the launch is as large as any lengths need, and what is past the last list leaves at once.
 #include <algorithm>
 
 #include "attn_q4.h"
@@ -13,6 +15,8 @@
 namespace sa {
 
 constexpr int DQ_WAVES = 4;
+constexpr int DQ_TARGET = 512;     // workgroups that a planned division aims at: two to a CU
+constexpr int DQ_MIN_UNIT = 8;     // steps of a workgroup of a planned division, two for each wave
 
 struct DecodeQ4Args {
   const elem_t* q;
@@ -34,24 +38,94 @@ struct DecodeQ4Args {
   elem_t* o;
   int64_t o_sb, o_sh;
   int B, Hq;
-  int unit, splits;                // steps of a workgroup; most workgroups of a list
-  float* part;                     // [splits, B, Hq, D], then [splits, B, Hq, 2] (splits > 1)
+  int unit;                        // steps of a workgroup; 0: planned
+  int splits;                      // with lists: workgroups of each
+  float* part;                     // NULL: no list is shared; else of workgroup x and its head r [x, r, D], ...
+  float* part_ml;                  // ... and row reference and sum [x, r, 2]
   float scale_log2;
 
-  // Chunks of 16 keys of list `row` of sequence b.
-  __device__ __forceinline__ int chunks(int b, int row, const int32_t*& list, int& len) const {
-    len = min(max(kv_lens[b], 0), MAX_KV_LEN);
-    const int last = (int)min((int64_t)len, (int64_t)max_blocks * page);
-    list = nullptr;
-    if (!sel_off) return (last + 15) / 16;
-    const int32_t* off = sel_off + b * off_sb + row * off_sr;
-    const int e0 = min(max(off[0], 0), sel_width), e1 = min(max(off[1], e0), sel_width);
-    list = sel + b * sel_sb + row * sel_sr + e0;
-    return last > 0 ? (e1 - e0) * (page / 16) : 0;
+  __device__ __forceinline__ int length(int b) const { return min(max(kv_lens[b], 0), MAX_KV_LEN); }
+  // Steps of a whole cache of `len` tokens, as far as the table goes.
+  __device__ __forceinline__ int steps(int len) const {
+    return ((int)min((int64_t)len, (int64_t)max_blocks * page) + 31) / 32;
   }
-  // Workgroups that share `chunks` chunks.
-  __device__ __forceinline__ int splits_of(int chunks) const {
-    return max(1, ((chunks + 1) / 2 + unit - 1) / unit);
+};
+
+// Which list a workgroup has, and which share of it.
+struct DecodeQ4Item {
+  int b, row, tile, len;
+  int split, splits;
+  int unit;
+  int first;                       // workgroup of the list's and tile's first share
+
+  // Workgroup x.  False if there is none.
+  __device__ __forceinline__ bool find(const DecodeQ4Args& a, int x) {
+    const int of_seq = a.rows * a.tiles;
+    if (a.sel_off) {
+      unit = a.unit;
+      splits = a.splits;
+      const int per = of_seq * splits;
+      b = x / per;
+      if (b >= a.B) return false;
+      set(a, x - b * per, x);
+      len = a.length(b);
+      return true;
+    }
+    const int lane = threadIdx.x & 63;
+    const int len64 = lane < a.B ? a.length(lane) : 0;
+    plan(a, len64, of_seq);
+    auto count = [&](int s) { return shares(a.steps(s < 64 ? len64 : a.length(s))) * of_seq; };
+    int local;
+    if (!find_item(a.B, x, count, b, local)) return false;
+    len = a.length(b);
+    splits = shares(a.steps(len));
+    set(a, local, x);
+    return true;
+  }
+  // The shares of list `row`'s tile `t` of sequence s (whole caches): splits and first.
+  __device__ __forceinline__ void of_list(const DecodeQ4Args& a, int s, int r, int t) {
+    const int of_seq = a.rows * a.tiles;
+    b = s, row = r, tile = t;
+    if (a.sel_off) {
+      splits = a.splits;
+      first = ((s * a.rows + r) * a.tiles + t) * splits;
+      return;
+    }
+    const int lane = threadIdx.x & 63;
+    const int len64 = lane < a.B ? a.length(lane) : 0;
+    plan(a, len64, of_seq);
+    first = 0;
+    for (int b0 = 0; b0 <= s; b0 += 64) {
+      const int l = b0 ? (b0 + lane < a.B ? a.length(b0 + lane) : 0) : len64;
+      const int k = b0 + lane < a.B ? shares(a.steps(l)) : 0, incl = scan_lanes(k);
+      if (s < b0 + 64) {
+        splits = __builtin_amdgcn_readlane(k, s - b0);
+        first += __builtin_amdgcn_readlane(incl, s - b0) - splits;
+      } else {
+        first += __builtin_amdgcn_readlane(incl, 63);
+      }
+    }
+    first = first * of_seq + (r * a.tiles + t) * splits;
+  }
+
+ private:
+  __device__ __forceinline__ int shares(int steps) const { return max(1, (steps + unit - 1) / unit); }
+  __device__ __forceinline__ void set(const DecodeQ4Args& a, int local, int x) {
+    split = local % splits;
+    const int l = local / splits;
+    tile = l % a.tiles;
+    row = l / a.tiles;
+    first = x - split;
+  }
+  // Sums in fp32, with a margin above their rounding: no more than DQ_TARGET shares beyond one for each list.
+  __device__ __forceinline__ void plan(const DecodeQ4Args& a, int len64, int of_seq) {
+    unit = a.unit;
+    if (unit) return;
+    const int lane = threadIdx.x & 63;
+    float sum = (float)a.steps(len64);
+    for (int s = 64 + lane; s < a.B; s += 64) sum += (float)a.steps(a.length(s));
+    sum = wave_sum(sum) * (float)of_seq;
+    unit = max(DQ_MIN_UNIT, (int)ceilf(sum * (1.001f / DQ_TARGET)));
   }
 };
 
@@ -61,28 +135,32 @@ struct DecodeQ4 {
   using Rows = Q4Fold<BF16, D, NQ>;
   static constexpr int ROWS = Rows::ROWS;
   static constexpr int ACC = ROWS * D * 4;
+  static_assert(ACC >= 4 * Q4Pairs<D>::WORDS, "the pairs lie in the accumulators' LDS");
 
   static __device__ void run(const DecodeQ4Args& a, char* s_acc, float* s_ml) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int x = blockIdx.x;
-    const int tile = x % a.tiles;
-    x /= a.tiles;
-    const int row = x % a.rows;
-    x /= a.rows;
-    const int b = x % a.B, split = x / a.B;
-    int len;
-    const int32_t* list;
-    const int chunks = a.chunks(b, row, list, len);
-    const int n = a.splits_of(chunks);
-    if (split >= n) return;
-    const int head0 = row * a.heads + tile * ROWS, live = min(ROWS, a.heads - tile * ROWS);
+    DecodeQ4Item it;
+    if (!it.find(a, blockIdx.x)) return;
+    const int b = it.b, row = it.row, len = it.len;
+    // Chunks of 16 keys of the list.
+    const int last = (int)min((int64_t)len, (int64_t)a.max_blocks * a.page);
+    int chunks = (last + 15) / 16;
+    const int32_t* list = nullptr;
+    if (a.sel_off) {
+      const int32_t* off = a.sel_off + b * a.off_sb + row * a.off_sr;
+      const int e0 = min(max(off[0], 0), a.sel_width), e1 = min(max(off[1], e0), a.sel_width);
+      list = a.sel + b * a.sel_sb + row * a.sel_sr + e0;
+      chunks = last > 0 ? (e1 - e0) * (a.page / 16) : 0;
+    }
+    const int head0 = row * a.heads + it.tile * ROWS, live = min(ROWS, a.heads - it.tile * ROWS);
     Rows w;
 #pragma unroll
     for (int x = 0; x < NQ; ++x)
       w.set_query(x, a.q + b * a.q_sb + (head0 + min(x * Rows::RPS + Rows::row_of(lane), live - 1)) * a.q_sh, len - 1);
     w.pos_min = len - 1;
     w.start();
+    w.pairs.at = reinterpret_cast<uint32_t*>(s_acc) + wave * Q4Pairs<D>::WORDS;
     Q4Keys ks;
     const int kvh = row / a.group;
     ks.k = a.k + kvh * a.sh;
@@ -92,11 +170,12 @@ struct DecodeQ4 {
     ks.list = list;
     ks.max_blocks = a.max_blocks, ks.num_pages = a.num_pages, ks.page = a.page;
     ks.mul_page = a.mul_page, ks.mul_ppc = a.mul_ppc;
-    ks.c0 = 2 * a.unit * split;
-    ks.c1 = min(chunks, ks.c0 + 2 * a.unit);
+    ks.c0 = min(chunks, 2 * it.unit * it.split);
+    ks.c1 = min(chunks, ks.c0 + 2 * it.unit);
     ks.end = len, ks.pos_max = len - 1;
     ks.wave = wave, ks.waves = DQ_WAVES;
     q4_run(w, ks, a.scale_log2);
+    __syncthreads();               // the pairs lie where the accumulators go
     // Merge in fp32: row r is D floats at r * 4 D, its 16-byte chunk x at position x ^ (r % (D / 4)).
     constexpr int NC4 = D / 4, OC = D / 8;
 #pragma unroll
@@ -133,15 +212,14 @@ struct DecodeQ4 {
         hi += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc + 1) ^ (r & (NC4 - 1))));
       }
       const int h = head0 + r;
-      if (n > 1) {
-        const int64_t at = ((int64_t)split * a.B + b) * a.Hq + h;
+      if (it.splits > 1) {
+        const int64_t at = (int64_t)blockIdx.x * ROWS + r;
         f32x4* d = reinterpret_cast<f32x4*>(a.part + at * D + 8 * oc);
         d[0] = lo;
         d[1] = hi;
         if (oc == 0) {
-          float* ml = a.part + (int64_t)a.splits * a.B * a.Hq * D + 2 * at;
-          ml[0] = M;
-          ml[1] = l;
+          a.part_ml[2 * at] = M;
+          a.part_ml[2 * at + 1] = l;
         }
       } else {
         const float inv = l > 0.f ? 1.f / l : 1.f;
@@ -161,52 +239,67 @@ static __global__ __launch_bounds__(64 * DQ_WAVES, NQ == 1 ? 3 : 2) void decode_
   K::run(a, s_acc, s_ml);
 }
 
-// Merges the partials of the query heads of lists that were shared, D / 8 lanes a head.
+// Merges the partials of a query head whose list was shared: a workgroup a head, D / 8 lanes a share, 2048 / D shares at a
+// time.
 template <bool BF16, int D>
-static __global__ __launch_bounds__(256) void decode_q4_combine_kernel(const DecodeQ4Args a) {
+static __global__ __launch_bounds__(256) void decode_q4_combine_kernel(const DecodeQ4Args a, int per_tile) {
   using E = Elem<BF16>;
-  constexpr int LPR = D / 8, U = 4;
-  const int x = (int)blockIdx.x * (256 / LPR) + (int)threadIdx.x / LPR, oc = threadIdx.x % LPR;
-  if (x >= a.B * a.Hq) return;
-  const int b = x / a.Hq, h = x - b * a.Hq;
-  int len;
-  const int32_t* list;
-  const int n = a.splits_of(a.chunks(b, h / a.heads, list, len));
-  if (n <= 1) return;
-  const int64_t step = (int64_t)a.B * a.Hq;
-  const float* ml = a.part + (int64_t)a.splits * step * D;
+  constexpr int LPR = D / 8, SH = 256 / LPR;
+  __shared__ __attribute__((aligned(16))) float s_acc[4][D + 4];
+  const int x = blockIdx.x, b = x / a.Hq, h = x - b * a.Hq;
+  const int oc = threadIdx.x % LPR, sh = threadIdx.x / LPR, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  DecodeQ4Item it;
+  const int row = h / a.heads, r = h - row * a.heads;
+  it.of_list(a, b, row, r / per_tile);
+  if (it.splits <= 1) return;
+  const int64_t at = (int64_t)it.first * per_tile + r % per_tile;
   float M = -__builtin_inff(), L = 0.f;
   f32x4 acc[2] = {f32x4{}, f32x4{}};
-  for (int s0 = 0; s0 < n; s0 += U) {
-    float m[U], l[U];
-    f32x4 v[U][2];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t p = x + min(s0 + u, n - 1) * step;   // past the last: a repeat, not used
-      m[u] = ml[2 * p];
-      l[u] = ml[2 * p + 1];
-      v[u][0] = reinterpret_cast<const f32x4*>(a.part + p * D + 8 * oc)[0];
-      v[u][1] = reinterpret_cast<const f32x4*>(a.part + p * D + 8 * oc)[1];
-    }
-    float Mc = M;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s0 + u < n) Mc = fmaxf(Mc, m[u]);
+  for (int s = sh; s < it.splits; s += SH) {
+    const int64_t p = at + (int64_t)s * per_tile;
+    const float m = a.part_ml[2 * p], l = a.part_ml[2 * p + 1];
+    const f32x4* v = reinterpret_cast<const f32x4*>(a.part + p * D + 8 * oc);
+    const f32x4 v0 = v[0], v1 = v[1];
     // As in chunk_items.h: a share of NaN scores has sums of NaN, which reach the row.
-    const float Mu = Mc == -__builtin_inff() ? 0.f : Mc;
-    const float f0 = fast_exp2(M - Mu);
-    L *= f0;
-    acc[0] *= f0;
-    acc[1] *= f0;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s0 + u < n) {
-        const float fs = fast_exp2(m[u] - Mu);
-        L += fs * l[u];
-        acc[0] += fs * v[u][0];
-        acc[1] += fs * v[u][1];
-      }
+    const float Mc = fmaxf(M, m), Mu = Mc == -__builtin_inff() ? 0.f : Mc;
+    const float f0 = fast_exp2(M - Mu), f1 = fast_exp2(m - Mu);
+    L = L * f0 + l * f1;
+    acc[0] = acc[0] * f0 + v0 * f1;
+    acc[1] = acc[1] * f0 + v1 * f1;
     M = Mc;
+  }
+  // Over the shares of a wave, then of the four waves, in a fixed order.
+#pragma unroll
+  for (int o = LPR; o < 64; o <<= 1) {
+    const float m = __shfl_xor(M, o, 64), l = __shfl_xor(L, o, 64);
+    const float Mc = fmaxf(M, m), Mu = Mc == -__builtin_inff() ? 0.f : Mc;
+    const float f0 = fast_exp2(M - Mu), f1 = fast_exp2(m - Mu);
+    L = L * f0 + l * f1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[k][e] = acc[k][e] * f0 + __shfl_xor(acc[k][e], o, 64) * f1;
+    M = Mc;
+  }
+  if (lane < LPR) {
+    f32x4* d = reinterpret_cast<f32x4*>(&s_acc[wave][8 * oc]);
+    d[0] = acc[0];
+    d[1] = acc[1];
+    if (lane == 0) s_acc[wave][D] = M, s_acc[wave][D + 1] = L;
+  }
+  __syncthreads();
+  if (threadIdx.x >= LPR) return;
+  M = fmaxf(fmaxf(s_acc[0][D], s_acc[1][D]), fmaxf(s_acc[2][D], s_acc[3][D]));
+  const float Mu = M == -__builtin_inff() ? 0.f : M;
+  L = 0.f;
+  acc[0] = acc[1] = f32x4{};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = fast_exp2(s_acc[w][D] - Mu);
+    const f32x4* d = reinterpret_cast<const f32x4*>(&s_acc[w][8 * oc]);
+    L += f * s_acc[w][D + 1];
+    acc[0] += f * d[0];
+    acc[1] += f * d[1];
   }
   const float inv = L > 0.f ? 1.f / L : 1.f;
   *reinterpret_cast<u32x4*>(a.o + b * a.o_sb + h * a.o_sh + 8 * oc) =
@@ -220,23 +313,53 @@ static int launch_decode_q4(const DecodeQ4Args& a, int64_t groups, int sets, hip
     hipLaunchKernelGGL((decode_q4_kernel<BF16, D, 1>), dim3((unsigned)groups), dim3(64 * DQ_WAVES), 0, s, a);
   else
     hipLaunchKernelGGL((decode_q4_kernel<BF16, D, 2>), dim3((unsigned)groups), dim3(64 * DQ_WAVES), 0, s, a);
-  if (a.splits > 1) {
-    const int per = 256 / (D / 8);
-    hipLaunchKernelGGL((decode_q4_combine_kernel<BF16, D>), dim3((unsigned)((a.B * a.Hq + per - 1) / per)), dim3(256), 0, s, a);
-  }
+  if (a.part)
+    hipLaunchKernelGGL((decode_q4_combine_kernel<BF16, D>), dim3((unsigned)(a.B * a.Hq)), dim3(256), 0, s, a, sets * 16 / (D / 32));
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? 0 : set_error((int)err, "sa_decode_q4: launch failed: %s", hipGetErrorString(err));
 }
 
-// Steps of 32 keys of the longest list.
-static int64_t decode_q4_steps(int64_t blocks, int page) { return std::max<int64_t>(1, (std::min<int64_t>(blocks * page, MAX_KV_LEN) + 31) / 32); }
+// Sizes of a launch.
+struct DecodeQ4Plan {
+  int sets, tiles;                 // column sets of a workgroup; workgroups that share the query heads of a list
+  int unit, splits;                // as in DecodeQ4Args; splits 1: nothing is shared
+  int64_t groups, bytes;           // workgroups; bytes of partials
+
+  DecodeQ4Plan(int B, int Hq, int rows, int D, int64_t keys, bool lists, int num_splits) {
+    const int per_set = 16 / (D / 32), heads = Hq / rows;
+    sets = heads > per_set ? 2 : 1;
+    tiles = (heads + sets * per_set - 1) / (sets * per_set);
+    const int64_t of = (int64_t)B * rows * tiles;
+    const int64_t steps = std::max<int64_t>(1, (std::min<int64_t>(keys, MAX_KV_LEN) + 31) / 32);
+    unit = (int)steps;
+    groups = of;
+    // Sharing up to 16 steps costs more than it saves: the merge is 3 us, and four waves have 4 steps each.  (16 lists of 16
+    // steps, D = 64: 6.9 us in one, 7.7 in two; 8 of 32, D = 128: 11.6 in one, 8.5 in 4.)
+    if (num_splits == 0 && steps > 16) {
+      if (lists) {
+        // Their lengths are taken to be about those of the longest.
+        num_splits = (int)std::max<int64_t>(1, std::min<int64_t>({64, DQ_TARGET / of, steps / DQ_MIN_UNIT}));
+      } else {
+        unit = 0;
+        groups = of + DQ_TARGET;
+      }
+    }
+    if (num_splits > 1) {
+      unit = (int)((steps + num_splits - 1) / num_splits);
+      groups = of * ((steps + unit - 1) / unit);
+    }
+    splits = unit ? (int)((steps + unit - 1) / unit) : 2;
+    bytes = splits > 1 ? groups * sets * per_set * (D + 2) * 4 : 0;
+  }
+};
 
 }  // namespace sa
 
 using namespace sa;
 
-extern "C" int64_t sa_decode_q4_workspace_bytes(int B, int Hq, int D, int num_splits) {
-  return num_splits > 1 && B > 0 && Hq > 0 && D > 0 ? (int64_t)num_splits * B * Hq * (D + 2) * 4 : 0;
+extern "C" int64_t sa_decode_q4_workspace_bytes(int B, int Hq, int rows, int D, int max_keys, int selected, int num_splits) {
+  if (B < 1 || Hq < 1 || rows < 1 || Hq % rows || (D != 64 && D != 128) || num_splits < 0) return 0;
+  return DecodeQ4Plan(B, Hq, rows, D, max_keys, selected != 0, num_splits).bytes;
 }
 
 extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
@@ -254,9 +377,9 @@ extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh
   if (page < 16 || page > 128 || page % 16)
     return set_error(SA_E_BLOCK, "%s: page %d is not a multiple of 16 in [16, 128]", name, page);
   if (B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > (1 << 15) || max_blocks < 0 || num_pages < 0 ||
-      block_table_stride < max_blocks || num_splits < 1 || num_splits > 64)
+      block_table_stride < max_blocks || num_splits < 0 || num_splits > 64)
     return set_error(SA_E_SHAPE, "%s: bad sizes B=%d Hq=%d Hkv=%d, table of %d columns (stride %lld), %d pages, "
-                     "%d splits (1..64)", name, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages, num_splits);
+                     "%d splits (0..64)", name, B, Hq, Hkv, max_blocks, (long long)block_table_stride, num_pages, num_splits);
   if (!(sm_scale >= 1e-30f && sm_scale <= 1e30f))
     return set_error(SA_E_SHAPE, "%s: scale %g is not in [1e-30, 1e30]", name, sm_scale);
   if (sel_off && sel_rows != Hq && sel_rows != Hkv)
@@ -273,13 +396,12 @@ extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh
     return set_error(SA_E_ALIGN, "%s: head rows and blocks must be 16-byte aligned", name);
   DecodeQ4Args a = {};
   a.max_blocks = num_pages ? max_blocks : 0;      // without pages no key is there, and none is loaded
-  const int64_t steps = decode_q4_steps(sel_off ? sel_width : a.max_blocks, page);
-  a.unit = (int)((steps + num_splits - 1) / num_splits);
-  a.splits = (int)((steps + a.unit - 1) / a.unit);
-  const int64_t need = sa_decode_q4_workspace_bytes(B, Hq, D, a.splits);
-  if (need && (!workspace || workspace_bytes < need))
+  a.rows = sel_off ? sel_rows : Hkv;
+  const int64_t keys = std::min<int64_t>((int64_t)(sel_off ? sel_width : max_blocks) * page, MAX_KV_LEN);
+  const DecodeQ4Plan plan(B, Hq, a.rows, D, keys, sel_off != nullptr, num_splits);
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
     return set_error(SA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", name, (long long)workspace_bytes,
-                     (long long)need);
+                     (long long)plan.bytes);
   a.q = static_cast<const elem_t*>(q);
   a.q_sb = q_sb, a.q_sh = q_sh;
   a.k = static_cast<const uint8_t*>(k_pages);
@@ -295,19 +417,22 @@ extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh
   a.sel_sb = sel_sb, a.sel_sr = sel_sr, a.sel_width = sel_width;
   a.sel_off = sel_off;
   a.off_sb = off_sb, a.off_sr = off_sr;
-  a.rows = sel_off ? sel_rows : Hkv;
   a.heads = Hq / a.rows;
   a.group = a.rows / Hkv;
-  // Query heads of a workgroup: one column set, or two.
-  const int per_set = 16 / (D / 32), sets = a.heads > per_set ? 2 : 1;
-  a.tiles = (a.heads + sets * per_set - 1) / (sets * per_set);
+  a.tiles = plan.tiles;
+  a.unit = plan.unit, a.splits = plan.splits;
   a.o = static_cast<elem_t*>(o);
   a.o_sb = o_sb, a.o_sh = o_sh;
   a.B = B, a.Hq = Hq;
-  a.part = static_cast<float*>(workspace);
+  const int per_tile = plan.sets * 16 / (D / 32);
+  if (plan.bytes) {
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + plan.groups * per_tile * D;
+  }
   a.scale_log2 = sm_scale * 1.44269504088896340736f;
-  const int64_t groups = (int64_t)B * a.rows * a.tiles * a.splits;
-  if (groups > MAX_WORKGROUPS || (int64_t)B * Hq > 0x7fffffff / 2)
+  const int64_t groups = plan.groups;
+  const int sets = plan.sets;
+  if (groups > MAX_WORKGROUPS || (int64_t)B * Hq > MAX_WORKGROUPS)
     return set_error(SA_E_SHAPE, "%s: %lld workgroups are too many for one launch", name, (long long)groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == SA_DTYPE_BF16)

@@ -1291,12 +1291,6 @@ def paged_chunk_attn_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     return out
 
 
-def decode_q4_splits(B: int, rows: int, steps: int) -> int:
-    """Workgroups that share the longest list of a :func:`paged_sparse_decode_q4` call, ``steps`` steps of 32 keys, where it
-    has ``B * rows`` lists."""
-    return max(1, min(64, -(-1024 // max(1, B * rows)), steps // 8))
-
-
 def paged_sparse_decode_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                            kv_lens: torch.Tensor, sel: torch.Tensor | None = None, sel_off: torch.Tensor | None = None, *,
                            num_splits: int = 0, workspace: torch.Tensor | None = None,
@@ -1307,9 +1301,9 @@ def paged_sparse_decode_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     :func:`paged_append_q4` writes them for the type of ``q``; ``block_table [B, max_blocks]``, ``kv_lens [B]``, ``sel
     [B, R, max_sel]`` and ``sel_off [B, R, 2]`` (R = Hq or Hkv) int32 as for :func:`paged_sparse_decode`; without ``sel`` and
     ``sel_off`` the whole cache is attended.  ``num_splits`` workgroups (at most 64) share the longest list that the sizes allow
-    and other lists as many as their lengths need of the same share; ``0`` picks the number from the sizes
-    (:func:`decode_q4_splits`).  More than one takes a byte workspace of ``sa_decode_q4_workspace_bytes`` (allocated if
-    omitted), which concurrent calls must not share.  A sequence without keys gets zeros.
+    and other lists as many as their lengths need of the same share; by default the share is worked out, over whole caches
+    on the device from the lengths.  Partial results take a byte workspace (allocated if omitted), which concurrent calls
+    must not share.  A sequence without keys gets zeros.
     """
     name = "paged_sparse_decode_q4"
     q3 = q.reshape(q.shape[0], q.shape[1], q.shape[-1]) if q.dim() == 4 else q
@@ -1341,9 +1335,8 @@ def paged_sparse_decode_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                    other="q and out must be [B, Hq, D] with Hq a multiple of the pools' heads, block_table [B, max_blocks], "
                          "sel and sel_off (both or neither) [B, Hq or Hkv, width] and [B, Hq or Hkv, 2]")
     Hq, D = qs[1], qs[2]
-    if num_splits == 0:
-        num_splits = decode_q4_splits(B, R, -(-width * page // 32))
-    ws = _workspace(name, workspace, _lib.load().sa_decode_q4_workspace_bytes(B, Hq, D, num_splits), dev)
+    ws = _workspace(name, workspace, _lib.load().sa_decode_q4_workspace_bytes(
+        B, Hq, R, D, min(width * page, 1 << 30), sel is not None, num_splits), dev)
     ost = out.stride()
     _call("sa_decode_q4", dev.index, _DTYPES[dt], q3.data_ptr(), qst[0], qst[1], k_pages.data_ptr(), v_pages.data_ptr(),
           k_pages.stride(0), k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0), block_table.size(1),

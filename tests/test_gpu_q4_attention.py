@@ -3,7 +3,7 @@ holds: lengths, pages, groups and lists where it can go wrong.  Slots without a 
 import pytest
 import torch
 
-from sparseattentioninfer_amd import ops
+from sparseattentioninfer_amd import _lib, ops
 from tests.chunk_reference import randn
 from tests.q4_reference import Q4Ragged, assert_attention, pack, unpack
 
@@ -187,6 +187,13 @@ def test_decode_splits(splits, D, dtype):
     _decode([5000, 700, 1, 0, 2048], 64, 8, 2, D, dtype, splits=splits)
 
 
+@pytest.mark.parametrize("B", [70, 130])
+def test_decode_many_sequences(B):
+    """More sequences than lanes of a wave, of uneven lengths."""
+    _say("decode many", B)
+    _decode([(1, 2000, 0, 65, 700, 33)[b % 6] for b in range(B)], 64, 4, 1, 64, HF)
+
+
 @pytest.mark.parametrize("rows", [2, 8])
 @pytest.mark.parametrize("splits", [0, 3])
 @pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
@@ -294,7 +301,8 @@ def test_other_stream_and_workspaces():
     q = randn(2, 8, 128, seed=7)
     args = (q.cuda(), *_cache(r), r.kv_lens.cuda())
     want = ops.paged_sparse_decode_q4(*args, num_splits=7)
-    ws = torch.full((int(2 * 8 * 130 * 4 * 7),), 255, dtype=torch.uint8, device="cuda")
+    need = _lib.load().sa_decode_q4_workspace_bytes(2, 8, 2, 128, r.table.size(1) * 64, 0, 7)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):

@@ -131,7 +131,7 @@ def _decode(lib, **o):
 
 @pytest.mark.parametrize("change,code,text", [
     (dict(dtype=7), -1, b"dtype 7"), (dict(D=32), -3, b"head dim 32"), (dict(page=136), -4, b"page 136"),
-    (dict(Hq=9), -2, b"Hq=9"), (dict(mb=5), -2, b"5 columns"), (dict(splits=65), -2, b"65 splits"), (dict(splits=0), -2, b"0 splits"),
+    (dict(Hq=9), -2, b"Hq=9"), (dict(mb=5), -2, b"5 columns"), (dict(splits=65), -2, b"65 splits"), (dict(splits=-1), -2, b"-1 splits"),
     (dict(scale=-1.0), -2, b"scale"), (dict(off=FAKE, sel=FAKE, rows=3, width=4), -5, b"sel_rows=3"),
     (dict(sel=FAKE), -2, b"selection"), (dict(off=FAKE, sel=FAKE, rows=2, width=-1), -2, b"selection"),
     (dict(off=FAKE, rows=2, width=4), -6, b"NULL"), (dict(lens=None), -6, b"NULL"), (dict(kp=None), -6, b"NULL"),
@@ -142,8 +142,11 @@ def test_decode_refusals(lib, change, code, text):
 
 def test_decode_nothing_to_do(lib):
     assert _decode(lib, B=0, q=None) == 0
-    assert lib.sa_decode_q4_workspace_bytes(2, 4, 128, 3) == 3 * 2 * 4 * 130 * 4
-    assert lib.sa_decode_q4_workspace_bytes(2, 4, 128, 1) == 0
+    # 4 heads a workgroup at D = 128: 2 sequences, 2 lists, 3 shares; none in one share, nor of short lists
+    assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 3) == 2 * 2 * 3 * 4 * 130 * 4
+    assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 1) == 0
+    assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 512, 0, 0) == 0
+    assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 0) > 0
 
 
 def test_attention_refuses_cpu_tensors():
