@@ -6,8 +6,7 @@
 // A workgroup has the query heads of one list (up to 8 at D = 128, 16 at 64) and `unit` steps of 32 keys of it, which its
 // four waves take in turn; a longer list is shared by workgroups whose fp32 partials a second kernel merges.  The unit is
 // the same for all lists, so the workgroups' loads are even whatever the lengths.  Over whole caches every workgroup works
-// it out for itself, an even share of all steps for each of DQ_TARGET workgroups, and finds its list by a scan of the
-// lengths: the launch is as large as any lengths need, and what is past the last list leaves at once.
+// it out for itself and finds its list by a scan of the lengths: the launch is as large as any lengths need, and what is past the last list leaves at once.
 #include <algorithm>
 
 #include "attn_q4.h"
@@ -15,8 +14,10 @@
 namespace sa {
 
 constexpr int DQ_WAVES = 4;
-constexpr int DQ_TARGET = 512;     // workgroups that a planned division aims at: two to a CU
+constexpr int DQ_TARGET = 512;     // workgroups that run at once, two to a CU
 constexpr int DQ_MIN_UNIT = 8;     // steps of a workgroup of a planned division, two for each wave
+constexpr int DQ_MOST = 1344;      // workgroups that a planned division adds to one for each list: DQ_TARGET / 0.381
+constexpr float DQ_START = 8.f;    // what a workgroup costs besides its steps, in steps: 4 us of 0.5
 
 struct DecodeQ4Args {
   const elem_t* q;
@@ -42,6 +43,7 @@ struct DecodeQ4Args {
   int splits;                      // with lists: workgroups of each
   float* part;                     // NULL: no list is shared; else of workgroup x and its head r [x, r, D], ...
   float* part_ml;                  // ... and row reference and sum [x, r, 2]
+  int* planned;                    // the planned unit, written by the launch's first workgroup for the merge
   float scale_log2;
 
   __device__ __forceinline__ int length(int b) const { return min(max(kv_lens[b], 0), MAX_KV_LEN); }
@@ -93,7 +95,7 @@ struct DecodeQ4Item {
     }
     const int lane = threadIdx.x & 63;
     const int len64 = lane < a.B ? a.length(lane) : 0;
-    plan(a, len64, of_seq);
+    unit = a.unit ? a.unit : *a.planned;
     first = 0;
     for (int b0 = 0; b0 <= s; b0 += 64) {
       const int l = b0 ? (b0 + lane < a.B ? a.length(b0 + lane) : 0) : len64;
@@ -117,15 +119,54 @@ struct DecodeQ4Item {
     row = l / a.tiles;
     first = x - split;
   }
-  // Sums in fp32, with a margin above their rounding: no more than DQ_TARGET shares beyond one for each list.
+  // The unit of a planned division: of no division, an even share of all steps and 0.76, 0.5 and 0.381 of it the one that
+  // ends first.  While the shares run at once that is when the longest ends; else the mean load and half the longest.
+  // (Equal lists are best left whole or cut evenly, uneven ones finely: 28 sequences of 64 to 30,000 tokens, 8 KV heads,
+  // 141 us with even shares, 114 with 0.38 of one; 64 of 4,096 67 us whole, 79 in two.)  Sums are fp32; the margin
+  // above their rounding keeps the shares within DQ_MOST.
   __device__ __forceinline__ void plan(const DecodeQ4Args& a, int len64, int of_seq) {
     unit = a.unit;
     if (unit) return;
     const int lane = threadIdx.x & 63;
-    float sum = (float)a.steps(len64);
-    for (int s = 64 + lane; s < a.B; s += 64) sum += (float)a.steps(a.length(s));
-    sum = wave_sum(sum) * (float)of_seq;
-    unit = max(DQ_MIN_UNIT, (int)ceilf(sum * (1.001f / DQ_TARGET)));
+    const float of = (float)of_seq;
+    const int n64 = a.steps(len64);
+    float sum = (float)n64, longest = (float)n64;
+    for (int s = 64 + lane; s < a.B; s += 64) {
+      const float n = (float)a.steps(a.length(s));
+      sum += n;
+      longest = fmaxf(longest, n);
+    }
+    sum = wave_sum(sum) * of;
+    longest = wave_max(longest);
+    const float even = sum * (1.001f / DQ_TARGET);
+    int u[5];
+    float groups[5], share[5];
+    auto weigh = [&](int c, float n) {
+      const float k = fmaxf(1.f, ceilf(n * __builtin_amdgcn_rcpf((float)u[c])));
+      groups[c] += n > 0.f ? k : 0.f;
+      share[c] = fmaxf(share[c], n * __builtin_amdgcn_rcpf(k));
+    };
+#pragma unroll
+    for (int c = 0; c < 5; ++c) {
+      const float f = c == 1 ? 1.f : c == 2 ? 0.76f : c == 3 ? 0.5f : 0.381f;
+      u[c] = c ? max(DQ_MIN_UNIT, (int)ceilf(even * f)) : max(1, (int)longest);
+      groups[c] = share[c] = 0.f;
+      weigh(c, (float)n64);
+    }
+    for (int s = 64 + lane; s < a.B; s += 64) {
+      const float n = (float)a.steps(a.length(s));
+#pragma unroll
+      for (int c = 0; c < 5; ++c) weigh(c, n);
+    }
+    float best = __builtin_inff();
+#pragma unroll
+    for (int c = 0; c < 5; ++c) {
+      const float g = wave_sum(groups[c]) * of, h = wave_max(share[c]) + DQ_START;
+      const float time = g <= DQ_TARGET ? h : (sum + g * DQ_START) * (1.f / DQ_TARGET) + 0.5f * h;
+      unit = time < best ? u[c] : unit;
+      best = fminf(time, best);
+    }
+    unit = __builtin_amdgcn_readfirstlane(unit);
   }
 };
 
@@ -142,6 +183,7 @@ struct DecodeQ4 {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     DecodeQ4Item it;
     if (!it.find(a, blockIdx.x)) return;
+    if (a.planned && blockIdx.x == 0 && threadIdx.x == 0) *a.planned = it.unit;
     const int b = it.b, row = it.row, len = it.len;
     // Chunks of 16 keys of the list.
     const int last = (int)min((int64_t)len, (int64_t)a.max_blocks * a.page);
@@ -323,7 +365,8 @@ static int launch_decode_q4(const DecodeQ4Args& a, int64_t groups, int sets, hip
 struct DecodeQ4Plan {
   int sets, tiles;                 // column sets of a workgroup; workgroups that share the query heads of a list
   int unit, splits;                // as in DecodeQ4Args; splits 1: nothing is shared
-  int64_t groups, bytes;           // workgroups; bytes of partials
+  int64_t groups, bytes;           // workgroups; bytes of the planned unit and the partials
+  static constexpr int HEADER = 64;
 
   DecodeQ4Plan(int B, int Hq, int rows, int D, int64_t keys, bool lists, int num_splits) {
     const int per_set = 16 / (D / 32), heads = Hq / rows;
@@ -341,7 +384,7 @@ struct DecodeQ4Plan {
         num_splits = (int)std::max<int64_t>(1, std::min<int64_t>({64, DQ_TARGET / of, steps / DQ_MIN_UNIT}));
       } else {
         unit = 0;
-        groups = of + DQ_TARGET;
+        groups = std::min(of + DQ_MOST, of * ((steps + DQ_MIN_UNIT - 1) / DQ_MIN_UNIT));
       }
     }
     if (num_splits > 1) {
@@ -349,7 +392,7 @@ struct DecodeQ4Plan {
       groups = of * ((steps + unit - 1) / unit);
     }
     splits = unit ? (int)((steps + unit - 1) / unit) : 2;
-    bytes = splits > 1 ? groups * sets * per_set * (D + 2) * 4 : 0;
+    bytes = splits > 1 ? HEADER + groups * sets * per_set * (D + 2) * 4 : 0;
   }
 };
 
@@ -426,7 +469,8 @@ extern "C" int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh
   a.B = B, a.Hq = Hq;
   const int per_tile = plan.sets * 16 / (D / 32);
   if (plan.bytes) {
-    a.part = static_cast<float*>(workspace);
+    a.planned = plan.unit ? nullptr : static_cast<int*>(workspace);
+    a.part = static_cast<float*>(workspace) + DecodeQ4Plan::HEADER / 4;
     a.part_ml = a.part + plan.groups * per_tile * D;
   }
   a.scale_log2 = sm_scale * 1.44269504088896340736f;

@@ -143,7 +143,7 @@ def test_decode_refusals(lib, change, code, text):
 def test_decode_nothing_to_do(lib):
     assert _decode(lib, B=0, q=None) == 0
     # 4 heads a workgroup at D = 128: 2 sequences, 2 lists, 3 shares; none in one share, nor of short lists
-    assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 3) == 2 * 2 * 3 * 4 * 130 * 4
+    assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 3) == 64 + 2 * 2 * 3 * 4 * 130 * 4
     assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 1) == 0
     assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 512, 0, 0) == 0
     assert lib.sa_decode_q4_workspace_bytes(2, 8, 2, 128, 6400, 0, 0) > 0
