@@ -1,5 +1,5 @@
-// Attention of one wave over keys held in 4 bits (gfx950): keys and values go from memory to the operands of
-// v_mfma 16x16x32 in registers, without LDS.
+// Attention of one wave over keys held in 4 bits (gfx950): codes go from memory to the operands of v_mfma 16x16x32 by way
+// of LDS of the wave's own, without a barrier and without a change of lanes.
 //
 // A step is 32 keys, two chunks of 16 that each lie in one page.  S^T = K Q^T: keys are the rows of the product, so a lane
 // of column n holds scores of row n of the queries for four keys of each chunk, and those of both chunks are, as they lie,
@@ -93,59 +93,89 @@ struct Q4Window {
 template <bool BF16>
 constexpr float Q4_REFIT = BF16 ? 65536.f : 32768.f;
 
-// The codes of a chunk's keys and values as they come from memory, and their pairs: those of key l % 16 and group l / 16
-// (of those that there are), which change lanes through LDS.
-template <int D>
-struct Q4Chunk {
+// A wave's steps on their way: a ring of DEPTH steps of codes and pairs in LDS of its own, filled by direct loads.  The
+// loads of the DEPTH - 1 steps ahead are in flight while one is worked on, without registers of their own.
+template <int D, int DEPTH>
+struct Q4Ring {
   using F = Kv4<D>;
   static constexpr int NG = F::NG;
-  Words<NG> k, v;
-  uint32_t ks, vs;
-  int key;
+  static constexpr int CODES = 16 * F::ROW, PAIRS = 64 * NG;       // bytes of a chunk's keys (or values)
+  static constexpr int STEP = 4 * (CODES + PAIRS);                 // [keys, values][chunk] codes, then so the pairs
+  static constexpr int BYTES = DEPTH * STEP;
+  static constexpr int LOADS = NG == 4 ? 8 : 4;                    // direct loads of a step
+  char* lds;
 
-  __device__ __forceinline__ void load(const Q4Keys& keys, const Q4Window& w, int step, int h) {
+  __device__ __forceinline__ void issue(const Q4Keys& keys, const Q4Window& w, int step, int slot) const {
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    const int slot = w.slot_of(step, h);
-    const int64_t off = w.off_of(step, h);
-    key = w.key_of(step, h);
-    const uint8_t *kb = keys.k + off, *vb = keys.v + off;
-    k.load(kb + slot * F::ROW + (i * F::ROW + 4 * NG * q));
-    v.load(vb + slot * F::ROW + (q * F::QUAD + 4 * NG * i));
-    const int st = F::stats_at(keys.page) + 4 * slot + 4 * (min(q, NG - 1) * keys.page + i);
-    ks = *reinterpret_cast<const uint32_t*>(kb + st);
-    vs = *reinterpret_cast<const uint32_t*>(vb + st);
-  }
-};
-
-// A step's pairs in a wave's own LDS, [keys, values][chunk][NG][16]; accesses of one wave run in order.
-template <int D>
-struct Q4Pairs {
-  static constexpr int NG = Kv4<D>::NG, WORDS = 4 * 16 * NG;
-  uint32_t* at;
-  __device__ __forceinline__ void put(const Q4Chunk<D> (&ch)[2], int end) const {
-    const int lane = threadIdx.x & 63;
-    if (lane < 16 * NG)
+    const uint32_t at = lds_addr(lds + slot * STEP), pairs_at = at + 4 * CODES;
+    if constexpr (NG == 4) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        at[16 * NG * h + lane] = ch[h].ks;
-        // 0 times what a slot without a token holds is 0
-        at[16 * NG * (2 + h) + lane] = ch[h].key + (lane & 15) < end ? ch[h].vs : 0u;
+        const int s = w.slot_of(step, h);
+        const int64_t off = w.off_of(step, h) + s * F::ROW;
+        const uint8_t *kb = keys.k + off, *vb = keys.v + off;
+        const int st = F::stats_at(keys.page) + s * (4 - F::ROW);
+        load_lds16(kb, i * F::ROW + 16 * q, at + h * CODES);
+        load_lds16(vb, q * F::QUAD + 16 * i, at + (2 + h) * CODES);
+        load_lds4(kb + st, 4 * (q * keys.page + i), pairs_at + h * PAIRS);
+        load_lds4(vb + st, 4 * (q * keys.page + i), pairs_at + (2 + h) * PAIRS);
       }
+    } else {
+      // Half a wave holds a chunk: both chunks in one load.
+      const int h = lane >> 5, s0 = w.slot_of(step, 0), s1 = w.slot_of(step, 1);
+      const int64_t o0 = w.off_of(step, 0), o1 = w.off_of(step, 1);
+      const int s = h ? s1 : s0;
+      const int64_t off = (h ? o1 : o0) + s * F::ROW + 16 * (lane & 31);
+      const int64_t st = (h ? o1 : o0) + F::stats_at(keys.page) + 4 * (s + (q & 1) * keys.page + i);
+      load_lds16(keys.k + off, at);
+      load_lds16(keys.v + off, at + 2 * CODES);
+      load_lds4(keys.k + st, pairs_at);
+      load_lds4(keys.v + st, pairs_at + 2 * PAIRS);
+    }
   }
-  __device__ __forceinline__ const uint32_t* keys(int h, int g) const { return at + 16 * (NG * h + g); }
-  __device__ __forceinline__ const uint32_t* values(int h, int g) const { return at + 16 * (NG * (2 + h) + g); }
+  // The lane's words of chunk h.
+  __device__ __forceinline__ Words<NG> keys(int slot, int h) const {
+    const int lane = threadIdx.x & 63;
+    Words<NG> x;
+    x.load(reinterpret_cast<const uint8_t*>(lds) + slot * STEP + h * CODES +
+           (NG == 4 ? 16 * lane : (lane & 15) * F::ROW + 8 * (lane >> 4)));
+    return x;
+  }
+  __device__ __forceinline__ Words<NG> values(int slot, int h) const {
+    const int lane = threadIdx.x & 63;
+    Words<NG> x;
+    x.load(reinterpret_cast<const uint8_t*>(lds) + slot * STEP + (2 + h) * CODES +
+           (NG == 4 ? 16 * lane : (lane >> 4) * F::QUAD + 8 * (lane & 15)));
+    return x;
+  }
+  // Pairs of group g: of key i of the chunk, and of keys 4 q .. + 3.
+  __device__ __forceinline__ uint32_t key_pair(int slot, int h, int g, int i) const {
+    return reinterpret_cast<const uint32_t*>(lds + slot * STEP + 4 * CODES + h * PAIRS)[16 * g + i];
+  }
+  __device__ __forceinline__ u32x4 key_pairs(int slot, int h, int g, int q) const {
+    return *reinterpret_cast<const u32x4*>(lds + slot * STEP + 4 * CODES + h * PAIRS + 64 * g + 16 * q);
+  }
+  // (0 times what a slot without a token holds is 0)
+  __device__ __forceinline__ u32x4 value_pairs(int slot, int h, int g, int q, int key, int end) const {
+    u32x4 x = *reinterpret_cast<const u32x4*>(lds + slot * STEP + 4 * CODES + (2 + h) * PAIRS + 64 * g + 16 * q);
+    if (key + 16 > end) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = key + 4 * q + j < end ? x[j] : 0u;
+    }
+    return x;
+  }
 };
 
 // 16 NC rows of queries.  Keys and values are brought to the element type in registers: m + s c in fp32, one rounding.
-template <bool BF16, int D, int NC>
+template <bool BF16, int D, int NC, int DEPTH>
 struct Q4Dequant {
   using E = Elem<BF16>;
   using F = Kv4<D>;
   static constexpr int NG = F::NG, NE = D / 16;
 
-  using Chunk = Q4Chunk<D>;
+  static constexpr int STEPS = DEPTH;
 
-  Q4Pairs<D> pairs;
+  Q4Ring<D, DEPTH> ring;
   u32x4 qf[NC][NG];
   int pos[NC];                     // position of the lane's row
   int pos_min;                     // of all rows
@@ -183,19 +213,21 @@ struct Q4Dequant {
     }
   }
 
-  __device__ __forceinline__ void step(const Chunk (&ch)[2], int end, float scale) {
+  // A step whose codes and pairs are in `slot` of the ring, of two chunks from keys key0 and key1 on.
+  __device__ __forceinline__ void step(int slot, int key0, int key1, int end, float scale) {
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    pairs.put(ch, end);
+    const int key[2] = {key0, key1};
     f32x4 S[NC][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const Words<NG> kw = ring.keys(slot, h);
 #pragma unroll
       for (int c = 0; c < NC; ++c) S[c][h] = f32x4{};
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t st = pairs.keys(h, g)[i];
+        const uint32_t st = ring.key_pair(slot, h, g, i);
         const float s = q4_scale<BF16>(st), m = q4_min<BF16>(st);
-        const uint32_t lo = q4_low(ch[h].k.w[g]), hi = q4_high(ch[h].k.w[g]);
+        const uint32_t lo = q4_low(kw.w[g]), hi = q4_high(kw.w[g]);
         const u32x4 kf = {E::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
                           E::pack2f(fmaf(q4_code<2>(lo), s, m), fmaf(q4_code<3>(lo), s, m)),
                           E::pack2f(fmaf(q4_code<0>(hi), s, m), fmaf(q4_code<1>(hi), s, m)),
@@ -203,10 +235,10 @@ struct Q4Dequant {
 #pragma unroll
         for (int c = 0; c < NC; ++c) S[c][h] = E::mfma16(kf, qf[c][g], S[c][h]);
       }
-      if (ch[h].key + 15 > pos_min) {              // keys past a row's position
+      if (key[h] + 15 > pos_min) {              // keys past a row's position
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const int lim = pos[c] - ch[h].key - 4 * q;
+          const int lim = pos[c] - key[h] - 4 * q;
 #pragma unroll
           for (int j = 0; j < 4; ++j) S[c][h][j] = j > lim ? -__builtin_inff() : S[c][h][j];
         }
@@ -240,12 +272,13 @@ struct Q4Dequant {
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) l_run[c] += ls[c];
+    const Words<NG> vw[2] = {ring.values(slot, 0), ring.values(slot, 1)};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float s[2][4], m[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const u32x4 st = *reinterpret_cast<const u32x4*>(pairs.values(h, g) + 4 * q);
+        const u32x4 st = ring.value_pairs(slot, h, g, q, key[h], end);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[h][j] = q4_scale<BF16>(st[j]), m[h][j] = q4_min<BF16>(st[j]);
       }
@@ -254,7 +287,7 @@ struct Q4Dequant {
         u32x4 vf;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t x = half ? q4_high(ch[h].v.w[g]) : q4_low(ch[h].v.w[g]);
+          const uint32_t x = half ? q4_high(vw[h].w[g]) : q4_low(vw[h].w[g]);
           vf[2 * h] = E::pack2f(fmaf(q4_code<0>(x), s[h][0], m[h][0]), fmaf(q4_code<1>(x), s[h][1], m[h][1]));
           vf[2 * h + 1] = E::pack2f(fmaf(q4_code<2>(x), s[h][2], m[h][2]), fmaf(q4_code<3>(x), s[h][3], m[h][3]));
         }
@@ -275,7 +308,7 @@ struct Q4Dequant {
 // What rounds: p s, once, to bf16.  Codes lie in 0 .. 15, so that would weigh with up to 15 s where half of it is the
 // values' own; sum_t (p s) 7.5, of the rounded products (a row of ones more in the matrix product), is taken out
 // and put back from the unrounded ones.  For fp16 the product is split in two bf16 parts instead, 16 bits in all.
-template <bool BF16, int D, int NQ>
+template <bool BF16, int D, int NQ, int DEPTH>
 struct Q4Fold {
   using E = Elem<BF16>;
   using F = Kv4<D>;
@@ -284,9 +317,9 @@ struct Q4Fold {
   static constexpr int ROWS = RPS * NQ;
   static constexpr float REFIT = 65536.f;
 
-  using Chunk = Q4Chunk<D>;
+  static constexpr int STEPS = DEPTH;
 
-  Q4Pairs<D> pairs;
+  Q4Ring<D, DEPTH> ring;
   u32x4 qz[NQ][NG];
   float qsum[NQ];                                  // of the lane's group and row
   int pos[NQ];                                     // position of the lane's row
@@ -355,33 +388,34 @@ struct Q4Fold {
     return op(x, dpp<0x128>(x));                       // row_ror:8
   }
 
-  __device__ __forceinline__ void step(const Chunk (&ch)[2], int end, float scale) {
+  __device__ __forceinline__ void step(int slot, int key0, int key1, int end, float scale) {
     const int lane = threadIdx.x & 63, q = lane >> 4, group = group_of(lane);
-    pairs.put(ch, end);
+    const int key[2] = {key0, key1};
     f32x4 S[NQ][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const Words<NG> kw = ring.keys(slot, h);
 #pragma unroll
       for (int x = 0; x < NQ; ++x) S[x][h] = f32x4{};
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t lo = q4_low(ch[h].k.w[g]), hi = q4_high(ch[h].k.w[g]);
+        const uint32_t lo = q4_low(kw.w[g]), hi = q4_high(kw.w[g]);
         const u32x4 kf = BF16 ? u32x4{q4_pair_bf16<false>(lo), q4_pair_bf16<true>(lo), q4_pair_bf16<false>(hi), q4_pair_bf16<true>(hi)}
                               : u32x4{q4_pair_f16<false>(lo), q4_pair_f16<true>(lo), q4_pair_f16<false>(hi), q4_pair_f16<true>(hi)};
 #pragma unroll
         for (int x = 0; x < NQ; ++x) S[x][h] = E::mfma16(kf, qz[x][g], S[x][h]);
       }
-      const u32x4 ks = *reinterpret_cast<const u32x4*>(pairs.keys(h, group) + 4 * q);
+      const u32x4 ks = ring.key_pairs(slot, h, group, q);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float s = q4_scale<BF16>(ks[j]), m = q4_min<BF16>(ks[j]);
 #pragma unroll
         for (int x = 0; x < NQ; ++x) S[x][h][j] = over_groups<SUM>(fmaf(s, S[x][h][j], m * qsum[x]));
       }
-      if (ch[h].key + 15 > pos_min) {              // keys past a row's position
+      if (key[h] + 15 > pos_min) {              // keys past a row's position
 #pragma unroll
         for (int x = 0; x < NQ; ++x) {
-          const int lim = pos[x] - ch[h].key - 4 * q;
+          const int lim = pos[x] - key[h] - 4 * q;
 #pragma unroll
           for (int j = 0; j < 4; ++j) S[x][h][j] = j > lim ? -__builtin_inff() : S[x][h][j];
         }
@@ -417,7 +451,7 @@ struct Q4Fold {
     u32x4 P[NQ], R[NQ];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const u32x4 vs = *reinterpret_cast<const u32x4*>(pairs.values(h, group) + 4 * q);
+      const u32x4 vs = ring.value_pairs(slot, h, group, q, key[h], end);
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         const float s0 = q4_scale<BF16>(vs[j]), s1 = q4_scale<BF16>(vs[j + 1]);
@@ -436,6 +470,7 @@ struct Q4Fold {
         }
       }
     }
+    const Words<NG> vw[2] = {ring.values(slot, 0), ring.values(slot, 1)};
     constexpr uint32_t ONE2 = 0x3f803f80u;
 #pragma unroll
     for (int x = 0; x < NQ; ++x)
@@ -447,7 +482,7 @@ struct Q4Fold {
         u32x4 vf;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t c = half ? q4_high(ch[h].v.w[g]) : q4_low(ch[h].v.w[g]);
+          const uint32_t c = half ? q4_high(vw[h].w[g]) : q4_low(vw[h].w[g]);
           vf[2 * h] = q4_pair_bf16<false>(c);
           vf[2 * h + 1] = q4_pair_bf16<true>(c);
         }
@@ -474,27 +509,29 @@ struct Q4Fold {
   }
 };
 
-// All steps of the wave; the loads of the next are in flight during one.
+// All steps of the wave.
 template <class W>
 __device__ __forceinline__ void q4_run(W& wave, const Q4Keys& ks, float scale) {
+  constexpr int DEPTH = W::STEPS, LOADS = decltype(wave.ring)::LOADS;
   const int ns = ks.steps();
   if (ns == 0) return;
   Q4Window w;
   w.fill(ks, 0);
-  typename W::Chunk a[2], b[2];
-  auto fetch = [&](typename W::Chunk (&ch)[2], int s) {
-    if (s - w.base >= 32) w.fill(ks, s);
-    ch[0].load(ks, w, s, 0);
-    ch[1].load(ks, w, s, 1);
-  };
-  fetch(a, 0);
+  for (int s = 0; s < min(ns, DEPTH - 1); ++s) wave.ring.issue(ks, w, s, s);
+  int slot = 0;
 #pragma unroll 1
-  for (int s = 0; s < ns; s += 2) {
-    if (s + 1 < ns) fetch(b, s + 1);
-    wave.step(a, ks.end, scale);
-    if (s + 1 >= ns) break;
-    if (s + 2 < ns) fetch(a, s + 2);
-    wave.step(b, ks.end, scale);
+  for (int s = 0; s < ns; ++s) {
+    const int ahead = s + DEPTH - 1;
+    if (ahead < ns) {
+      if (ahead - w.base >= 32) w.fill(ks, s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the slot's last step has been read
+      wave.ring.issue(ks, w, ahead, slot == 0 ? DEPTH - 1 : slot - 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"((DEPTH - 1) * LOADS) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    wave.step(slot, w.key_of(s, 0), w.key_of(s, 1), ks.end, scale);
+    slot = slot == DEPTH - 1 ? 0 : slot + 1;
   }
 }
 

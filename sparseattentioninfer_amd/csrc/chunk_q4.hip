@@ -17,6 +17,8 @@ struct ChunkQ4 {
   static constexpr int NW = 8;
   static constexpr int ACC = CK_ROWS * D * 4;
   static constexpr int LDS_BYTES = NW * ACC;
+  static constexpr int DEPTH = 3;
+  static_assert(ACC >= Q4Ring<D, DEPTH>::BYTES, "the waves' rings lie in the accumulators' LDS");
 
   static __device__ __forceinline__ Q4Keys keys_of(const ChunkQ4Args& a, const ChunkItem& it) {
     Q4Keys ks;
@@ -49,11 +51,11 @@ struct ChunkQ4 {
   // Up to 16 NC rows, by scaled keys and values.
   template <int NC>
   static __device__ __forceinline__ void scaled(const ChunkQ4Args& a, const ChunkItem& it, const Q4Keys& ks, int pos_min,
-                                                char* acc, float* ml, uint32_t* pairs) {
-    using W = Q4Dequant<BF16, D, NC>;
+                                                char* acc, float* ml, char* ring) {
+    using W = Q4Dequant<BF16, D, NC, DEPTH>;
     const int lane = threadIdx.x & 63;
     W w;
-    w.pairs.at = pairs;
+    w.ring.lds = ring;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const elem_t* qs = query(a, it, 16 * c + (lane & 15), w.pos[c]) + 8 * (lane >> 4);
@@ -63,7 +65,7 @@ struct ChunkQ4 {
     w.pos_min = pos_min;
     w.start();
     q4_run(w, ks, a.c.scale_log2);
-    __syncthreads();               // the pairs lie where the accumulators go
+    __syncthreads();               // the rings lie where the accumulators go
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int r = 16 * c + (lane & 15);
@@ -80,11 +82,11 @@ struct ChunkQ4 {
   // Up to Q4Fold::ROWS rows, by codes.
   template <int NQ>
   static __device__ __forceinline__ void folded(const ChunkQ4Args& a, const ChunkItem& it, const Q4Keys& ks, int pos_min,
-                                                char* acc, float* ml, uint32_t* pairs) {
-    using W = Q4Fold<BF16, D, NQ>;
+                                                char* acc, float* ml, char* ring) {
+    using W = Q4Fold<BF16, D, NQ, DEPTH>;
     const int lane = threadIdx.x & 63;
     W w;
-    w.pairs.at = pairs;
+    w.ring.lds = ring;
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       int pos;
@@ -94,7 +96,7 @@ struct ChunkQ4 {
     w.pos_min = pos_min;
     w.start();
     q4_run(w, ks, a.c.scale_log2);
-    __syncthreads();               // the pairs lie where the accumulators go
+    __syncthreads();               // the rings lie where the accumulators go
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const int r = x * W::RPS + W::row_of(lane);
@@ -120,16 +122,16 @@ struct ChunkQ4 {
     const int rows = it.row_end - it.row0;
     char* acc = s_acc + wave * ACC;
     float* ml = s_ml + 2 * CK_ROWS * wave;
-    uint32_t* pairs = reinterpret_cast<uint32_t*>(s_acc) + wave * Q4Pairs<D>::WORDS;
-    constexpr int SET = Q4Fold<BF16, D, 1>::RPS;
+    char* ring = s_acc + wave * Q4Ring<D, DEPTH>::BYTES;
+    constexpr int SET = Q4Fold<BF16, D, 1, DEPTH>::RPS;
     if (rows <= SET) {
-      folded<1>(a, it, ks, pos_min, acc, ml, pairs);
+      folded<1>(a, it, ks, pos_min, acc, ml, ring);
     } else if (rows <= 2 * SET) {
-      folded<2>(a, it, ks, pos_min, acc, ml, pairs);
+      folded<2>(a, it, ks, pos_min, acc, ml, ring);
     } else if (2 * SET < 16 && rows <= 16) {
-      scaled<1>(a, it, ks, pos_min, acc, ml, pairs);
+      scaled<1>(a, it, ks, pos_min, acc, ml, ring);
     } else {
-      scaled<2>(a, it, ks, pos_min, acc, ml, pairs);
+      scaled<2>(a, it, ks, pos_min, acc, ml, ring);
     }
     // Merge in fp32.
     __syncthreads();
@@ -255,24 +257,14 @@ struct ChunkQ4Wide : StagedTile {
     }
   };
 
-  // A lane's words of a tile and their pairs.  Keys: token 8 (wave % 2) + l / 4 % 8 of the wave's chunk, words NWD p + u of
-  // quarter l % 4, p = l / 32.  Values: tokens 8 (wave % 2) + 4 (l % 2) .. + 3, dims l / 2 % 16 of the groups NWD p + u.
+  // A lane's words of a tile and their pairs.
   struct KeyWords {
     uint32_t w[NWD], st[NWD];
   };
   struct ValueWords {
     uint32_t w[NWD];
-    u32x4 st[NWD];
+    u32x4 st;
   };
-
-  static __device__ __forceinline__ void load_words(uint32_t (&w)[NWD], const uint8_t* p) {
-    if constexpr (NWD == 2) {
-      const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-      w[0] = v[0], w[1] = v[1];
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-  }
 
   // A operand of O^T = V^T P^T: lane l holds d = 32 dt + l % 32 of keys 32 j + 16 h + 8 (l / 32) + 0..7.
   static __device__ __forceinline__ u32x4 vtfrag(const char* cV, int v0, int swz, int j, int h, int dt) {
@@ -308,14 +300,17 @@ struct ChunkQ4Wide : StagedTile {
     const int rb = wave >> 1;
     const uint8_t* kh = x.k + it.kvh * x.sh;
     const uint8_t* vh = x.v + it.kvh * x.sh;
+    // Keys: words NWD p + u of quarter kq of a token.
     const int ktok = 8 * (wave & 1) + ((lane >> 2) & 7), kq = lane & 3, p = lane >> 5;
-    const int vtok = 8 * (wave & 1) + 4 * (lane & 1), vi = (lane >> 1) & 15;
+    // Values: four tokens of one group vg; at D = 128 its dims vi and vi + 8 of both halves, at 64 dim vi.
+    const int vtok = 8 * (wave & 1) + 4 * (lane & 1);
+    const int vi = NWD == 2 ? (lane >> 1) & 7 : (lane >> 1) & 15, vg = NWD == 2 ? lane >> 4 : lane >> 5;
     const int k_at = ktok * F::ROW + 4 * F::NG * kq + 4 * NWD * p;
-    const int v_at = (vtok >> 2) * F::QUAD + 4 * F::NG * vi + 4 * NWD * p;
+    const int v_at = (vtok >> 2) * F::QUAD + 4 * F::NG * vi + 4 * vg;
     const int stats = F::stats_at(a.page);
     const int krow16 = krow(ktok);
     char* const lds_k = sK + rb * 1024 + krow16 * 64 + 16 * (kq ^ ((krow16 >> 2) & 3)) + 4096 * NWD * p;
-    char* const lds_v = sV + (32 * NWD * p + vi) * 128 + 16 * (wave ^ (vi & 7)) + 8 * (lane & 1);
+    char* const lds_v = sV + (32 * vg + vi) * 128 + 16 * (wave ^ (vi & 7)) + 8 * (lane & 1);
     Window w;
     KeyWords kw;
     ValueWords vw;
@@ -323,7 +318,12 @@ struct ChunkQ4Wide : StagedTile {
       if (t - w.base >= 64) w.fill(a, it, x.sp, t - AHEAD, rb, s_keys);
       const uint8_t* b = kh + w.off_of(t);
       const int slot = w.slot_of(t), key = w.key_of(t);
-      load_words(kw.w, b + slot * F::ROW + k_at);
+      if constexpr (NWD == 2) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(b + slot * F::ROW + k_at);
+        kw.w[0] = v[0], kw.w[1] = v[1];
+      } else {
+        kw.w[0] = *reinterpret_cast<const uint32_t*>(b + slot * F::ROW + k_at);
+      }
 #pragma unroll
       for (int u = 0; u < NWD; ++u)
         kw.st[u] = *reinterpret_cast<const uint32_t*>(b + stats + 4 * slot + 4 * ((NWD * p + u) * a.page + ktok));
@@ -335,44 +335,44 @@ struct ChunkQ4Wide : StagedTile {
     auto load_v = [&](int t) {
       const uint8_t* b = vh + w.off_of(t);
       const int slot = w.slot_of(t), key = w.key_of(t);
-      load_words(vw.w, b + slot * F::ROW + v_at);
 #pragma unroll
       for (int u = 0; u < NWD; ++u)
-        vw.st[u] = *reinterpret_cast<const u32x4*>(b + stats + 4 * slot + 4 * ((NWD * p + u) * a.page + vtok));
+        vw.w[u] = *reinterpret_cast<const uint32_t*>(b + slot * F::ROW + v_at + 8 * u * 4 * F::NG);
+      vw.st = *reinterpret_cast<const u32x4*>(b + stats + 4 * slot + 4 * (vg * a.page + vtok));
       if (key + 16 > it.end) {
 #pragma unroll
-        for (int u = 0; u < NWD; ++u)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vw.st[u][j] = key + vtok + j < it.end ? vw.st[u][j] : 0u;
+        for (int j = 0; j < 4; ++j) vw.st[j] = key + vtok + j < it.end ? vw.st[j] : 0u;
       }
     };
-    // Scales the loaded words into buffer kb / vb.
+    // Scales the loaded words into buffers kb and vb, in 4 NWD pieces: halves of words of keys, then of values.
+    constexpr int PIECES = 4 * NWD;
+    uint32_t half[2];
+    auto put = [&](int piece, int kb, int vb) {
+      const int u = (piece >> 1) % NWD;
+      if (piece < 2 * NWD) {
+        const float s = q4_scale<BF16>(kw.st[u]), m = q4_min<BF16>(kw.st[u]);
+        const uint32_t cs = piece & 1 ? q4_high(kw.w[u]) : q4_low(kw.w[u]);
+        const uint32_t d0 = q4_scaled<BF16, false>(cs, s, m), d1 = q4_scaled<BF16, true>(cs, s, m);
+        if (piece & 1)
+          *reinterpret_cast<u32x4*>(lds_k + kb * TILE_BYTES + 4096 * u) = u32x4{half[0], half[1], d0, d1};
+        else
+          half[0] = d0, half[1] = d1;
+      } else {
+        const uint32_t cs = piece & 1 ? q4_high(vw.w[u]) : q4_low(vw.w[u]);
+        *reinterpret_cast<u32x2*>(lds_v + vb * TILE_BYTES + 1024 * u + 2048 * (piece & 1)) =
+            u32x2{q4_scaled<BF16, false>(cs, q4_scale<BF16>(vw.st[0]), q4_min<BF16>(vw.st[0]), q4_scale<BF16>(vw.st[1]),
+                                         q4_min<BF16>(vw.st[1])),
+                  q4_scaled<BF16, true>(cs, q4_scale<BF16>(vw.st[2]), q4_min<BF16>(vw.st[2]), q4_scale<BF16>(vw.st[3]),
+                                        q4_min<BF16>(vw.st[3]))};
+      }
+    };
     auto put_k = [&](int kb) {
 #pragma unroll
-      for (int u = 0; u < NWD; ++u) {
-        const float s = q4_scale<BF16>(kw.st[u]), m = q4_min<BF16>(kw.st[u]);
-        const uint32_t lo = q4_low(kw.w[u]), hi = q4_high(kw.w[u]);
-        *reinterpret_cast<u32x4*>(lds_k + kb * TILE_BYTES + 4096 * u) =
-            u32x4{E::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
-                  E::pack2f(fmaf(q4_code<2>(lo), s, m), fmaf(q4_code<3>(lo), s, m)),
-                  E::pack2f(fmaf(q4_code<0>(hi), s, m), fmaf(q4_code<1>(hi), s, m)),
-                  E::pack2f(fmaf(q4_code<2>(hi), s, m), fmaf(q4_code<3>(hi), s, m))};
-      }
+      for (int y = 0; y < 2 * NWD; ++y) put(y, kb, 0);
     };
     auto put_v = [&](int vb) {
 #pragma unroll
-      for (int u = 0; u < NWD; ++u) {
-        float s[4], m[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = q4_scale<BF16>(vw.st[u][j]), m[j] = q4_min<BF16>(vw.st[u][j]);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t cs = half ? q4_high(vw.w[u]) : q4_low(vw.w[u]);
-          *reinterpret_cast<u32x2*>(lds_v + vb * TILE_BYTES + 4096 * u + 2048 * half) =
-              u32x2{E::pack2f(fmaf(q4_code<0>(cs), s[0], m[0]), fmaf(q4_code<1>(cs), s[1], m[1])),
-                    E::pack2f(fmaf(q4_code<2>(cs), s[2], m[2]), fmaf(q4_code<3>(cs), s[3], m[3]))};
-        }
-      }
+      for (int y = 2 * NWD; y < PIECES; ++y) put(y, 0, vb);
     };
     // Scores of tile t past a row's position become -inf.
     auto mask = [&](f32x16 (&S)[2], int t) {
@@ -430,8 +430,10 @@ struct ChunkQ4Wide : StagedTile {
     constexpr int NQ = D / 8;    // QK MFMAs of a tile: i -> (key half i % 2, cc = i / 2)
     constexpr int PE = 32 / NQ;  // probabilities per QK MFMA
     constexpr int NP = D / 8;    // PV MFMAs: i -> (dt = i % NCG, h, j)
+    static_assert(NP == 2 * PIECES, "a piece of the scaling to every other one");
 
-    auto block_b = [&](const char* cV) {
+    // Block B; work(i) after its i-th product.
+    auto block_b = [&](const char* cV, auto work) {
       auto vfr = [&](int i) { return vtfrag(cV, v0, vswz, i / (2 * NCG), (i / NCG) & 1, i % NCG); };
       u32x4 vf[2] = {vfr(0), vfr(1)};
       __builtin_amdgcn_s_setprio(0);
@@ -440,9 +442,11 @@ struct ChunkQ4Wide : StagedTile {
       for (int i = 0; i < NP; ++i) {
         O[i % NCG] = E::mfma32(vf[i & 1], P[i / (2 * NCG)][(i / NCG) & 1], O[i % NCG]);
         if (i + 2 < NP) vf[i & 1] = vfr(i + 2);
+        work(i);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
+    auto nothing = [](int) {};
     auto probs = [&](const f32x16 (&Sc)[2], float& ls) {
       ls = 0.f;
 #pragma unroll
@@ -477,11 +481,11 @@ struct ChunkQ4Wide : StagedTile {
 
     // One step on tile t, whose scores are in Sc; fills Sx with the next tile's.
     auto step = [&](int t, f32x16 (&Sc)[2], f32x16 (&Sx)[2]) {
-      if (t + 2 < nt) put_k(kb_cur);
-      put_v(ring(vb_cur + 1, NBV));            // of tile t + 1: there is one
+      put_k(kb_cur);                            // of tile t + 2 (a repeat where there is none, to a buffer that no one reads)
+      put_v(ring(vb_cur + 1, NBV));             // of tile t + 1
       if (t + 3 < nt) load_k(t + 3);
       if (t + 2 < nt) load_v(t + 2);
-      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES);
+      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES, nothing);
       const char* cK = sK + (kb_cur ^ 1) * TILE_BYTES;
       auto kfr = [&](int i) { return kfrag(cK, f, i & 1, i >> 1); };
       u32x4 kf[3] = {kfr(0), kfr(1), kfr(2)};
@@ -514,7 +518,7 @@ struct ChunkQ4Wide : StagedTile {
       if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(Sc, ls);
       l_run += ls;
       mask(Sx, t + 1);
-      if (!lag) block_b(sV + vb_cur * TILE_BYTES);
+      if (!lag) block_b(sV + vb_cur * TILE_BYTES, nothing);
       pending = true;
       __syncthreads();
       vb_cur = ring(vb_cur + 1, NBV);
@@ -534,12 +538,12 @@ struct ChunkQ4Wide : StagedTile {
         S[1] = Sn[1];
       }
       // The last tile: no next one, nothing to load.
-      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES);
+      if (lag && pending) block_b(sV + ring(vb_cur + NBV - 1, NBV) * TILE_BYTES, nothing);
       float ls;
       probs(S, ls);
       if (!ref_ok || __any(!(ls <= REFIT_SUM))) raise(S, ls);
       l_run += ls;
-      block_b(sV + vb_cur * TILE_BYTES);
+      block_b(sV + vb_cur * TILE_BYTES, nothing);
     }
     __syncthreads();   // the K/V buffers are free
     const float lt = halves_sum(l_run);

@@ -14,6 +14,7 @@
 namespace sa {
 
 constexpr int DQ_WAVES = 4;
+constexpr int DQ_DEPTH = 2;        // steps of a wave's ring
 constexpr int DQ_TARGET = 512;     // workgroups that run at once, two to a CU
 constexpr int DQ_MIN_UNIT = 8;     // steps of a workgroup of a planned division, two for each wave
 constexpr int DQ_MOST = 1344;      // workgroups that a planned division adds to one for each list: DQ_TARGET / 0.381
@@ -173,12 +174,12 @@ struct DecodeQ4Item {
 template <bool BF16, int D, int NQ>
 struct DecodeQ4 {
   using E = Elem<BF16>;
-  using Rows = Q4Fold<BF16, D, NQ>;
+  using Rows = Q4Fold<BF16, D, NQ, DQ_DEPTH>;
   static constexpr int ROWS = Rows::ROWS;
   static constexpr int ACC = ROWS * D * 4;
-  static_assert(ACC >= 4 * Q4Pairs<D>::WORDS, "the pairs lie in the accumulators' LDS");
+  static constexpr int LDS_BYTES = DQ_WAVES * (ACC > Q4Ring<D, DQ_DEPTH>::BYTES ? ACC : Q4Ring<D, DQ_DEPTH>::BYTES);
 
-  static __device__ void run(const DecodeQ4Args& a, char* s_acc, float* s_ml) {
+  static __device__ void run(const DecodeQ4Args& a, char* s_lds, float* s_ml) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     DecodeQ4Item it;
@@ -202,7 +203,7 @@ struct DecodeQ4 {
       w.set_query(x, a.q + b * a.q_sb + (head0 + min(x * Rows::RPS + Rows::row_of(lane), live - 1)) * a.q_sh, len - 1);
     w.pos_min = len - 1;
     w.start();
-    w.pairs.at = reinterpret_cast<uint32_t*>(s_acc) + wave * Q4Pairs<D>::WORDS;
+    w.ring.lds = s_lds + wave * Q4Ring<D, DQ_DEPTH>::BYTES;
     Q4Keys ks;
     const int kvh = row / a.group;
     ks.k = a.k + kvh * a.sh;
@@ -217,7 +218,7 @@ struct DecodeQ4 {
     ks.end = len, ks.pos_max = len - 1;
     ks.wave = wave, ks.waves = DQ_WAVES;
     q4_run(w, ks, a.scale_log2);
-    __syncthreads();               // the pairs lie where the accumulators go
+    __syncthreads();               // the rings lie where the accumulators go
     // Merge in fp32: row r is D floats at r * 4 D, its 16-byte chunk x at position x ^ (r % (D / 4)).
     constexpr int NC4 = D / 4, OC = D / 8;
 #pragma unroll
@@ -227,7 +228,7 @@ struct DecodeQ4 {
       w.result(x, out);
 #pragma unroll
       for (int half = 0; half < 2; ++half)
-        *reinterpret_cast<f32x4*>(s_acc + wave * ACC + r * 4 * D + 16 * ((8 * g + 4 * half + (lane >> 4)) ^ (r & (NC4 - 1)))) = out[half];
+        *reinterpret_cast<f32x4*>(s_lds + wave * ACC + r * 4 * D + 16 * ((8 * g + 4 * half + (lane >> 4)) ^ (r & (NC4 - 1)))) = out[half];
       const float l = quarters_sum(w.l_run[x]);
       if (lane < Rows::RPS) {
         s_ml[2 * (wave * ROWS + r)] = w.m_ref[x];
@@ -249,7 +250,7 @@ struct DecodeQ4 {
       for (int s = 0; s < DQ_WAVES; ++s) {
         const float fs = fast_exp2(m[s] - Mu);
         l += fs * s_ml[2 * (s * ROWS + r) + 1];
-        const char* p = s_acc + s * ACC + r * 4 * D;
+        const char* p = s_lds + s * ACC + r * 4 * D;
         lo += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc) ^ (r & (NC4 - 1))));
         hi += fs * *reinterpret_cast<const f32x4*>(p + 16 * ((2 * oc + 1) ^ (r & (NC4 - 1))));
       }
@@ -274,11 +275,11 @@ struct DecodeQ4 {
 };
 
 template <bool BF16, int D, int NQ>
-static __global__ __launch_bounds__(64 * DQ_WAVES, NQ == 1 ? 3 : 2) void decode_q4_kernel(const DecodeQ4Args a) {
+static __global__ __launch_bounds__(64 * DQ_WAVES, 2) void decode_q4_kernel(const DecodeQ4Args a) {
   using K = DecodeQ4<BF16, D, NQ>;
-  __shared__ __attribute__((aligned(16))) char s_acc[DQ_WAVES * K::ACC];
+  __shared__ __attribute__((aligned(16))) char s_lds[K::LDS_BYTES];
   __shared__ float s_ml[2 * DQ_WAVES * K::ROWS];
-  K::run(a, s_acc, s_ml);
+  K::run(a, s_lds, s_ml);
 }
 
 // Merges the partials of a query head whose list was shared: a workgroup a head, D / 8 lanes a share, 2048 / D shares at a

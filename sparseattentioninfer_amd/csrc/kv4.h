@@ -65,8 +65,23 @@ __device__ __forceinline__ uint32_t q4_high(uint32_t w) { return (w >> 4) & 0x0f
 template <int E>
 __device__ __forceinline__ float q4_code(uint32_t codes) { return (float)((codes >> (8 * E)) & 0xffu); }
 
-// Two of four codes as numbers of 16 bits, exact: a code in a byte is an e4m3 number of that many 2^-9, subnormals and the
+// Two of four codes as fp32 and as 16-bit numbers, exact: a code in a byte is an e4m3 number of that many 2^-9, subnormals and the
 // first binade together, so the conversion scales by 2^9.
+template <bool HIGH>
+__device__ __forceinline__ f32x2 q4_pair_f32(uint32_t codes) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((int)codes, 512.f, HIGH);
+}
+// m + s c of two codes, rounded to the element type.
+template <bool BF16, bool HIGH>
+__device__ __forceinline__ uint32_t q4_scaled(uint32_t codes, float s, float m) {
+  const f32x2 c = q4_pair_f32<HIGH>(codes);
+  return Elem<BF16>::pack2f(fmaf(c[0], s, m), fmaf(c[1], s, m));
+}
+template <bool BF16, bool HIGH>      // the same with a scale and a minimum of its own for each
+__device__ __forceinline__ uint32_t q4_scaled(uint32_t codes, float s0, float m0, float s1, float m1) {
+  const f32x2 c = q4_pair_f32<HIGH>(codes);
+  return Elem<BF16>::pack2f(fmaf(c[0], s0, m0), fmaf(c[1], s1, m1));
+}
 template <bool HIGH>
 __device__ __forceinline__ uint32_t q4_pair_bf16(uint32_t codes) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)codes, 512.f, HIGH));

@@ -92,6 +92,26 @@ __device__ __forceinline__ void load_lds16(const void* vaddr, uint32_t lds) {
       : "memory", "m0");
 }
 
+// The same for 4 bytes per lane: lane l's land at the LDS address plus 4 l.
+__device__ __forceinline__ void load_lds4(const void* vaddr, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %0, off"
+      :
+      : "v"(vaddr), "s"(lds)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds4(const void* sbase, uint32_t voff, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %0, %1"
+      :
+      : "v"(voff), "s"(sbase), "s"(lds)
+      : "memory", "m0");
+}
+
 // Waits for the calling wave's direct loads (and any other vector memory access).
 __device__ __forceinline__ void wait_dma() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 
