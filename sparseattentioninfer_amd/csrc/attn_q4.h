@@ -228,10 +228,8 @@ struct Q4Dequant {
         const uint32_t st = ring.key_pair(slot, h, g, i);
         const float s = q4_scale<BF16>(st), m = q4_min<BF16>(st);
         const uint32_t lo = q4_low(kw.w[g]), hi = q4_high(kw.w[g]);
-        const u32x4 kf = {E::pack2f(fmaf(q4_code<0>(lo), s, m), fmaf(q4_code<1>(lo), s, m)),
-                          E::pack2f(fmaf(q4_code<2>(lo), s, m), fmaf(q4_code<3>(lo), s, m)),
-                          E::pack2f(fmaf(q4_code<0>(hi), s, m), fmaf(q4_code<1>(hi), s, m)),
-                          E::pack2f(fmaf(q4_code<2>(hi), s, m), fmaf(q4_code<3>(hi), s, m))};
+        const u32x4 kf = {q4_scaled<BF16, false>(lo, s, m), q4_scaled<BF16, true>(lo, s, m),
+                          q4_scaled<BF16, false>(hi, s, m), q4_scaled<BF16, true>(hi, s, m)};
 #pragma unroll
         for (int c = 0; c < NC; ++c) S[c][h] = E::mfma16(kf, qf[c][g], S[c][h]);
       }
@@ -288,8 +286,8 @@ struct Q4Dequant {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t x = half ? q4_high(vw[h].w[g]) : q4_low(vw[h].w[g]);
-          vf[2 * h] = E::pack2f(fmaf(q4_code<0>(x), s[h][0], m[h][0]), fmaf(q4_code<1>(x), s[h][1], m[h][1]));
-          vf[2 * h + 1] = E::pack2f(fmaf(q4_code<2>(x), s[h][2], m[h][2]), fmaf(q4_code<3>(x), s[h][3], m[h][3]));
+          vf[2 * h] = q4_scaled<BF16, false>(x, s[h][0], m[h][0], s[h][1], m[h][1]);
+          vf[2 * h + 1] = q4_scaled<BF16, true>(x, s[h][2], m[h][2], s[h][3], m[h][3]);
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) O[c][2 * g + half] = E::mfma16(vf, P[c], O[c][2 * g + half]);

@@ -199,21 +199,19 @@ struct ChunkQ4Wide : StagedTile {
   static_assert(NW * STAGE <= LDS_BYTES, "O is staged in the K/V buffers");
   static constexpr float REFIT_SUM = BF16 ? 65536.f : 32768.f;
 
-  // 64 tiles looked up at once: lane i holds, for tile base + i, the place and first key of the chunk of which this
-  // wave scales half, and the tile's largest key; the first keys of its four chunks go to LDS, for the tiles that need
-  // a mask.  Tiles are looked up three ahead of the one whose mask is due, so a window starts three tiles back.
+  // 64 tiles looked up at once: lane i holds, for tile base + i, the page and first key of the chunk of which this wave
+  // scales half (a multiple of 16, and its 16 keys' place in the page in the low bits), and the tile's largest key; the
+  // first keys of its four chunks go to LDS, for the tiles that need a mask.  Tiles are looked up three ahead of the one
+  // whose mask is due, so a window starts three tiles back.
   static constexpr int AHEAD = 3;
   struct Window {
-    int base;
-    int64_t off;
-    int key, slot, last;
+    int base, page, key, last;
 
-    __device__ __forceinline__ void fill(const ChunkArgs& a, const ChunkItem& it, int64_t sp, int first, int rb, int* s_keys) {
+    __device__ __forceinline__ void fill(const ChunkArgs& a, const ChunkItem& it, int first, int rb, int* s_keys) {
       base = first;
       const int lane = threadIdx.x & 63;
       key = CK_NO_KEY;
-      off = 0;
-      slot = 0;
+      page = 0;
       last = -1;
       int keys[4];
 #pragma unroll
@@ -236,9 +234,8 @@ struct ChunkQ4Wide : StagedTile {
             if (pg >= 0 && pg < a.num_pages) {
               keys[x] = lb * a.page + s;
               if (x == rb) {
-                off = (int64_t)pg * sp;
-                key = keys[x];
-                slot = s;
+                page = pg;
+                key = keys[x] | (s >> 4);
               }
             }
           }
@@ -248,13 +245,8 @@ struct ChunkQ4Wide : StagedTile {
       *reinterpret_cast<int4*>(s_keys + 4 * lane) = int4{keys[0], keys[1], keys[2], keys[3]};
     }
     __device__ __forceinline__ int key_of(int t) const { return __builtin_amdgcn_readlane(key, t - base); }
-    __device__ __forceinline__ int slot_of(int t) const { return __builtin_amdgcn_readlane(slot, t - base); }
+    __device__ __forceinline__ int page_of(int t) const { return __builtin_amdgcn_readlane(page, t - base); }
     __device__ __forceinline__ int last_of(int t) const { return __builtin_amdgcn_readlane(last, t - base); }
-    __device__ __forceinline__ int64_t off_of(int t) const {
-      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(uint64_t)off, t - base);
-      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)off >> 32), t - base);
-      return (int64_t)(((uint64_t)hi << 32) | lo);
-    }
   };
 
   // A lane's words of a tile and their pairs.
@@ -315,9 +307,9 @@ struct ChunkQ4Wide : StagedTile {
     KeyWords kw;
     ValueWords vw;
     auto load_k = [&](int t) {
-      if (t - w.base >= 64) w.fill(a, it, x.sp, t - AHEAD, rb, s_keys);
-      const uint8_t* b = kh + w.off_of(t);
-      const int slot = w.slot_of(t), key = w.key_of(t);
+      if (t - w.base >= 64) w.fill(a, it, t - AHEAD, rb, s_keys);
+      const uint8_t* b = kh + w.page_of(t) * x.sp;
+      const int packed = w.key_of(t), slot = 16 * (packed & 15), key = packed & ~15;
       if constexpr (NWD == 2) {
         const u32x2 v = *reinterpret_cast<const u32x2*>(b + slot * F::ROW + k_at);
         kw.w[0] = v[0], kw.w[1] = v[1];
@@ -333,8 +325,8 @@ struct ChunkQ4Wide : StagedTile {
       }
     };
     auto load_v = [&](int t) {
-      const uint8_t* b = vh + w.off_of(t);
-      const int slot = w.slot_of(t), key = w.key_of(t);
+      const uint8_t* b = vh + w.page_of(t) * x.sp;
+      const int packed = w.key_of(t), slot = 16 * (packed & 15), key = packed & ~15;
 #pragma unroll
       for (int u = 0; u < NWD; ++u)
         vw.w[u] = *reinterpret_cast<const uint32_t*>(b + slot * F::ROW + v_at + 8 * u * 4 * F::NG);
@@ -394,7 +386,7 @@ struct ChunkQ4Wide : StagedTile {
     float m_ref = -__builtin_inff(), l_run = 0.f;
     f32x16 S[2] = {f32x16{}, f32x16{}};
     if (nt > 0) {
-      w.fill(a, it, x.sp, 0, rb, s_keys);
+      w.fill(a, it, 0, rb, s_keys);
       load_k(0);
       load_v(0);
       put_k(0);
