@@ -68,12 +68,16 @@ struct ChunkArgs {
 //
 // Key tiles are what is balanced.  With the chip full a wide item takes 1.75 us for one (256 rows on its matrix
 // cores), a narrow one 1.45 us where narrow items are most of the work (32 KB at a CU's share of HBM) and about half of
-// a wide one's beside wide ones.  A workgroup costs CK_START of them besides its own: 9.6 us, of which finding its item
+// a wide one's beside wide ones.  A workgroup costs `start` of them (5.5) besides its own: 9.6 us, of which finding its item
 // takes 2.5, the pages of its first tiles 2.6, the tiles 1.5 and the end 3.
-constexpr float CK_START = 5.5f;
 // A division costs the merge, 4 us after narrow and 6.5 after wide items, and for each row of partials its write and
 // read: 1,040 bytes at D = 128, 0.2 ns at the rate of a copy.
-constexpr float CK_MERGE_WIDE = 4.f, CK_MERGE_NARROW = 2.5f, CK_MERGE_ROW = 1.3e-4f;
+struct ChunkCost {
+  static constexpr float MERGE_WIDE = 4.f, MERGE_NARROW = 2.5f, MERGE_ROW = 1.3e-4f;
+  static __device__ __forceinline__ float start(int) { return 5.5f; }
+  // Narrow items that do not fill the chip are not bound by HBM: 0.5 us for a tile instead of 1.45.
+  static __device__ __forceinline__ float alone(float groups, float cus) { return fminf(fmaxf(0.35f, groups / cus), 1.f); }
+};
 constexpr int CK_NARROW = 64;
 constexpr int CK_WIDE_ROWS = 256;
 
@@ -145,6 +149,7 @@ struct SplitRule {
 // the sequences y, y + 8, ...  The sums are fp32: exact where they decide between neighbouring choices (below 2^24),
 // and the room for partials is kept with a margin above their rounding; a fixed division, which fills its room
 // exactly, is summed in 64 bits.
+template <class Cost>
 __device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqShape& first64) {
   const int lane = threadIdx.x & 63;
   if (a.splits) {
@@ -173,6 +178,7 @@ __device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqSh
   tiles = wave_sum(tiles);
   longest = wave_max(longest);
   const int half = narrow > wide ? 0 : 1;
+  const float start = Cost::start(half);
   const float nw = half ? 0.5f : 1.f, work = wide + nw * narrow;
   const float even = fminf(ceilf(work / cus), (float)(CK_NO_LIMIT / 16));
   if (longest <= 0.5f * even) return SplitRule(CK_NO_LIMIT, half);   // there are row tiles enough
@@ -205,13 +211,12 @@ __device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqSh
   rows = over_eights<SUM>(rows) * (float)a.Hq;
   // When it ends.  In one round: with the longest workgroup.  Else, handed out longest first: the mean load, or
   // two of those longer than half of it where they outnumber the CUs (their lengths taken as spread evenly).
-  const float mean = (work + groups * CK_START) / cus;
-  // Narrow items that do not fill the chip are not bound by HBM: 0.5 us for a tile instead of 1.45.
-  const float alone = half ? 1.f : fminf(fmaxf(0.35f, groups / cus), 1.f);
+  const float mean = (work + groups * start) / cus;
+  const float alone = half ? 1.f : Cost::alone(groups, cus);
   float one = 0.f, many = 0.f, lo = __builtin_inff(), hi = 0.f;
   each([&](float st, float k, float nt, float nt0, float, float w) {
     if (st == 0.f) return;
-    const float x = w * alone * __builtin_amdgcn_rcpf(k), h = nt * x + CK_START, l = nt0 * x + CK_START;
+    const float x = w * alone * __builtin_amdgcn_rcpf(k), h = nt * x + start, l = nt0 * x + start;
     one = fmaxf(one, h);
     if (h <= 0.5f * mean) return;
     const float from = fmaxf(l, 0.5f * mean);
@@ -226,7 +231,7 @@ __device__ __forceinline__ SplitRule plan_splits(const ChunkArgs& a, const SeqSh
   float time = one;
   if (groups > cus) time = fmaxf(one, 1.08f * mean);
   if (groups > cus && many > cus) time = fmaxf(time, 2.f * (lo + (hi - lo) * (many - cus) / many));
-  if (rows > 0.f) time += (half ? CK_MERGE_WIDE : CK_MERGE_NARROW) + CK_MERGE_ROW * rows;
+  if (rows > 0.f) time += (half ? Cost::MERGE_WIDE : Cost::MERGE_NARROW) + Cost::MERGE_ROW * rows;
   // The partials must fit, and no more workgroups are added than there are CUs (chunk_items: the launch has that
   // many to spare, and idle ones cost time too).  No division always does.
   if (rows * 1.001f > (float)a.part_rows || groups > tiles * heads + cus) time = __builtin_inff();
@@ -268,6 +273,7 @@ struct ChunkItem {
 // are eight of them).  Longest first, so that the launch ends evenly: up to 64 sequences in the order of their
 // workgroups' key tiles (a narrow one's take half as long while the matrix cores bound the rest), more as they come;
 // within a sequence later row tiles, which see more keys, first.
+template <class Cost = ChunkCost>
 __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, ChunkItem& it) {
   const int lane = threadIdx.x & 63;
   const int t = (int)fast_div((uint32_t)id, (uint32_t)a.Hkv, a.mul_heads);
@@ -275,7 +281,7 @@ __device__ __forceinline__ bool find_chunk_item(const ChunkArgs& a, int id, Chun
   SeqShape s64 = {};
   if (lane < a.seqs.B) s64 = seq_shape(a, lane);
   const bool split = a.part != nullptr;
-  const SplitRule rule = split ? plan_splits(a, s64) : SplitRule(CK_NO_LIMIT, 0);
+  const SplitRule rule = split ? plan_splits<Cost>(a, s64) : SplitRule(CK_NO_LIMIT, 0);
   const bool first = id == 0 && split && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
   const bool ranked = a.seqs.B > 1 && a.seqs.B <= 64;
   int base = 0, block0 = 0, part0 = 0, local = 0;
