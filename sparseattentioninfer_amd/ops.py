@@ -1121,9 +1121,19 @@ def _q4_page(nbytes: int, D: int) -> int:
     return 0 if odd or page % 16 or not 16 <= page <= 128 else page
 
 
-def _q4_pools_ok(kp: torch.Tensor, vp: torch.Tensor, dev) -> bool:
-    return (kp.dtype == torch.uint8 and vp.dtype == torch.uint8 and kp.device == dev and vp.device == dev and kp.dim() == 3
-            and kp.shape == vp.shape and kp.stride() == vp.stride() and kp.stride(2) == 1)
+_I32, _U8 = torch.int32, torch.uint8
+
+
+def _q4_pools_ok(kp: torch.Tensor, vp: torch.Tensor, pst, dev) -> bool:
+    """Whether kp (of strides pst) and vp are pools of one form on `dev`."""
+    return (kp.dtype == _U8 and vp.dtype == _U8 and vp.device == dev and len(pst) == 3 and pst[2] == 1 and vp.shape == kp.shape
+            and vp.stride() == pst and kp.device == dev)
+
+
+def _q4_index_ok(table: torch.Tensor, bs, bst, lens: torch.Tensor, B: int, dev) -> bool:
+    """Whether table (of shape bs and strides bst) is [B, max_blocks] and lens [B], int32 on `dev`."""
+    return (table.dtype == _I32 and lens.dtype == _I32 and table.device == dev and lens.device == dev and len(bs) == 2
+            and bs[0] == B and (bs[1] <= 1 or bst[1] == 1) and lens.shape == (B,) and (B < 2 or lens.stride(0) == 1))
 
 
 def _refuse_q4(name: str, like: torch.Tensor, dtype, D: int, kp: torch.Tensor, vp: torch.Tensor, *, heads: dict, index: dict,
@@ -1154,15 +1164,13 @@ def paged_append_q4(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     smallest and largest key per dim as they are read back.
     """
     name = "paged_append_q4"
-    dt, dev, ks, ps, B = k.dtype, k.device, k.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
-    kst, vst = k.stride(), v.stride()
+    dt, dev, ks, ps, bs = k.dtype, k.device, k.shape, k_pages.shape, block_table.shape
+    kst, vst, pst, bst, B = k.stride(), v.stride(), k_pages.stride(), block_table.stride(), bs[0] if bs else 0
     page = _q4_page(ps[2], ks[2]) if len(ps) == 3 and len(ks) == 3 else 0
     ok = (k.is_cuda and dt in _DTYPES and len(ks) == 3 and v.shape == ks and v.dtype == dt and v.device == dev
-          and kst[2] == 1 and vst[2] == 1 and _q4_pools_ok(k_pages, v_pages, dev) and ps[1] == ks[1] and page > 0
-          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
-          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
-          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
-          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+          and kst[2] == 1 and vst[2] == 1 and _q4_pools_ok(k_pages, v_pages, pst, dev) and ps[1] == ks[1] and page > 0
+          and _q4_index_ok(block_table, bs, bst, kv_lens, B, dev) and cu_seqlens.dtype == _I32 and cu_seqlens.device == dev
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.stride(0) == 1
           and (k_weight is None or (k_weight.shape == (ks[2],) and k_weight.dtype == dt and k_weight.device == dev
                                     and k_weight.is_contiguous()))
           and (inv_freq is None or (inv_freq.dtype == torch.float32 and inv_freq.shape == (ks[2] // 2,)
@@ -1197,8 +1205,7 @@ def paged_append_q4(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     _call("sa_paged_append_q4", dev.index, _DTYPES[dt], *qargs, k.data_ptr(), kst[0], kst[1], v.data_ptr(), vst[0], vst[1],
           *oargs, None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
           None if inv_freq is None else inv_freq.data_ptr(), *at, k_pages.data_ptr(), v_pages.data_ptr(),
-          k_pages.stride(0), k_pages.stride(1), ps[0], *bargs, block_table.data_ptr(), block_table.stride(0),
-          block_table.size(1), cu_seqlens.data_ptr(), kv_lens.data_ptr(), ks[0], B, Hq, ks[1], ks[2], page, eps)
+          pst[0], pst[1], ps[0], *bargs, block_table.data_ptr(), bst[0], bs[1], cu_seqlens.data_ptr(), kv_lens.data_ptr(), ks[0], B, Hq, ks[1], ks[2], page, eps)
     return q_out
 
 
@@ -1213,16 +1220,16 @@ def paged_read_q4(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: tor
     lengths are on the device).  Rows of given outputs that belong to no sequence are left as they are.
     """
     name = "paged_read_q4"
-    dev, ps, B = k_pages.device, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
+    dev, ps, bs, pst, bst = k_pages.device, k_pages.shape, block_table.shape, k_pages.stride(), block_table.stride()
+    B = bs[0] if bs else 0
     page = _q4_page(ps[2], head_dim) if len(ps) == 3 else 0
-    ok = (k_pages.is_cuda and dtype in _DTYPES and _q4_pools_ok(k_pages, v_pages, dev) and page > 0 and rows >= 0
-          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
-          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
-          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
-          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous())
+    ok = (k_pages.is_cuda and dtype in _DTYPES and _q4_pools_ok(k_pages, v_pages, pst, dev) and page > 0 and rows >= 0
+          and _q4_index_ok(block_table, bs, bst, kv_lens, B, dev) and cu_seqlens.dtype == _I32 and cu_seqlens.device == dev
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.stride(0) == 1)
     shape = (rows, ps[1] if len(ps) == 3 else 0, head_dim)
-    for out in (k_out, v_out):
-        ok = ok and (out is None or (out.shape == shape and out.dtype == dtype and out.device == dev and out.stride(2) == 1))
+    if k_out is not None or v_out is not None:
+        for out in (k_out, v_out):
+            ok = ok and (out is None or (out.shape == shape and out.dtype == dtype and out.device == dev and out.stride(2) == 1))
     if not ok:
         outs = {label: t for label, t in (("k_out", k_out), ("v_out", v_out)) if t is not None}
         like = next(iter(outs.values()), torch.empty(0, dtype=dtype, device=dev)) if k_pages.is_cuda else k_pages
@@ -1234,8 +1241,8 @@ def paged_read_q4(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: tor
     if v_out is None:
         v_out = torch.empty(shape, dtype=dtype, device=dev)
     kst, vst = k_out.stride(), v_out.stride()
-    _call("sa_paged_read_q4", dev.index, _DTYPES[dtype], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0),
-          k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0), block_table.size(1), cu_seqlens.data_ptr(),
+    _call("sa_paged_read_q4", dev.index, _DTYPES[dtype], k_pages.data_ptr(), v_pages.data_ptr(), pst[0], pst[1], ps[0],
+          block_table.data_ptr(), bst[0], bs[1], cu_seqlens.data_ptr(),
           kv_lens.data_ptr(), k_out.data_ptr(), kst[0], kst[1], v_out.data_ptr(), vst[0], vst[1], rows, B, ps[1], head_dim, page)
     return k_out, v_out
 
@@ -1250,26 +1257,23 @@ def paged_chunk_attn_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     everything else is as for :func:`paged_chunk_attn`.
     """
     name = "paged_chunk_attn_q4"
-    dt, dev, qs, ps, B = q.dtype, q.device, q.shape, k_pages.shape, kv_lens.size(0) if kv_lens.dim() else 0
-    qst = q.stride()
+    dt, dev, qs, ps, bs = q.dtype, q.device, q.shape, k_pages.shape, block_table.shape
+    qst, pst, bst, B = q.stride(), k_pages.stride(), block_table.stride(), bs[0] if bs else 0
     page = _q4_page(ps[2], qs[2]) if len(ps) == 3 and len(qs) == 3 else 0
-    ok = (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and _q4_pools_ok(k_pages, v_pages, dev) and page > 0
+    ok = (q.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and _q4_pools_ok(k_pages, v_pages, pst, dev) and page > 0
           and ps[1] > 0 and qs[1] % ps[1] == 0
-          and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32 and kv_lens.dtype == torch.int32
-          and block_table.device == dev and cu_seqlens.device == dev and kv_lens.device == dev
-          and block_table.dim() == 2 and block_table.size(0) == B and (block_table.size(1) <= 1 or block_table.stride(1) == 1)
-          and cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous() and kv_lens.dim() == 1 and kv_lens.is_contiguous()
+          and _q4_index_ok(block_table, bs, bst, kv_lens, B, dev) and cu_seqlens.dtype == _I32 and cu_seqlens.device == dev
+          and cu_seqlens.shape == (B + 1,) and cu_seqlens.stride(0) == 1
           and (sel is None) == (sel_off is None))
     if out is None:
         out = _empty_like(q)
     elif ok:
         ok = out.shape == qs and out.dtype == dt and out.device == dev and out.stride(2) == 1
     sargs = (None, 0, 0, 0, 0, None, 0, 0)
-    max_blocks = block_table.size(-1) if ok else 0
-    keys = max_blocks
+    keys = max_blocks = bs[1] if ok else 0
     if ok and sel is not None:
         ss, sst = sel.shape, sel.stride()
-        ok = (sel.dtype == torch.int32 and sel_off.dtype == torch.int32 and sel.device == dev and sel_off.device == dev
+        ok = (sel.dtype == _I32 and sel_off.dtype == _I32 and sel.device == dev and sel_off.device == dev
               and len(ss) == 3 and ss[0] >= qs[0] // CHUNK_BLOCK + B and ss[1] == ps[1]
               and sel_off.shape == (ss[0], ss[1], 2) and (ss[2] <= 1 or sst[2] == 1) and sel_off.stride(2) == 1)
         if ok:
@@ -1285,8 +1289,7 @@ def paged_chunk_attn_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     ws = _workspace(name, workspace, _lib.load().sa_paged_chunk_workspace_bytes(
         N, B, Hq, ps[1], D, min(keys * page, 1 << 30), num_splits), dev)
     _call("sa_paged_chunk_attn_q4", dev.index, _DTYPES[dt], q.data_ptr(), qst[0], qst[1], k_pages.data_ptr(),
-          v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0),
-          max_blocks, cu_seqlens.data_ptr(), kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], N, B, Hq, ps[1], D,
+          v_pages.data_ptr(), pst[0], pst[1], ps[0], block_table.data_ptr(), bst[0], max_blocks, cu_seqlens.data_ptr(), kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], N, B, Hq, ps[1], D,
           page, D ** -0.5 if sm_scale is None else sm_scale, num_splits, *_ws_bytes(ws))
     return out
 
@@ -1307,23 +1310,21 @@ def paged_sparse_decode_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """
     name = "paged_sparse_decode_q4"
     q3 = q.reshape(q.shape[0], q.shape[1], q.shape[-1]) if q.dim() == 4 else q
-    dt, dev, qs, ps = q3.dtype, q3.device, q3.shape, k_pages.shape
-    qst = q3.stride()
+    dt, dev, qs, ps, bs = q3.dtype, q3.device, q3.shape, k_pages.shape, block_table.shape
+    qst, pst, bst = q3.stride(), k_pages.stride(), block_table.stride()
     B = qs[0] if len(qs) == 3 else 0
     page = _q4_page(ps[2], qs[2]) if len(ps) == 3 and len(qs) == 3 else 0
-    ok = (q3.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and _q4_pools_ok(k_pages, v_pages, dev) and page > 0
-          and ps[1] > 0 and qs[1] % ps[1] == 0 and block_table.dtype == torch.int32 and kv_lens.dtype == torch.int32
-          and block_table.device == dev and kv_lens.device == dev and block_table.dim() == 2 and block_table.size(0) == B
-          and (block_table.size(1) <= 1 or block_table.stride(1) == 1) and kv_lens.shape == (B,) and kv_lens.is_contiguous()
+    ok = (q3.is_cuda and dt in _DTYPES and len(qs) == 3 and qst[2] == 1 and _q4_pools_ok(k_pages, v_pages, pst, dev) and page > 0
+          and ps[1] > 0 and qs[1] % ps[1] == 0 and _q4_index_ok(block_table, bs, bst, kv_lens, B, dev)
           and (sel is None) == (sel_off is None))
     if out is None:
         out = _empty_like(q3)
     elif ok:
         ok = out.shape == qs and out.dtype == dt and out.device == dev and out.stride(2) == 1
-    sargs, R, width = (None, 0, 0, 0, None, 0, 0, 0), ps[1] if len(ps) == 3 else 1, block_table.size(-1) if ok else 0
+    sargs, R, width = (None, 0, 0, 0, None, 0, 0, 0), ps[1] if len(ps) == 3 else 1, bs[1] if ok else 0
     if ok and sel is not None:
         ss, sst = sel.shape, sel.stride()
-        ok = (sel.dtype == torch.int32 and sel_off.dtype == torch.int32 and sel.device == dev and sel_off.device == dev
+        ok = (sel.dtype == _I32 and sel_off.dtype == _I32 and sel.device == dev and sel_off.device == dev
               and len(ss) == 3 and ss[0] == B and (ss[1] == qs[1] or ss[1] == ps[1]) and sel_off.shape == (B, ss[1], 2)
               and (ss[2] <= 1 or sst[2] == 1) and sel_off.stride(2) == 1)
         if ok:
@@ -1339,7 +1340,6 @@ def paged_sparse_decode_q4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         B, Hq, R, D, min(width * page, 1 << 30), sel is not None, num_splits), dev)
     ost = out.stride()
     _call("sa_decode_q4", dev.index, _DTYPES[dt], q3.data_ptr(), qst[0], qst[1], k_pages.data_ptr(), v_pages.data_ptr(),
-          k_pages.stride(0), k_pages.stride(1), ps[0], block_table.data_ptr(), block_table.stride(0), block_table.size(1),
-          kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], B, Hq, ps[1], D, page, D ** -0.5, num_splits,
+          pst[0], pst[1], ps[0], block_table.data_ptr(), bst[0], bs[1], kv_lens.data_ptr(), *sargs, out.data_ptr(), ost[0], ost[1], B, Hq, ps[1], D, page, D ** -0.5, num_splits,
           *_ws_bytes(ws))
     return out.reshape(q.shape) if q.dim() == 4 else out
