@@ -192,17 +192,25 @@ class HipBlockSparseBackend(AttentionBackend):
         self._last_actual_backend = "hip_block_sparse"
         return out
 
+    @staticmethod
+    def _check_store(q: torch.Tensor, store) -> None:
+        # 4-bit pools are bytes: what type they were written for is the store's to say.
+        if getattr(store, "bits", 16) == 4 and q.dtype != store.dtype:
+            raise ValueError(f"queries of {q.dtype} over a 4-bit store of {store.dtype}")
+
     def forward_paged(self, q: torch.Tensor, store, pattern: PatternMetadata) -> torch.Tensor:
         """One decode token per sequence (``q [B, H, 1, D]``) against a paged store.
 
         ``store`` is a :class:`~sparseattentioninfer_amd.models.kv_cache.PagedKVStore` already
         holding the new token; the pattern's single CSR query block (the row of the last
-        position) is shared by the batch, and its block size must equal the page size.
+        position) is shared by the batch, and its block size must equal the page size.  Stores of 4 bits run
+        ``ops.paged_sparse_decode_q4``.
         """
         if not q.is_cuda:
             raise RuntimeError("hip_block_sparse runs on ROCm GPU tensors only")
         if q.size(2) != 1:
             raise ValueError(f"forward_paged decodes one token per sequence; got T_q={q.size(2)}")
+        self._check_store(q, store)
         pairs, offsets, bs = self._schedule(1, store.seq_len(), store.heads, q.device, pattern)
         if bs != store.page:
             raise ValueError(f"schedule block {bs} differs from the cache page {store.page}")
@@ -211,8 +219,8 @@ class HipBlockSparseBackend(AttentionBackend):
         B, R = q.size(0), pairs.size(0)
         sel = pairs.contiguous()[None].expand(B, R, pairs.size(1))
         sel_off = offsets.contiguous()[None].expand(B, R, 2)
-        out = ops.paged_sparse_decode(q, store.k_pages, store.v_pages, store.block_table, store.kv_lens,
-                                      sel, sel_off, num_splits=0)
+        decode = ops.paged_sparse_decode_q4 if getattr(store, "bits", 16) == 4 else ops.paged_sparse_decode
+        out = decode(q, store.k_pages, store.v_pages, store.block_table, store.kv_lens, sel, sel_off, num_splits=0)
         self.last_kernel = "decode"
         self._last_actual_backend = "hip_block_sparse"
         return out
@@ -223,13 +231,21 @@ class HipBlockSparseBackend(AttentionBackend):
         ``q [N, H, D]`` packs the new tokens of all sequences, any number of them each, as the ``chunk`` that
         :meth:`~sparseattentioninfer_amd.models.kv_cache.PagedKVStore.append` returned lists them; the store
         already holds their keys and values.  ``kind == "dense"`` attends the whole cache; ``"block_topk"`` the
-        pages that the store's key bounds rank highest for each query (single tokens) or block of 64 queries.
+        pages that the store's key bounds rank highest for each query (single tokens) or block of 64 queries.  Stores
+        of 4 bits run the operators of a 4-bit cache.
         """
         if not q.is_cuda:
             raise RuntimeError("hip_block_sparse runs on ROCm GPU tensors only")
+        self._check_store(q, store)
         paged = (store.k_pages, store.v_pages, store.block_table)
+        decode, attend = ops.paged_sparse_decode, ops.paged_chunk_attn
+        if getattr(store, "bits", 16) == 4:
+            decode, attend = ops.paged_sparse_decode_q4, ops.paged_chunk_attn_q4
         if pattern.kind == "dense":
-            out = ops.paged_chunk_attn(q, *paged, chunk.cu_seqlens, store.kv_lens)
+            if getattr(store, "bits", 16) == 4 and chunk.single_tokens:
+                out = decode(q, *paged, store.kv_lens)
+            else:
+                out = attend(q, *paged, chunk.cu_seqlens, store.kv_lens)
         elif pattern.kind == "block_topk":
             if store.k_bounds is None:
                 raise ValueError("block_topk needs a paged store with key bounds (bounds=True)")
@@ -238,11 +254,11 @@ class HipBlockSparseBackend(AttentionBackend):
             pick = dict(page=store.page, top_k=pattern.topk, sink=pattern.sink, recent=pattern.recent)
             if chunk.single_tokens:
                 sel, off = ops.paged_block_select(q, store.k_bounds, store.block_table, store.kv_lens, **pick)
-                out = ops.paged_sparse_decode(q, *paged, store.kv_lens, sel, off, num_splits=0)
+                out = decode(q, *paged, store.kv_lens, sel, off, num_splits=0)
             else:
                 sel, off = ops.paged_block_select(q, store.k_bounds, store.block_table, store.kv_lens,
                                                   cu_seqlens=chunk.cu_seqlens, **pick)
-                out = ops.paged_chunk_attn(q, *paged, chunk.cu_seqlens, store.kv_lens, sel=sel, sel_off=off)
+                out = attend(q, *paged, chunk.cu_seqlens, store.kv_lens, sel=sel, sel_off=off)
         else:
             raise NotImplementedError(f"forward_packed runs dense and block_topk patterns, not {pattern.kind!r}")
         self.last_kernel = "decode" if chunk.single_tokens else "chunk"

@@ -13,7 +13,9 @@ copy) only when exceeded.
 ``[B, max_blocks]`` (logical block -> page) and the sequence lengths; pages
 are taken from a free list as sequences grow.  It is the layout
 ``sa_decode`` reads in paged mode.  ``append`` takes a chunk of new tokens whose
-number differs from sequence to sequence.
+number differs from sequence to sequence.  With ``bits=4`` the pages hold 4-bit
+codes with a scale and a minimum for each 32 dims (``ops.paged_append_q4``),
+3.2 times fewer bytes.
 """
 from __future__ import annotations
 
@@ -137,11 +139,19 @@ class PagedKVStore:
     sequences grow; ``lens`` counts the valid tokens per sequence on the host
     and ``kv_lens`` mirrors it on the device.  With ``bounds`` (on the GPU) ``k_bounds [P, H, 2, D]`` keeps
     the smallest and largest key of each page in each dim, which ``ops.paged_block_select`` ranks pages by.
+    With ``bits=4`` (on the GPU) the pools are uint8 ``[P, H, ops.q4_block_bytes(page, D)]``, for tensors of ``dtype``; what
+    is read and attended is what the codes stand for.
     """
 
     def __init__(self, batch: int, heads: int, head_dim: int, max_len: int, *, page: int = 64,
                  dtype=torch.bfloat16, device="cuda", num_pages: int | None = None,
-                 shuffle_seed: int | None = None, bounds: bool = False):
+                 shuffle_seed: int | None = None, bounds: bool = False, bits: int = 16):
+        if bits not in (4, 16):
+            raise ValueError(f"a PagedKVStore holds 16 or 4 bits, not {bits}")
+        if bits == 4 and torch.device(device).type != "cuda":
+            raise ValueError("a PagedKVStore of 4 bits lives on the GPU (its append kernel quantises)")
+        if bits == 4 and (dtype not in (torch.bfloat16, torch.float16) or head_dim not in (64, 128)):
+            raise ValueError(f"a PagedKVStore of 4 bits holds fp16 or bf16 heads of 64 or 128 dims, not {dtype} of {head_dim}")
         if bounds and torch.device(device).type != "cuda":
             raise ValueError("a PagedKVStore with key bounds lives on the GPU (its append kernel keeps them)")
         if page % 16 or not 16 <= page <= 128:
@@ -149,7 +159,11 @@ class PagedKVStore:
         self.batch, self.heads, self.head_dim, self.page = batch, heads, head_dim, page
         self.max_blocks = -(-max_len // page)
         self.num_pages = num_pages if num_pages is not None else batch * self.max_blocks
-        self.k_pages = torch.empty(self.num_pages, heads, page, head_dim, dtype=dtype, device=device)
+        self.bits, self.dtype = bits, dtype
+        if bits == 4:
+            self.k_pages = torch.empty(self.num_pages, heads, ops.q4_block_bytes(page, head_dim), dtype=torch.uint8, device=device)
+        else:
+            self.k_pages = torch.empty(self.num_pages, heads, page, head_dim, dtype=dtype, device=device)
         self.v_pages = torch.empty_like(self.k_pages)
         self.k_bounds = torch.zeros(self.num_pages, heads, 2, head_dim, dtype=dtype, device=device) if bounds else None
         self.block_table = torch.zeros(batch, self.max_blocks, dtype=torch.int32, device=device)
@@ -214,7 +228,7 @@ class PagedKVStore:
 
         Keys are normed (``k_weight``) and rotated (``inv_freq``, by their places in the cache or by ``positions``
         int64 ``[N]``) on the way where those are given, and queries ``q [N, Hq, D]`` with them
-        (:func:`~sparseattentioninfer_amd.ops.paged_append`, one launch).  A call that is refused leaves the store as it was.
+        (:func:`~sparseattentioninfer_amd.ops.paged_append` or, in 4 bits, ``paged_append_q4``; one launch).  A call that is refused leaves the store as it was.
         Nothing here waits for the GPU.  The lengths are kept on the host, so the call cannot be captured into a graph.
         """
         if self.kv_lens.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -234,9 +248,12 @@ class PagedKVStore:
                 self.kv_lens.fill_(new_lens[0])
             else:
                 self.kv_lens.copy_(self._upload(new_lens))
-            q_out = ops.paged_append(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
-                                     inv_freq=inv_freq, positions=positions, k_weight=k_weight, eps=eps,
-                                     k_bounds=self.k_bounds, q=q, q_weight=q_weight)
+            if self.bits == 4 and k_new.dtype != self.dtype:
+                raise ValueError(f"tensors of {k_new.dtype} for a store of {self.dtype}")
+            write = ops.paged_append_q4 if self.bits == 4 else ops.paged_append
+            q_out = write(k_new, v_new, self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens,
+                          inv_freq=inv_freq, positions=positions, k_weight=k_weight, eps=eps, k_bounds=self.k_bounds,
+                          q=q, q_weight=q_weight)
         except BaseException:
             self._shrink_each(blocks)
             self.kv_lens.copy_(torch.tensor(self.lens, dtype=torch.int32))
@@ -252,11 +269,24 @@ class PagedKVStore:
         if self.k_bounds is None or first >= last:
             return
         pages = self.block_table[:, first:last].long()                         # [B, nb]
-        k = self.k_pages[pages]                                                 # [B, nb, H, page, D]
+        if self.bits == 4:                                                      # what the keys are read back as
+            t = n - first * self.page
+            k = torch.zeros(self.batch, (last - first) * self.page, self.heads, self.head_dim, dtype=self.dtype,
+                            device=self.kv_lens.device)
+            k[:, :t] = self._read(t)[0].unflatten(0, (self.batch, t))
+            k = k.unflatten(1, (last - first, self.page)).transpose(2, 3)
+        else:
+            k = self.k_pages[pages]                                             # [B, nb, H, page, D]
         pos = torch.arange(first * self.page, last * self.page, device=k.device).view(-1, 1, self.page, 1)
         held = (pos < n) & ~k.isnan()
         lo, hi = torch.where(held, k, math.inf).amin(3), torch.where(held, k, -math.inf).amax(3)
         self.k_bounds[pages] = torch.stack([lo, hi], dim=3)
+
+    def _read(self, t: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The last ``t`` tokens of each sequence of a 4-bit store, ``[B * t, H, D]`` keys and values."""
+        cu = torch.arange(self.batch + 1, dtype=torch.int32, device=self.kv_lens.device) * t
+        return ops.paged_read_q4(self.k_pages, self.v_pages, self.block_table, cu, self.kv_lens, rows=self.batch * t,
+                                 head_dim=self.head_dim, dtype=self.dtype)
 
     def _page_col(self, lb: int) -> torch.Tensor:
         """Pages of logical block ``lb`` for every sequence, as a device index tensor (cached)."""
@@ -273,8 +303,8 @@ class PagedKVStore:
             raise ValueError(f"write of {tuple(k_new.shape)} into a [{self.batch}, {self.heads}, *, "
                              f"{self.head_dim}] store")
         start = self._uniform_len("write")
-        if self.k_bounds is not None:      # the append kernel keeps the bounds
-            k, v = (x.to(self.k_pages.dtype).transpose(1, 2).reshape(B * t, H, D) for x in (k_new, v_new))
+        if self.k_bounds is not None or self.bits == 4:      # the append kernel keeps the bounds, and quantises
+            k, v = (x.to(self.dtype).transpose(1, 2).reshape(B * t, H, D) for x in (k_new, v_new))
             self.append(k, v, [t] * B)
             return
         self._grow_all(start + t)
@@ -296,6 +326,9 @@ class PagedKVStore:
     def gather(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Contiguous ``[B, H, T, D]`` copies of the cached K/V (slow path for generic callers)."""
         T = self._uniform_len("gather")
+        if self.bits == 4:
+            k, v = (x.view(self.batch, T, self.heads, self.head_dim).transpose(1, 2).contiguous() for x in self._read(T))
+            return k, v
         nb = -(-T // self.page)
         pages = self.block_table[:, :nb].long()                         # [B, nb]
         k = self.k_pages[pages].permute(0, 2, 1, 3, 4).reshape(self.batch, self.heads, nb * self.page, -1)

@@ -33,7 +33,9 @@ up projections with the SwiGLU in its epilogue (``sa_gemm_skinny_swiglu``, on
 the weights interleaved once), the down GEMM and ``sa_rmsnorm`` (residual add +
 the next layer's input norm).  ``fused=False`` calls the model's
 own modules instead (Hugging Face's arithmetic op by op, about 66 launches per
-layer).
+layer).  Over a cache of 4 bits (``PagedKVCache(bits=4)``) the write is
+``sa_paged_append_q4`` (norms, rotation, quantisation) and the decode
+``sa_decode_q4``.
 
 The graph holds no ``hipMemsetAsync`` node: the argmax over the vocabulary is
 taken in two small stages, so no multi-block reduction needs a zeroed
@@ -114,6 +116,9 @@ class _LayerSchedule:
         self.row_of = row_of
         self.sel = self.sel_off = None  # views of the decoder's gathered selections (set by the decoder)
         self.rows = R
+        if getattr(store, "bits", 16) == 4:      # the call picks its splits and takes its workspace itself
+            self.num_splits, self.workspace = 0, None
+            return
         self.num_splits = ops.decode_splits(batch, H, R, self.width)   # as the eager paged decode picks it
         need = ops.decode_workspace_bytes(batch, H, D, self.num_splits)
         self.workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
@@ -171,6 +176,7 @@ class GraphDecoder:
         # device state
         self.ids = ids.reshape(self.B).to(torch.long).clone()
         self.pos = torch.full((1,), self.start, dtype=torch.long, device=self.dev)
+        self.cu = torch.arange(self.B + 1, dtype=torch.int32, device=self.dev)   # one new token each (4-bit stores)
         self.graph = None
         self.warmup = warmup
         self.steps_done = 0
@@ -235,13 +241,17 @@ class GraphDecoder:
         for i, (layer, store, sched) in enumerate(zip(self.layers, self.stores, self.sched)):
             attn = layer.self_attn
             ops.gemm_skinny(self.x, self.w_qkv[i], out=self.qkv)
-            ops.qk_rope_kv(self.qkv, attn.q_norm.weight, attn.k_norm.weight, self.inv_freq, self.pos, store, self.q,
-                           num_heads=self.num_heads, eps=self.eps)
-            ops.paged_sparse_decode(
-                self.q, store.k_pages, store.v_pages, store.block_table, self.kv_lens,
-                sched.sel.expand(B, sched.rows, sched.width), sched.sel_off.expand(B, sched.rows, 2),
-                num_splits=sched.num_splits, workspace=sched.workspace if sched.num_splits > 1 else None,
-                out=self.att)
+            if getattr(store, "bits", 16) == 4:
+                heads = self.qkv.view(B, -1, self.head_dim)
+                H, Hkv = self.num_heads, store.heads
+                ops.paged_append_q4(heads[:, H:H + Hkv], heads[:, H + Hkv:], store.k_pages, store.v_pages,
+                                    store.block_table, self.cu, self.kv_lens, inv_freq=self.inv_freq,
+                                    k_weight=attn.k_norm.weight, eps=self.eps, q=heads[:, :H],
+                                    q_weight=attn.q_norm.weight, q_out=self.q)
+            else:
+                ops.qk_rope_kv(self.qkv, attn.q_norm.weight, attn.k_norm.weight, self.inv_freq, self.pos, store, self.q,
+                               num_heads=self.num_heads, eps=self.eps)
+            self._attend(self.q, store, sched, self.kv_lens, self.att)
             ops.gemm_skinny(self.att.view(B, -1), attn.o_proj.weight, out=self.a)
             ops.rmsnorm(self.a, layer.post_attention_layernorm.weight, self.eps, residual=self.h, out=self.x)
             ops.gemm_skinny_swiglu(self.x, self.w_gu[i], out=self.mid)
@@ -256,6 +266,14 @@ class GraphDecoder:
             self.logits.copy_(self.lg)
         self.ids.copy_(_argmax_rows(self.lg, self.chunk))
         self.pos.add_(1)
+
+    def _attend(self, q, store, sched, kv_lens, out=None) -> torch.Tensor:
+        """The layer's paged decode over the selection at hand."""
+        B = self.B
+        decode = ops.paged_sparse_decode_q4 if getattr(store, "bits", 16) == 4 else ops.paged_sparse_decode
+        return decode(q, store.k_pages, store.v_pages, store.block_table, kv_lens,
+                      sched.sel.expand(B, sched.rows, sched.width), sched.sel_off.expand(B, sched.rows, 2),
+                      num_splits=sched.num_splits, workspace=sched.workspace if sched.num_splits > 1 else None, out=out)
 
     def _merge_selections(self) -> None:
         """Stacks the distinct combinations of every schedule's selection (one per position the run
@@ -316,13 +334,14 @@ class GraphDecoder:
             v = attn.v_proj(x).view(shape).transpose(1, 2)
             q, k = apply_rotary_pos_emb(q, k, cos, sin)
             pg = store.block_table.index_select(1, blk).view(B).long()
-            store.k_pages[pg, :, slot] = k[:, :, 0].to(store.k_pages.dtype)
-            store.v_pages[pg, :, slot] = v[:, :, 0].to(store.v_pages.dtype)
             store.kv_lens.copy_(kv_len)
-            out = ops.paged_sparse_decode(
-                q.reshape(B, attn.num_heads, D).contiguous(), store.k_pages, store.v_pages, store.block_table,
-                store.kv_lens, sched.sel.expand(B, sched.rows, sched.width), sched.sel_off.expand(B, sched.rows, 2),
-                num_splits=sched.num_splits, workspace=sched.workspace if sched.num_splits > 1 else None)
+            if getattr(store, "bits", 16) == 4:
+                ops.paged_append_q4(k[:, :, 0].to(store.dtype), v[:, :, 0].to(store.dtype), store.k_pages, store.v_pages,
+                                    store.block_table, self.cu, store.kv_lens)
+            else:
+                store.k_pages[pg, :, slot] = k[:, :, 0].to(store.k_pages.dtype)
+                store.v_pages[pg, :, slot] = v[:, :, 0].to(store.v_pages.dtype)
+            out = self._attend(q.reshape(B, attn.num_heads, D).contiguous(), store, sched, store.kv_lens)
             h = res + attn.o_proj(out.reshape(B, 1, -1))
             res = h
             h = res + layer.mlp(layer.post_attention_layernorm(h))

@@ -22,9 +22,9 @@ class PagedKVLayer(CacheLayerMixin):
     is_sliding = False
     is_compileable = False
 
-    def __init__(self, max_len: int, *, page: int = 64, shuffle_seed: int | None = None, bounds: bool = False):
+    def __init__(self, max_len: int, *, page: int = 64, shuffle_seed: int | None = None, bounds: bool = False, bits: int = 16):
         super().__init__()
-        self.max_len, self.page, self.shuffle_seed, self.bounds = max_len, page, shuffle_seed, bounds
+        self.max_len, self.page, self.shuffle_seed, self.bounds, self.bits = max_len, page, shuffle_seed, bounds, bits
         self.store: PagedKVStore | None = None
 
     def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
@@ -34,7 +34,7 @@ class PagedKVLayer(CacheLayerMixin):
     def _make_store(self, B: int, H: int, D: int, like: torch.Tensor) -> None:
         self.dtype, self.device = like.dtype, like.device
         self.store = PagedKVStore(B, H, D, self.max_len, page=self.page, dtype=like.dtype, device=like.device,
-                                  shuffle_seed=self.shuffle_seed, bounds=self.bounds)
+                                  shuffle_seed=self.shuffle_seed, bounds=self.bounds, bits=self.bits)
         self.is_initialized = True
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, counts, **rope) -> PagedChunk:
@@ -88,13 +88,15 @@ class PagedKVLayer(CacheLayerMixin):
 
 class PagedKVCache(Cache):
     """``num_layers`` paged layers of up to ``max_len`` tokens per sequence; with ``bounds`` their pages keep the
-    key bounds that the ``"block_topk"`` pattern selects by."""
+    key bounds that the ``"block_topk"`` pattern selects by, with ``bits=4`` they hold 4-bit codes."""
 
     def __init__(self, num_layers: int, max_len: int, *, page: int = 64, shuffle_seed: int | None = None,
-                 bounds: bool = False):
-        super().__init__(layers=[PagedKVLayer(max_len, page=page, shuffle_seed=shuffle_seed, bounds=bounds)
+                 bounds: bool = False, bits: int = 16):
+        if bits not in (4, 16):
+            raise ValueError(f"a PagedKVCache holds 16 or 4 bits, not {bits}")
+        super().__init__(layers=[PagedKVLayer(max_len, page=page, shuffle_seed=shuffle_seed, bounds=bounds, bits=bits)
                                  for _ in range(num_layers)])
-        self.page = page
+        self.page, self.bits = page, bits
 
     @property
     def max_cache_len(self) -> int:

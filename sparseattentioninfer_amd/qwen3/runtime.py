@@ -73,13 +73,15 @@ def _sync(device):
 
 @torch.inference_mode()
 def greedy_generate(model, input_ids: torch.Tensor, steps: int, *, cache: str = "paged",
-                    max_len: int | None = None, shuffle_seed: int | None = None, graph: bool = False) -> dict:
+                    max_len: int | None = None, shuffle_seed: int | None = None, graph: bool = False,
+                    cache_bits: int = 16) -> dict:
     """Prompt forward (timed: TTFT) then ``steps`` greedy decode forwards (each timed).
 
     ``cache``: ``"paged"`` (:class:`PagedKVCache`, decode reads pages) or
     ``"dynamic"`` (HF ``DynamicCache``).  ``graph`` (paged cache only): decode
     with :class:`~sparseattentioninfer_amd.qwen3.graph_decode.GraphDecoder`, one
     HIP graph replay per token, instead of the eager Hugging Face forward.
+    ``cache_bits=4`` (paged cache only) holds the cache in 4 bits.
     Returns the timings, the generated ids ``[B, steps + 1]`` and the
     last-position logits of the prompt forward.
     """
@@ -89,7 +91,9 @@ def greedy_generate(model, input_ids: torch.Tensor, steps: int, *, cache: str = 
     if cache == "paged":
         pkv = PagedKVCache(cfg.num_hidden_layers, max_len or (T + steps + 1),
                            page=getattr(cfg, "sparse_attention_block_size", 64), shuffle_seed=shuffle_seed,
-                           bounds=getattr(cfg, "sparse_attention_pattern", None) == "block_topk")
+                           bounds=getattr(cfg, "sparse_attention_pattern", None) == "block_topk", bits=cache_bits)
+    elif cache_bits != 16:
+        raise ValueError("only the paged cache holds 4 bits")
     elif cache == "dynamic":
         from transformers.cache_utils import DynamicCache
         pkv = DynamicCache(config=cfg)

@@ -157,3 +157,19 @@ def test_attention_refuses_cpu_tensors():
         ops.paged_chunk_attn_q4(x, pool, pool, i(0)[None], i(0, 1), i(1))
     with pytest.raises(AssertionError, match="on the GPU"):
         ops.paged_sparse_decode_q4(x, pool, pool, i(0)[None], i(1))
+
+
+def test_stores_and_caches_of_4_bits_say_what_they_hold():
+    from sparseattentioninfer_amd.models import PagedKVStore
+    from sparseattentioninfer_amd.qwen3 import PagedKVCache
+    with pytest.raises(ValueError, match="16 or 4 bits"):
+        PagedKVStore(1, 1, 64, 64, device="cpu", bits=8)
+    with pytest.raises(ValueError, match="GPU"):
+        PagedKVStore(1, 1, 64, 64, device="cpu", bits=4)
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        PagedKVStore(1, 1, 64, 64, device="cuda", bits=4, dtype=torch.float32)
+    with pytest.raises(ValueError, match="64 or 128"):
+        PagedKVStore(1, 1, 96, 64, device="cuda", bits=4)
+    with pytest.raises(ValueError, match="16 or 4 bits"):
+        PagedKVCache(1, 64, bits=2)
+    assert PagedKVStore(1, 1, 64, 64, device="cpu").bits == 16 and PagedKVCache(2, 64, bits=4).layers[1].bits == 4
