@@ -108,12 +108,16 @@ struct Group4 {
     mx = fmaxf(mx, dpp<0x4E>(mx));
     odd += dpp<0x4E>(odd);
     // Halves: the range of large bf16 values passes fp32's.
-    const float half = 0.5f * mn;
-    float s = cut(fmaf(0.5f, mx, -half) / 7.5f);
+    const float half = 0.5f * mn, range = fmaf(0.5f, mx, -half);
+    // range / 7.5 toward zero to the element type: a quotient that is too large, by less than 2^-21 of it (2^-22, and three
+    // roundings of 2^-24), cut, and one step less where 7.5 of it (exact: 15 times at most 11 bits) pass the range.
+    float s = cut(range * (1.f / 7.5f) * 1.0000002384185791f);
+    s = fmaf(s, 7.5f, -range) > 0.f ? step_down(s) : s;
     s = s < 1.17549435e-38f ? 0.f : s;
-    // 2 / s, and so much more that the rounded products below never bring a tie under the code it goes up to: 2^-22
-    // against 2^-24 each of the quotient and the product.
-    const float r = s > 0.f ? 2.f / s * 1.0000002384185791f : 0.f;
+    // 2 / s, and so much more that the rounded products below never bring a tie under the code it goes up to: 2^-21
+    // against 2^-23 of the reciprocal after one Newton step and 2^-24 each of the difference and of the two products.
+    const float r0 = __builtin_amdgcn_rcpf(s);
+    const float r = s > 0.f ? fmaf(fmaf(-s, r0, 1.f), r0, r0) * 2.0000009536743164f : 0.f;
     uint32_t c[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) c[e] = (uint32_t)fminf(fmaf(fmaf(0.5f, x[e], -half), r, 0.5f), 15.f);
@@ -126,7 +130,12 @@ struct Group4 {
   static __device__ __forceinline__ float cut(float s) {
     if constexpr (BF16) return __uint_as_float(__float_as_uint(s) & 0xffff0000u);
     const float t = Elem<false>::to_f32(Elem<false>::from_f32(s));
-    return t > s ? Elem<false>::to_f32((elem_t)(Elem<false>::from_f32(s) - 1)) : t;
+    return t > s ? step_down(t) : t;
+  }
+  // The next smaller value of the element type; x > 0 is one.
+  static __device__ __forceinline__ float step_down(float x) {
+    if constexpr (BF16) return __uint_as_float(__float_as_uint(x) - 0x10000u);
+    return Elem<false>::to_f32((elem_t)(Elem<false>::from_f32(x) - 1));
   }
   // The lane's 8 values as they are read back.
   __device__ __forceinline__ u32x4 values() const {
