@@ -586,7 +586,9 @@ int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks)
  *           bits) and 32 g + 16 + i (high), i < 16
  * then the pairs (s, m) of type T, [D / 32][page].
  *
- * What a slot holds that no token was written to is never used, whatever its bytes.
+ * What a slot holds that no token was written to is never used, whatever its bytes.  A token whose key reads back as NaN
+ * makes NaN of the rows that see it and of no others.  One whose value does makes NaN of those dims in the rows that see it,
+ * and in a chunk possibly in rows before it as well: they share its tile, where its weight of 0 meets the NaN.
  */
 
 /*

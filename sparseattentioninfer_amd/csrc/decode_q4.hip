@@ -6,7 +6,8 @@
 // A workgroup has the query heads of one list (up to 8 at D = 128, 16 at 64) and `unit` steps of 32 keys of it, which its
 // four waves take in turn; a longer list is shared by workgroups whose fp32 partials a second kernel merges.  The unit is
 // the same for all lists, so the workgroups' loads are even whatever the lengths.  Over whole caches every workgroup works
-// it out for itself and finds its list by a scan of the lengths: the launch is as large as any lengths need, and what is past the last list leaves at once.
+// it out for itself and finds its list by a scan of the lengths: the launch is as large as any lengths need, and what is past
+// the last list leaves at once.
 #include <algorithm>
 
 #include "attn_q4.h"
@@ -124,7 +125,8 @@ struct DecodeQ4Item {
   // ends first.  While the shares run at once that is when the longest ends; else the mean load and half the longest.
   // (Equal lists are best left whole or cut evenly, uneven ones finely: 28 sequences of 64 to 30,000 tokens, 8 KV heads,
   // 141 us with even shares, 114 with 0.38 of one; 64 of 4,096 67 us whole, 79 in two.)  Sums are fp32; the margin
-  // above their rounding keeps the shares within DQ_MOST.
+  // above their rounding keeps the shares within DQ_MOST, and a unit of no division is one step more where fp32 may have
+  // rounded the longest list down (past 2^24 steps, of at most 2^25).
   __device__ __forceinline__ void plan(const DecodeQ4Args& a, int len64, int of_seq) {
     unit = a.unit;
     if (unit) return;
@@ -150,7 +152,8 @@ struct DecodeQ4Item {
 #pragma unroll
     for (int c = 0; c < 5; ++c) {
       const float f = c == 1 ? 1.f : c == 2 ? 0.76f : c == 3 ? 0.5f : 0.381f;
-      u[c] = c ? max(DQ_MIN_UNIT, (int)ceilf(even * f)) : max(1, (int)longest);
+      u[c] = c ? max(DQ_MIN_UNIT, (int)fminf(ceilf(even * f), 33554432.f))
+             : max(1, (int)longest + (longest >= 16777216.f ? 1 : 0));
       groups[c] = share[c] = 0.f;
       weigh(c, (float)n64);
     }

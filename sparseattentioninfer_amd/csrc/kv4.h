@@ -26,7 +26,6 @@ struct Kv4 {
   static constexpr int ROW = D / 2;        // bytes of codes of a token
   static constexpr int QUAD = 2 * D;       // bytes of codes of four tokens
   static __device__ __host__ constexpr int stats_at(int page) { return page * ROW; }   // byte of the first pair
-  static __device__ __host__ constexpr int block_bytes(int page) { return page * (ROW + 4 * NG); }
 };
 
 // Loads and words of a lane: NG of them, 8 or 16 bytes.
