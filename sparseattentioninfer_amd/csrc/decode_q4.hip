@@ -147,28 +147,25 @@ struct DecodeQ4Item {
     const float even = sum * (1.001f / DQ_TARGET);
     int u[5];
     float rcp[5], groups[5], share[5];
-    // Shares as shares() counts them.  The reciprocal is off by a step for some units (of 1,535, times 1,535 it passes 1), so
-    // the product is corrected; it is off by one at most, as no list has more than DQ_MOST shares and one.
-    auto weigh = [&](int c, int n) {
-      const int x = n + u[c] - 1;
-      int q = (int)((float)x * rcp[c]);
-      q += (q + 1) * u[c] <= x ? 1 : 0;
-      q -= q * u[c] > x ? 1 : 0;
-      const float k = (float)max(1, q);
-      groups[c] += n > 0 ? k : 0.f;
-      share[c] = fmaxf(share[c], (float)n * __builtin_amdgcn_rcpf(k));
+    // Shares as shares() counts them, up to 2^20 steps (past that a rest of a step may go uncounted).  The reciprocal is off by
+    // a step for some units (of 1,535, times 1,535 it passes 1): with 2^-21 less than it the product stays below a whole
+    // number that it should be (2^-23 and three roundings of 2^-24), and above one that n passes by a step.
+    auto weigh = [&](int c, float n) {
+      const float k = fmaxf(1.f, ceilf(n * rcp[c]));
+      groups[c] += n > 0.f ? k : 0.f;
+      share[c] = fmaxf(share[c], n * __builtin_amdgcn_rcpf(k));
     };
 #pragma unroll
     for (int c = 0; c < 5; ++c) {
       const float f = c == 1 ? 1.f : c == 2 ? 0.76f : c == 3 ? 0.5f : 0.381f;
       u[c] = c ? max(DQ_MIN_UNIT, (int)fminf(ceilf(even * f), 33554432.f))
              : max(1, (int)longest + (longest >= 16777216.f ? 1 : 0));
-      rcp[c] = __builtin_amdgcn_rcpf((float)u[c]);
+      rcp[c] = __builtin_amdgcn_rcpf((float)u[c]) * 0.9999995231628418f;
       groups[c] = share[c] = 0.f;
-      weigh(c, n64);
+      weigh(c, (float)n64);
     }
     for (int s = 64 + lane; s < a.B; s += 64) {
-      const int n = a.steps(a.length(s));
+      const float n = (float)a.steps(a.length(s));
 #pragma unroll
       for (int c = 0; c < 5; ++c) weigh(c, n);
     }
