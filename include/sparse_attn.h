@@ -579,8 +579,11 @@ int64_t sa_paged_block_select_workspace_bytes(int rows, int Hkv, int max_blocks)
  * A pool is [num_pages, Hkv] blocks of page * D * 5 / 8 bytes (strides of pages and heads in bytes, blocks 16-byte aligned),
  * written for one element type T, the dtype of the calls that read it.  32 dims of one token's head are a group, held as
  * m + s c: m = min x, s = (max x - min x) / 15 toward zero to T (a scale below 2^-126 is 0), c = floor((x - m) / s + 1/2)
- * and at most 15, 0 where s is.  x is of type T, so a value is off by at most s / 2 (the group's largest by at most what
- * cutting s takes from 15 s: 0.12 s in bf16).  A group with a NaN or an infinity reads back as NaN.  In a block, first the codes:
+ * and at most 15, 0 where s is.  x is of type T, so a value is off by at most s / 2 or, past the code 15, by what 15 s leave
+ * of the range.  That is less than 0.12 s, but in fp16 up to 15 of its smallest steps 2^-24 where s is a subnormal (below
+ * 2^-14), and in bf16 up to 15 2^-126 where s is 0.  Ranges and quotients are formed in fp32: one less than 2^-20 of itself
+ * below the border to the next s or c may be taken for the border.  A group with a NaN or an infinity reads back as NaN.  In a
+ * block, first the codes:
  *   keys    word (D / 32) q + g of a token's D / 2 bytes: dims 32 g + 8 q + e at bit 8 (e % 4) + 4 (e / 4), e < 8
  *   values  byte t % 4 of word (D / 32) i + g of the 2 D bytes that tokens t with one t / 4 share: dims 32 g + i (low four
  *           bits) and 32 g + 16 + i (high), i < 16

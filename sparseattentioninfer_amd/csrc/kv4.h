@@ -3,9 +3,11 @@
 // 32 dims of one token's head are a group, held as m + s c with codes c of 4 bits:
 //   m = min x,   s = (max x - min x) / 15, toward zero to the element type,   c = min(floor((x - m) / s + 1/2), 15).
 // x is of the element type (what a 16-bit cache would hold), so m is exact.  s is cut and not rounded, so that no value
-// is read back past the group's largest; the largest is then off by at most 15 s 2^-7 (bf16), less than the half step
-// s / 2 that bounds the others.  A scale below 2^-126 is taken for 0, and c for 0 with it.  A group with a NaN or an
-// infinity has s = m = NaN.
+// is read back past the group's largest.  A value is off by at most s / 2 or, past the code 15, by what the cut leaves of the
+// range, max x - min x - 15 s: less than 15 s 2^-7 (bf16) and 15 s 2^-10 (fp16), which is less than s / 2, but 15 2^-24 where
+// s is one of fp16's subnormal multiples of 2^-24.  A scale below 2^-126 (bf16) is taken for 0, and c for 0 with it: off by
+// less than 15 2^-126.  Ranges and quotients are formed in fp32: one less than 2^-20 of itself below the border to the next s
+// or c may be taken for the border, which moves the bound by that much.  A group with a NaN or an infinity has s = m = NaN.
 //
 // First the codes, page * D / 2 bytes; then (s, m) pairs of the element type, [D / 32][page].  The order of the codes is
 // that of the matrix instructions' operands, so that attention takes them from memory to registers with 16-byte loads

@@ -114,12 +114,14 @@ struct Group4 {
     // Halves: the range of large bf16 values passes fp32's.
     const float half = 0.5f * mn, range = fmaf(0.5f, mx, -half);
     // range / 7.5 toward zero to the element type: a quotient that is too large, by less than 2^-21 of it (2^-22, and three
-    // roundings of 2^-24), cut, and one step less where 7.5 of it (exact: 15 times at most 11 bits) pass the range.
+    // roundings of 2^-24), cut, and one step less where 7.5 of it (exact: 15 times at most 11 bits) pass the range as
+    // fp32 holds it.
     float s = cut(range * (1.f / 7.5f) * 1.0000002384185791f);
     s = fmaf(s, 7.5f, -range) > 0.f ? step_down(s) : s;
     s = s < 1.17549435e-38f ? 0.f : s;
     // 2 / s, and so much more that the rounded products below never bring a tie under the code it goes up to: 2^-21
-    // against 2^-23 of the reciprocal after one Newton step and 2^-24 each of the difference and of the two products.
+    // against 2^-23 of the reciprocal after one Newton step and 2^-24 each of the difference and of the two products.  A
+    // quotient less than 2^-20 of itself below a tie goes up with it: off by half a step and that much, as its neighbour would be.
     const float r0 = __builtin_amdgcn_rcpf(s);
     const float r = s > 0.f ? fmaf(fmaf(-s, r0, 1.f), r0, r0) * 2.0000009536743164f : 0.f;
     uint32_t c[8];

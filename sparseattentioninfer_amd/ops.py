@@ -1160,8 +1160,8 @@ def paged_append_q4(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
 
     ``k_pages, v_pages [P, Hkv, q4_block_bytes(page, D)]`` uint8; everything else is as for :func:`paged_append`, and
     the pools belong to the element type of ``k``.  Each group of 32 dims of a token's head keeps its minimum and a
-    fifteenth of its range, so a value is off by at most half of that step.  ``k_bounds [P, Hkv, 2, D]`` holds the
-    smallest and largest key per dim as they are read back.
+    fifteenth of its range, so a value is off by at most half of that step (in fp16, where the step is a subnormal, by up to
+    ``15 * 2**-24``).  ``k_bounds [P, Hkv, 2, D]`` holds the smallest and largest key per dim as they are read back.
     """
     name = "paged_append_q4"
     dt, dev, ks, ps, bs = k.dtype, k.device, k.shape, k_pages.shape, block_table.shape
