@@ -140,7 +140,7 @@ class PagedKVStore:
     and ``kv_lens`` mirrors it on the device.  With ``bounds`` (on the GPU) ``k_bounds [P, H, 2, D]`` keeps
     the smallest and largest key of each page in each dim, which ``ops.paged_block_select`` ranks pages by.
     With ``bits=4`` (on the GPU) the pools are uint8 ``[P, H, ops.q4_block_bytes(page, D)]``, for tensors of ``dtype``; what
-    is read and attended is what the codes stand for.
+    is read or attended from the pages is what the codes stand for, not the tensors that were written.
     """
 
     def __init__(self, batch: int, heads: int, head_dim: int, max_len: int, *, page: int = 64,

@@ -88,7 +88,8 @@ class PagedKVLayer(CacheLayerMixin):
 
 class PagedKVCache(Cache):
     """``num_layers`` paged layers of up to ``max_len`` tokens per sequence; with ``bounds`` their pages keep the
-    key bounds that the ``"block_topk"`` pattern selects by, with ``bits=4`` they hold 4-bit codes."""
+    key bounds that the ``"block_topk"`` pattern selects by, with ``bits=4`` they hold 4-bit codes.  A prompt into an empty
+    cache attends its own keys and values (``block_topk``: the pages), everything after it what the pages hold."""
 
     def __init__(self, num_layers: int, max_len: int, *, page: int = 64, shuffle_seed: int | None = None,
                  bounds: bool = False, bits: int = 16):
