@@ -621,7 +621,10 @@ int sa_paged_read_q4(int dtype, const void* k_pages, const void* v_pages, int64_
 
 /*
  * sa_paged_chunk_attn over such pools: causal attention of the new tokens, over every page or a selection's, with the
- * division of keys, the workspace (sa_paged_chunk_workspace_bytes) and the rules for rows and pages given there.
+ * division of keys, the workspace (sa_paged_chunk_workspace_bytes) and the rules for rows and pages given there.  A sequence's
+ * rows of a KV head (new tokens times Hq / Hkv) are taken 32 at a time where it has at most 64, and up to 8 of them at D = 128,
+ * 16 at 64, are attended as by sa_decode_q4.  For more rows keys, values and probabilities are rounded to T for the products;
+ * statistics and sums are fp32.
  */
 int sa_paged_chunk_attn_q4(int dtype, const void* q, int64_t q_st, int64_t q_sh,
                            const void* k_pages, const void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,
@@ -641,7 +644,8 @@ int sa_paged_chunk_attn_q4(int dtype, const void* q, int64_t q_st, int64_t q_sh,
  * its own length needs of the same share.  0: worked out, over whole caches on the device from the lengths; 1: one; up to
  * 64.  Partial results take sa_decode_q4_workspace_bytes() bytes where that is not 0 (rows: sel_rows, or Hkv without lists;
  * max_keys: sel_width or max_blocks times page, at most 2^30; selected: whether there are lists), 16-byte aligned, contents arbitrary,
- * which calls that may run concurrently must not share.
+ * which calls that may run concurrently must not share.  Codes enter the products as they are; a probability times its scale
+ * is rounded to bf16 (two parts of it where T is fp16), statistics and sums are fp32.
  */
 int sa_decode_q4(int dtype, const void* q, int64_t q_sb, int64_t q_sh,
                  const void* k_pages, const void* v_pages, int64_t pages_sp, int64_t pages_sh, int num_pages,

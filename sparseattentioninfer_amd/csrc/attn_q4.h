@@ -166,7 +166,10 @@ struct Q4Ring {
   }
 };
 
-// 16 NC rows of queries.  Keys and values are brought to the element type in registers: m + s c in fp32, one rounding.
+// 16 NC rows of queries.  Keys and values are brought to the element type in registers, m + s c in fp32 and one rounding, and
+// probabilities are rounded to it as well, since both products are 16-bit matrix instructions (fp32 ones have a sixteenth of
+// their rate); the sums that divide are of the unrounded ones.  Outputs are off by 0.0032 of their size in bf16 and 0.00036 in
+// fp16, their own rounding included; fp32 arithmetic on m + s c leaves 0.0017 and 0.0002, nearly all of it that rounding.
 template <bool BF16, int D, int NC, int DEPTH>
 struct Q4Dequant {
   using E = Elem<BF16>;
@@ -303,7 +306,8 @@ struct Q4Dequant {
 // the operand of column (g, r) is row r of the queries in group g and 0 in the others, so that one accumulator holds the
 // partial scores of all groups, each lane needs the pairs of one group only, and a rotation over 16 lanes adds them up.  In
 // the second product column (g, r) is p s[., g], of use in the dims of g.
-// What rounds: p s, once, to bf16.  Codes lie in 0 .. 15, so that would weigh with up to 15 s where half of it is the
+// What rounds: p s, once, to bf16, for the 16-bit product; outputs are off by 0.0023 of their size in bf16, their own rounding
+// of 0.0017 included.  Codes lie in 0 .. 15, so that would weigh with up to 15 s where half of it is the
 // values' own; sum_t (p s) 7.5, of the rounded products (a row of ones more in the matrix product), is taken out
 // and put back from the unrounded ones.  For fp16 the product is split in two bf16 parts instead, 16 bits in all.
 template <bool BF16, int D, int NQ, int DEPTH>

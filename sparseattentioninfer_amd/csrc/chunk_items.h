@@ -61,7 +61,7 @@ struct ChunkArgs {
 // ---- which workgroup does what ----------------------------------------------------------------
 //
 // A sequence of few rows (CK_NARROW or less: one token, a few drafts) is read by narrow items, 32 rows whose keys
-// four waves divide; others by wide items, 256 rows that share every key tile.  Where there are fewer items than
+// the waves of a workgroup divide (four over 16 bits, eight over 4); others by wide items, 256 rows that share every key tile.  Where there are fewer items than
 // CUs, or one sequence is much longer than the rest, each item's keys are divided over `splits` workgroups.  The
 // lengths are device memory, so the launch is as large as any lengths need and every workgroup works out the
 // division for itself, the same in all of them: `limit` key tiles to a workgroup, from the total.

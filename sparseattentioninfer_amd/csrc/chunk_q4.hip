@@ -2,14 +2,18 @@
 // caches or the pages that a selection lists for each 64-query block.  Rows, items, the division of keys and the merge
 // are those of the 16-bit cache (chunk_items.h).
 //
-// Few rows are bound by latency (8 sequences of 4 tokens over 4K, 32 + 8 heads: 23 us and 5 for the merge, for 42 MB), many by
-// vector and matrix issue (8K tokens over 32K: 3.80 ms, 1.01 PFLOP/s; a 16-bit cache reaches 1.16 to 1.24).
+// Few rows are bound by latency (8 sequences of 4 tokens over 4K, 32 + 8 heads: 23 to 24 us and 4 to 5 for the merge, for
+// 42 MB; 31 to 38 in all over a 16-bit cache), many by vector and matrix issue (8K tokens over 32K: 3.65 to 4.0 ms on four cards,
+// 0.96 to 1.05 PFLOP/s; a 16-bit cache reaches 1.16 to 1.24).
 #include "attn_q4.h"
 
 namespace sa {
 
 // What the division of keys weighs (chunk_items.h), in key tiles: 2.07 us for a wide item's, 0.77 for a narrow one's
-// with the chip full and 0.37 where it is not.
+// with the chip full and 0.37 where it is not.  With the 16-bit cache's weights 8 sequences of 4 tokens over 4K take 31.3 us
+// instead of 28.0 (replayed), 1,000 tokens beside 8 single ones over 8K 53.4 instead of 47.4, nine other batches within 3 %.
+// MERGE_ROW is in wide tiles, 0.27 ns a row; where all items are narrow it stands for 0.1 ns, and twice the number there
+// divides those eleven batches no differently.
 struct ChunkQ4Cost {
   static constexpr float MERGE_WIDE = 3.f, MERGE_NARROW = 5.f, MERGE_ROW = 1.3e-4f;
   static __device__ __forceinline__ float start(int half) { return half ? 4.6f : 12.f; }   // 9.6 us
@@ -195,7 +199,7 @@ struct ChunkQ4 {
 // A row's reference is the maximum of its first tile and is raised only when its probabilities would pass the
 // element type's range (REFIT_SUM), so the common step never touches O with vector instructions.
 // Scaling is some 88 of about 225 vector instructions of a wave's step.  256 rows are what the registers hold, and so what a
-// tile's scaling is shared by.
+// tile's scaling is shared by; each row tile of a KV head scales its key tiles again.  Roundings are those of Q4Dequant.
 template <bool BF16, int D>
 struct ChunkQ4Wide : StagedTile {
   using E = Elem<BF16>;

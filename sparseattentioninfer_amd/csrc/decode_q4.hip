@@ -9,8 +9,9 @@
 // it out for itself and finds its list by a scan of the lengths: the launch is as large as any lengths need, and what is past
 // the last list leaves at once.
 //
-// Up to 4 heads of a KV head at D = 128 are bound by HBM (64 sequences of 4,096 tokens: 67 to 72 us, 5.0 TB/s), up to 8 by
-// vector issue (75 to 80 us), few short lists by latency.
+// Up to 4 heads of a KV head at D = 128 are bound by HBM (64 sequences of 4,096 tokens, 8 KV heads, 335 MB: 67 to 72 us,
+// 4.7 to 5.0 TB/s; over 16 bits 170), up to 8 by vector issue (81 to 83 us; fp16, with two products for p s, 89 to 91),
+// few short lists by latency.
 #include <algorithm>
 
 #include "attn_q4.h"
@@ -126,10 +127,11 @@ struct DecodeQ4Item {
   }
   // The unit of a planned division: of no division, an even share of all steps and 0.76, 0.5 and 0.381 of it the one that
   // ends first.  While the shares run at once that is when the longest ends; else the mean load and half the longest.
-  // (Equal lists are best left whole or cut evenly, uneven ones finely: 28 sequences of 64 to 30,000 tokens, 8 KV heads,
-  // 141 us with even shares, 114 with 0.38 of one; 64 of 4,096 67 us whole, 79 in two.)  Sums are fp32; the margin
-  // above their rounding keeps the shares within DQ_MOST, and a unit of no division is one step more where fp32 may have
-  // rounded the longest list down (past 2^24 steps, of at most 2^25).
+  // (Equal lists are best left whole or cut evenly, uneven ones finely.  Replayed, whole / even / 0.76 / 0.5 / 0.381 of it / as
+  // planned: 28 sequences of 64 to 30,000 tokens, 40 heads, 319 / 131 / 117 / 114 / 111 / 114 us; 48 of 500 to 16,010, 32
+  // heads, 162 / 129 / 125 / 122 / 116 / 117; 64 of 4,096 71 / 71 / 92 / 76 / 80 / 72; one of 32,001 275 / 18.8 / 20.2 / 22.3 /
+  // 22.2 / 19.9.)  Sums are fp32; the margin above their rounding keeps the shares within DQ_MOST, and a unit of no division
+  // is one step more where fp32 may have rounded the longest list down (past 2^24 steps, of at most 2^25).
   __device__ __forceinline__ void plan(const DecodeQ4Args& a, int len64, int of_seq) {
     unit = a.unit;
     if (unit) return;
